@@ -37,7 +37,7 @@
 extern "C" {
 #endif
 
-#define VDN_FP8_ABI_VERSION 6
+#define VDN_FP8_ABI_VERSION 7
 
 /* status codes */
 #define VDN_FP8_OK 0
@@ -339,6 +339,123 @@ int vdn_fp8_gated_residual(const void *residual, int64_t ldr, const void *gate, 
                            const int32_t *gate_index, int64_t gate_rows, const void *branch,
                            int64_t ldb, void *out, int64_t ldo, int64_t M, int64_t N,
                            hipStream_t stream);
+
+/*
+ * The 8-bit key/value cache: a pool of pages of VDN_FP8_KV_PAGE tokens, each page holding every
+ * key/value head of its tokens.
+ *   k       e4m3 [pages, heads, 64, head_dim]
+ *   v       e4m3 [pages, heads, head_dim, 64]   (transposed: a page's tokens are contiguous)
+ *   k_scale, v_scale   e8m0 [pages, heads]: a page's keys are code * 2^(k_scale - 127)
+ *   k_mean  bf16 [pages, heads, head_dim], each page's mean key, or NULL (then kv_select is not
+ *           available and kv_append does not keep it)
+ * k, v and k_mean 16-byte aligned; head_dim in {64, 128, 256}.
+ */
+#define VDN_FP8_KV_PAGE 64
+typedef struct {
+    void *k, *v, *k_scale, *v_scale, *k_mean;
+    int64_t pages, heads, head_dim;
+} vdn_fp8_kv_cache;
+
+/*
+ * The sequences of a call. Row b of page_table (int32, row stride ldtable >= 0) lists the pool pages of
+ * sequence b in order, max_pages at most; an entry outside the pool means that the page is not there:
+ * nothing is stored in it, and its tokens are not attended to. lengths[b] (int32) counts the tokens of
+ * sequence b in the cache INCLUDING the call's own, of which sequence b has rows
+ * [q_start[b], q_start[b + 1]) (int32 [batch + 1], not decreasing, from 0), or tokens / batch each where
+ * q_start is NULL. Its n rows are its last n positions. All arrays are in device memory; a length
+ * beyond the table counts as the table's. Rows behind q_start[batch] belong to no sequence.
+ */
+typedef struct {
+    const int32_t *page_table;
+    int64_t ldtable, max_pages;
+    const int32_t *lengths, *q_start;
+    int64_t batch, tokens;
+} vdn_fp8_kv_batch;
+
+/*
+ * Stores keys and values (dtype: VDN_FP8_DTYPE_*; [tokens, heads, head_dim], token strides ldk, ldv,
+ * heads contiguous) at their positions. For the tokens that a page receives, per head, with amax over
+ * their finite elements:
+ *   e      = the least integer with amax <= 448 * 2^e, in [-100, 120] (-100 for zeros), and no less than
+ *            the page's own where it keeps earlier tokens
+ *   code   = e4m3(x * 2^-e)                   (one rounding; infinities and NaN become NaN)
+ *   k_mean = bf16(mean of the page's codes * 2^e)
+ * Codes of earlier tokens in the page become e4m3(code * 2^(own - e)); tokens behind the call's last
+ * keep their bytes. A page may receive tokens from one sequence of a call only.
+ * Replaces: nothing in the reference, whose attention reads the k and v of one call
+ *           (src/models/softmax_attention).
+ * Requires: ldk, ldv multiples of 8 and >= heads * head_dim; key, value 16-byte aligned.
+ */
+int vdn_fp8_kv_append(const vdn_fp8_kv_cache *cache, const vdn_fp8_kv_batch *batch, const void *key,
+                      int64_t ldk, const void *value, int64_t ldv, int dtype, hipStream_t stream);
+
+/*
+ * vdn_fp8_qk_prep of the query (bf16 [tokens, q_heads, head_dim] -> out) and of the key, and the store
+ * of that key and the value, in one launch: the bits of vdn_fp8_qk_prep twice, then vdn_fp8_kv_append
+ * with VDN_FP8_DTYPE_BF16. weight_q, weight_k bf16 [head_dim] or NULL; cos, sin [tokens, rotary_dim]
+ * as in vdn_fp8_qk_prep.
+ * Replaces: _qk_prep (src/models/softmax_attention/kernels.py:33-45) as HybridAttention._qkv calls it
+ *           (src/models/hybrid_attention.py:128-130), with the store behind it.
+ * Requires: as vdn_fp8_kv_append and vdn_fp8_qk_prep, but any number of heads.
+ */
+int vdn_fp8_qk_prep_append(const vdn_fp8_kv_cache *cache, const vdn_fp8_kv_batch *batch, const void *query,
+                           int64_t q_heads, int64_t ldq, const void *key, int64_t ldk, const void *value,
+                           int64_t ldv, const void *weight_q, float eps_q, const void *weight_k,
+                           float eps_k, const void *cos, const void *sin, int64_t rotary_dim,
+                           int64_t ldcs, int cs_bf16, void *out, int64_t ldo, hipStream_t stream);
+
+/*
+ * Softmax attention of the call's queries over the cache:
+ *   out[t][h] = sum_j p_j v_j,  p = softmax_j(scale * query[t][h] . k_j)
+ * over the tokens j of t's sequence, with `causal` those up to t's own position, of key/value head
+ * h / (q_heads / heads). query (dtype bf16 or binary16, [tokens, q_heads, head_dim], token stride
+ * ldq, heads contiguous); out of its type, contiguous; lse (or NULL) binary32 [tokens, q_heads]
+ * receives log(sum_j exp(scale * query . k_j)). A row that sees no token gets zeros, and -inf in lse;
+ * so do rows behind the last sequence. Scores, weights' sums and outputs are accumulated in binary32;
+ * queries take part with all their bits, weights rounded to 11 bits. A NaN that is stored reaches the
+ * rows that attend to it and no others.
+ * blocks (int32 [rows, heads, top], or NULL for all pages) lists, for each block of query_block
+ * consecutive queries of a sequence and each key/value head, the pages (numbers within the
+ * sequence) that it attends to; entries outside the sequence are skipped, a page listed twice counts
+ * twice. The block that holds token i of sequence b is row floor(q_start[b] / query_block) + b +
+ * floor(i / query_block) with q_start and query_block > 1, b ceil(n / query_block) + floor(i /
+ * query_block) without; with query_block = 1 the token's own row.
+ * max_query: at least the rows of the longest sequence where q_start is given (0: unknown).
+ * The workspace has the bytes that the size query gives for the same arguments (top = 0 without
+ * blocks), 16-byte aligned; nothing in it needs to be set, and calls that overlap need their own.
+ * Replaces: the attention of HybridAttention's softmax branch (src/models/softmax_attention/window.py:56,
+ *           decomposed.py:190) for keys and values held in a cache.
+ * Requires: q_heads a multiple of heads; tokens * q_heads < 2^30; query_block 1 or query_block *
+ *           q_heads / heads a multiple of 128; scale > 0; ldq % 8 == 0; query, out 16-byte aligned.
+ */
+int vdn_fp8_kv_attention_workspace_size(const vdn_fp8_kv_cache *cache, const vdn_fp8_kv_batch *batch,
+                                        int64_t q_heads, int64_t max_query, int64_t top,
+                                        int64_t query_block, int64_t *bytes);
+int vdn_fp8_kv_attention(const vdn_fp8_kv_cache *cache, const vdn_fp8_kv_batch *batch, const void *query,
+                         int dtype, int64_t q_heads, int64_t ldq, int64_t max_query, float scale,
+                         int causal, const int32_t *blocks, int64_t top, int64_t query_block, void *out,
+                         float *lse, void *workspace, int64_t workspace_bytes, hipStream_t stream);
+
+/*
+ * The pages that each block of queries attends to, by a cheap score: for each block of query_block
+ * consecutive queries of a sequence and each key/value head
+ *   score[w] = (sum of the block's queries over its tokens and the head's group) . k_mean[page w]
+ * (the sum rounded to binary32 once, the products summed in binary64) over the pages that the block's
+ * last query sees. The first `first` and last `last` of those are taken in any case, then those of the
+ * largest scores, `top` in all; equal scores go to the lower page, NaN counts as -inf, and a page that is not
+ * in the pool is never taken. blocks (int32 [rows, heads, top], rows as vdn_fp8_kv_attention numbers
+ * them) receives them in ascending order, then -1; rows without a query hold -1.
+ * The workspace as above.
+ * Replaces: nothing in the reference (its softmax branch attends to fixed windows,
+ *           src/models/softmax_attention/window.py).
+ * Requires: as vdn_fp8_kv_attention; k_mean; first, last >= 0; first + last <= top.
+ */
+int vdn_fp8_kv_select_workspace_size(const vdn_fp8_kv_cache *cache, const vdn_fp8_kv_batch *batch,
+                                     int64_t q_heads, int64_t query_block, int64_t *bytes);
+int vdn_fp8_kv_select(const vdn_fp8_kv_cache *cache, const vdn_fp8_kv_batch *batch, const void *query,
+                      int dtype, int64_t q_heads, int64_t ldq, int causal, int64_t top, int64_t first,
+                      int64_t last, int64_t query_block, int32_t *blocks, void *workspace,
+                      int64_t workspace_bytes, hipStream_t stream);
 
 /* The message of the last failed call on this host thread ("" if none). */
 const char *vdn_fp8_last_error(void);

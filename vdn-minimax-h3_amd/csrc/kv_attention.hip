@@ -1,0 +1,840 @@
+// Softmax attention over the 8-bit key/value cache.
+//
+// For a query row q (one token, one head) over the visible tokens j of its sequence:
+//   x_j = log2(e) scale (q . k_j),  k_j = code 2^ek,   o = sum_j 2^(x_j) v_j / sum_j 2^(x_j)
+// in one pass over the pages with a running maximum. Three choices carry the arithmetic:
+//
+//   Scores on the fp8 matrix cores, without rounding the queries to 8 bits. A bf16 value has eight
+//   significant bits, so it is exactly hi + lo with hi = e4m3(q 2^-eq) and lo the e4m3 of the
+//   rest times 2^4 (eq: a power of two for each row that brings its largest element to [224, 448];
+//   elements 2^-11 below that one lose bits under 2^-21 of it). Two fp8 products cost what one bf16
+//   product does, and the keys, the larger operand, go to the matrix cores as they are stored. A
+//   binary16 query has eleven bits and takes a third term. The lower terms' factors are the
+//   instruction's own block scales.
+//
+//   Values in binary16: e4m3 codes are binary16 numbers, and weights in [0, 2^8] keep eleven bits
+//   (bf16 weights would leave eight, an error as large as the output's own rounding). The value's scale
+//   2^ev never meets the codes: it joins the exponent of the weight, P' = 2^(x + ev - m), where m
+//   is the running maximum of x + ev, so that the product's sum is that of the real values, and a
+//   page's sum of weights is 2^-ev times its sum of P'. Sums, maxima and accumulators are binary32.
+//
+//   The transposed scores S^T = K Q^T leave each lane 16 consecutive keys of one query (the key that
+//   a matrix row stands for is a matter of which row is loaded where), and those are the operand of
+//   O^T = V^T P^T as they are: P goes from one product to the next in registers.
+//
+// A running maximum is raised only when it would move by more than 8 (weights up to 2^8 stay in
+// binary16's range), so most pages rescale nothing.
+//
+// Rows are (token, head of a group) pairs of one key/value head, so grouped heads share the pages
+// that they read. Two kernels:
+//   k_kv_attn_rows    128 rows, 32 for each of four waves, which share the pages through LDS (copied
+//                     there asynchronously, two pages ahead). For chunks and prompts.
+//   k_kv_attn_step    up to 32 rows; each of the four waves takes every fourth page, straight from
+//                     memory into the operands' registers, and they join at the end. For single tokens.
+// Both cut long key axes into splits where there are few rows, joined by k_kv_attn_join.
+#include <stdint.h>
+
+#include <atomic>
+
+#include "gemm_common.h"
+#include "kv_common.h"
+#include "vdn_common.h"
+
+namespace vdn {
+namespace {
+
+constexpr int kRows = 128, kWaveRows = 32;
+constexpr int kMostSplits = 64;
+constexpr float kNoMax = -3.0e38f;      // the running maximum of no keys: finite, so that differences stay numbers
+constexpr float kSlack = 8.0f;          // the maximum moves only past this
+constexpr int kAbsent = 1 << 30;        // first key of a page that is not there: behind every sequence
+
+typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
+
+struct KvAttnArgs {
+    KvCacheArgs c;
+    KvBatchArgs b;
+    KvUnits units;          // the units of rows
+    const uint16_t* q;
+    int64_t ldq;
+    int group, q_heads;     // query heads for each key/value head, and in all
+    float scale;            // of the scores, times log2(e)
+    int causal;
+    const int32_t* blocks;  // [listed units, heads, top] pages that a query block attends to, or NULL
+    int top, query_block;
+    KvUnits listed;
+    uint16_t* out;
+    float* lse;
+    float* part;            // splits > 1: [tokens * q_heads][splits][d], then the (maximum, sum) pairs
+    int splits, column_tiles;
+    int step_rows;          // rows of a unit of k_kv_attn_step at most
+    uint32_t items;         // workgroups of k_kv_attn_rows
+};
+
+__device__ __forceinline__ float* part_sums(const KvAttnArgs& p)
+{
+    return p.part + p.b.tokens * p.q_heads * p.splits * p.c.d;
+}
+
+// The key of each 32 that row r of the matrix stands for: lane group g = (r >> 2) & 1 of the output
+// then holds keys 16 g .. 16 g + 15 in its registers' order.
+__device__ __forceinline__ int row_key(int r) { return 16 * ((r >> 2) & 1) + 4 * (r >> 3) + (r & 3); }
+
+// max / sum with the lane that holds the same query's other 16 keys.
+__device__ __forceinline__ float half_max(float v)
+{
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float half_sum(float v)
+{
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+__device__ __forceinline__ float exponent_f32(int e) { return __uint_as_float((uint32_t)(min(max(e, -126), 127) + 127) << 23); }
+
+// 16 codes of one operand row -> two operands of eight binary16 values (exact).
+__device__ __forceinline__ void decode16(uint4 w, f16x8_t o[2])
+{
+    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const f16x2_t lo = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(u[i], 1.0f, false);
+        const f16x2_t hi = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(u[i], 1.0f, true);
+        o[i / 2][4 * (i % 2)] = lo.x, o[i / 2][4 * (i % 2) + 1] = lo.y;
+        o[i / 2][4 * (i % 2) + 2] = hi.x, o[i / 2][4 * (i % 2) + 3] = hi.y;
+    }
+}
+
+// One wave's 32 rows: the queries as fp8 terms, the running softmax, the output's accumulators.
+// Lane (column l % 32, half g = l / 32): the column is the row of the problem.
+template <int D, bool F16>
+struct WaveRows {
+    static constexpr int kSteps = D / 64, kTerms = F16 ? 3 : 2, kTiles = D / 32;
+    i32x8_t q[kTerms][kSteps];
+    f32x16_t acc[kTiles];
+    float m, l, c;     // running maximum and sum (of this half's keys), factor of the raw scores
+    int limit;         // keys below it are visible to the row
+
+    // row: the row's values (NULL: none, zeros).
+    __device__ __forceinline__ void load(const uint16_t* row, int g, float scale)
+    {
+        float x[kSteps][32];
+        uint32_t top = 0;
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                uint4 v = make_uint4(0, 0, 0, 0);
+                if (row) v = *reinterpret_cast<const uint4*>(row + 64 * s + 32 * g + 8 * i);
+                const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    float lo, hi;
+                    if (F16) {
+                        lo = (float)__builtin_bit_cast(_Float16, (uint16_t)w[e]);
+                        hi = (float)__builtin_bit_cast(_Float16, (uint16_t)(w[e] >> 16));
+                    } else {
+                        lo = bf16_lo(w[e]), hi = bf16_hi(w[e]);
+                    }
+                    x[s][8 * i + 2 * e] = lo, x[s][8 * i + 2 * e + 1] = hi;
+                    const uint32_t a = __float_as_uint(lo) & 0x7fffffffu, b = __float_as_uint(hi) & 0x7fffffffu;
+                    top = max(top, max(a < 0x7f800000u ? a : 0u, b < 0x7f800000u ? b : 0u));
+                }
+            }
+        const auto other = __builtin_amdgcn_permlane32_swap(top, top, false, false);
+        top = max((uint32_t)other[0], (uint32_t)other[1]);
+        int e = (int)(top >> 23) - 127 - 8 + ((top & 0x7fffffu) > 0x600000u ? 1 : 0);
+        e = top == 0 ? 0 : min(max(e, -120), 120);
+        const float f = exponent_f32(-e);
+        c = scale * exponent_f32(e);
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                float r[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) r[j] = x[s][4 * i + j] * f;
+#pragma unroll
+                for (int t = 0; t < kTerms; ++t) {
+                    const uint32_t w = pack_e4m3x4(r[0], r[1], r[2], r[3]);
+                    q[t][s][i] = (int)w;
+                    // the rest, exact; times the next term's factor: 2^4, then 2^5
+                    const float up = t == 0 ? 16.0f : 32.0f;
+                    r[0] = (r[0] - __builtin_amdgcn_cvt_f32_fp8(w, 0)) * up;
+                    r[1] = (r[1] - __builtin_amdgcn_cvt_f32_fp8(w, 1)) * up;
+                    r[2] = (r[2] - __builtin_amdgcn_cvt_f32_fp8(w, 2)) * up;
+                    r[3] = (r[3] - __builtin_amdgcn_cvt_f32_fp8(w, 3)) * up;
+                }
+            }
+        m = kNoMax, l = 0.0f;
+#pragma unroll
+        for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) acc[t][i] = 0.0f;
+    }
+
+    // Scores of 64 keys: key(kt, s) gives 32 codes of this lane's matrix row.
+    template <typename Key>
+    __device__ __forceinline__ void scores(Key key, f32x16_t s[2]) const
+    {
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s[kt][i] = 0.0f;
+#pragma unroll
+            for (int st = 0; st < kSteps; ++st) {
+                const i32x8_t a = key(kt, st);
+                s[kt] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a, q[0][st], s[kt], 0, 0, 0, 0x7f7f7f7f, 0, 0x7f7f7f7f);
+                s[kt] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a, q[1][st], s[kt], 0, 0, 0, 0x7f7f7f7f, 0, 0x7b7b7b7b);
+                if (kTerms == 3)
+                    s[kt] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a, q[kTerms - 1][st], s[kt], 0, 0, 0, 0x7f7f7f7f, 0, 0x76767676);
+            }
+        }
+    }
+
+    // Keys from key0 on that the row does not see.
+    __device__ __forceinline__ void mask(f32x16_t s[2], int key0, int g) const
+    {
+        const int seen = limit - key0 - 16 * g;   // visible ones of this half's keys, counted from its first
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s[kt][i] = 32 * kt + i < seen ? s[kt][i] : -__builtin_inff();
+    }
+
+    // Scores -> weights in binary16, for a page whose scales are 2^ek and 2^ev.
+    __device__ __forceinline__ void weights(f32x16_t s[2], int ek, int ev, f16x8_t w[2][2])
+    {
+        const float f = fmaxf(c * exponent_f32(ek), 1e-37f);   // (never 0: a masked score stays -inf)
+        const float shift = (float)ev;
+        float top = fmaxf(s[0][0], s[1][0]);
+#pragma unroll
+        for (int i = 1; i < 16; ++i) top = fmaxf(top, fmaxf(s[0][i], s[1][i]));
+        top = half_max(top) * f + shift;
+        if (__any(top > m + kSlack)) {
+            const float now = fmaxf(m, top), a = __builtin_amdgcn_exp2f(m - now);
+            m = now;
+            l *= a;
+#pragma unroll
+            for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) acc[t][i] *= a;
+        }
+        const float base = shift - m;
+        float sum = 0.0f;
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kt][8 * h + j], f, base));
+                    sum += p;
+                    w[kt][h][j] = (_Float16)p;
+                }
+        l = __builtin_fmaf(sum, exponent_f32(-ev), l);
+    }
+
+    // Adds the weighted values of a page: value(kt, t) gives 16 tokens' codes of one element. MASKED:
+    // the page has tokens that some row does not see. Those behind the sequence's end hold what an
+    // earlier owner left and count as zeros; a NaN code of a token that some rows see and others do
+    // not reaches the rows that see it, through a product of indicators.
+    template <bool MASKED, typename Value>
+    __device__ __forceinline__ void add_values(Value value, const f16x8_t w[2][2], int key0, int end, int g)
+    {
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt) {
+#pragma unroll
+            for (int t = 0; t < kTiles; ++t) {
+                uint4 v = value(kt, t);
+                f16x8_t a[2];
+                if (MASKED) {
+                    const int have = end - (key0 + 32 * kt + 16 * g);   // of these 16 tokens
+                    uint32_t u[4] = {v.x, v.y, v.z, v.w}, nan[4], any = 0;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int n = have - 4 * i;
+                        u[i] = n >= 4 ? u[i] : n <= 0 ? 0u : u[i] & (0xffffffffu >> (32 - 8 * n));
+                        nan[i] = ((u[i] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
+                        any |= nan[i];
+                    }
+                    if (__any(any != 0)) {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            u[i] &= ~((nan[i] >> 7) * 0xffu);
+                            nan[i] = (nan[i] >> 7) * 0x38u;   // e4m3 1.0
+                        }
+                        f16x8_t is_nan[2];
+                        decode16(make_uint4(nan[0], nan[1], nan[2], nan[3]), is_nan);
+                        f32x16_t hit;
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) hit[i] = 0.0f;
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            f16x8_t seen;
+#pragma unroll
+                            for (int j = 0; j < 8; ++j) seen[j] = key0 + 32 * kt + 16 * g + 8 * h + j < limit ? (_Float16)1.0f : (_Float16)0.0f;
+                            hit = __builtin_amdgcn_mfma_f32_32x32x16_f16(is_nan[h], seen, hit, 0, 0, 0);
+                        }
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) acc[t][i] = hit[i] > 0.0f ? __builtin_nanf("") : acc[t][i];
+                    }
+                    v = make_uint4(u[0], u[1], u[2], u[3]);
+                }
+                decode16(v, a);
+                acc[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[0], w[kt][0], acc[t], 0, 0, 0);
+                acc[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[1], w[kt][1], acc[t], 0, 0, 0);
+            }
+        }
+    }
+};
+
+// A page's place in the sequence and in the pool.
+struct PageAt {
+    int key0;       // its first token, kAbsent where there is none
+    int64_t ph;     // page * heads + head
+    int ek, ev;
+};
+
+__device__ __forceinline__ PageAt page_at(const KvAttnArgs& p, int b, int h, int length, const int32_t* list, int i)
+{
+    PageAt a;
+    int w = list ? list[i] : i;
+    const int have = (length + kPage - 1) / kPage;
+    const int page = w >= 0 && w < have ? kv_page(p.b, p.c, b, w) : -1;
+    a.key0 = page >= 0 ? w * kPage : kAbsent;
+    a.ph = (int64_t)max(page, 0) * p.c.heads + h;
+    a.ek = scalar_byte(p.c.k_scale, a.ph) - 127;
+    a.ev = scalar_byte(p.c.v_scale, a.ph) - 127;
+    return a;
+}
+
+template <bool F16>
+__device__ __forceinline__ uint32_t pack_out(float lo, float hi)
+{
+    if (!F16) return pack_bf16x2(lo, hi);
+    const f16x2_t p = {(_Float16)lo, (_Float16)hi};
+    return __builtin_bit_cast(uint32_t, p);
+}
+
+// The rows of key/value head h for the tokens behind the last sequence: zeros, and no weight.
+__device__ __forceinline__ void clear_rows(const KvAttnArgs& p, int64_t first, int64_t end, int h)
+{
+    const int64_t rows = (end - first) * p.group;
+    const int chunks = p.c.d / 8;
+    for (int64_t i = threadIdx.x; i < rows * chunks; i += blockDim.x) {
+        const int64_t row = i / chunks, at = (first + row / p.group) * p.q_heads + h * p.group + row % p.group;
+        *reinterpret_cast<uint4*>(p.out + at * p.c.d + 8 * (i % chunks)) = make_uint4(0, 0, 0, 0);
+        if (p.lse && i % chunks == 0) p.lse[at] = -__builtin_inff();
+    }
+}
+
+// The rows [r0, r0 + 128) of one sequence and key/value head, or the part of their keys that is split
+// `split`'s.
+template <int D, bool F16>
+__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_kv_attn_rows(KvAttnArgs p)
+{
+    constexpr int kBuffers = D == 256 ? 2 : 3;
+    constexpr int kPageBytes = kPage * D;            // of k, and of v
+    constexpr int kCopies = D / 64;                  // 4 KB each, of k and of v
+    extern __shared__ __attribute__((aligned(128))) uint8_t lds[];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int r = lane & 31, g = lane >> 5;
+
+    // XCD (blockIdx % 8) takes a run of items, neighbours in which read the same pages
+    uint32_t item;
+    {
+        const uint32_t per = p.items / 8, rest = p.items % 8, x = blockIdx.x % 8, i = blockIdx.x / 8;
+        item = (x < rest ? x * (per + 1) : rest * (per + 1) + (x - rest) * per) + i;
+    }
+    const int split = (int)(item % p.splits);
+    item /= p.splits;
+    const uint32_t units = p.items / p.splits / p.c.heads;
+    const int h = __builtin_amdgcn_readfirstlane((int)(item / units));
+    int64_t at64;
+    // (the last units of a sequence first: with a causal mask they are the longest)
+    const int b = __builtin_amdgcn_readfirstlane(kv_locate(p.b, p.units, units - 1 - item % units, at64));
+    if (b == p.b.batch) {   // behind the last sequence
+        if (split == 0) {
+            const int64_t end = min(max((int64_t)p.b.q_start[b], (int64_t)0), p.b.tokens);
+            const int64_t each = max(kRows / p.group, 1);   // tokens; as many units as kv_unit_count leaves take turns
+            for (int64_t t = end + at64 * each; t < p.b.tokens; t += each * (int64_t)(units - kv_first_unit(p.b, p.units, b)))
+                clear_rows(p, t, min(t + each, p.b.tokens), h);
+        }
+        return;
+    }
+    const int at = __builtin_amdgcn_readfirstlane((int)at64);
+    const KvSequence s = kv_sequence(p.b, b);
+    const int r0 = at * kRows, rows = s.n * p.group;   // (tokens * q_heads < 2^30)
+    if (at >= (rows + kRows - 1) / kRows) return;
+    const int last = min(r0 + kRows, rows) - 1;
+    auto limit_of = [&](int row) -> int {
+        if (!p.causal) return s.length;
+        return (int)min(max(s.first + (uint32_t)row / (uint32_t)p.group + 1, (int64_t)0), (int64_t)s.length);
+    };
+    const int32_t* list = nullptr;
+    int lo, hi;
+    if (p.blocks) {
+        // the query block's number, as p.listed counts them
+        const int64_t block = r0 / (p.query_block * p.group);
+        const int64_t unit = p.b.q_start ? kv_first_unit(p.b, p.listed, b) + block : (int64_t)b * p.listed.each + block;
+        list = p.blocks + (unit * p.c.heads + h) * p.top;
+        lo = 0, hi = p.b.width > 0 ? p.top : 0;   // (no pages, no list to look at)
+    } else {
+        lo = 0, hi = (limit_of(last) + kPage - 1) / kPage;
+    }
+    if (p.splits > 1) {
+        const int per = max((hi + p.splits - 1) / p.splits, 1);
+        lo = min(split * per, hi);
+        hi = min(lo + per, hi);
+    }
+
+    WaveRows<D, F16> rowset;
+    const int w0 = r0 + wave * kWaveRows;
+    const bool idle = w0 >= rows;   // this wave copies only
+    const int row = w0 + r;
+    const bool valid = row < rows;
+    const int64_t token = s.start + (uint32_t)row / (uint32_t)p.group;
+    const int head = h * p.group + (uint32_t)row % (uint32_t)p.group;
+    rowset.load(valid ? p.q + token * p.ldq + (int64_t)head * D : nullptr, g, p.scale);
+    rowset.limit = valid ? limit_of(row) : 0;
+    const int least = limit_of(min(w0, last)), most = limit_of(min(w0 + kWaveRows - 1, last));
+
+    // Copies: this thread's 16 bytes of each 4 KB. In LDS, k lies in 128-byte lines (a row's d = 64, or
+    // 128 elements of it, the next 128 behind all rows; two rows of 64), v in rows of 64 tokens, two to
+    // a line; chunk c of line L at c ^ (L & 7), of 128-byte rows at c ^ ((row >> 1) & 7): the reads of
+    // 32 rows by 64 lanes fall on all banks. Rows are in the matrix's order (row_key).
+    const int line = tid / 8, slot = tid % 8;
+    uint32_t from_k, from_v;
+    {
+        const int x = slot ^ (line & 7), row_v = 2 * line + (x >> 2);
+        from_v = (uint32_t)(((row_v & 32) + row_key(row_v & 31)) * kPage + (x & 3) * 16);
+        if (D == 64) from_k = (uint32_t)(((row_v & 32) + row_key(row_v & 31)) * D + (x & 3) * 16);
+        else from_k = (uint32_t)(row_key(line) * D + (slot ^ ((line >> 1) & 7)) * 16);
+    }
+    const uint32_t base = (uint32_t)(uintptr_t)(lds_void_t*)lds + wave * 1024;
+    auto copy = [&](const PageAt& a, int buffer) {
+        const i32x4_t rk = rsrc_words(p.c.k + a.ph * kPageBytes, kPageBytes);
+        const i32x4_t rv = rsrc_words(p.c.v + a.ph * kPageBytes, kPageBytes);
+        const uint32_t to = __builtin_amdgcn_readfirstlane(base + buffer * (2 * kPageBytes));
+#pragma unroll
+        for (int j = 0; j < kCopies; ++j) {
+            const int off = D == 64 ? 0 : (j & 1) * 32 * D + (j >> 1) * 128;
+            copy16_to_lds(rk, to + j * 4096, from_k, off);
+            copy16_to_lds(rv, to + kPageBytes + j * 4096, from_v, j * 4096);
+        }
+    };
+    // Reads: lane (r, g) takes 32 codes of a key in two pieces, 16 tokens of a value's element in one.
+    const int sw = (r >> 1) & 7;
+    const int k_line = D == 64 ? (r >> 1) * 128 : r * 128, k_chunk = D == 64 ? (r & 1) * 4 + 2 * g : 2 * g;
+    const int v_line = (r >> 1) * 128, v_chunk = (r & 1) * 4 + g;
+
+    PageAt now{}, next{}, after{};
+    if (lo < hi) {
+        now = page_at(p, b, h, s.length, list, lo);
+        copy(now, 0);
+        if (lo + 1 < hi) {
+            next = page_at(p, b, h, s.length, list, lo + 1);
+            if (kBuffers == 3) copy(next, 1);
+        }
+    }
+    int buffer = 0;
+    for (int i = lo; i < hi; ++i) {
+        if (kBuffers == 3 && i + 1 < hi) wave_sync<2 * kCopies>();
+        else wave_sync<0>();
+        if (kBuffers == 3) {
+            if (i + 2 < hi) {
+                after = page_at(p, b, h, s.length, list, i + 2);
+                copy(after, buffer == 0 ? 2 : buffer - 1);
+            }
+        } else {
+            if (i + 1 < hi) copy(next, buffer ^ 1);
+            if (i + 2 < hi) after = page_at(p, b, h, s.length, list, i + 2);
+        }
+        if (!idle && now.key0 < most) {
+            const uint8_t* const kb = lds + buffer * (2 * kPageBytes);
+            const uint8_t* const vb = kb + kPageBytes;
+            auto key = [&](int kt, int st) {
+                const uint8_t* const at_k = kb + k_line + (D == 64 ? kt * 2048 : kt * 4096 + (st >> 1) * 8192);
+                const int c = D == 64 ? k_chunk : k_chunk + 4 * (st & 1);
+                const uint4 x = *reinterpret_cast<const uint4*>(at_k + ((c ^ sw) * 16));
+                const uint4 y = *reinterpret_cast<const uint4*>(at_k + (((c + 1) ^ sw) * 16));
+                return i32x8_t{(int)x.x, (int)x.y, (int)x.z, (int)x.w, (int)y.x, (int)y.y, (int)y.z, (int)y.w};
+            };
+            auto value = [&](int kt, int t) {
+                return *reinterpret_cast<const uint4*>(vb + v_line + t * 2048 + (((v_chunk + 2 * kt) ^ sw) * 16));
+            };
+            f32x16_t sc[2];
+            f16x8_t w[2][2];
+            rowset.scores(key, sc);
+            const bool masked = now.key0 + kPage > least;
+            if (masked) rowset.mask(sc, now.key0, g);
+            rowset.weights(sc, now.ek, now.ev, w);
+            if (masked) rowset.template add_values<true>(value, w, now.key0, s.length, g);
+            else rowset.template add_values<false>(value, w, now.key0, s.length, g);
+        }
+        now = next, next = after;
+        buffer = buffer + 1 == kBuffers ? 0 : buffer + 1;
+    }
+
+    if (!valid) return;
+    const float l = half_sum(rowset.l);
+    const int64_t out_row = token * p.q_heads + head;
+    if (p.splits > 1) {
+        float* const dst = p.part + (out_row * p.splits + split) * D + 16 * g;
+        if (lo < hi)
+#pragma unroll
+            for (int t = 0; t < D / 32; ++t)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    *reinterpret_cast<float4*>(dst + 32 * t + 4 * i) = make_float4(rowset.acc[t][4 * i], rowset.acc[t][4 * i + 1],
+                                                                                 rowset.acc[t][4 * i + 2], rowset.acc[t][4 * i + 3]);
+        if (g == 0) *reinterpret_cast<float2*>(part_sums(p) + 2 * (out_row * p.splits + split)) = make_float2(rowset.m, l);
+        return;
+    }
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    uint16_t* const dst = p.out + out_row * D + 16 * g;
+#pragma unroll
+    for (int t = 0; t < D / 32; ++t)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const f32x16_t& a = rowset.acc[t];
+            *reinterpret_cast<uint4*>(dst + 32 * t + 8 * i) =
+                make_uint4(pack_out<F16>(a[8 * i] * inv, a[8 * i + 1] * inv), pack_out<F16>(a[8 * i + 2] * inv, a[8 * i + 3] * inv),
+                           pack_out<F16>(a[8 * i + 4] * inv, a[8 * i + 5] * inv), pack_out<F16>(a[8 * i + 6] * inv, a[8 * i + 7] * inv));
+        }
+    if (p.lse && g == 0)
+        p.lse[out_row] = l == 0.0f ? -__builtin_inff() : (rowset.m + __builtin_log2f(l)) * 0.6931471805599453f;
+}
+
+// Up to 32 rows of one sequence (or of one token, where each has its own pages) and key/value head.
+template <int D, bool F16>
+__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_kv_attn_step(KvAttnArgs p)
+{
+    constexpr int kTiles = D / 32, kSteps = D / 64;
+    extern __shared__ __attribute__((aligned(128))) uint8_t lds[];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int r = lane & 31, g = lane >> 5;
+
+    uint32_t item = blockIdx.x;
+    const int split = (int)(item % p.splits);
+    item /= p.splits;
+    const int tile = (int)(item % p.column_tiles);
+    item /= p.column_tiles;
+    const int h = __builtin_amdgcn_readfirstlane((int)(item % p.c.heads));
+    const uint32_t unit = item / p.c.heads;
+    int b = (int)unit;
+    if (p.blocks) {   // a unit is a token
+        if (p.b.q_start) {
+            int64_t none;
+            b = kv_locate(p.b, KvUnits{1, 1, 1, 0}, unit, none);
+        } else {
+            b = (int)(unit / (uint32_t)(p.b.tokens / p.b.batch));
+        }
+    }
+    b = __builtin_amdgcn_readfirstlane(b);
+    if (b == p.b.batch) {   // behind the last sequence
+        if (split == 0 && tile == 0) {
+            const int64_t end = min(max((int64_t)p.b.q_start[b], (int64_t)0), p.b.tokens);
+            clear_rows(p, p.blocks ? unit : end, p.blocks ? unit + 1 : p.b.tokens, h);
+        }
+        return;
+    }
+    const KvSequence s = kv_sequence(p.b, b);
+    const int at = p.blocks ? (int)((int64_t)unit - s.start) : 0;   // the unit's first token in its sequence
+    if (at < 0 || at >= s.n) return;
+    const int rows = min(p.blocks ? p.group : s.n * p.group, p.step_rows);
+    if (tile * kWaveRows >= rows) return;
+    const int row = tile * kWaveRows + r;
+    const bool valid = row < rows;
+    const int first_token = at + tile * kWaveRows / p.group, last_token = at + (min((tile + 1) * kWaveRows, rows) - 1) / p.group;
+    auto limit_of = [&](int t) -> int {
+        return p.causal ? (int)min(max(s.first + t + 1, (int64_t)0), (int64_t)s.length) : s.length;
+    };
+    const int own = at + row / p.group;
+    const int64_t token = s.start + own;
+    const int head = h * p.group + row % p.group;
+
+    const int32_t* list = p.blocks ? p.blocks + ((int64_t)unit * p.c.heads + h) * p.top : nullptr;
+    int lo = 0, hi = list ? (p.b.width > 0 ? p.top : 0) : (limit_of(last_token) + kPage - 1) / kPage;
+    if (p.splits > 1) {
+        const int per = max((hi + p.splits - 1) / p.splits, 4);
+        lo = min(split * per, hi);
+        hi = min(lo + per, hi);
+    }
+
+    WaveRows<D, F16> rowset;
+    rowset.load(valid ? p.q + token * p.ldq + (int64_t)head * D : nullptr, g, p.scale);
+    rowset.limit = valid ? limit_of(own) : 0;
+    const int least = limit_of(first_token), most = limit_of(last_token);
+
+    const int from_k = row_key(r) * D + 32 * g, from_v = row_key(r) * kPage + 16 * g;
+    uint4 kr[2][kSteps][2], vr[2][kTiles];
+    auto load_k = [&](const PageAt& a) {
+        const uint8_t* const src = p.c.k + a.ph * (kPage * D);
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+            for (int st = 0; st < kSteps; ++st)
+#pragma unroll
+                for (int j = 0; j < 2; ++j)
+                    kr[kt][st][j] = *reinterpret_cast<const uint4*>(src + from_k + kt * 32 * D + st * 64 + j * 16);
+    };
+    auto load_v = [&](const PageAt& a) {
+        const uint8_t* const src = p.c.v + a.ph * (kPage * D);
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+            for (int t = 0; t < kTiles; ++t) vr[kt][t] = *reinterpret_cast<const uint4*>(src + from_v + t * 32 * kPage + kt * 32);
+    };
+    PageAt now{}, next{};
+    int i = lo + wave;
+    if (i < hi) {
+        now = page_at(p, b, h, s.length, list, i);
+        load_k(now);
+        load_v(now);
+    }
+    for (; i < hi; i += 4) {
+        const bool more = i + 4 < hi;
+        if (more) next = page_at(p, b, h, s.length, list, i + 4);
+        f32x16_t sc[2];
+        f16x8_t w[2][2];
+        rowset.scores([&](int kt, int st) {
+            const uint4 x = kr[kt][st][0], y = kr[kt][st][1];
+            return i32x8_t{(int)x.x, (int)x.y, (int)x.z, (int)x.w, (int)y.x, (int)y.y, (int)y.z, (int)y.w};
+        }, sc);
+        if (more) load_k(next);
+        if (now.key0 < most) {
+            const bool masked = now.key0 + kPage > least;
+            if (masked) rowset.mask(sc, now.key0, g);
+            rowset.weights(sc, now.ek, now.ev, w);
+            auto value = [&](int kt, int t) { return vr[kt][t]; };
+            if (masked) rowset.template add_values<true>(value, w, now.key0, s.length, g);
+            else rowset.template add_values<false>(value, w, now.key0, s.length, g);
+        }
+        if (more) load_v(next);
+        now = next;
+    }
+
+    // The four waves' parts of each row, joined in LDS: [wave][row][d], then their maxima and sums.
+    const int kept = min(rows - tile * kWaveRows, kWaveRows);
+    float* const acc = reinterpret_cast<float*>(lds);
+    float* const sums = acc + 4 * kept * D;
+    const float l = half_sum(rowset.l);
+    if (r < kept) {
+        float* const dst = acc + (wave * kept + r) * D + 16 * g;
+#pragma unroll
+        for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                *reinterpret_cast<float4*>(dst + 32 * t + 4 * j) = make_float4(rowset.acc[t][4 * j], rowset.acc[t][4 * j + 1],
+                                                                             rowset.acc[t][4 * j + 2], rowset.acc[t][4 * j + 3]);
+        if (g == 0) sums[2 * (wave * kept + r)] = rowset.m, sums[2 * (wave * kept + r) + 1] = l;
+    }
+    __syncthreads();
+    for (int e = tid; e < kept * (D / 4); e += 256) {
+        const int row_e = e / (D / 4), d = 4 * (e % (D / 4));
+        float m = kNoMax;
+#pragma unroll
+        for (int wv = 0; wv < 4; ++wv) m = fmaxf(m, sums[2 * (wv * kept + row_e)]);
+        float total = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int wv = 0; wv < 4; ++wv) {
+            const float f = __builtin_amdgcn_exp2f(sums[2 * (wv * kept + row_e)] - m);
+            const float4 a = *reinterpret_cast<const float4*>(acc + (wv * kept + row_e) * D + d);
+            total += f * sums[2 * (wv * kept + row_e) + 1];
+            o[0] += f * a.x, o[1] += f * a.y, o[2] += f * a.z, o[3] += f * a.w;
+        }
+        const int row_at = tile * kWaveRows + row_e;
+        const int64_t out_row = (s.start + at + row_at / p.group) * p.q_heads + h * p.group + row_at % p.group;
+        if (p.splits > 1) {
+            *reinterpret_cast<float4*>(p.part + (out_row * p.splits + split) * D + d) = make_float4(o[0], o[1], o[2], o[3]);
+            if (d == 0) *reinterpret_cast<float2*>(part_sums(p) + 2 * (out_row * p.splits + split)) = make_float2(m, total);
+        } else {
+            const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+            *reinterpret_cast<uint2*>(p.out + out_row * D + d) =
+                make_uint2(pack_out<F16>(o[0] * inv, o[1] * inv), pack_out<F16>(o[2] * inv, o[3] * inv));
+            if (p.lse && d == 0) p.lse[out_row] = total == 0.0f ? -__builtin_inff() : (m + __builtin_log2f(total)) * 0.6931471805599453f;
+        }
+    }
+}
+
+// One wave joins the splits of one row.
+template <int D, bool F16>
+__global__ __launch_bounds__(256) void k_kv_attn_join(KvAttnArgs p)
+{
+    constexpr int E = D / 64;
+    const int lane = threadIdx.x & 63;
+    const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (row >= p.b.tokens * p.q_heads) return;
+    if (p.b.q_start && row / p.q_heads >= p.b.q_start[p.b.batch]) return;   // behind the last sequence
+    const float* const sums = part_sums(p) + 2 * row * p.splits;
+    float2 own = make_float2(kNoMax, 0.0f);
+    if (lane < p.splits) own = *reinterpret_cast<const float2*>(sums + 2 * lane);
+    float m = own.x;
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) m = fmaxf(m, __shfl_xor(m, off, 64));
+    const float f = __builtin_amdgcn_exp2f(own.x - m);
+    float total = f * own.y;
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) total += __shfl_xor(total, off, 64);
+    float o[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) o[e] = 0.0f;
+    for (int i = 0; i < p.splits; ++i) {
+        if (__shfl(own.y, i, 64) == 0.0f) continue;   // no keys there (uniform): its accumulators are not written
+        const float w = __shfl(f, i, 64);
+        const float* const src = p.part + (row * p.splits + i) * D + lane * E;
+#pragma unroll
+        for (int e = 0; e < E; ++e) o[e] += w * src[e];
+    }
+    const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+    uint16_t* const dst = p.out + row * D + lane * E;
+    if (E == 1) dst[0] = (uint16_t)pack_out<F16>(o[0] * inv, 0.0f);
+    else
+#pragma unroll
+        for (int e = 0; e + 1 < E; e += 2) *reinterpret_cast<uint32_t*>(dst + e) = pack_out<F16>(o[e] * inv, o[e + 1] * inv);
+    if (p.lse && lane == 0) p.lse[row] = total == 0.0f ? -__builtin_inff() : (m + __builtin_log2f(total)) * 0.6931471805599453f;
+}
+
+// Which kernel a call takes, its units and its splits.
+struct Plan {
+    bool step;
+    int64_t items;          // workgroups
+    int splits, column_tiles, step_rows;
+    int64_t bytes;          // of workspace
+};
+
+Plan make_plan(KvAttnArgs& p, int64_t max_query, int cus)
+{
+    Plan plan{};
+    const int64_t n = p.b.q_start ? (max_query > 0 && max_query < p.b.tokens ? max_query : p.b.tokens) : p.b.tokens / p.b.batch;
+    const int64_t most = p.blocks ? p.query_block : n;   // tokens of a unit of the step kernel
+    plan.step = p.blocks ? p.query_block == 1 : n * p.group <= kWaveRows;
+    const int64_t pages = p.blocks ? p.top : p.b.width;
+    int64_t groups;
+    if (plan.step) {
+        plan.step_rows = (int)(most * p.group);
+        plan.column_tiles = (plan.step_rows + kWaveRows - 1) / kWaveRows;
+        // (and one unit that clears what is behind the last sequence)
+        groups = (p.blocks ? p.b.tokens : (int64_t)p.b.batch + (p.b.q_start ? 1 : 0)) * p.c.heads * plan.column_tiles;
+    } else {
+        plan.column_tiles = 1;
+        p.units = KvUnits{kRows, (n * p.group + kRows - 1) / kRows, p.group, 1};
+        groups = (kv_unit_count(p.b, p.units) + (p.b.q_start ? 1 : 0)) * p.c.heads;
+    }
+    // Splits where the workgroups alone leave compute units idle: enough for four workgroups (steps) or
+    // two (rows) on each, of at least four pages.
+    const int64_t want = (int64_t)cus * (plan.step ? 4 : 2), least = 4;
+    int64_t splits = groups > 0 ? want / groups : 1;
+    splits = splits < pages / least ? splits : pages / least;
+    plan.splits = (int)(splits < 1 ? 1 : splits > kMostSplits ? kMostSplits : splits);
+    plan.items = groups * plan.splits;
+    plan.bytes = plan.splits > 1 ? p.b.tokens * p.q_heads * plan.splits * (int64_t)(p.c.d + 2) * 4 : 0;
+    return plan;
+}
+
+template <int D, bool F16>
+int launch(const KvAttnArgs& p, bool step, hipStream_t stream)
+{
+    const dim3 grid((unsigned)p.items), block(256);
+    if (step) {
+        const size_t bytes = (size_t)(4 * (p.step_rows < kWaveRows ? p.step_rows : kWaveRows)) * (D + 2) * 4;
+        if (bytes > 65536) {
+            static std::atomic<bool> raised[64];
+            int dev = 0;
+            if (hipGetDevice(&dev) != hipSuccess) return set_error(VDN_FP8_ELAUNCH, "kv_attention: no device");
+            if (dev >= 64 || !raised[dev].load(std::memory_order_relaxed)) {
+                if (hipFuncSetAttribute((const void*)k_kv_attn_step<D, F16>, hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024) != hipSuccess)
+                    return set_error(VDN_FP8_ELAUNCH, "kv_attention: the device refuses %zu bytes of LDS", bytes);
+                if (dev < 64) raised[dev].store(true, std::memory_order_relaxed);
+            }
+        }
+        hipLaunchKernelGGL((k_kv_attn_step<D, F16>), grid, block, bytes, stream, p);
+    } else {
+        const size_t bytes = (size_t)(D == 256 ? 2 : 3) * 2 * kPage * D;
+        hipLaunchKernelGGL((k_kv_attn_rows<D, F16>), grid, block, bytes, stream, p);
+    }
+    int st = check_launch("kv_attention");
+    if (st != VDN_FP8_OK || p.splits == 1) return st;
+    hipLaunchKernelGGL((k_kv_attn_join<D, F16>), dim3((unsigned)((p.b.tokens * p.q_heads + 3) / 4)), block, 0, stream, p);
+    return check_launch("kv_attention join");
+}
+
+// The arguments that the size query and the call share.
+int attn_arguments(const vdn_fp8_kv_cache* cache, const vdn_fp8_kv_batch* batch, int64_t q_heads, int64_t max_query, int64_t top,
+                   int64_t query_block, bool listed, KvAttnArgs& p)
+{
+    const int st = kv_arguments("kv_attention", cache, batch, p.c, p.b);
+    if (st != VDN_FP8_OK) return st;
+    if (q_heads < 1 || q_heads > (1 << 16) || q_heads % p.c.heads)
+        return set_error(VDN_FP8_EINVAL, "kv_attention: %lld query heads for %d key/value heads", (long long)q_heads, p.c.heads);
+    if (max_query < 0) return set_error(VDN_FP8_EINVAL, "kv_attention: negative max_query");
+    p.group = (int)(q_heads / p.c.heads), p.q_heads = (int)q_heads;
+    if (listed) {
+        if (top < 1 || top > (1 << 24)) return set_error(VDN_FP8_EINVAL, "kv_attention: top must be in [1, 2^24]");
+        if (query_block < 1 || query_block > (1 << 20) || (query_block > 1 && query_block * p.group % kRows))
+            return set_error(VDN_FP8_EINVAL, "kv_attention: query_block must be 1, or such that query_block * group is a multiple of %d "
+                             "(got %lld with groups of %d)", kRows, (long long)query_block, p.group);
+        p.top = (int)top, p.query_block = (int)query_block;
+        const int64_t n = p.b.batch > 0 ? p.b.tokens / p.b.batch : 0;
+        p.listed = KvUnits{query_block, (n + query_block - 1) / query_block, 1, query_block == 1 ? 0 : 1};
+        p.blocks = (const int32_t*)(uintptr_t)4;   // replaced by the call
+    }
+    if (p.b.tokens * q_heads >= ((int64_t)1 << 30))
+        return set_error(VDN_FP8_EINVAL, "kv_attention: %lld tokens of %lld heads, 2^30 rows at most", (long long)p.b.tokens, (long long)q_heads);
+    return VDN_FP8_OK;
+}
+
+}  // namespace
+}  // namespace vdn
+
+using namespace vdn;
+
+extern "C" int vdn_fp8_kv_attention_workspace_size(const vdn_fp8_kv_cache* cache, const vdn_fp8_kv_batch* batch, int64_t q_heads,
+                                                   int64_t max_query, int64_t top, int64_t query_block, int64_t* bytes)
+{
+    KvAttnArgs p{};
+    if (!bytes) return set_error(VDN_FP8_EINVAL, "kv_attention_workspace_size: null pointer");
+    *bytes = 0;
+    const int st = attn_arguments(cache, batch, q_heads, max_query, top, query_block, top > 0, p);
+    if (st != VDN_FP8_OK || p.b.tokens == 0) return st;
+    const int cus = device_cus();
+    if (cus == 0) return set_error(VDN_FP8_ELAUNCH, "kv_attention_workspace_size: the device cannot be queried");
+    *bytes = make_plan(p, max_query, cus).bytes;
+    return VDN_FP8_OK;
+}
+
+extern "C" int vdn_fp8_kv_attention(const vdn_fp8_kv_cache* cache, const vdn_fp8_kv_batch* batch, const void* query, int dtype,
+                                    int64_t q_heads, int64_t ldq, int64_t max_query, float scale, int causal, const int32_t* blocks,
+                                    int64_t top, int64_t query_block, void* out, float* lse, void* workspace, int64_t workspace_bytes,
+                                    hipStream_t stream)
+{
+    KvAttnArgs p{};
+    if (dtype != VDN_FP8_DTYPE_BF16 && dtype != VDN_FP8_DTYPE_F16) return set_error(VDN_FP8_EINVAL, "kv_attention: dtype must be bf16 or binary16");
+    const int st = attn_arguments(cache, batch, q_heads, max_query, top, query_block, blocks != nullptr, p);
+    if (st != VDN_FP8_OK || p.b.tokens == 0) return st;
+    if (!query || !out) return set_error(VDN_FP8_EINVAL, "kv_attention: null pointer");
+    if (ldq % 8 || ldq < q_heads * p.c.d) return set_error(VDN_FP8_EINVAL, "kv_attention: need ldq a multiple of 8 and >= q_heads * head_dim");
+    if (!aligned(query, 16) || !aligned(out, 16) || !aligned(lse, 4) || !aligned(blocks, 4) || !aligned(workspace, 16))
+        return set_error(VDN_FP8_EINVAL, "kv_attention: misaligned pointer (query, out, workspace 16 B; lse, blocks 4 B)");
+    if (!(scale > 0.0f) || scale > 3e38f) return set_error(VDN_FP8_EINVAL, "kv_attention: scale must be positive and finite");
+    const int cus = device_cus();
+    if (cus == 0) return set_error(VDN_FP8_ELAUNCH, "kv_attention: the device cannot be queried");
+    const Plan plan = make_plan(p, max_query, cus);
+    if (plan.items >= ((int64_t)1 << 24)) return set_error(VDN_FP8_EINVAL, "kv_attention: %lld workgroups, 2^24 at most", (long long)plan.items);
+    if (plan.bytes > 0 && (!workspace || workspace_bytes < plan.bytes))
+        return set_error(VDN_FP8_EINVAL, "kv_attention: workspace of %lld bytes, %lld needed", (long long)workspace_bytes, (long long)plan.bytes);
+    p.q = (const uint16_t*)query, p.ldq = ldq, p.scale = scale * 1.4426950408889634f, p.causal = causal != 0;
+    p.blocks = blocks, p.out = (uint16_t*)out, p.lse = lse, p.part = (float*)workspace;
+    p.splits = plan.splits, p.column_tiles = plan.column_tiles, p.step_rows = plan.step_rows, p.items = (uint32_t)plan.items;
+    const bool f16 = dtype == VDN_FP8_DTYPE_F16;
+    switch (p.c.d) {
+        case 64: return f16 ? launch<64, true>(p, plan.step, stream) : launch<64, false>(p, plan.step, stream);
+        case 128: return f16 ? launch<128, true>(p, plan.step, stream) : launch<128, false>(p, plan.step, stream);
+        default: return f16 ? launch<256, true>(p, plan.step, stream) : launch<256, false>(p, plan.step, stream);
+    }
+}

@@ -20,6 +20,7 @@
 // so its weight and cos/sin values are loaded once per token.
 #include <stdint.h>
 
+#include "qk_prep.h"
 #include "vdn_common.h"
 
 namespace vdn {
@@ -45,49 +46,6 @@ struct QkArgs {
     uint16_t* out;
     int64_t ldo;
 };
-
-// Eight table values for elements i0 .. i0 + 7 of one row, rounded to bf16 and
-// returned as binary32, from the 32 bytes at the row's element i0 (binary32
-// tables use both halves, bf16 tables the first).
-__device__ __forceinline__ void decode_table8(uint4 lo, uint4 hi, bool bf16, float v[8])
-{
-    if (bf16) {
-        const uint32_t w[4] = {lo.x, lo.y, lo.z, lo.w};
-#pragma unroll
-        for (int e = 0; e < 4; ++e) { v[2 * e] = bf16_lo(w[e]); v[2 * e + 1] = bf16_hi(w[e]); }
-    } else {
-        const uint32_t raw[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
-#pragma unroll
-        for (int e = 0; e < 8; e += 2) {
-            const uint32_t r = pack_bf16x2(__uint_as_float(raw[e]), __uint_as_float(raw[e + 1]));
-            v[e] = bf16_lo(r);
-            v[e + 1] = bf16_hi(r);
-        }
-    }
-}
-
-// Lane exchanges inside a 16-lane DPP row (d = 128: one head per row), as
-// register moves rather than LDS round trips.
-template <int CTRL>
-__device__ __forceinline__ float dpp_f32(float v)
-{
-    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xf, 0xf, false));
-}
-constexpr int kDppXor1 = 0xb1;         // quad_perm [1, 0, 3, 2]
-constexpr int kDppXor2 = 0x4e;         // quad_perm [2, 3, 0, 1]
-constexpr int kDppHalfMirror = 0x141;  // lane i <- 7 - i within each half row
-constexpr int kDppMirror = 0x140;      // lane i <- 15 - i within each row
-constexpr int kDppRor8 = 0x128;        // lane i <- lane (i + 8) mod 16 within each row
-
-// Sum over the 16 lanes of a row, every lane receiving it.
-__device__ __forceinline__ float row16_sum(float v)
-{
-    v += dpp_f32<kDppXor1>(v);
-    v += dpp_f32<kDppXor2>(v);
-    v += dpp_f32<kDppHalfMirror>(v);
-    v += dpp_f32<kDppMirror>(v);
-    return v;
-}
 
 // G = d / 8 lanes per head; CPL = chunks per lane; NT: non-temporal output stores.
 template <int G, int CPL, bool NT, int WPR>
@@ -165,37 +123,13 @@ __global__ __launch_bounds__(kWavesPerBlock * kLanes) void k_qk_prep(QkArgs p)
         float x[8];
 #pragma unroll
         for (int e = 0; e < 4; ++e) { x[2 * e] = bf16_lo(xw[e]); x[2 * e + 1] = bf16_hi(xw[e]); }
-        float ss = 0.0f;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) ss += x[e] * x[e];
-        if (G == 16) {
-            ss = row16_sum(ss);
-        } else {
-#pragma unroll
-            for (int off = 1; off < G; off <<= 1) ss += __shfl_xor(ss, off, kLanes);
-        }
+        const float ss = head_sum_squares<G>(x);
         const float rstd = 1.0f / __builtin_sqrtf(ss / (float)p.d + p.eps);
         float n[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) n[e] = (x[e] * rstd) * w[e];
-        // every lane takes part in the exchange (the lanes of pass-through chunks
-        // read a value they do not use)
         float o[8];
-        if (G == 16 && full_rot) {
-            // R = d = 128: the partner chunk is 8 lanes away inside the row
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const float pe = dpp_f32<kDppRor8>(n[e]);
-                o[e] = n[e] * cs[e] + (first ? -pe : pe) * sn[e];
-            }
-        } else {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const float pe = __shfl(n[e], rot ? partner : lane, kLanes);
-                const float r = first ? -pe : pe;
-                o[e] = rot ? n[e] * cs[e] + r * sn[e] : n[e];
-            }
-        }
+        rotate8<G>(n, cs, sn, full_rot, rot, first, partner, lane, o);
         if (q < nch) {
             const u32x4_t ov = {pack_bf16x2(o[0], o[1]), pack_bf16x2(o[2], o[3]), pack_bf16x2(o[4], o[5]),
                                 pack_bf16x2(o[6], o[7])};

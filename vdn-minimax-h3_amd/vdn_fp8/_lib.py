@@ -12,7 +12,7 @@ import os
 
 from .build import CSRC, INCLUDE, LIB_PATH, compiler_id, source_manifest
 
-ABI_VERSION = 6
+ABI_VERSION = 7
 
 OK, EINVAL, ELAUNCH = 0, 1, 2
 EPI_NONE, EPI_GELU_TANH, EPI_GATE, EPI_F32 = 0, 1, 2, 3
@@ -23,6 +23,21 @@ _build_info = None
 
 # (name, restype, argtypes) of every exported symbol, in header order.
 _P, _I64, _F32, _I32 = ctypes.c_void_p, ctypes.c_int64, ctypes.c_float, ctypes.c_int
+
+
+class KvCacheStruct(ctypes.Structure):
+    """vdn_fp8_kv_cache."""
+    _fields_ = [("k", _P), ("v", _P), ("k_scale", _P), ("v_scale", _P), ("k_mean", _P),
+                ("pages", _I64), ("heads", _I64), ("head_dim", _I64)]
+
+
+class KvBatchStruct(ctypes.Structure):
+    """vdn_fp8_kv_batch."""
+    _fields_ = [("page_table", _P), ("ldtable", _I64), ("max_pages", _I64), ("lengths", _P), ("q_start", _P),
+                ("batch", _I64), ("tokens", _I64)]
+
+
+_CACHE, _BATCH = ctypes.POINTER(KvCacheStruct), ctypes.POINTER(KvBatchStruct)
 EXPORTS = (
     ("vdn_fp8_quantize_rows", _I32, [_P, _I64, _I64, _I64, _P, _I64, _P, _P]),
     ("vdn_fp8_gelu_quantize_rows", _I32, [_P, _I64, _I64, _I64, _P, _I64, _P, _P]),
@@ -44,6 +59,14 @@ EXPORTS = (
                                     _P, _I64, _P, _I64, _P]),
     ("vdn_fp8_qk_prep", _I32, [_P, _I64, _I64, _I64, _I64, _P, _F32, _P, _P, _I64, _I64, _I32, _P, _I64, _P]),
     ("vdn_fp8_gated_residual", _I32, [_P, _I64, _P, _I64, _P, _I64, _P, _I64, _P, _I64, _I64, _I64, _P]),
+    ("vdn_fp8_kv_append", _I32, [_CACHE, _BATCH, _P, _I64, _P, _I64, _I32, _P]),
+    ("vdn_fp8_qk_prep_append", _I32, [_CACHE, _BATCH, _P, _I64, _I64, _P, _I64, _P, _I64, _P, _F32, _P, _F32, _P, _P,
+                                      _I64, _I64, _I32, _P, _I64, _P]),
+    ("vdn_fp8_kv_attention_workspace_size", _I32, [_CACHE, _BATCH, _I64, _I64, _I64, _I64, _P]),
+    ("vdn_fp8_kv_attention", _I32, [_CACHE, _BATCH, _P, _I32, _I64, _I64, _I64, _F32, _I32, _P, _I64, _I64, _P, _P, _P,
+                                    _I64, _P]),
+    ("vdn_fp8_kv_select_workspace_size", _I32, [_CACHE, _BATCH, _I64, _I64, _P]),
+    ("vdn_fp8_kv_select", _I32, [_CACHE, _BATCH, _P, _I32, _I64, _I64, _I32, _I64, _I64, _I64, _I64, _P, _P, _I64, _P]),
     ("vdn_fp8_last_error", ctypes.c_char_p, []),
     ("vdn_fp8_abi_version", _I32, []),
     ("vdn_fp8_build_info", ctypes.c_char_p, []),
