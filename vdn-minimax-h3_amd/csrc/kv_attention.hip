@@ -43,7 +43,9 @@
 namespace vdn {
 namespace {
 
-constexpr int kRows = 128, kWaveRows = 32;
+constexpr int kRows = 128, kWaveRows = 32;   // of k_kv_attn_rows
+constexpr int kStepRows = 32;                  // of k_kv_attn_step, at most
+constexpr int kInfo = 256;                     // pages that a workgroup looks up at a time
 constexpr int kMostSplits = 64;
 constexpr float kNoMax = -3.0e38f;      // the running maximum of no keys: finite, so that differences stay numbers
 constexpr float kSlack = 8.0f;          // the maximum moves only past this
@@ -81,17 +83,22 @@ __device__ __forceinline__ float* part_sums(const KvAttnArgs& p)
 // then holds keys 16 g .. 16 g + 15 in its registers' order.
 __device__ __forceinline__ int row_key(int r) { return 16 * ((r >> 2) & 1) + 4 * (r >> 3) + (r & 3); }
 
-// max / sum with the lane that holds the same query's other 16 keys.
-__device__ __forceinline__ float half_max(float v)
+// The value of the lane 32 (16) away joined with one's own: lanes that hold the same row.
+template <typename F>
+__device__ __forceinline__ float across32(float v, F f)
 {
     const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+    return f(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
-__device__ __forceinline__ float half_sum(float v)
+template <typename F>
+__device__ __forceinline__ float across16(float v, F f)
 {
-    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return f(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
+// (NaN wins: the row becomes NaN anyway, and one instruction takes two values without quieting them first)
+__device__ __forceinline__ float larger(float a, float b) { return __builtin_elementwise_maximum(a, b); }
+__device__ __forceinline__ float added(float a, float b) { return a + b; }
 
 __device__ __forceinline__ float exponent_f32(int e) { return __uint_as_float((uint32_t)(min(max(e, -126), 127) + 127) << 23); }
 
@@ -108,8 +115,132 @@ __device__ __forceinline__ void decode16(uint4 w, f16x8_t o[2])
     }
 }
 
-// One wave's 32 rows: the queries as fp8 terms, the running softmax, the output's accumulators.
-// Lane (column l % 32, half g = l / 32): the column is the row of the problem.
+// The fp8 terms of 32 elements of a query row (row: at its first element of these, NULL: zeros), and the
+// exponent e that they are scaled by: TERMS values whose sum is x 2^-e, term t times 2^(5 t - 1) (t > 0).
+// Every lane of a row passes all elements' largest magnitude through `join`.
+template <bool F16, int STEPS, int TERMS, typename Join>
+__device__ __forceinline__ int split_query(const uint16_t* const (&row)[STEPS], Join join, i32x8_t (&q)[TERMS][STEPS])
+{
+    float x[STEPS][32];
+    uint32_t top = 0;
+#pragma unroll
+    for (int s = 0; s < STEPS; ++s)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            uint4 v = make_uint4(0, 0, 0, 0);
+            if (row[s]) v = *reinterpret_cast<const uint4*>(row[s] + 8 * i);
+            const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                float lo, hi;
+                if (F16) {
+                    lo = (float)__builtin_bit_cast(_Float16, (uint16_t)w[e]);
+                    hi = (float)__builtin_bit_cast(_Float16, (uint16_t)(w[e] >> 16));
+                } else {
+                    lo = bf16_lo(w[e]), hi = bf16_hi(w[e]);
+                }
+                x[s][8 * i + 2 * e] = lo, x[s][8 * i + 2 * e + 1] = hi;
+                const uint32_t a = __float_as_uint(lo) & 0x7fffffffu, b = __float_as_uint(hi) & 0x7fffffffu;
+                top = max(top, max(a < 0x7f800000u ? a : 0u, b < 0x7f800000u ? b : 0u));
+            }
+        }
+    top = join(top);
+    int e = (int)(top >> 23) - 127 - 8 + ((top & 0x7fffffu) > 0x600000u ? 1 : 0);
+    e = top == 0 ? 0 : min(max(e, -120), 120);
+    const float f = exponent_f32(-e);
+#pragma unroll
+    for (int s = 0; s < STEPS; ++s)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            float r[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) r[j] = x[s][4 * i + j] * f;
+#pragma unroll
+            for (int t = 0; t < TERMS; ++t) {
+                const uint32_t w = pack_e4m3x4(r[0], r[1], r[2], r[3]);
+                q[t][s][i] = (int)w;
+                // the rest, exact; times the next term's factor: 2^4, then 2^5
+                const float up = t == 0 ? 16.0f : 32.0f;
+                r[0] = (r[0] - __builtin_amdgcn_cvt_f32_fp8(w, 0)) * up;
+                r[1] = (r[1] - __builtin_amdgcn_cvt_f32_fp8(w, 1)) * up;
+                r[2] = (r[2] - __builtin_amdgcn_cvt_f32_fp8(w, 2)) * up;
+                r[3] = (r[3] - __builtin_amdgcn_cvt_f32_fp8(w, 3)) * up;
+            }
+        }
+    return e;
+}
+
+// The block scales of the terms, as the matrix instructions take them.
+constexpr int waitcnt_lgkm0() { return 15 | (7 << 4) | (0 << 8) | (3 << 14); }   // any vmcnt
+
+constexpr int kOne = 0x7f7f7f7f, kTerm1 = 0x7b7b7b7b, kTerm2 = 0x76767676;
+
+// What the workgroup knows of a page: its number in the pool (-1: not there), its number in the
+// sequence, and its scales' exponents. Looked up by all threads at once, kInfo pages at a time, so
+// that the loops over pages meet no chain of dependent loads.
+struct PageInfo {
+    int page, w, ek, ev;
+};
+
+__device__ __forceinline__ void look_up(const KvAttnArgs& p, int b, int h, int length, const int32_t* list, int i0, int hi, PageInfo* info)
+{
+    const int i = i0 + (int)threadIdx.x;
+    if (threadIdx.x < kInfo && i < hi) {
+        PageInfo a;
+        a.w = list ? list[i] : i;
+        a.page = a.w >= 0 && a.w < (length + kPage - 1) / kPage ? kv_page(p.b, p.c, b, a.w) : -1;
+        const int64_t ph = (int64_t)max(a.page, 0) * p.c.heads + h;
+        a.ek = p.c.k_scale[ph] - 127, a.ev = p.c.v_scale[ph] - 127;
+        info[threadIdx.x] = a;
+    }
+}
+
+// One entry, in scalar registers.
+__device__ __forceinline__ PageInfo info_at(const PageInfo* info, int i)
+{
+    const int4 v = *reinterpret_cast<const int4*>(info + i);
+    return PageInfo{__builtin_amdgcn_readfirstlane(v.x), __builtin_amdgcn_readfirstlane(v.y), __builtin_amdgcn_readfirstlane(v.z),
+                    __builtin_amdgcn_readfirstlane(v.w)};
+}
+__device__ __forceinline__ int first_key(const PageInfo& a) { return a.page >= 0 ? a.w * kPage : kAbsent; }
+
+// Codes of 16 tokens of which the first `have` are in the sequence: the others become zeros (they hold what
+// an earlier owner of the page left). The NaN codes left are marked in `nan` by their top bits.
+__device__ __forceinline__ uint4 keep_tokens(uint4 v, int have, uint4& nan)
+{
+    uint32_t u[4] = {v.x, v.y, v.z, v.w}, n[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int k = have - 4 * i;
+        u[i] = k >= 4 ? u[i] : k <= 0 ? 0u : u[i] & (0xffffffffu >> (32 - 8 * k));
+        n[i] = ((u[i] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
+    }
+    nan = make_uint4(n[0], n[1], n[2], n[3]);
+    return make_uint4(u[0], u[1], u[2], u[3]);
+}
+__device__ __forceinline__ bool any_of(uint4 v) { return (v.x | v.y | v.z | v.w) != 0; }
+// The marked codes without their bytes; the marks as e4m3 ones.
+__device__ __forceinline__ uint4 without(uint4 v, uint4 nan)
+{
+    return make_uint4(v.x & ~((nan.x >> 7) * 0xffu), v.y & ~((nan.y >> 7) * 0xffu), v.z & ~((nan.z >> 7) * 0xffu), v.w & ~((nan.w >> 7) * 0xffu));
+}
+__device__ __forceinline__ uint4 as_ones(uint4 nan)
+{
+    return make_uint4((nan.x >> 7) * 0x38u, (nan.y >> 7) * 0x38u, (nan.z >> 7) * 0x38u, (nan.w >> 7) * 0x38u);
+}
+// Which of eight tokens from `first` on a row sees, as ones. (Opaque, so that it is computed where it is
+// rarely needed and not kept in registers where it is not.)
+__device__ __forceinline__ f16x8_t seen_ones(int first, int limit)
+{
+    asm volatile("" : "+v"(limit));
+    f16x8_t o;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) o[j] = first + j < limit ? (_Float16)1.0f : (_Float16)0.0f;
+    return o;
+}
+
+// One wave's 32 rows of k_kv_attn_rows: the queries' terms, the running softmax, the output's accumulators.
+// Lane l: column l % 32 is the row of the problem, g = l / 32 its half of the keys.
 template <int D, bool F16>
 struct WaveRows {
     static constexpr int kSteps = D / 64, kTerms = F16 ? 3 : 2, kTiles = D / 32;
@@ -118,57 +249,16 @@ struct WaveRows {
     float m, l, c;     // running maximum and sum (of this half's keys), factor of the raw scores
     int limit;         // keys below it are visible to the row
 
-    // row: the row's values (NULL: none, zeros).
     __device__ __forceinline__ void load(const uint16_t* row, int g, float scale)
     {
-        float x[kSteps][32];
-        uint32_t top = 0;
+        const uint16_t* at[kSteps];
 #pragma unroll
-        for (int s = 0; s < kSteps; ++s)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                uint4 v = make_uint4(0, 0, 0, 0);
-                if (row) v = *reinterpret_cast<const uint4*>(row + 64 * s + 32 * g + 8 * i);
-                const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    float lo, hi;
-                    if (F16) {
-                        lo = (float)__builtin_bit_cast(_Float16, (uint16_t)w[e]);
-                        hi = (float)__builtin_bit_cast(_Float16, (uint16_t)(w[e] >> 16));
-                    } else {
-                        lo = bf16_lo(w[e]), hi = bf16_hi(w[e]);
-                    }
-                    x[s][8 * i + 2 * e] = lo, x[s][8 * i + 2 * e + 1] = hi;
-                    const uint32_t a = __float_as_uint(lo) & 0x7fffffffu, b = __float_as_uint(hi) & 0x7fffffffu;
-                    top = max(top, max(a < 0x7f800000u ? a : 0u, b < 0x7f800000u ? b : 0u));
-                }
-            }
-        const auto other = __builtin_amdgcn_permlane32_swap(top, top, false, false);
-        top = max((uint32_t)other[0], (uint32_t)other[1]);
-        int e = (int)(top >> 23) - 127 - 8 + ((top & 0x7fffffu) > 0x600000u ? 1 : 0);
-        e = top == 0 ? 0 : min(max(e, -120), 120);
-        const float f = exponent_f32(-e);
+        for (int s = 0; s < kSteps; ++s) at[s] = row ? row + 64 * s + 32 * g : nullptr;
+        const int e = split_query<F16>(at, [](uint32_t v) {
+            const auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+            return max((uint32_t)r[0], (uint32_t)r[1]);
+        }, q);
         c = scale * exponent_f32(e);
-#pragma unroll
-        for (int s = 0; s < kSteps; ++s)
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                float r[4];
-#pragma unroll
-                for (int j = 0; j < 4; ++j) r[j] = x[s][4 * i + j] * f;
-#pragma unroll
-                for (int t = 0; t < kTerms; ++t) {
-                    const uint32_t w = pack_e4m3x4(r[0], r[1], r[2], r[3]);
-                    q[t][s][i] = (int)w;
-                    // the rest, exact; times the next term's factor: 2^4, then 2^5
-                    const float up = t == 0 ? 16.0f : 32.0f;
-                    r[0] = (r[0] - __builtin_amdgcn_cvt_f32_fp8(w, 0)) * up;
-                    r[1] = (r[1] - __builtin_amdgcn_cvt_f32_fp8(w, 1)) * up;
-                    r[2] = (r[2] - __builtin_amdgcn_cvt_f32_fp8(w, 2)) * up;
-                    r[3] = (r[3] - __builtin_amdgcn_cvt_f32_fp8(w, 3)) * up;
-                }
-            }
         m = kNoMax, l = 0.0f;
 #pragma unroll
         for (int t = 0; t < kTiles; ++t)
@@ -187,10 +277,10 @@ struct WaveRows {
 #pragma unroll
             for (int st = 0; st < kSteps; ++st) {
                 const i32x8_t a = key(kt, st);
-                s[kt] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a, q[0][st], s[kt], 0, 0, 0, 0x7f7f7f7f, 0, 0x7f7f7f7f);
-                s[kt] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a, q[1][st], s[kt], 0, 0, 0, 0x7f7f7f7f, 0, 0x7b7b7b7b);
+                s[kt] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a, q[0][st], s[kt], 0, 0, 0, kOne, 0, kOne);
+                s[kt] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a, q[1][st], s[kt], 0, 0, 0, kOne, 0, kTerm1);
                 if (kTerms == 3)
-                    s[kt] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a, q[kTerms - 1][st], s[kt], 0, 0, 0, 0x7f7f7f7f, 0, 0x76767676);
+                    s[kt] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a, q[kTerms - 1][st], s[kt], 0, 0, 0, kOne, 0, kTerm2);
             }
         }
     }
@@ -210,10 +300,10 @@ struct WaveRows {
     {
         const float f = fmaxf(c * exponent_f32(ek), 1e-37f);   // (never 0: a masked score stays -inf)
         const float shift = (float)ev;
-        float top = fmaxf(s[0][0], s[1][0]);
+        float top = larger(s[0][0], s[1][0]);
 #pragma unroll
-        for (int i = 1; i < 16; ++i) top = fmaxf(top, fmaxf(s[0][i], s[1][i]));
-        top = half_max(top) * f + shift;
+        for (int i = 1; i < 16; ++i) top = larger(top, larger(s[0][i], s[1][i]));
+        top = across32(top, larger) * f + shift;
         if (__any(top > m + kSlack)) {
             const float now = fmaxf(m, top), a = __builtin_amdgcn_exp2f(m - now);
             m = now;
@@ -238,79 +328,186 @@ struct WaveRows {
         l = __builtin_fmaf(sum, exponent_f32(-ev), l);
     }
 
-    // Adds the weighted values of a page: value(kt, t) gives 16 tokens' codes of one element. MASKED:
-    // the page has tokens that some row does not see. Those behind the sequence's end hold what an
-    // earlier owner left and count as zeros; a NaN code of a token that some rows see and others do
-    // not reaches the rows that see it, through a product of indicators.
-    template <bool MASKED, typename Value>
-    __device__ __forceinline__ void add_values(Value value, const f16x8_t w[2][2], int key0, int end, int g)
+    // Adds the weighted values of a page: value(kt, h, t) gives one element's values of the eight tokens from
+    // 32 kt + 16 g + 8 h on.
+    template <typename Value>
+    __device__ __forceinline__ void add_values(Value value, const f16x8_t w[2][2])
     {
 #pragma unroll
-        for (int kt = 0; kt < 2; ++kt) {
+        for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
-            for (int t = 0; t < kTiles; ++t) {
-                uint4 v = value(kt, t);
-                f16x8_t a[2];
-                if (MASKED) {
-                    const int have = end - (key0 + 32 * kt + 16 * g);   // of these 16 tokens
-                    uint32_t u[4] = {v.x, v.y, v.z, v.w}, nan[4], any = 0;
+            for (int h = 0; h < 2; ++h)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const int n = have - 4 * i;
-                        u[i] = n >= 4 ? u[i] : n <= 0 ? 0u : u[i] & (0xffffffffu >> (32 - 8 * n));
-                        nan[i] = ((u[i] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
-                        any |= nan[i];
-                    }
-                    if (__any(any != 0)) {
+                for (int t = 0; t < kTiles; ++t)
+                    acc[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(value(kt, h, t), w[kt][h], acc[t], 0, 0, 0);
+    }
+
+    // A page in which some rows see NaN values that others do not (its NaN were stored as zeros): the rows
+    // that see one become NaN, by a product of indicators. codes(kt, t): 16 tokens from 32 kt + 16 g on.
+    template <typename Codes>
+    __device__ __forceinline__ void add_nan(Codes codes, int key0, int end, int g)
+    {
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            u[i] &= ~((nan[i] >> 7) * 0xffu);
-                            nan[i] = (nan[i] >> 7) * 0x38u;   // e4m3 1.0
-                        }
-                        f16x8_t is_nan[2];
-                        decode16(make_uint4(nan[0], nan[1], nan[2], nan[3]), is_nan);
-                        f32x16_t hit;
+        for (int t = 0; t < kTiles; ++t) {
+            __builtin_amdgcn_sched_barrier(0);
+            f32x16_t hit;
 #pragma unroll
-                        for (int i = 0; i < 16; ++i) hit[i] = 0.0f;
+            for (int i = 0; i < 16; ++i) hit[i] = 0.0f;
 #pragma unroll
-                        for (int h = 0; h < 2; ++h) {
-                            f16x8_t seen;
+            for (int kt = 0; kt < 2; ++kt) {
+                const int first = key0 + 32 * kt + 16 * g;
+                uint4 nan;
+                keep_tokens(codes(kt, t), end - first, nan);
+                f16x8_t is_nan[2];
+                decode16(as_ones(nan), is_nan);
 #pragma unroll
-                            for (int j = 0; j < 8; ++j) seen[j] = key0 + 32 * kt + 16 * g + 8 * h + j < limit ? (_Float16)1.0f : (_Float16)0.0f;
-                            hit = __builtin_amdgcn_mfma_f32_32x32x16_f16(is_nan[h], seen, hit, 0, 0, 0);
-                        }
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) acc[t][i] = hit[i] > 0.0f ? __builtin_nanf("") : acc[t][i];
-                    }
-                    v = make_uint4(u[0], u[1], u[2], u[3]);
-                }
-                decode16(v, a);
-                acc[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[0], w[kt][0], acc[t], 0, 0, 0);
-                acc[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[1], w[kt][1], acc[t], 0, 0, 0);
+                for (int h = 0; h < 2; ++h)
+                    hit = __builtin_amdgcn_mfma_f32_32x32x16_f16(is_nan[h], seen_ones(first + 8 * h, limit), hit, 0, 0, 0);
             }
+#pragma unroll
+            for (int i = 0; i < 16; ++i) acc[t][i] = hit[i] > 0.0f ? __builtin_nanf("") : acc[t][i];
         }
     }
 };
 
-// A page's place in the sequence and in the pool.
-struct PageAt {
-    int key0;       // its first token, kAbsent where there is none
-    int64_t ph;     // page * heads + head
-    int ek, ev;
-};
+// One wave's rows of k_kv_attn_step, NT columns of 16: lane l holds row l % 16 of each, and the keys
+// 16 g .. 16 g + 15 of a page (g = l / 16), tile t of the scores standing for keys 16 g + 4 t + i.
+// (Half the accumulators and scores that 32 columns would take, at the group sizes that are usual.)
+template <int D, bool F16, int NT>
+struct StepRows {
+    static constexpr int kSteps = D <= 128 ? 1 : D / 128, kTerms = F16 ? 3 : 2, kTiles = D / 16;
+    i32x8_t q[NT][kTerms][kSteps];
+    f32x4_t acc[NT][kTiles];
+    float m[NT], l[NT], c[NT];
+    int limit[NT];
 
-__device__ __forceinline__ PageAt page_at(const KvAttnArgs& p, int b, int h, int length, const int32_t* list, int i)
-{
-    PageAt a;
-    int w = list ? list[i] : i;
-    const int have = (length + kPage - 1) / kPage;
-    const int page = w >= 0 && w < have ? kv_page(p.b, p.c, b, w) : -1;
-    a.key0 = page >= 0 ? w * kPage : kAbsent;
-    a.ph = (int64_t)max(page, 0) * p.c.heads + h;
-    a.ek = scalar_byte(p.c.k_scale, a.ph) - 127;
-    a.ev = scalar_byte(p.c.v_scale, a.ph) - 127;
-    return a;
-}
+    // (a head of 64 fills half of the instruction's 128: the upper lanes repeat the keys against zeros)
+    __device__ __forceinline__ void load(int n, const uint16_t* row, int g, float scale)
+    {
+        const uint16_t* at[kSteps];
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) at[s] = row && (D > 64 || g < 2) ? row + 128 * s + 32 * g : nullptr;
+        const int e = split_query<F16>(at, [](uint32_t v) {
+            const auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+            v = max((uint32_t)r[0], (uint32_t)r[1]);
+            const auto s = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+            return max((uint32_t)s[0], (uint32_t)s[1]);
+        }, q[n]);
+        c[n] = scale * exponent_f32(e);
+        m[n] = kNoMax, l[n] = 0.0f;
+#pragma unroll
+        for (int t = 0; t < kTiles; ++t) acc[n][t] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+
+    template <typename Key>
+    __device__ __forceinline__ void scores(Key key, f32x4_t s[NT][4]) const
+    {
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+#pragma unroll
+            for (int n = 0; n < NT; ++n) s[n][t] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int st = 0; st < kSteps; ++st) {
+                const i32x8_t a = key(t, st);
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    s[n][t] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, q[n][0][st], s[n][t], 0, 0, 0, kOne, 0, kOne);
+                    s[n][t] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, q[n][1][st], s[n][t], 0, 0, 0, kOne, 0, kTerm1);
+                    if (kTerms == 3)
+                        s[n][t] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, q[n][kTerms - 1][st], s[n][t], 0, 0, 0, kOne, 0, kTerm2);
+                }
+            }
+        }
+    }
+
+    __device__ __forceinline__ void mask(f32x4_t s[NT][4], int key0, int g) const
+    {
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            const int seen = limit[n] - key0 - 16 * g;
+#pragma unroll
+            for (int t = 0; t < 4; ++t)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) s[n][t][i] = 4 * t + i < seen ? s[n][t][i] : -__builtin_inff();
+        }
+    }
+
+    __device__ __forceinline__ void weights(const f32x4_t s[NT][4], int ek, int ev, f16x8_t w[NT][2])
+    {
+        const float shift = (float)ev;
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            const float f = fmaxf(c[n] * exponent_f32(ek), 1e-37f);
+            float top = s[n][0][0];
+#pragma unroll
+            for (int i = 1; i < 16; ++i) top = larger(top, s[n][i / 4][i % 4]);
+            top = across16(across32(top, larger), larger) * f + shift;
+            if (__any(top > m[n] + kSlack)) {
+                const float now = fmaxf(m[n], top), a = __builtin_amdgcn_exp2f(m[n] - now);
+                m[n] = now;
+                l[n] *= a;
+#pragma unroll
+                for (int t = 0; t < kTiles; ++t) acc[n][t] *= a;
+            }
+            const float base = shift - m[n];
+            float sum = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][i / 4][i % 4], f, base));
+                sum += p;
+                w[n][i / 8][i % 8] = (_Float16)p;
+            }
+            l[n] = __builtin_fmaf(sum, exponent_f32(-ev), l[n]);
+        }
+    }
+
+    // v[t]: the codes of 16 tokens, one element.
+    __device__ __forceinline__ void add_values(const uint4 v[kTiles], const f16x8_t w[NT][2])
+    {
+#pragma unroll
+        for (int t = 0; t < kTiles; ++t) {
+            f16x8_t a[2];
+            decode16(v[t], a);
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                acc[n][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a[0], w[n][0], acc[n][t], 0, 0, 0);
+                acc[n][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a[1], w[n][1], acc[n][t], 0, 0, 0);
+            }
+        }
+    }
+
+    // A page with tokens that some row does not see: tokens behind the end become zeros, and so do NaN
+    // values, after the rows that see one have become NaN.
+    __device__ __forceinline__ void settle_values(uint4 v[kTiles], int key0, int end, int g)
+    {
+        bool some = false;
+#pragma unroll
+        for (int t = 0; t < kTiles; ++t) {
+            uint4 nan;
+            v[t] = keep_tokens(v[t], end - (key0 + 16 * g), nan);
+            some |= any_of(nan);
+        }
+        if (!__any(some)) return;
+#pragma unroll
+        for (int t = 0; t < kTiles; ++t) {
+            __builtin_amdgcn_sched_barrier(0);
+            uint4 nan;
+            keep_tokens(v[t], 16, nan);
+            f16x8_t is_nan[2];
+            decode16(as_ones(nan), is_nan);
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                f32x4_t hit = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+                    hit = __builtin_amdgcn_mfma_f32_16x16x32_f16(is_nan[h], seen_ones(key0 + 16 * g + 8 * h, limit[n]), hit, 0, 0, 0);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) acc[n][t][i] = hit[i] > 0.0f ? __builtin_nanf("") : acc[n][t][i];
+            }
+            v[t] = without(v[t], nan);
+        }
+    }
+};
 
 template <bool F16>
 __device__ __forceinline__ uint32_t pack_out(float lo, float hi)
@@ -337,10 +534,13 @@ __device__ __forceinline__ void clear_rows(const KvAttnArgs& p, int64_t first, i
 template <int D, bool F16>
 __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_kv_attn_rows(KvAttnArgs p)
 {
-    constexpr int kBuffers = D == 256 ? 2 : 3;
     constexpr int kPageBytes = kPage * D;            // of k, and of v
-    constexpr int kCopies = D / 64;                  // 4 KB each, of k and of v
-    extern __shared__ __attribute__((aligned(128))) uint8_t lds[];
+    constexpr int kCopies = D / 64;                  // of 4 KB, of k and of v
+    // three pages of k codes, two of v in binary16
+    __shared__ __attribute__((aligned(128))) uint8_t lds_k[3 * kPageBytes];
+    __shared__ __attribute__((aligned(128))) uint8_t lds_v[2 * 2 * kPageBytes];
+    __shared__ __attribute__((aligned(16))) PageInfo info[kInfo];
+    __shared__ int nan_page[2];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int r = lane & 31, g = lane >> 5;
 
@@ -403,85 +603,130 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_kv_attn_rows(KvAttnAr
     rowset.limit = valid ? limit_of(row) : 0;
     const int least = limit_of(min(w0, last)), most = limit_of(min(w0 + kWaveRows - 1, last));
 
-    // Copies: this thread's 16 bytes of each 4 KB. In LDS, k lies in 128-byte lines (a row's d = 64, or
-    // 128 elements of it, the next 128 behind all rows; two rows of 64), v in rows of 64 tokens, two to
-    // a line; chunk c of line L at c ^ (L & 7), of 128-byte rows at c ^ ((row >> 1) & 7): the reads of
-    // 32 rows by 64 lanes fall on all banks. Rows are in the matrix's order (row_key).
+    // k goes to LDS as it is, by asynchronous copies of this thread's 16 bytes of each 4 KB; v passes through
+    // registers, where each thread decodes its share for all four waves. Lines of 128 bytes: of k a row (64
+    // codes: two rows) of 128 codes, the next 128 behind all rows; of v a row's 64 tokens. Chunk c of row r
+    // lies at c ^ ((r >> 1) & 7) (two rows a line: chunk c of line L at c ^ (L & 7)), so that the
+    // reads of 32 rows by 64 lanes fall on all banks. Rows are in the matrix's order (row_key).
     const int line = tid / 8, slot = tid % 8;
-    uint32_t from_k, from_v;
+    uint32_t from_k;
     {
-        const int x = slot ^ (line & 7), row_v = 2 * line + (x >> 2);
-        from_v = (uint32_t)(((row_v & 32) + row_key(row_v & 31)) * kPage + (x & 3) * 16);
-        if (D == 64) from_k = (uint32_t)(((row_v & 32) + row_key(row_v & 31)) * D + (x & 3) * 16);
+        const int x = slot ^ (line & 7), row2 = 2 * line + (x >> 2);
+        if (D == 64) from_k = (uint32_t)(((row2 & 32) + row_key(row2 & 31)) * D + (x & 3) * 16);
         else from_k = (uint32_t)(row_key(line) * D + (slot ^ ((line >> 1) & 7)) * 16);
     }
-    const uint32_t base = (uint32_t)(uintptr_t)(lds_void_t*)lds + wave * 1024;
-    auto copy = [&](const PageAt& a, int buffer) {
-        const i32x4_t rk = rsrc_words(p.c.k + a.ph * kPageBytes, kPageBytes);
-        const i32x4_t rv = rsrc_words(p.c.v + a.ph * kPageBytes, kPageBytes);
-        const uint32_t to = __builtin_amdgcn_readfirstlane(base + buffer * (2 * kPageBytes));
+    const uint32_t base_k = (uint32_t)(uintptr_t)(lds_void_t*)lds_k + wave * 1024;
+    auto copy_k = [&](const PageInfo& a, int buffer) {
+        const i32x4_t rk = rsrc_words(p.c.k + ((int64_t)max(a.page, 0) * p.c.heads + h) * kPageBytes, kPageBytes);
+        const uint32_t to = __builtin_amdgcn_readfirstlane(base_k + buffer * kPageBytes);
+#pragma unroll
+        for (int j = 0; j < kCopies; ++j) copy16_to_lds(rk, to + j * 4096, from_k, D == 64 ? 0 : (j & 1) * 32 * D + (j >> 1) * 128);
+    };
+    const int v_row = tid / 4, v_part = tid % 4;   // this thread's rows (v_row + 64 j), 16 tokens of each
+    const int from_v = ((v_row & 32) + row_key(v_row & 31)) * kPage + v_part * 16;
+    uint4 vr[kCopies];
+    auto load_v = [&](const PageInfo& a) {
+        const uint8_t* const src = p.c.v + ((int64_t)max(a.page, 0) * p.c.heads + h) * kPageBytes;
+#pragma unroll
+        for (int j = 0; j < kCopies; ++j) vr[j] = *reinterpret_cast<const uint4*>(src + from_v + j * 4096);
+    };
+    // Of a page with tokens that some row does not see, those behind the end and NaN become zeros, and
+    // nan_page remembers a page with NaN.
+    const int least_all = limit_of(r0);
+    auto store_v = [&](const PageInfo& a, int i, int buffer) {
+        const int sv = (v_row >> 1) & 7, key0 = first_key(a);
+        if (key0 + kPage > least_all) {
+            bool some = false;
+#pragma unroll
+            for (int j = 0; j < kCopies; ++j) {
+                uint4 nan;
+                vr[j] = keep_tokens(vr[j], s.length - (key0 + 16 * v_part), nan);
+                if (any_of(nan)) some = true, vr[j] = without(vr[j], nan);
+            }
+            if (some) nan_page[buffer] = i;
+        }
+        uint8_t* const to = lds_v + buffer * (2 * kPageBytes) + v_row * 128;
 #pragma unroll
         for (int j = 0; j < kCopies; ++j) {
-            const int off = D == 64 ? 0 : (j & 1) * 32 * D + (j >> 1) * 128;
-            copy16_to_lds(rk, to + j * 4096, from_k, off);
-            copy16_to_lds(rv, to + kPageBytes + j * 4096, from_v, j * 4096);
+            f16x8_t o[2];
+            decode16(vr[j], o);
+            *reinterpret_cast<f16x8_t*>(to + j * 8192 + ((2 * v_part) ^ sv) * 16) = o[0];
+            *reinterpret_cast<f16x8_t*>(to + j * 8192 + ((2 * v_part + 1) ^ sv) * 16) = o[1];
         }
     };
-    // Reads: lane (r, g) takes 32 codes of a key in two pieces, 16 tokens of a value's element in one.
+    // Reads: lane (r, g) takes 32 codes of a key in two pieces, eight tokens of a value's element in one.
     const int sw = (r >> 1) & 7;
     const int k_line = D == 64 ? (r >> 1) * 128 : r * 128, k_chunk = D == 64 ? (r & 1) * 4 + 2 * g : 2 * g;
-    const int v_line = (r >> 1) * 128, v_chunk = (r & 1) * 4 + g;
 
-    PageAt now{}, next{}, after{};
-    if (lo < hi) {
-        now = page_at(p, b, h, s.length, list, lo);
-        copy(now, 0);
-        if (lo + 1 < hi) {
-            next = page_at(p, b, h, s.length, list, lo + 1);
-            if (kBuffers == 3) copy(next, 1);
+    for (int first = lo; first < hi; first += kInfo) {
+        const int count = min(hi - first, kInfo);
+        __syncthreads();   // (all reads of the pages before are done)
+        look_up(p, b, h, s.length, list, first, hi, info);
+        if (tid < 2) nan_page[tid] = -1;
+        __syncthreads();
+        PageInfo now = info_at(info, 0), next = now;
+        copy_k(now, 0);
+        load_v(now);
+        __builtin_amdgcn_s_waitcnt(waitcnt_vm_lgkm0(0));   // (the copies too, which the compiler does not count)
+        store_v(now, first, 0);
+        if (count > 1) {
+            next = info_at(info, 1);
+            copy_k(next, 1);
+            load_v(next);
         }
-    }
-    int buffer = 0;
-    for (int i = lo; i < hi; ++i) {
-        if (kBuffers == 3 && i + 1 < hi) wave_sync<2 * kCopies>();
-        else wave_sync<0>();
-        if (kBuffers == 3) {
-            if (i + 2 < hi) {
-                after = page_at(p, b, h, s.length, list, i + 2);
-                copy(after, buffer == 0 ? 2 : buffer - 1);
+        int buffer = 0;   // of k; page i of v is in buffer i & 1
+        for (int i = 0; i < count; ++i) {
+            // All waves' stores of page i, and their copies of it, which each waited for before it stored the
+            // page's values, are done; so are the reads of page i - 1.
+            __builtin_amdgcn_sched_barrier(0);
+            __builtin_amdgcn_s_waitcnt(waitcnt_lgkm0());
+            __builtin_amdgcn_s_barrier();
+            asm volatile("" ::: "memory");
+            __builtin_amdgcn_sched_barrier(0);
+            PageInfo after = next;
+            if (i + 1 < count) {
+                __builtin_amdgcn_s_waitcnt(waitcnt_vm_lgkm0(0));   // issued one page ago
+                asm volatile("" ::: "memory");
+                store_v(next, first + i + 1, (i + 1) & 1);
+                if (i + 2 < count) {
+                    after = info_at(info, i + 2);
+                    copy_k(after, buffer == 0 ? 2 : buffer - 1);
+                    load_v(after);
+                }
             }
-        } else {
-            if (i + 1 < hi) copy(next, buffer ^ 1);
-            if (i + 2 < hi) after = page_at(p, b, h, s.length, list, i + 2);
+            const int key0 = first_key(now);
+            if (!idle && key0 < most) {
+                const uint8_t* const kb = lds_k + buffer * kPageBytes;
+                const uint8_t* const vb = lds_v + (i & 1) * (2 * kPageBytes) + r * 128;
+                auto key = [&](int kt, int st) {
+                    const uint8_t* const at_k = kb + k_line + (D == 64 ? kt * 2048 : kt * 4096 + (st >> 1) * 8192);
+                    const int c = D == 64 ? k_chunk : k_chunk + 4 * (st & 1);
+                    const uint4 x = *reinterpret_cast<const uint4*>(at_k + ((c ^ sw) * 16));
+                    const uint4 y = *reinterpret_cast<const uint4*>(at_k + (((c + 1) ^ sw) * 16));
+                    return i32x8_t{(int)x.x, (int)x.y, (int)x.z, (int)x.w, (int)y.x, (int)y.y, (int)y.z, (int)y.w};
+                };
+                auto value = [&](int kt, int half, int t) {
+                    return *reinterpret_cast<const f16x8_t*>(vb + t * 4096 + (((4 * kt + 2 * g + half) ^ sw) * 16));
+                };
+                f32x16_t sc[2];
+                f16x8_t w[2][2];
+                rowset.scores(key, sc);
+                const bool masked = key0 + kPage > least;
+                if (masked) rowset.mask(sc, key0, g);
+                rowset.weights(sc, now.ek, now.ev, w);
+                if (key0 + kPage > least_all && nan_page[i & 1] == first + i) {   // (also where this wave sees the whole page)
+                    const uint8_t* const src = p.c.v + ((int64_t)now.page * p.c.heads + h) * kPageBytes + row_key(r) * kPage + 16 * g;
+                    rowset.add_nan([&](int kt, int t) { return *reinterpret_cast<const uint4*>(src + t * 32 * kPage + 32 * kt); }, key0, s.length, g);
+                }
+                rowset.add_values(value, w);
+            }
+            now = next, next = after;
+            buffer = buffer == 2 ? 0 : buffer + 1;
         }
-        if (!idle && now.key0 < most) {
-            const uint8_t* const kb = lds + buffer * (2 * kPageBytes);
-            const uint8_t* const vb = kb + kPageBytes;
-            auto key = [&](int kt, int st) {
-                const uint8_t* const at_k = kb + k_line + (D == 64 ? kt * 2048 : kt * 4096 + (st >> 1) * 8192);
-                const int c = D == 64 ? k_chunk : k_chunk + 4 * (st & 1);
-                const uint4 x = *reinterpret_cast<const uint4*>(at_k + ((c ^ sw) * 16));
-                const uint4 y = *reinterpret_cast<const uint4*>(at_k + (((c + 1) ^ sw) * 16));
-                return i32x8_t{(int)x.x, (int)x.y, (int)x.z, (int)x.w, (int)y.x, (int)y.y, (int)y.z, (int)y.w};
-            };
-            auto value = [&](int kt, int t) {
-                return *reinterpret_cast<const uint4*>(vb + v_line + t * 2048 + (((v_chunk + 2 * kt) ^ sw) * 16));
-            };
-            f32x16_t sc[2];
-            f16x8_t w[2][2];
-            rowset.scores(key, sc);
-            const bool masked = now.key0 + kPage > least;
-            if (masked) rowset.mask(sc, now.key0, g);
-            rowset.weights(sc, now.ek, now.ev, w);
-            if (masked) rowset.template add_values<true>(value, w, now.key0, s.length, g);
-            else rowset.template add_values<false>(value, w, now.key0, s.length, g);
-        }
-        now = next, next = after;
-        buffer = buffer + 1 == kBuffers ? 0 : buffer + 1;
     }
 
     if (!valid) return;
-    const float l = half_sum(rowset.l);
+    const float l = across32(rowset.l, added);
     const int64_t out_row = token * p.q_heads + head;
     if (p.splits > 1) {
         float* const dst = p.part + (out_row * p.splits + split) * D + 16 * g;
@@ -510,14 +755,15 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_kv_attn_rows(KvAttnAr
         p.lse[out_row] = l == 0.0f ? -__builtin_inff() : (rowset.m + __builtin_log2f(l)) * 0.6931471805599453f;
 }
 
-// Up to 32 rows of one sequence (or of one token, where each has its own pages) and key/value head.
-template <int D, bool F16>
+// Up to 16 NT rows of one sequence (or of one token, where each has its own pages) and key/value head.
+template <int D, bool F16, int NT>
 __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_kv_attn_step(KvAttnArgs p)
 {
-    constexpr int kTiles = D / 32, kSteps = D / 64;
-    extern __shared__ __attribute__((aligned(128))) uint8_t lds[];
+    constexpr int kTiles = D / 16, kSteps = StepRows<D, F16, NT>::kSteps;
+    extern __shared__ __attribute__((aligned(128))) uint8_t lds[];   // [4][rows][D], then the maxima and sums
+    __shared__ __attribute__((aligned(16))) PageInfo info[kInfo];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int r = lane & 31, g = lane >> 5;
+    const int r = lane & 15, g = lane >> 4;
 
     uint32_t item = blockIdx.x;
     const int split = (int)(item % p.splits);
@@ -547,17 +793,11 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_kv_attn_step(KvAttnAr
     const int at = p.blocks ? (int)((int64_t)unit - s.start) : 0;   // the unit's first token in its sequence
     if (at < 0 || at >= s.n) return;
     const int rows = min(p.blocks ? p.group : s.n * p.group, p.step_rows);
-    if (tile * kWaveRows >= rows) return;
-    const int row = tile * kWaveRows + r;
-    const bool valid = row < rows;
-    const int first_token = at + tile * kWaveRows / p.group, last_token = at + (min((tile + 1) * kWaveRows, rows) - 1) / p.group;
+    if (tile * kStepRows >= rows) return;
+    const int first_token = at + tile * kStepRows / p.group, last_token = at + (min((tile + 1) * kStepRows, rows) - 1) / p.group;
     auto limit_of = [&](int t) -> int {
         return p.causal ? (int)min(max(s.first + t + 1, (int64_t)0), (int64_t)s.length) : s.length;
     };
-    const int own = at + row / p.group;
-    const int64_t token = s.start + own;
-    const int head = h * p.group + row % p.group;
-
     const int32_t* list = p.blocks ? p.blocks + ((int64_t)unit * p.c.heads + h) * p.top : nullptr;
     int lo = 0, hi = list ? (p.b.width > 0 ? p.top : 0) : (limit_of(last_token) + kPage - 1) / kPage;
     if (p.splits > 1) {
@@ -566,73 +806,82 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_kv_attn_step(KvAttnAr
         hi = min(lo + per, hi);
     }
 
-    WaveRows<D, F16> rowset;
-    rowset.load(valid ? p.q + token * p.ldq + (int64_t)head * D : nullptr, g, p.scale);
-    rowset.limit = valid ? limit_of(own) : 0;
+    StepRows<D, F16, NT> rowset;
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+        const int row = tile * kStepRows + 16 * n + r, own = at + row / p.group;
+        const bool valid = row < rows;
+        rowset.load(n, valid ? p.q + (s.start + own) * p.ldq + (int64_t)(h * p.group + row % p.group) * D : nullptr, g, p.scale);
+        rowset.limit[n] = valid ? limit_of(own) : 0;
+    }
     const int least = limit_of(first_token), most = limit_of(last_token);
 
-    const int from_k = row_key(r) * D + 32 * g, from_v = row_key(r) * kPage + 16 * g;
-    uint4 kr[2][kSteps][2], vr[2][kTiles];
-    auto load_k = [&](const PageAt& a) {
-        const uint8_t* const src = p.c.k + a.ph * (kPage * D);
+    const int from_k = (16 * (r >> 2) + (r & 3)) * D + 32 * (D == 64 ? g & 1 : g), from_v = r * kPage + 16 * g;
+    uint4 kr[4][kSteps][2], vr[kTiles];
+    auto load_k = [&](const PageInfo& a) {
+        const uint8_t* const src = p.c.k + ((int64_t)max(a.page, 0) * p.c.heads + h) * (kPage * D);
 #pragma unroll
-        for (int kt = 0; kt < 2; ++kt)
+        for (int t = 0; t < 4; ++t)
 #pragma unroll
             for (int st = 0; st < kSteps; ++st)
 #pragma unroll
-                for (int j = 0; j < 2; ++j)
-                    kr[kt][st][j] = *reinterpret_cast<const uint4*>(src + from_k + kt * 32 * D + st * 64 + j * 16);
+                for (int j = 0; j < 2; ++j) kr[t][st][j] = *reinterpret_cast<const uint4*>(src + from_k + t * 4 * D + st * 128 + j * 16);
     };
-    auto load_v = [&](const PageAt& a) {
-        const uint8_t* const src = p.c.v + a.ph * (kPage * D);
+    auto load_v = [&](const PageInfo& a) {
+        const uint8_t* const src = p.c.v + ((int64_t)max(a.page, 0) * p.c.heads + h) * (kPage * D);
 #pragma unroll
-        for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-            for (int t = 0; t < kTiles; ++t) vr[kt][t] = *reinterpret_cast<const uint4*>(src + from_v + t * 32 * kPage + kt * 32);
+        for (int t = 0; t < kTiles; ++t) vr[t] = *reinterpret_cast<const uint4*>(src + from_v + t * 16 * kPage);
     };
-    PageAt now{}, next{};
-    int i = lo + wave;
-    if (i < hi) {
-        now = page_at(p, b, h, s.length, list, i);
-        load_k(now);
-        load_v(now);
-    }
-    for (; i < hi; i += 4) {
-        const bool more = i + 4 < hi;
-        if (more) next = page_at(p, b, h, s.length, list, i + 4);
-        f32x16_t sc[2];
-        f16x8_t w[2][2];
-        rowset.scores([&](int kt, int st) {
-            const uint4 x = kr[kt][st][0], y = kr[kt][st][1];
-            return i32x8_t{(int)x.x, (int)x.y, (int)x.z, (int)x.w, (int)y.x, (int)y.y, (int)y.z, (int)y.w};
-        }, sc);
-        if (more) load_k(next);
-        if (now.key0 < most) {
-            const bool masked = now.key0 + kPage > least;
-            if (masked) rowset.mask(sc, now.key0, g);
-            rowset.weights(sc, now.ek, now.ev, w);
-            auto value = [&](int kt, int t) { return vr[kt][t]; };
-            if (masked) rowset.template add_values<true>(value, w, now.key0, s.length, g);
-            else rowset.template add_values<false>(value, w, now.key0, s.length, g);
+    for (int first = lo; first < hi; first += kInfo) {
+        const int count = min(hi - first, kInfo);
+        __syncthreads();
+        look_up(p, b, h, s.length, list, first, hi, info);
+        __syncthreads();
+        PageInfo now{}, next{};
+        int i = wave;
+        if (i < count) {
+            now = info_at(info, i);
+            load_k(now);
+            load_v(now);
         }
-        if (more) load_v(next);
-        now = next;
+        for (; i < count; i += 4) {
+            const bool more = i + 4 < count;
+            if (more) next = info_at(info, i + 4);
+            f32x4_t sc[NT][4];
+            f16x8_t w[NT][2];
+            rowset.scores([&](int t, int st) {
+                const uint4 x = kr[t][st][0], y = kr[t][st][1];
+                return i32x8_t{(int)x.x, (int)x.y, (int)x.z, (int)x.w, (int)y.x, (int)y.y, (int)y.z, (int)y.w};
+            }, sc);
+            if (more) load_k(next);
+            const int key0 = first_key(now);
+            if (key0 < most) {
+                const bool masked = key0 + kPage > least;
+                if (masked) rowset.mask(sc, key0, g);
+                rowset.weights(sc, now.ek, now.ev, w);
+                if (masked) rowset.settle_values(vr, key0, s.length, g);
+                rowset.add_values(vr, w);
+            }
+            if (more) load_v(next);
+            now = next;
+        }
     }
 
-    // The four waves' parts of each row, joined in LDS: [wave][row][d], then their maxima and sums.
-    const int kept = min(rows - tile * kWaveRows, kWaveRows);
+    // The four waves' parts of each row, joined in LDS.
+    const int kept = min(rows - tile * kStepRows, kStepRows);
     float* const acc = reinterpret_cast<float*>(lds);
     float* const sums = acc + 4 * kept * D;
-    const float l = half_sum(rowset.l);
-    if (r < kept) {
-        float* const dst = acc + (wave * kept + r) * D + 16 * g;
 #pragma unroll
-        for (int t = 0; t < kTiles; ++t)
+    for (int n = 0; n < NT; ++n) {
+        const float l = across16(across32(rowset.l[n], added), added);
+        const int at_row = 16 * n + r;
+        if (at_row < kept) {
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-                *reinterpret_cast<float4*>(dst + 32 * t + 4 * j) = make_float4(rowset.acc[t][4 * j], rowset.acc[t][4 * j + 1],
-                                                                             rowset.acc[t][4 * j + 2], rowset.acc[t][4 * j + 3]);
-        if (g == 0) sums[2 * (wave * kept + r)] = rowset.m, sums[2 * (wave * kept + r) + 1] = l;
+            for (int t = 0; t < kTiles; ++t)
+                *reinterpret_cast<float4*>(acc + (wave * kept + at_row) * D + 16 * t + 4 * g) =
+                    make_float4(rowset.acc[n][t][0], rowset.acc[n][t][1], rowset.acc[n][t][2], rowset.acc[n][t][3]);
+            if (g == 0) sums[2 * (wave * kept + at_row)] = rowset.m[n], sums[2 * (wave * kept + at_row) + 1] = l;
+        }
     }
     __syncthreads();
     for (int e = tid; e < kept * (D / 4); e += 256) {
@@ -648,7 +897,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_kv_attn_step(KvAttnAr
             total += f * sums[2 * (wv * kept + row_e) + 1];
             o[0] += f * a.x, o[1] += f * a.y, o[2] += f * a.z, o[3] += f * a.w;
         }
-        const int row_at = tile * kWaveRows + row_e;
+        const int row_at = tile * kStepRows + row_e;
         const int64_t out_row = (s.start + at + row_at / p.group) * p.q_heads + h * p.group + row_at % p.group;
         if (p.splits > 1) {
             *reinterpret_cast<float4*>(p.part + (out_row * p.splits + split) * D + d) = make_float4(o[0], o[1], o[2], o[3]);
@@ -713,12 +962,12 @@ Plan make_plan(KvAttnArgs& p, int64_t max_query, int cus)
     Plan plan{};
     const int64_t n = p.b.q_start ? (max_query > 0 && max_query < p.b.tokens ? max_query : p.b.tokens) : p.b.tokens / p.b.batch;
     const int64_t most = p.blocks ? p.query_block : n;   // tokens of a unit of the step kernel
-    plan.step = p.blocks ? p.query_block == 1 : n * p.group <= kWaveRows;
+    plan.step = p.blocks ? p.query_block == 1 : n * p.group <= kStepRows;
     const int64_t pages = p.blocks ? p.top : p.b.width;
     int64_t groups;
     if (plan.step) {
         plan.step_rows = (int)(most * p.group);
-        plan.column_tiles = (plan.step_rows + kWaveRows - 1) / kWaveRows;
+        plan.column_tiles = (plan.step_rows + kStepRows - 1) / kStepRows;
         // (and one unit that clears what is behind the last sequence)
         groups = (p.blocks ? p.b.tokens : (int64_t)p.b.batch + (p.b.q_start ? 1 : 0)) * p.c.heads * plan.column_tiles;
     } else {
@@ -737,30 +986,37 @@ Plan make_plan(KvAttnArgs& p, int64_t max_query, int cus)
     return plan;
 }
 
+template <int D, bool F16, int NT>
+int launch_step(const KvAttnArgs& p, hipStream_t stream)
+{
+    const size_t bytes = (size_t)(4 * (p.step_rows < kStepRows ? p.step_rows : kStepRows)) * (D + 2) * 4;
+    if (bytes + kInfo * sizeof(PageInfo) > 65536) {   // (beyond what a launch may take unasked; once per device)
+        static std::atomic<bool> raised[64];
+        int dev = 0;
+        if (hipGetDevice(&dev) != hipSuccess) return set_error(VDN_FP8_ELAUNCH, "kv_attention: no device");
+        if (dev >= 64 || !raised[dev].load(std::memory_order_relaxed)) {
+            if (hipFuncSetAttribute((const void*)k_kv_attn_step<D, F16, NT>, hipFuncAttributeMaxDynamicSharedMemorySize,
+                                    4 * kStepRows * (D + 2) * 4) != hipSuccess)
+                return set_error(VDN_FP8_ELAUNCH, "kv_attention: the device refuses %zu bytes of LDS", bytes);
+            if (dev < 64) raised[dev].store(true, std::memory_order_relaxed);
+        }
+    }
+    hipLaunchKernelGGL((k_kv_attn_step<D, F16, NT>), dim3(p.items), dim3(256), bytes, stream, p);
+    return check_launch("kv_attention");
+}
+
 template <int D, bool F16>
 int launch(const KvAttnArgs& p, bool step, hipStream_t stream)
 {
-    const dim3 grid((unsigned)p.items), block(256);
+    int st;
     if (step) {
-        const size_t bytes = (size_t)(4 * (p.step_rows < kWaveRows ? p.step_rows : kWaveRows)) * (D + 2) * 4;
-        if (bytes > 65536) {
-            static std::atomic<bool> raised[64];
-            int dev = 0;
-            if (hipGetDevice(&dev) != hipSuccess) return set_error(VDN_FP8_ELAUNCH, "kv_attention: no device");
-            if (dev >= 64 || !raised[dev].load(std::memory_order_relaxed)) {
-                if (hipFuncSetAttribute((const void*)k_kv_attn_step<D, F16>, hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024) != hipSuccess)
-                    return set_error(VDN_FP8_ELAUNCH, "kv_attention: the device refuses %zu bytes of LDS", bytes);
-                if (dev < 64) raised[dev].store(true, std::memory_order_relaxed);
-            }
-        }
-        hipLaunchKernelGGL((k_kv_attn_step<D, F16>), grid, block, bytes, stream, p);
+        st = p.step_rows <= 16 ? launch_step<D, F16, 1>(p, stream) : launch_step<D, F16, 2>(p, stream);
     } else {
-        const size_t bytes = (size_t)(D == 256 ? 2 : 3) * 2 * kPage * D;
-        hipLaunchKernelGGL((k_kv_attn_rows<D, F16>), grid, block, bytes, stream, p);
+        hipLaunchKernelGGL((k_kv_attn_rows<D, F16>), dim3(p.items), dim3(256), 0, stream, p);
+        st = check_launch("kv_attention");
     }
-    int st = check_launch("kv_attention");
     if (st != VDN_FP8_OK || p.splits == 1) return st;
-    hipLaunchKernelGGL((k_kv_attn_join<D, F16>), dim3((unsigned)((p.b.tokens * p.q_heads + 3) / 4)), block, 0, stream, p);
+    hipLaunchKernelGGL((k_kv_attn_join<D, F16>), dim3((unsigned)((p.b.tokens * p.q_heads + 3) / 4)), dim3(256), 0, stream, p);
     return check_launch("kv_attention join");
 }
 
