@@ -12,9 +12,10 @@
 // five orders below the attention that follows, and the matrix cores take binary64.
 //
 // What bounds it: at many queries the query sum's bytes (each query read once); at single tokens the
-// page means' bytes (2 d a page and head, 1/64 of the cache) and the latency of three launches.
+// page means' bytes (2 d a page and head, 1/64 of the cache) and the latency of two launches.
 //   k_kv_query_sum   one workgroup per block and head
 //   k_kv_scores      one wave per 16 pages, all blocks of the sequence, 16 at a time
+//   k_kv_scores_step both of these where each query has its own pages
 //   k_kv_top         one workgroup per block and head: radix selection on the scores' bits,
 //                    eight bits a pass, until what is left of a digit is wanted as a whole
 #include <stdint.h>
@@ -56,6 +57,23 @@ __device__ __forceinline__ bool block_of(const KvSelectArgs& p, int64_t row, int
     return true;
 }
 
+// Adds eight elements.
+template <bool F16>
+__device__ __forceinline__ void add8(uint4 v, double sum[8])
+{
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        if (F16) {
+            sum[2 * e] += (double)(float)__builtin_bit_cast(_Float16, (uint16_t)w[e]);
+            sum[2 * e + 1] += (double)(float)__builtin_bit_cast(_Float16, (uint16_t)(w[e] >> 16));
+        } else {
+            sum[2 * e] += (double)bf16_lo(w[e]);
+            sum[2 * e + 1] += (double)bf16_hi(w[e]);
+        }
+    }
+}
+
 template <bool F16>
 __global__ __launch_bounds__(kThreads) void k_kv_query_sum(KvSelectArgs p)
 {
@@ -71,18 +89,7 @@ __global__ __launch_bounds__(kThreads) void k_kv_query_sum(KvSelectArgs p)
 #pragma unroll 4
     for (int i = tid / chunks; i < n; i += lanes) {
         const int64_t token = s.start + from + i / p.group;
-        const uint4 v = *reinterpret_cast<const uint4*>(p.q + token * p.ldq + (int64_t)(h * p.group + i % p.group) * d + 8 * ch);
-        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            if (F16) {
-                sum[2 * e] += (double)(float)__builtin_bit_cast(_Float16, (uint16_t)w[e]);
-                sum[2 * e + 1] += (double)(float)__builtin_bit_cast(_Float16, (uint16_t)(w[e] >> 16));
-            } else {
-                sum[2 * e] += (double)bf16_lo(w[e]);
-                sum[2 * e + 1] += (double)bf16_hi(w[e]);
-            }
-        }
+        add8<F16>(*reinterpret_cast<const uint4*>(p.q + token * p.ldq + (int64_t)(h * p.group + i % p.group) * d + 8 * ch), sum);
     }
 #pragma unroll
     for (int e = 0; e < 8; ++e) part[e * kThreads + tid] = sum[e];
@@ -139,6 +146,52 @@ __global__ __launch_bounds__(kThreads) void k_kv_scores(KvSelectArgs p)
     }
 }
 
+// One query (its group's heads) against all pages of its sequence, where each query has its own pages: 16
+// lanes a page, eight elements each. The matrix instruction would use one of its 16 rows: 64 cycles for four
+// products of 16 pages, where four fma here take 16 for four pages.
+template <int D, bool F16>
+__global__ __launch_bounds__(kThreads) void k_kv_scores_step(KvSelectArgs p)
+{
+    constexpr int L = D / 8, kPages = 64 / L, kSweeps = 4;   // lanes of a page, pages of a sweep, sweeps of a wave
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int h = blockIdx.y;
+    const int64_t row = blockIdx.z;   // the query
+    int b, from, to;
+    KvSequence s;
+    if (!block_of(p, row, b, s, from, to)) return;
+    const int have = (s.length + kPage - 1) / kPage;
+    const int w0 = (blockIdx.x * 4 + wave) * (kPages * kSweeps) + lane / L, i0 = 8 * (lane % L);
+    if (w0 - lane / L >= have) return;
+    uint4 mean[kSweeps];
+#pragma unroll
+    for (int j = 0; j < kSweeps; ++j) {
+        const int w = w0 + j * kPages;
+        const int page = w < have ? kv_page(p.b, p.c, b, w) : -1;
+        mean[j] = make_uint4(0, 0, 0, 0);
+        if (page >= 0) mean[j] = *reinterpret_cast<const uint4*>(p.c.k_mean + ((int64_t)page * p.c.heads + h) * D + i0);
+    }
+    double q[8] = {0.0, 0.0, 0.0, 0.0, 0.0, 0.0, 0.0, 0.0};
+    const uint16_t* const src = p.q + (s.start + from) * p.ldq + (int64_t)h * p.group * D + i0;
+#pragma unroll 8
+    for (int g = 0; g < p.group; ++g) add8<F16>(*reinterpret_cast<const uint4*>(src + (int64_t)g * D), q);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) q[e] = (double)(float)q[e];
+#pragma unroll
+    for (int j = 0; j < kSweeps; ++j) {
+        const uint32_t m[4] = {mean[j].x, mean[j].y, mean[j].z, mean[j].w};
+        double sum = 0.0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            sum = __builtin_fma(q[2 * e], (double)bf16_lo(m[e]), sum);
+            sum = __builtin_fma(q[2 * e + 1], (double)bf16_hi(m[e]), sum);
+        }
+#pragma unroll
+        for (int off = 1; off < L; off <<= 1) sum += __shfl_xor(sum, off, 64);
+        const int w = w0 + j * kPages;
+        if (lane % L == 0 && w < have) p.score[(row * p.c.heads + h) * p.b.width + w] = sum;
+    }
+}
+
 // A score's bits, ordered as the scores are, above 0; NaN as -inf.
 __device__ __forceinline__ uint64_t score_key(double v)
 {
@@ -147,12 +200,18 @@ __device__ __forceinline__ uint64_t score_key(double v)
     return (u >> 63) ? ~u : u | 0x8000000000000000ull;
 }
 
+// HELD: at most kHeld * 256 pages, whose keys stay in registers; else they are read again in every pass.
+// A pass counts one digit of the keys that share the digits before it, in LDS; the first wave finds the
+// digit in which the last wanted key lies. What is taken then goes through bitmaps, whose bits in
+// order are the pages in order.
 template <bool HELD>
 __global__ __launch_bounds__(kThreads) void k_kv_top(KvSelectArgs p)
 {
-    __shared__ uint32_t hist[256];
-    __shared__ uint32_t wave_sum[4];
-    __shared__ uint32_t picked[3];   // digit, how many of it are wanted, how many it has
+    constexpr int kWords = kHeld * kThreads / 32;   // of a bitmap, one lane each
+    static_assert(kWords == 64, "a wave reads a bitmap at once");
+    __shared__ __attribute__((aligned(16))) uint32_t hist[8][256];
+    __shared__ uint32_t picked[4];   // digit, how many of it are wanted, how many it has, keys counted in all
+    __shared__ uint32_t above[kWords], same[kWords];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int64_t row = blockIdx.x / (uint32_t)p.c.heads;
     const int h = (int)(blockIdx.x % (uint32_t)p.c.heads);
@@ -165,100 +224,129 @@ __global__ __launch_bounds__(kThreads) void k_kv_top(KvSelectArgs p)
         have = (seen + kPage - 1) / kPage;
     }
     const double* const score = p.score + (row * p.c.heads + h) * p.b.width;
-    const int turns = (have + kThreads - 1) / kThreads;
-    auto key_at = [&](int w) -> uint64_t {
+    auto key_at = [&](int w) -> uint64_t {   // 0: not to be taken
         if (w >= have || kv_page(p.b, p.c, b, w) < 0) return 0;
         if (w < p.first || w >= have - p.last) return ~0ull;
         return score_key(score[w]);
     };
+    const int turns = (have + kThreads - 1) / kThreads;
     uint64_t held[HELD ? kHeld : 1];
     if (HELD)
 #pragma unroll
         for (int j = 0; j < kHeld; ++j) held[j] = j < turns ? key_at(tid + j * kThreads) : 0;
-    // (a thread's scores: pages tid, tid + 256, ...)
     auto each = [&](auto f) {
         if (HELD) {
 #pragma unroll
             for (int j = 0; j < kHeld; ++j)
-                if (j < turns) f(held[j], j);
+                if (j < turns) f(held[j]);
         } else {
-            for (int j = 0; j < turns; ++j) f(key_at(tid + j * kThreads), j);
+            for (int j = 0; j < turns; ++j) f(key_at(tid + j * kThreads));
         }
     };
-    // sum over the workgroup of what comes before this thread's value, and in all
-    auto prefix = [&](uint32_t v, uint32_t& all) {
-        uint32_t run = v;
 #pragma unroll
-        for (int off = 1; off < 64; off <<= 1) {
-            const uint32_t t = __shfl_up(run, off, 64);
-            if (lane >= off) run += t;
-        }
-        __syncthreads();
-        if (lane == 63) wave_sum[wave] = run;
-        __syncthreads();
-        uint32_t before = run - v;
-        all = 0;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            if (i < wave) before += wave_sum[i];
-            all += wave_sum[i];
-        }
-        return before;
-    };
+    for (int i = 0; i < 8; ++i) hist[i][tid] = 0;
+    __syncthreads();
 
-    uint32_t candidates = 0;
-    {
-        uint32_t mine = 0;
-        each([&](uint64_t k, int) { mine += k != 0; });
-        prefix(mine, candidates);
-    }
-    // The least key that is taken (`least`), and how many of those equal to it: all but at the end.
-    uint64_t least = 1;
-    uint32_t equal = ~0u, wanted = (uint32_t)p.top;
-    if (candidates > wanted) {
-        uint64_t high = 0;
-        for (int shift = 56;; shift -= 8) {
-            hist[tid] = 0;
-            __syncthreads();
-            const uint64_t mask = shift == 56 ? 0 : ~0ull << (shift + 8);
-            each([&](uint64_t k, int) {
-                if (k != 0 && (k & mask) == high) atomicAdd(&hist[(k >> shift) & 255], 1u);
-            });
-            __syncthreads();
-            // thread t: digit 255 - t, so that what comes before it is what is larger
-            const uint32_t own = hist[255 - tid];
-            uint32_t all;
-            const uint32_t before = prefix(own, all);
-            if (before < wanted && before + own >= wanted) picked[0] = 255 - tid, picked[1] = wanted - before, picked[2] = own;
-            __syncthreads();
-            high |= (uint64_t)picked[0] << shift;
-            wanted = picked[1];
-            const bool whole = picked[2] == wanted;
-            __syncthreads();
-            if (whole || shift == 0) {
-                least = high;
-                equal = whole ? ~0u : wanted;   // (at shift 0: the first `wanted` of the equal ones)
-                break;
+    // Taken: the keys above `least`, and of those equal to it the first `equal`.
+    uint64_t least = 0;
+    uint32_t equal = 0, wanted = (uint32_t)p.top;
+    uint64_t high = 0;
+    for (int pass = 0; pass < 8; ++pass) {
+        const int shift = 56 - 8 * pass;
+        each([&](uint64_t k) {
+            if (k != 0 && (pass == 0 || (k >> (shift + 8)) == (high >> (shift + 8)))) atomicAdd(&hist[pass][(k >> shift) & 255], 1u);
+        });
+        __syncthreads();
+        if (wave == 0) {
+            // lane l: digits 255 - 4 l and the three below it; what comes before them is what is larger
+            const uint4 v = *reinterpret_cast<const uint4*>(&hist[pass][252 - 4 * lane]);
+            const uint32_t n[4] = {v.w, v.z, v.y, v.x}, own = n[0] + n[1] + n[2] + n[3];
+            uint32_t run = own;
+#pragma unroll
+            for (int off = 1; off < 64; off <<= 1) {
+                const uint32_t t = __shfl_up(run, off, 64);
+                if (lane >= off) run += t;
             }
+            uint32_t before = run - own;
+            if (before < wanted && run >= wanted)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    if (before < wanted && before + n[i] >= wanted) picked[0] = 255 - 4 * lane - i, picked[1] = wanted - before, picked[2] = n[i];
+                    before += n[i];
+                }
+            if (lane == 63) picked[3] = run;
+        }
+        __syncthreads();
+        if (pass == 0 && picked[3] <= wanted) break;   // all that there are: least = 0
+        high |= (uint64_t)picked[0] << shift;
+        wanted = picked[1];
+        least = high, equal = wanted;
+        if (picked[2] == wanted) {   // the whole digit: every key from its least one on
+            least = high - 1;
+            equal = 0;
+            break;
         }
     }
-    // In ascending order: pages of a turn come before those of the next.
-    uint32_t taken = 0, equal_before = 0;
-    auto turn = [&](uint64_t k, int j) {
-        const bool same = equal != ~0u && k == least;
-        uint32_t all;
-        uint32_t n = 0;
-        if (equal != ~0u) {   // (uniform)
-            n = equal_before + prefix(same, all);
-            equal_before += all;
+    // (high > 0 where the loop went past its first test, since every key counted has a bit of it or
+    // more: 0 itself is no key)
+
+    uint32_t taken = 0, equal_left = equal;
+    for (int w0 = 0; w0 < have; w0 += kWords * 32) {
+        if (w0) __syncthreads();   // the bitmaps before have been read
+        if (tid < kWords) above[tid] = same[tid] = 0;
+        __syncthreads();
+        auto mark = [&](uint64_t k, int j) {
+            const uint64_t more = __ballot(k > least), alike = __ballot(k == least && k != 0);
+            // this wave's 64 pages of the turn: two words
+            if (lane < 2) {
+                above[8 * j + 2 * wave + lane] = (uint32_t)(more >> (32 * lane));
+                same[8 * j + 2 * wave + lane] = (uint32_t)(alike >> (32 * lane));
+            }
+        };
+        if (HELD) {
+#pragma unroll
+            for (int j = 0; j < kHeld; ++j)
+                if (j < turns) mark(held[j], j);
+        } else {
+            for (int j = 0; j < kHeld && w0 + j * kThreads < have; ++j) mark(key_at(w0 + tid + j * kThreads), j);
         }
-        const bool take = k != 0 && (equal == ~0u ? k >= least : k > least || (same && n < equal));
-        const uint32_t at = taken + prefix(take, all);
-        taken += all;
-        if (take && at < (uint32_t)p.top) out[at] = tid + j * kThreads;
-    };
-    each(turn);
-    for (int i = (int)taken + tid; i < p.top; i += kThreads) out[i] = -1;
+        __syncthreads();
+        if (wave == 0) {
+            uint32_t alike = same[lane], bits = above[lane], run = __builtin_popcount(alike);
+            if (equal_left > 0) {   // (uniform)
+                const uint32_t own = run;
+#pragma unroll
+                for (int off = 1; off < 64; off <<= 1) {
+                    const uint32_t t = __shfl_up(run, off, 64);
+                    if (lane >= off) run += t;
+                }
+                uint32_t room = equal_left > run - own ? equal_left - (run - own) : 0;   // of this word's
+                while (alike && room) {
+                    bits |= alike & (0u - alike);
+                    alike &= alike - 1;
+                    --room;
+                }
+                const uint32_t all = __shfl(run, 63, 64);
+                equal_left = equal_left > all ? equal_left - all : 0;
+            }
+            const uint32_t own = __builtin_popcount(bits);
+            run = own;
+#pragma unroll
+            for (int off = 1; off < 64; off <<= 1) {
+                const uint32_t t = __shfl_up(run, off, 64);
+                if (lane >= off) run += t;
+            }
+            uint32_t at = taken + run - own;
+            while (bits) {
+                if (at < (uint32_t)p.top) out[at] = w0 + 32 * lane + __builtin_ctz(bits);
+                bits &= bits - 1;
+                ++at;
+            }
+            taken += __shfl(run, 63, 64);
+        }
+    }
+    if (wave == 0)
+        for (int i = (int)taken + lane; i < p.top; i += 64) out[i] = -1;
 }
 
 int select_arguments(const vdn_fp8_kv_cache* cache, const vdn_fp8_kv_batch* batch, int64_t q_heads, int64_t query_block, KvSelectArgs& p,
@@ -321,8 +409,21 @@ extern "C" int vdn_fp8_kv_select(const vdn_fp8_kv_cache* cache, const vdn_fp8_kv
     p.sum = (float*)workspace;   // (a multiple of 256 bytes)
     p.score = (double*)(p.sum + p.rows * p.c.heads * p.c.d);
     const dim3 block(kThreads), per_row((unsigned)(p.rows * p.c.heads));
-    if (p.b.width > 0) {
-        if (dtype == VDN_FP8_DTYPE_F16) hipLaunchKernelGGL((k_kv_query_sum<true>), per_row, block, 0, stream, p);
+    const bool f16 = dtype == VDN_FP8_DTYPE_F16;
+    if (p.b.width > 0 && p.query_block == 1 && p.rows <= 65535) {
+        const int64_t pages = 4 * 4 * (64 / (p.c.d / 8));   // of a workgroup
+        const dim3 grid((unsigned)((p.b.width + pages - 1) / pages), (unsigned)p.c.heads, (unsigned)p.rows);
+#define VDN_STEP(n)                                                                                         \
+    case n:                                                                                                 \
+        if (f16) hipLaunchKernelGGL((k_kv_scores_step<n, true>), grid, block, 0, stream, p);                \
+        else hipLaunchKernelGGL((k_kv_scores_step<n, false>), grid, block, 0, stream, p);                   \
+        break;
+        switch (p.c.d) { VDN_STEP(64) VDN_STEP(128) VDN_STEP(256) }
+#undef VDN_STEP
+        const int launched = check_launch("kv_select scores");
+        if (launched != VDN_FP8_OK) return launched;
+    } else if (p.b.width > 0) {
+        if (f16) hipLaunchKernelGGL((k_kv_query_sum<true>), per_row, block, 0, stream, p);
         else hipLaunchKernelGGL((k_kv_query_sum<false>), per_row, block, 0, stream, p);
         int launched = check_launch("kv_select query sum");
         if (launched != VDN_FP8_OK) return launched;

@@ -21,6 +21,7 @@ replayed with other lengths and tables in the same buffers.
 Everything runs on torch's current stream of the tensors' device, in hand-written kernels
 (include/vdn_fp8.h); there is no CPU path and no autograd.
 """
+import contextlib
 import ctypes
 from typing import NamedTuple, Optional
 
@@ -111,20 +112,12 @@ def _ld(t):
     return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1] * t.shape[2])
 
 
-class _on:
+_HERE = contextlib.nullcontext()
+
+
+def _on(device):
     """The tensors' device as the current one, for a launch (nothing where it is already)."""
-
-    def __init__(self, device):
-        self.device = device
-
-    def __enter__(self):
-        self.before = torch.cuda.current_device()
-        if self.before != self.device.index:
-            torch.cuda.set_device(self.device)
-
-    def __exit__(self, *exc):
-        if self.before != self.device.index:
-            torch.cuda.set_device(self.before)
+    return _HERE if torch._C._cuda_getDevice() == device.index else torch.cuda.device(device)
 
 
 def kv_append(key, value, cache, page_table, lengths, *, q_start=None):
@@ -153,6 +146,8 @@ def _norm(norm, d, device, name):
     weight, eps = norm
     if weight is None:
         return None, float(eps)
+    if weight.shape == (d,) and weight.dtype == torch.bfloat16 and weight.device == device and weight.stride(0) == 1:
+        return _aligned16(weight), float(eps)
     if weight.numel() != d or weight.dtype != torch.bfloat16:
         raise ValueError(f"{name}'s weight must be a bfloat16 [{d}] tensor")
     return _aligned16(weight.detach().to(device).reshape(d).contiguous()), float(eps)
@@ -176,7 +171,8 @@ def qk_prep_append(query, key, value, norm_q, norm_k, cache, page_table, lengths
     if (cos is None) != (sin is None):
         raise ValueError("cos and sin go together")
     if cos is not None:
-        cos, sin = cos.detach().to(dev).reshape(-1, cos.shape[-1]), sin.detach().to(dev).reshape(-1, sin.shape[-1])
+        if cos.dim() != 2 or cos.device != dev or sin.dim() != 2 or sin.device != dev:
+            cos, sin = cos.detach().to(dev).reshape(-1, cos.shape[-1]), sin.detach().to(dev).reshape(-1, sin.shape[-1])
         if cos.shape != sin.shape or cos.shape[0] != T or cos.dtype != sin.dtype:
             raise ValueError(f"cos/sin must both be [T={T}, R] of one dtype (got {tuple(cos.shape)}, {tuple(sin.shape)})")
         if cos.dtype not in (torch.float32, torch.bfloat16):
