@@ -115,12 +115,12 @@ __global__ __launch_bounds__(kThreads) void k_kv_scores(KvSelectArgs p)
     const int w0 = (blockIdx.x * 4 + wave) * 16;
     if (w0 >= have || s.n == 0) return;
     const int w = w0 + lane % 16, g = lane / 16;
-    const int page = w < have ? kv_page(p.b, p.c, b, w) : -1;
+    // (a page that is not there: any page's mean, as k_kv_top passes it over)
+    const int page = max(kv_page(p.b, p.c, b, min(w, have - 1)), 0);
     uint32_t mean[E / 2];
 #pragma unroll
     for (int i = 0; i < E / 8; ++i) {
-        uint4 v = make_uint4(0, 0, 0, 0);
-        if (page >= 0) v = *reinterpret_cast<const uint4*>(p.c.k_mean + ((int64_t)page * p.c.heads + h) * D + g * E + 8 * i);
+        const uint4 v = *reinterpret_cast<const uint4*>(p.c.k_mean + ((int64_t)page * p.c.heads + h) * D + g * E + 8 * i);
         mean[4 * i] = v.x, mean[4 * i + 1] = v.y, mean[4 * i + 2] = v.z, mean[4 * i + 3] = v.w;
     }
     const int blocks = (s.n + p.query_block - 1) / p.query_block;
@@ -162,18 +162,20 @@ __global__ __launch_bounds__(kThreads) void k_kv_scores_step(KvSelectArgs p)
     const int have = (s.length + kPage - 1) / kPage;
     const int w0 = (blockIdx.x * 4 + wave) * (kPages * kSweeps) + lane / L, i0 = 8 * (lane % L);
     if (w0 - lane / L >= have) return;
+    // (every load before any use, and none under a condition: each of its own would be a round trip to memory)
+    const uint16_t* const src = p.q + (s.start + from) * p.ldq + (int64_t)h * p.group * D + i0;
+    const uint4 q0 = *reinterpret_cast<const uint4*>(src);
+    int page[kSweeps];
+#pragma unroll
+    for (int j = 0; j < kSweeps; ++j) page[j] = max(kv_page(p.b, p.c, b, min(w0 + j * kPages, have - 1)), 0);
     uint4 mean[kSweeps];
 #pragma unroll
-    for (int j = 0; j < kSweeps; ++j) {
-        const int w = w0 + j * kPages;
-        const int page = w < have ? kv_page(p.b, p.c, b, w) : -1;
-        mean[j] = make_uint4(0, 0, 0, 0);
-        if (page >= 0) mean[j] = *reinterpret_cast<const uint4*>(p.c.k_mean + ((int64_t)page * p.c.heads + h) * D + i0);
-    }
+    for (int j = 0; j < kSweeps; ++j)
+        mean[j] = *reinterpret_cast<const uint4*>(p.c.k_mean + ((int64_t)page[j] * p.c.heads + h) * D + i0);
     double q[8] = {0.0, 0.0, 0.0, 0.0, 0.0, 0.0, 0.0, 0.0};
-    const uint16_t* const src = p.q + (s.start + from) * p.ldq + (int64_t)h * p.group * D + i0;
+    add8<F16>(q0, q);
 #pragma unroll 8
-    for (int g = 0; g < p.group; ++g) add8<F16>(*reinterpret_cast<const uint4*>(src + (int64_t)g * D), q);
+    for (int g = 1; g < p.group; ++g) add8<F16>(*reinterpret_cast<const uint4*>(src + (int64_t)g * D), q);
 #pragma unroll
     for (int e = 0; e < 8; ++e) q[e] = (double)(float)q[e];
 #pragma unroll
@@ -224,16 +226,26 @@ __global__ __launch_bounds__(kThreads) void k_kv_top(KvSelectArgs p)
         have = (seen + kPage - 1) / kPage;
     }
     const double* const score = p.score + (row * p.c.heads + h) * p.b.width;
-    auto key_at = [&](int w) -> uint64_t {   // 0: not to be taken
-        if (w >= have || kv_page(p.b, p.c, b, w) < 0) return 0;
-        if (w < p.first || w >= have - p.last) return ~0ull;
-        return score_key(score[w]);
+    auto key_of = [&](int w, int page, double v) -> uint64_t {   // 0: not to be taken
+        return w >= have || page < 0 ? 0 : w < p.first || w >= have - p.last ? ~0ull : score_key(v);
+    };
+    auto key_at = [&](int w) {
+        const int at = min(w, have - 1);
+        return key_of(w, kv_page(p.b, p.c, b, at), score[at]);
     };
     const int turns = (have + kThreads - 1) / kThreads;
     uint64_t held[HELD ? kHeld : 1];
-    if (HELD)
+    if (HELD && have > 0) {   // (all loads before their uses)
+        int page[kHeld];
+        double v[kHeld];
 #pragma unroll
-        for (int j = 0; j < kHeld; ++j) held[j] = j < turns ? key_at(tid + j * kThreads) : 0;
+        for (int j = 0; j < kHeld; ++j) {
+            const int at = min(tid + j * kThreads, have - 1);
+            page[j] = kv_page(p.b, p.c, b, at), v[j] = score[at];
+        }
+#pragma unroll
+        for (int j = 0; j < kHeld; ++j) held[j] = key_of(tid + j * kThreads, page[j], v[j]);
+    }
     auto each = [&](auto f) {
         if (HELD) {
 #pragma unroll
