@@ -36,7 +36,7 @@ struct KvAppendArgs {
     KvCacheArgs c;
     KvBatchArgs b;
     KvUnits units;
-    int64_t page_units;   // pages of all sequences that the call may touch, times the heads
+    uint32_t page_units;  // pages of all sequences that the call may touch, times the heads
     int page_groups;      // workgroups that store pages; the others prepare queries
     const void* key;
     const void* value;
@@ -205,15 +205,15 @@ __device__ __forceinline__ void prepare_query(const KvAppendArgs& p, int64_t tok
 }
 
 template <int D, int DTYPE, bool PREP>
-__device__ __forceinline__ void store_page(const KvAppendArgs& p, int64_t unit, uint32_t* vt, float* part, uint32_t* top)
+__device__ __forceinline__ void store_page(const KvAppendArgs& p, uint32_t unit, uint32_t* vt, float* part, uint32_t* top)
 {
     constexpr int CH = D / 8;               // chunks of a row: one lane each
     constexpr int P = kPage * CH / kThreads;   // consecutive tokens of a thread: 2, 4, 8
     constexpr int kRow = 17;                // dwords of a v row in LDS (16 and one to spread the banks)
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int h = (int)(unit % p.c.heads);
-    int64_t at;
-    const int b = kv_locate(p.b, p.units, unit / p.c.heads, at);
+    const int h = (int)(unit % (uint32_t)p.c.heads);
+    uint32_t at;
+    const int b = kv_locate(p.b, p.units, unit / (uint32_t)p.c.heads, at);
     if (b == p.b.batch) return;   // behind the last sequence
     const KvSequence s = kv_sequence(p.b, b);
     const int64_t w64 = max(s.first, (int64_t)0) / kPage + at;
@@ -373,7 +373,7 @@ __global__ __launch_bounds__(kThreads) void k_kv_append(KvAppendArgs p)
     __shared__ float part[4 * D];
     __shared__ uint32_t top[8];
     if ((int)blockIdx.x < p.page_groups) {
-        for (int64_t u = blockIdx.x; u < p.page_units; u += p.page_groups) {
+        for (uint32_t u = blockIdx.x; u < p.page_units; u += p.page_groups) {
             store_page<D, DTYPE, PREP>(p, u, vt, part, top);
             __syncthreads();   // before the next page's values overwrite LDS
         }
@@ -409,9 +409,11 @@ int append_arguments(const char* what, const vdn_fp8_kv_cache* cache, const vdn_
         return set_error(VDN_FP8_EINVAL, "%s: need ldk, ldv multiples of 8 and >= heads * head_dim", what);
     if (!aligned(key, 16) || !aligned(value, 16)) return set_error(VDN_FP8_EINVAL, "%s: key and value must be 16-byte aligned", what);
     // n tokens touch at most floor(n / 64) + 2 pages; none where they start at one's first token and end with it
-    const int64_t n = p.b.q_start ? p.b.tokens : p.b.tokens / p.b.batch;
-    p.units = KvUnits{kPage, (n + kPage - 2) / kPage + 1, 1, 2};
-    p.page_units = kv_unit_count(p.b, p.units) * p.c.heads;
+    const int64_t n = p.b.q_start ? p.b.tokens : p.b.each;
+    p.units = KvUnits{kPage, (uint32_t)((n + kPage - 2) / kPage + 1), 1, 2};
+    const int64_t units = kv_unit_count(p.b, p.units) * p.c.heads;
+    if (units >= INT32_MAX) return set_error(VDN_FP8_EINVAL, "%s: %lld pages and heads, 2^31 at most", what, (long long)units);
+    p.page_units = (uint32_t)units;
     p.page_groups = (int)(p.page_units < kMostGroups ? p.page_units : kMostGroups);
     p.key = key, p.value = value, p.ldk = ldk, p.ldv = ldv;
     return VDN_FP8_OK;
@@ -447,7 +449,8 @@ int kv_arguments(const char* what, const vdn_fp8_kv_cache* c, const vdn_fp8_kv_b
     cache = KvCacheArgs{(uint8_t*)c->k, (uint8_t*)c->v, (uint8_t*)c->k_scale, (uint8_t*)c->v_scale, (uint16_t*)c->k_mean,
                         c->pages, (int)c->heads, (int)c->head_dim};
     // (without pages every table entry is outside the pool: a table of no columns says the same)
-    batch = KvBatchArgs{b->page_table, b->ldtable, c->pages > 0 ? (int)b->max_pages : 0, b->lengths, b->q_start, (int)b->batch, b->tokens};
+    batch = KvBatchArgs{b->page_table, b->ldtable, c->pages > 0 ? (int)b->max_pages : 0, b->lengths, b->q_start, (int)b->batch, b->tokens,
+                        b->batch > 0 ? (int)(b->tokens / b->batch) : 0};
     return VDN_FP8_OK;
 }
 

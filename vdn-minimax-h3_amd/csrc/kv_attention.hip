@@ -554,14 +554,14 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_kv_attn_rows(KvAttnAr
     item /= p.splits;
     const uint32_t units = p.items / p.splits / p.c.heads;
     const int h = __builtin_amdgcn_readfirstlane((int)(item / units));
-    int64_t at64;
+    uint32_t at64;
     // (the last units of a sequence first: with a causal mask they are the longest)
     const int b = __builtin_amdgcn_readfirstlane(kv_locate(p.b, p.units, units - 1 - item % units, at64));
     if (b == p.b.batch) {   // behind the last sequence
         if (split == 0) {
             const int64_t end = min(max((int64_t)p.b.q_start[b], (int64_t)0), p.b.tokens);
             const int64_t each = max(kRows / p.group, 1);   // tokens; as many units as kv_unit_count leaves take turns
-            for (int64_t t = end + at64 * each; t < p.b.tokens; t += each * (int64_t)(units - kv_first_unit(p.b, p.units, b)))
+            for (int64_t t = end + (int64_t)at64 * each; t < p.b.tokens; t += each * (int64_t)(units - kv_first_unit(p.b, p.units, b)))
                 clear_rows(p, t, min(t + each, p.b.tokens), h);
         }
         return;
@@ -580,7 +580,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_kv_attn_rows(KvAttnAr
     if (p.blocks) {
         // the query block's number, as p.listed counts them
         const int64_t block = r0 / (p.query_block * p.group);
-        const int64_t unit = p.b.q_start ? kv_first_unit(p.b, p.listed, b) + block : (int64_t)b * p.listed.each + block;
+        const int64_t unit = (p.b.q_start ? (int64_t)kv_first_unit(p.b, p.listed, b) : (int64_t)b * p.listed.each) + block;
         list = p.blocks + (unit * p.c.heads + h) * p.top;
         lo = 0, hi = p.b.width > 0 ? p.top : 0;   // (no pages, no list to look at)
     } else {
@@ -775,10 +775,10 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_kv_attn_step(KvAttnAr
     int b = (int)unit;
     if (p.blocks) {   // a unit is a token
         if (p.b.q_start) {
-            int64_t none;
+            uint32_t none;
             b = kv_locate(p.b, KvUnits{1, 1, 1, 0}, unit, none);
         } else {
-            b = (int)(unit / (uint32_t)(p.b.tokens / p.b.batch));
+            b = (int)(unit / (uint32_t)p.b.each);
         }
     }
     b = __builtin_amdgcn_readfirstlane(b);
@@ -972,7 +972,7 @@ Plan make_plan(KvAttnArgs& p, int64_t max_query, int cus)
         groups = (p.blocks ? p.b.tokens : (int64_t)p.b.batch + (p.b.q_start ? 1 : 0)) * p.c.heads * plan.column_tiles;
     } else {
         plan.column_tiles = 1;
-        p.units = KvUnits{kRows, (n * p.group + kRows - 1) / kRows, p.group, 1};
+        p.units = KvUnits{kRows, (uint32_t)((n * p.group + kRows - 1) / kRows), p.group, 1};
         groups = (kv_unit_count(p.b, p.units) + (p.b.q_start ? 1 : 0)) * p.c.heads;
     }
     // Splits where the workgroups alone leave compute units idle: enough for four workgroups (steps) or two
@@ -1038,7 +1038,7 @@ int attn_arguments(const vdn_fp8_kv_cache* cache, const vdn_fp8_kv_batch* batch,
                              "(got %lld with groups of %d)", kRows, (long long)query_block, p.group);
         p.top = (int)top, p.query_block = (int)query_block;
         const int64_t n = p.b.batch > 0 ? p.b.tokens / p.b.batch : 0;
-        p.listed = KvUnits{query_block, (n + query_block - 1) / query_block, 1, query_block == 1 ? 0 : 1};
+        p.listed = KvUnits{(uint32_t)query_block, (uint32_t)((n + query_block - 1) / query_block), 1, query_block == 1 ? 0 : 1};
         p.blocks = (const int32_t*)(uintptr_t)4;   // replaced by the call
     }
     if (p.b.tokens * q_heads >= ((int64_t)1 << 30))

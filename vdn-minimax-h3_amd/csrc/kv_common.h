@@ -31,7 +31,8 @@ struct KvBatchArgs {
     const int32_t* lengths;    // [batch], the call's tokens included
     const int32_t* q_start;    // [batch + 1] or NULL: tokens / batch each
     int batch;
-    int64_t tokens;
+    int64_t tokens;            // < 2^31
+    int each;                  // tokens of every sequence, where q_start is NULL
 };
 
 // Sequence b of the batch: its rows [start, start + n) of the call (clamped into it), the position
@@ -51,8 +52,8 @@ __device__ __forceinline__ KvSequence kv_sequence(const KvBatchArgs& p, int b)
         s.start = lo;
         s.n = (int)(hi - lo);
     } else {
-        s.n = (int)(p.tokens / p.batch);
-        s.start = (int64_t)b * s.n;
+        s.n = p.each;
+        s.start = (int64_t)b * p.each;
     }
     const int64_t length = max((int64_t)p.lengths[b], (int64_t)0);
     s.first = length - s.n;
@@ -65,25 +66,26 @@ __device__ __forceinline__ KvSequence kv_sequence(const KvBatchArgs& p, int b)
 // sequence b's begin at floor(mult start / size) + more b: n tokens take at most
 // floor(mult n / size) + 1 units of rows (more = 1), or that many + 1 where the rows begin inside a
 // unit, as the pages of a cache do (more = 2), so they never reach the next sequence's, and all fit
-// mult tokens / size + more batch. Without q_start every sequence has `each` units.
+// mult tokens / size + more batch. Without q_start every sequence has `each` units. The host keeps
+// tokens * mult and the units below 2^31.
 struct KvUnits {
-    int64_t size, each;
+    uint32_t size, each;
     int mult, more;
 };
 
-__device__ __forceinline__ int64_t kv_first_unit(const KvBatchArgs& p, const KvUnits& u, int b)
+__device__ __forceinline__ uint32_t kv_first_unit(const KvBatchArgs& p, const KvUnits& u, int b)
 {
-    return min(max((int64_t)p.q_start[b], (int64_t)0), p.tokens) * u.mult / u.size + (int64_t)u.more * b;
+    return (uint32_t)(min(max(p.q_start[b], 0), (int)p.tokens) * u.mult) / u.size + (uint32_t)(u.more * b);
 }
 
 // The sequence that a unit belongs to, and its number `at` within it; with q_start, the batch's
 // size stands for the rows behind the last sequence.
-__device__ __forceinline__ int kv_locate(const KvBatchArgs& p, const KvUnits& u, int64_t unit, int64_t& at)
+__device__ __forceinline__ int kv_locate(const KvBatchArgs& p, const KvUnits& u, uint32_t unit, uint32_t& at)
 {
     if (!p.q_start) {
-        const int b = (int)(unit / u.each);
-        at = unit - (int64_t)b * u.each;
-        return b;
+        const uint32_t b = unit / u.each;
+        at = unit - b * u.each;
+        return (int)b;
     }
     int lo = 0, hi = p.batch;   // the last sequence whose first unit is not behind this one
     while (lo < hi) {
@@ -97,7 +99,7 @@ __device__ __forceinline__ int kv_locate(const KvBatchArgs& p, const KvUnits& u,
 
 inline int64_t kv_unit_count(const KvBatchArgs& p, const KvUnits& u)
 {
-    return p.q_start ? p.tokens * u.mult / u.size + (int64_t)u.more * p.batch : u.each * p.batch;
+    return p.q_start ? p.tokens * u.mult / u.size + (int64_t)u.more * p.batch : (int64_t)u.each * p.batch;
 }
 
 // The pool page of page w of sequence b, -1 where the table's entry is outside the pool.
@@ -105,15 +107,6 @@ __device__ __forceinline__ int kv_page(const KvBatchArgs& p, const KvCacheArgs& 
 {
     const int page = p.table[(int64_t)b * p.ldtable + w];
     return page >= 0 && page < c.pages ? page : -1;
-}
-
-// One byte of an array by a load of the aligned dword around it (uniform: a scalar load; the
-// dword lies in the byte's own memory page).
-__device__ __forceinline__ int scalar_byte(const uint8_t* a, int64_t i)
-{
-    const uint64_t at = (uint64_t)a + (uint64_t)i;
-    const uint32_t w = *reinterpret_cast<const uint32_t*>(at & ~(uint64_t)3);
-    return (int)((w >> (8 * (at & 3))) & 0xffu);
 }
 
 // Host: the checks that every entry point makes, and the two argument structs. Returns a status.

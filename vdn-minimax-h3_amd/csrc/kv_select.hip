@@ -39,6 +39,7 @@ struct KvSelectArgs {
     int64_t ldq;
     int group, causal, query_block;
     int top, first, last;
+    int row_turns;       // workgroups of k_kv_scores that share the blocks of a sequence
     int32_t* blocks;     // [rows, heads, top]
     double* score;       // [rows, heads, width]
     float* sum;          // [rows, heads, d]
@@ -47,11 +48,11 @@ struct KvSelectArgs {
 // Row `row` of the list: its sequence, the tokens [from, to) of it that make the block. False: none.
 __device__ __forceinline__ bool block_of(const KvSelectArgs& p, int64_t row, int& b, KvSequence& s, int& from, int& to)
 {
-    int64_t at;
-    b = kv_locate(p.b, p.listed, row, at);
+    uint32_t at;
+    b = kv_locate(p.b, p.listed, (uint32_t)row, at);
     if (b == p.b.batch) return false;
     s = kv_sequence(p.b, b);
-    if (at * p.query_block >= s.n) return false;
+    if ((int64_t)at * p.query_block >= s.n) return false;
     from = (int)at * p.query_block;
     to = min(from + p.query_block, s.n);
     return true;
@@ -109,7 +110,7 @@ __global__ __launch_bounds__(kThreads) void k_kv_scores(KvSelectArgs p)
 {
     constexpr int E = D / 4;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int b = blockIdx.z, h = blockIdx.y;
+    const int b = blockIdx.z / p.row_turns, h = blockIdx.y;
     const KvSequence s = kv_sequence(p.b, b);
     const int have = (s.length + kPage - 1) / kPage;
     const int w0 = (blockIdx.x * 4 + wave) * 16;
@@ -124,8 +125,8 @@ __global__ __launch_bounds__(kThreads) void k_kv_scores(KvSelectArgs p)
         mean[4 * i] = v.x, mean[4 * i + 1] = v.y, mean[4 * i + 2] = v.z, mean[4 * i + 3] = v.w;
     }
     const int blocks = (s.n + p.query_block - 1) / p.query_block;
-    const int64_t row0 = p.b.q_start ? kv_first_unit(p.b, p.listed, b) : (int64_t)b * p.listed.each;
-    for (int r0 = 0; r0 < blocks; r0 += 16) {
+    const int64_t row0 = p.b.q_start ? (int64_t)kv_first_unit(p.b, p.listed, b) : (int64_t)b * p.listed.each;
+    for (int r0 = 16 * (blockIdx.z % p.row_turns); r0 < blocks; r0 += 16 * p.row_turns) {
         const int r = min(r0 + lane % 16, blocks - 1);
         const float4* const src = reinterpret_cast<const float4*>(p.sum + ((row0 + r) * p.c.heads + h) * D + g * E);
         f64x4_t acc = {0.0, 0.0, 0.0, 0.0};
@@ -375,11 +376,11 @@ int select_arguments(const vdn_fp8_kv_cache* cache, const vdn_fp8_kv_batch* batc
     if (p.b.batch > 65535) return set_error(VDN_FP8_EINVAL, "kv_select: batch above 65535");
     p.query_block = (int)query_block;
     const int64_t n = p.b.batch > 0 ? p.b.tokens / p.b.batch : 0;
-    p.listed = KvUnits{query_block, (n + query_block - 1) / query_block, 1, query_block == 1 ? 0 : 1};
+    p.listed = KvUnits{(uint32_t)query_block, (uint32_t)((n + query_block - 1) / query_block), 1, query_block == 1 ? 0 : 1};
     p.rows = p.b.tokens == 0 ? 0 : kv_unit_count(p.b, p.listed);
     if (p.rows * p.c.heads >= (1 << 24)) return set_error(VDN_FP8_EINVAL, "kv_select: %lld blocks of queries and heads, 2^24 at most", (long long)(p.rows * p.c.heads));
-    if ((p.b.width + 63ll) / 64 * p.c.heads * p.b.batch >= (1 << 24))
-        return set_error(VDN_FP8_EINVAL, "kv_select: 2^30 pages and heads of the page table at most");
+    if ((p.b.width + 63ll) / 64 * p.c.heads * p.b.batch >= (1 << 21))
+        return set_error(VDN_FP8_EINVAL, "kv_select: 2^27 pages and heads of the page table at most");
     bytes = p.rows * p.c.heads * (8 * (int64_t)p.b.width + 4 * p.c.d);
     return VDN_FP8_OK;
 }
@@ -439,7 +440,10 @@ extern "C" int vdn_fp8_kv_select(const vdn_fp8_kv_cache* cache, const vdn_fp8_kv
         else hipLaunchKernelGGL((k_kv_query_sum<false>), per_row, block, 0, stream, p);
         int launched = check_launch("kv_select query sum");
         if (launched != VDN_FP8_OK) return launched;
-        const dim3 grid((unsigned)((p.b.width + 63) / 64), (unsigned)p.c.heads, (unsigned)p.b.batch);
+        const int64_t tiles = ((p.b.q_start ? p.b.tokens / query_block : (int64_t)p.listed.each) + 15) / 16, most = 65535 / p.b.batch;
+        p.row_turns = (int)(tiles < 1 ? 1 : tiles < 8 ? tiles : 8);
+        if (p.row_turns > most) p.row_turns = (int)most;
+        const dim3 grid((unsigned)((p.b.width + 63) / 64), (unsigned)p.c.heads, (unsigned)(p.b.batch * p.row_turns));
         switch (p.c.d) {
             case 64: hipLaunchKernelGGL((k_kv_scores<64>), grid, block, 0, stream, p); break;
             case 128: hipLaunchKernelGGL((k_kv_scores<128>), grid, block, 0, stream, p); break;
