@@ -115,11 +115,26 @@ __device__ __forceinline__ void decode16(uint4 w, f16x8_t o[2])
     }
 }
 
-// The fp8 terms of 32 elements of a query row (row: at its first element of these, NULL: zeros), and the
-// exponent e that they are scaled by: TERMS values whose sum is x 2^-e, term t times 2^(5 t - 1) (t > 0).
-// Every lane of a row passes all elements' largest magnitude through `join`.
+// 32 elements of a query row for each step of the inner dimension, as they are (row[s] NULL: zeros).
+template <int STEPS>
+struct RawQuery {
+    uint4 v[STEPS][4];
+    __device__ __forceinline__ void load(const uint16_t* const (&row)[STEPS])
+    {
+#pragma unroll
+        for (int s = 0; s < STEPS; ++s)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                v[s][i] = make_uint4(0, 0, 0, 0);
+                if (row[s]) v[s][i] = *reinterpret_cast<const uint4*>(row[s] + 8 * i);
+            }
+    }
+};
+
+// Their fp8 terms, and the exponent e that they are scaled by: TERMS values whose sum is x 2^-e, term t
+// times 2^(5 t - 1) (t > 0). Every lane of a row passes its largest magnitude through `join`.
 template <bool F16, int STEPS, int TERMS, typename Join>
-__device__ __forceinline__ int split_query(const uint16_t* const (&row)[STEPS], Join join, i32x8_t (&q)[TERMS][STEPS])
+__device__ __forceinline__ int split_query(const RawQuery<STEPS>& raw, Join join, i32x8_t (&q)[TERMS][STEPS])
 {
     float x[STEPS][32];
     uint32_t top = 0;
@@ -127,8 +142,7 @@ __device__ __forceinline__ int split_query(const uint16_t* const (&row)[STEPS], 
     for (int s = 0; s < STEPS; ++s)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            uint4 v = make_uint4(0, 0, 0, 0);
-            if (row[s]) v = *reinterpret_cast<const uint4*>(row[s] + 8 * i);
+            const uint4 v = raw.v[s][i];
             const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
@@ -186,11 +200,15 @@ __device__ __forceinline__ void look_up(const KvAttnArgs& p, int b, int h, int l
 {
     const int i = i0 + (int)threadIdx.x;
     if (threadIdx.x < kInfo && i < hi) {
+        // (no load under a condition on another; an entry outside the sequence is read at 0 and passed over)
         PageInfo a;
+        const int have = (length + kPage - 1) / kPage;
         a.w = list ? list[i] : i;
-        a.page = a.w >= 0 && a.w < (length + kPage - 1) / kPage ? kv_page(p.b, p.c, b, a.w) : -1;
+        const bool inside = a.w >= 0 && a.w < have;
+        a.page = kv_page(p.b, p.c, b, inside ? a.w : 0);
         const int64_t ph = (int64_t)max(a.page, 0) * p.c.heads + h;
         a.ek = p.c.k_scale[ph] - 127, a.ev = p.c.v_scale[ph] - 127;
+        if (!inside) a.page = -1;
         info[threadIdx.x] = a;
     }
 }
@@ -249,16 +267,23 @@ struct WaveRows {
     float m, l, c;     // running maximum and sum (of this half's keys), factor of the raw scores
     int limit;         // keys below it are visible to the row
 
-    __device__ __forceinline__ void load(const uint16_t* row, int g, float scale)
+    __device__ __forceinline__ static void read(RawQuery<kSteps>& raw, const uint16_t* row, int g)
     {
         const uint16_t* at[kSteps];
 #pragma unroll
         for (int s = 0; s < kSteps; ++s) at[s] = row ? row + 64 * s + 32 * g : nullptr;
-        const int e = split_query<F16>(at, [](uint32_t v) {
+        raw.load(at);
+    }
+    __device__ __forceinline__ void start(const RawQuery<kSteps>& raw, float scale)
+    {
+        const int e = split_query<F16>(raw, [](uint32_t v) {
             const auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
             return max((uint32_t)r[0], (uint32_t)r[1]);
         }, q);
         c = scale * exponent_f32(e);
+    }
+    __device__ __forceinline__ void clear()
+    {
         m = kNoMax, l = 0.0f;
 #pragma unroll
         for (int t = 0; t < kTiles; ++t)
@@ -331,15 +356,23 @@ struct WaveRows {
     // Adds the weighted values of a page: value(kt, h, t) gives one element's values of the eight tokens from
     // 32 kt + 16 g + 8 h on.
     template <typename Value>
-    __device__ __forceinline__ void add_values(Value value, const f16x8_t w[2][2])
+    __device__ __forceinline__ void add_values(const f16x8_t (&v0)[2][kTiles], Value value, const f16x8_t w[2][2])
     {
+        f16x8_t v1[2][kTiles];
 #pragma unroll
-        for (int kt = 0; kt < 2; ++kt)
+        for (int h = 0; h < 2; ++h)
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
+            for (int t = 0; t < kTiles; ++t) {
+                acc[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v0[h][t], w[0][h], acc[t], 0, 0, 0);
+                v1[h][t] = value(1, h, t);
+                __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+                __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+            }
 #pragma unroll
-                for (int t = 0; t < kTiles; ++t)
-                    acc[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(value(kt, h, t), w[kt][h], acc[t], 0, 0, 0);
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int t = 0; t < kTiles; ++t)
+                acc[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v1[h][t], w[1][h], acc[t], 0, 0, 0);
     }
 
     // A page in which some rows see NaN values that others do not (its NaN were stored as zeros): the rows
@@ -382,18 +415,25 @@ struct StepRows {
     int limit[NT];
 
     // (a head of 64 fills half of the instruction's 128: the upper lanes repeat the keys against zeros)
-    __device__ __forceinline__ void load(int n, const uint16_t* row, int g, float scale)
+    __device__ __forceinline__ static void read(RawQuery<kSteps>& raw, const uint16_t* row, int g)
     {
         const uint16_t* at[kSteps];
 #pragma unroll
         for (int s = 0; s < kSteps; ++s) at[s] = row && (D > 64 || g < 2) ? row + 128 * s + 32 * g : nullptr;
-        const int e = split_query<F16>(at, [](uint32_t v) {
+        raw.load(at);
+    }
+    __device__ __forceinline__ void start(int n, const RawQuery<kSteps>& raw, float scale)
+    {
+        const int e = split_query<F16>(raw, [](uint32_t v) {
             const auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
             v = max((uint32_t)r[0], (uint32_t)r[1]);
             const auto s = __builtin_amdgcn_permlane16_swap(v, v, false, false);
             return max((uint32_t)s[0], (uint32_t)s[1]);
         }, q[n]);
         c[n] = scale * exponent_f32(e);
+    }
+    __device__ __forceinline__ void clear(int n)
+    {
         m[n] = kNoMax, l[n] = 0.0f;
 #pragma unroll
         for (int t = 0; t < kTiles; ++t) acc[n][t] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
@@ -599,7 +639,8 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_kv_attn_rows(KvAttnAr
     const bool valid = row < rows;
     const int64_t token = s.start + (uint32_t)row / (uint32_t)p.group;
     const int head = h * p.group + (uint32_t)row % (uint32_t)p.group;
-    rowset.load(valid ? p.q + token * p.ldq + (int64_t)head * D : nullptr, g, p.scale);
+    RawQuery<WaveRows<D, F16>::kSteps> raw;   // (on its way while the pages are looked up)
+    rowset.read(raw, valid ? p.q + token * p.ldq + (int64_t)head * D : nullptr, g);
     rowset.limit = valid ? limit_of(row) : 0;
     const int least = limit_of(min(w0, last)), most = limit_of(min(w0 + kWaveRows - 1, last));
 
@@ -658,12 +699,19 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_kv_attn_rows(KvAttnAr
     const int sw = (r >> 1) & 7;
     const int k_line = D == 64 ? (r >> 1) * 128 : r * 128, k_chunk = D == 64 ? (r & 1) * 4 + 2 * g : 2 * g;
 
+    look_up(p, b, h, s.length, list, lo, hi, info);
+    if (tid < 2) nan_page[tid] = -1;
+    __syncthreads();
+    rowset.start(raw, p.scale);
+    rowset.clear();
     for (int first = lo; first < hi; first += kInfo) {
         const int count = min(hi - first, kInfo);
-        __syncthreads();   // (all reads of the pages before are done)
-        look_up(p, b, h, s.length, list, first, hi, info);
-        if (tid < 2) nan_page[tid] = -1;
-        __syncthreads();
+        if (first > lo) {
+            __syncthreads();   // (all reads of the pages before are done)
+            look_up(p, b, h, s.length, list, first, hi, info);
+            if (tid < 2) nan_page[tid] = -1;
+            __syncthreads();
+        }
         PageInfo now = info_at(info, 0), next = now;
         copy_k(now, 0);
         load_v(now);
@@ -708,17 +756,24 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_kv_attn_rows(KvAttnAr
                 auto value = [&](int kt, int half, int t) {
                     return *reinterpret_cast<const f16x8_t*>(vb + t * 4096 + (((4 * kt + 2 * g + half) ^ sw) * 16));
                 };
-                f32x16_t sc[2];
-                f16x8_t w[2][2];
-                rowset.scores(key, sc);
-                const bool masked = key0 + kPage > least;
-                if (masked) rowset.mask(sc, key0, g);
-                rowset.weights(sc, now.ek, now.ev, w);
                 if (key0 + kPage > least_all && nan_page[i & 1] == first + i) {   // (also where this wave sees the whole page)
                     const uint8_t* const src = p.c.v + ((int64_t)now.page * p.c.heads + h) * kPageBytes + row_key(r) * kPage + 16 * g;
                     rowset.add_nan([&](int kt, int t) { return *reinterpret_cast<const uint4*>(src + t * 32 * kPage + 32 * kt); }, key0, s.length, g);
                 }
-                rowset.add_values(value, w);
+                f32x16_t sc[2];
+                f16x8_t w[2][2];
+                rowset.scores(key, sc);
+                const bool masked = key0 + kPage > least;
+                f16x8_t v0[2][D / 32];
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int hf = 0; hf < 2; ++hf)
+#pragma unroll
+                    for (int tt = 0; tt < D / 32; ++tt) v0[hf][tt] = value(0, hf, tt);
+                __builtin_amdgcn_sched_barrier(0);
+                if (masked) rowset.mask(sc, key0, g);
+                rowset.weights(sc, now.ek, now.ev, w);
+                rowset.add_values(v0, value, w);
             }
             now = next, next = after;
             buffer = buffer == 2 ? 0 : buffer + 1;
@@ -807,11 +862,13 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_kv_attn_step(KvAttnAr
     }
 
     StepRows<D, F16, NT> rowset;
+    RawQuery<kSteps> raw[NT];   // (on their way while the pages are looked up)
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
         const int row = tile * kStepRows + 16 * n + r, own = at + row / p.group;
         const bool valid = row < rows;
-        rowset.load(n, valid ? p.q + (s.start + own) * p.ldq + (int64_t)(h * p.group + row % p.group) * D : nullptr, g, p.scale);
+        rowset.read(raw[n], valid ? p.q + (s.start + own) * p.ldq + (int64_t)(h * p.group + row % p.group) * D : nullptr, g);
+        rowset.clear(n);
         rowset.limit[n] = valid ? limit_of(own) : 0;
     }
     const int least = limit_of(first_token), most = limit_of(last_token);
@@ -832,11 +889,17 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_kv_attn_step(KvAttnAr
 #pragma unroll
         for (int t = 0; t < kTiles; ++t) vr[t] = *reinterpret_cast<const uint4*>(src + from_v + t * 16 * kPage);
     };
+    look_up(p, b, h, s.length, list, lo, hi, info);
+    __syncthreads();
+#pragma unroll
+    for (int n = 0; n < NT; ++n) rowset.start(n, raw[n], p.scale);
     for (int first = lo; first < hi; first += kInfo) {
         const int count = min(hi - first, kInfo);
-        __syncthreads();
-        look_up(p, b, h, s.length, list, first, hi, info);
-        __syncthreads();
+        if (first > lo) {
+            __syncthreads();
+            look_up(p, b, h, s.length, list, first, hi, info);
+            __syncthreads();
+        }
         PageInfo now{}, next{};
         int i = wave;
         if (i < count) {
@@ -933,12 +996,21 @@ __global__ __launch_bounds__(256) void k_kv_attn_join(KvAttnArgs p)
     float o[E];
 #pragma unroll
     for (int e = 0; e < E; ++e) o[e] = 0.0f;
-    for (int i = 0; i < p.splits; ++i) {
-        if (__shfl(own.y, i, 64) == 0.0f) continue;   // no keys there (uniform): its accumulators are not written
-        const float w = __shfl(f, i, 64);
-        const float* const src = p.part + (row * p.splits + i) * D + lane * E;
+    const float* const src = p.part + row * p.splits * D + lane * E;
+    for (int i0 = 0; i0 < p.splits; i0 += 8) {   // (eight splits' loads before their use)
+        float v[8][E];
 #pragma unroll
-        for (int e = 0; e < E; ++e) o[e] += w * src[e];
+        for (int i = 0; i < 8; ++i)
+#pragma unroll
+            for (int e = 0; e < E; ++e) v[i][e] = src[(int64_t)min(i0 + i, p.splits - 1) * D + e];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            // (a split without keys has not written its accumulators; lanes beyond the splits hold none)
+            const bool some = __shfl(own.y, (i0 + i) & 63, 64) != 0.0f && i0 + i < p.splits;
+            const float w = __shfl(f, (i0 + i) & 63, 64);
+#pragma unroll
+            for (int e = 0; e < E; ++e) o[e] += some ? w * v[i][e] : 0.0f;
+        }
     }
     const float inv = total == 0.0f ? 0.0f : 1.0f / total;
     uint16_t* const dst = p.out + row * D + lane * E;

@@ -59,51 +59,63 @@ class KvCache(NamedTuple):
 def _cache(cache, device):
     """The C struct of a cache, checked."""
     k, v, ks, vs, mean = cache
-    if k.dim() != 4 or k.dtype != FP8_DTYPE or k.shape[2] != KV_PAGE:
-        raise ValueError(f"cache.k must be float8_e4m3fn [pages, heads, {KV_PAGE}, d] (got {k.dtype} {tuple(k.shape)})")
-    P, H, _, d = k.shape
+    shape = k.shape
+    if len(shape) != 4 or k.dtype != FP8_DTYPE or shape[2] != KV_PAGE:
+        raise ValueError(f"cache.k must be float8_e4m3fn [pages, heads, {KV_PAGE}, d] (got {k.dtype} {tuple(shape)})")
+    P, H, _, d = shape
     if v.shape != (P, H, d, KV_PAGE) or v.dtype != FP8_DTYPE:
         raise ValueError(f"cache.v must be float8_e4m3fn [{P}, {H}, {d}, {KV_PAGE}] (got {v.dtype} {tuple(v.shape)})")
     if ks.shape != (P, H) or vs.shape != (P, H) or ks.dtype != SCALE_DTYPE or vs.dtype != SCALE_DTYPE:
         raise ValueError(f"cache.k_scale and v_scale must be float8_e8m0fnu [{P}, {H}]")
     if mean is not None and (mean.shape != (P, H, d) or mean.dtype != torch.bfloat16):
         raise ValueError(f"cache.k_mean must be bfloat16 [{P}, {H}, {d}]")
-    for t in cache:
-        if t is not None and (t.device != device or not t.is_contiguous()):
+    at = _index(device)
+    for t in (k, v, ks, vs, mean):
+        if t is not None and (t.get_device() != at or not t.is_contiguous()):
             raise ValueError(f"the cache's tensors must be contiguous, on {device}")
-    return _lib.KvCacheStruct(k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr(), _ptr(mean), P, H, d)
+    return _lib.KvCacheStruct(k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr(), None if mean is None else mean.data_ptr(), P, H, d)
+
+
+def _index(device):
+    """What get_device() gives for tensors on `device` (cheaper to compare than devices are)."""
+    return device.index if device.type == "cuda" else -1
 
 
 def _batch(page_table, lengths, q_start, tokens, pages, device):
     """The C struct of a batch, checked (and what it points to, to be kept until the launch)."""
-    if page_table.dim() != 2 or page_table.dtype != torch.int32 or (page_table.shape[1] > 1 and page_table.stride(1) != 1):
+    shape = page_table.shape
+    if len(shape) != 2 or page_table.dtype != torch.int32 or (shape[1] > 1 and page_table.stride(1) != 1):
         raise ValueError("page_table must be int32 [B, W] with unit column stride")
-    B, W = page_table.shape
+    B, W = shape
     if lengths.shape != (B,) or lengths.dtype != torch.int32 or not lengths.is_contiguous():
         raise ValueError(f"lengths must be a contiguous int32 [{B}] tensor")
     if q_start is not None and (q_start.shape != (B + 1,) or q_start.dtype != torch.int32 or not q_start.is_contiguous()):
         raise ValueError(f"q_start must be a contiguous int32 [{B + 1}] tensor")
-    if page_table.device != device or lengths.device != device or (q_start is not None and q_start.device != device):
+    at = _index(device)
+    if page_table.get_device() != at or lengths.get_device() != at or (q_start is not None and q_start.get_device() != at):
         raise ValueError(f"page_table, lengths and q_start must be on {device}")
     if tokens and not B:
         raise ValueError(f"{tokens} tokens of an empty batch")
     if q_start is None and B and tokens % B:
         raise ValueError(f"{tokens} tokens do not divide among {B} sequences: pass q_start")
     check_index_range(lengths, W * KV_PAGE + 1, "lengths")
-    check_index_range(q_start, tokens + 1, "q_start")
+    if q_start is not None:
+        check_index_range(q_start, tokens + 1, "q_start")
     ld = page_table.stride(0) if B > 1 else W
-    return _lib.KvBatchStruct(page_table.data_ptr(), ld, W, lengths.data_ptr(), _ptr(q_start), B, tokens)
+    return _lib.KvBatchStruct(page_table.data_ptr(), ld, W, lengths.data_ptr(), None if q_start is None else q_start.data_ptr(), B, tokens)
 
 
 def _rows(t, heads, d, name, dtypes):
     """[T, heads, d] with contiguous heads on the GPU, 16-byte aligned rows; a copy where it is not."""
     if not t.is_cuda:
         raise ValueError(f"the cache's kernels run on the GPU; {name} is a CPU tensor")
-    if t.dim() != 3 or t.dtype not in dtypes or t.shape[2] != d or (heads is not None and t.shape[1] != heads):
+    shape = t.shape
+    if len(shape) != 3 or t.dtype not in dtypes or shape[2] != d or (heads is not None and shape[1] != heads):
         names = ", ".join(str(x).replace("torch.", "") for x in dtypes)
         raise ValueError(f"{name} must be a {names} [T, {'heads' if heads is None else heads}, {d}] tensor "
                          f"(got {t.dtype} {tuple(t.shape)})")
-    if t.stride(2) != 1 or t.stride(1) != d or t.stride(0) % 8 or t.stride(0) < t.shape[1] * d or t.data_ptr() % 16:
+    token, head, unit = t.stride()
+    if unit != 1 or head != d or token % 8 or token < shape[1] * d or t.data_ptr() % 16:
         t = t.clone(memory_format=torch.contiguous_format)
     return t
 
@@ -171,7 +183,8 @@ def qk_prep_append(query, key, value, norm_q, norm_k, cache, page_table, lengths
     if (cos is None) != (sin is None):
         raise ValueError("cos and sin go together")
     if cos is not None:
-        if cos.dim() != 2 or cos.device != dev or sin.dim() != 2 or sin.device != dev:
+        at = _index(dev)
+        if cos.dim() != 2 or cos.get_device() != at or sin.dim() != 2 or sin.get_device() != at:
             cos, sin = cos.detach().to(dev).reshape(-1, cos.shape[-1]), sin.detach().to(dev).reshape(-1, sin.shape[-1])
         if cos.shape != sin.shape or cos.shape[0] != T or cos.dtype != sin.dtype:
             raise ValueError(f"cos/sin must both be [T={T}, R] of one dtype (got {tuple(cos.shape)}, {tuple(sin.shape)})")
