@@ -15,10 +15,13 @@
 //
 // What bounds it: bytes, each key and value read once (16-byte loads) and each code written once.
 // One workgroup takes a page of one head, so that the page's maximum needs no second pass over
-// memory: the rows stay in registers between the maximum and the cast. A thread holds P = d / 32
-// consecutive tokens of one 8-element chunk; k is packed along the chunk, v along the tokens, so the
-// transposition is a matter of which values one conversion takes, and one pass through LDS makes
-// whole 16-byte stores of it.
+// memory: the rows stay in registers between the maximum and the cast. A thread holds two consecutive
+// tokens of one 8-element chunk, packed as they came (4 d threads a page; with four tokens and 256 threads
+// the registers left a compute unit 2.3 waves a SIMD: 67 us for 3120 tokens of 40 + 2 x 40 heads, 50 us now).
+// k is packed along the chunk, v along the tokens, so the transposition is a matter of which values one
+// conversion takes, and one pass through LDS makes whole 16-byte stores of it. Where pages alone fill the
+// part, a workgroup takes up to four heads of a page (1: 59 us): it reads the next head's rows while it
+// stores one, and keeps the tokens' rotations.
 #include <stdint.h>
 
 #include "kv_common.h"
@@ -28,16 +31,22 @@
 namespace vdn {
 namespace {
 
-constexpr int kThreads = 256;
+// Threads of a workgroup: two consecutive tokens of one chunk each.
+constexpr int threads_of(int d) { return 4 * d; }
 // Workgroups of a launch at most; each takes further units in steps of the grid.
 constexpr int64_t kMostGroups = 1 << 20;
+// Waves from which on the part is full (16 a compute unit), and heads of a unit at most.
+constexpr int64_t kFill = 4096;
+constexpr int kMostHeads = 4;
 
 struct KvAppendArgs {
     KvCacheArgs c;
     KvBatchArgs b;
     KvUnits units;
-    uint32_t page_units;  // pages of all sequences that the call may touch, times the heads
+    uint32_t page_units;  // pages of all sequences that the call may touch, times the heads' shares
     int page_groups;      // workgroups that store pages; the others prepare queries
+    int unit_heads;       // heads of a unit
+    int query_parts;      // waves that share a token's queries: all of a workgroup's or 1
     const void* key;
     const void* value;
     int64_t ldk, ldv;
@@ -55,19 +64,37 @@ struct KvAppendArgs {
     int R, cs_bf16;
 };
 
-// Eight elements of a row as binary32.
+// Eight elements of a row, as they are stored and as binary32.
 template <int DTYPE>
-__device__ __forceinline__ void load8(const void* base, int64_t i, float x[8])
-{
-    if (DTYPE == VDN_FP8_DTYPE_F32) {
-        const uint4* p = reinterpret_cast<const uint4*>(static_cast<const float*>(base) + i);
-        const uint4 lo = load_once(p), hi = load_once(p + 1);
-        const uint32_t w[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+struct Chunk {
+    static constexpr int kWords = DTYPE == VDN_FP8_DTYPE_F32 ? 2 : 1;
+    uint4 v[kWords];
+    __device__ __forceinline__ void load(const void* base, int64_t i)
+    {
+        const int size = DTYPE == VDN_FP8_DTYPE_F32 ? 4 : 2;
+        const uint4* const p = reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(base) + i * size);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = __uint_as_float(w[e]);
-    } else {
-        const uint4 v = load_once(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(base) + i));
-        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+        for (int j = 0; j < kWords; ++j) v[j] = load_once(p + j);
+    }
+    __device__ __forceinline__ void clear()
+    {
+#pragma unroll
+        for (int j = 0; j < kWords; ++j) v[j] = make_uint4(0, 0, 0, 0);
+    }
+    // (what is unpacked from it before and after is unpacked twice, and not kept in registers in between)
+    __device__ __forceinline__ void hide()
+    {
+#pragma unroll
+        for (int j = 0; j < kWords; ++j) asm volatile("" : "+v"(v[j].x), "+v"(v[j].y), "+v"(v[j].z), "+v"(v[j].w));
+    }
+    __device__ __forceinline__ void get(float x[8]) const
+    {
+        const uint32_t w[8] = {v[0].x, v[0].y, v[0].z, v[0].w, v[kWords - 1].x, v[kWords - 1].y, v[kWords - 1].z, v[kWords - 1].w};
+        if (DTYPE == VDN_FP8_DTYPE_F32) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] = __uint_as_float(w[e]);
+            return;
+        }
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             if (DTYPE == VDN_FP8_DTYPE_BF16) {
@@ -79,7 +106,7 @@ __device__ __forceinline__ void load8(const void* base, int64_t i, float x[8])
             }
         }
     }
-}
+};
 
 __device__ __forceinline__ float power_of_two(int e)   // e in [-126, 127]
 {
@@ -108,35 +135,37 @@ __device__ __forceinline__ uint32_t rescale4(uint32_t w, int delta)
                        __builtin_amdgcn_cvt_f32_fp8(w, 2) * f, __builtin_amdgcn_cvt_f32_fp8(w, 3) * f);
 }
 
-// What one lane of QK preparation keeps of its token: the rotation of its chunk.
+// The rotation of one chunk of a token, as the bf16 that its cosines and sines are rounded to.
 struct Rotation {
-    float cs[8], sn[8];
-};
-
-template <int D>
-__device__ __forceinline__ Rotation load_rotation(const KvAppendArgs& p, int64_t token, int i0, bool rot)
-{
-    Rotation r;
-    if (rot) {
-        const int64_t at = token * p.ldcs + i0;
-        uint4 c0, c1, s0, s1;
-        if (p.cs_bf16) {
-            c0 = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.cos) + at);
-            s0 = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.sin) + at);
-            c1 = s1 = make_uint4(0, 0, 0, 0);
-        } else {
-            const uint4* c = reinterpret_cast<const uint4*>(static_cast<const float*>(p.cos) + at);
-            const uint4* s = reinterpret_cast<const uint4*>(static_cast<const float*>(p.sin) + at);
-            c0 = c[0], c1 = c[1], s0 = s[0], s1 = s[1];
-        }
-        decode_table8(c0, c1, p.cs_bf16, r.cs);
-        decode_table8(s0, s1, p.cs_bf16, r.sn);
-    } else {
+    uint32_t cs[4], sn[4];
+    __device__ __forceinline__ void hide()
+    {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) r.cs[e] = 1.0f, r.sn[e] = 0.0f;
+        for (int j = 0; j < 4; ++j) asm volatile("" : "+v"(cs[j]), "+v"(sn[j]));
     }
-    return r;
-}
+    // (i0 < R: the chunk rotates; otherwise zeros that nothing uses)
+    __device__ __forceinline__ void load(const KvAppendArgs& p, int64_t token, int i0)
+    {
+        if (i0 >= p.R) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) cs[j] = sn[j] = 0;
+            return;
+        }
+        const int64_t at = token * p.ldcs + i0;
+        if (p.cs_bf16) {
+            const uint4 c = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.cos) + at);
+            const uint4 s = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.sin) + at);
+            cs[0] = c.x, cs[1] = c.y, cs[2] = c.z, cs[3] = c.w;
+            sn[0] = s.x, sn[1] = s.y, sn[2] = s.z, sn[3] = s.w;
+        } else {
+            const float4* const c = reinterpret_cast<const float4*>(static_cast<const float*>(p.cos) + at);
+            const float4* const s = reinterpret_cast<const float4*>(static_cast<const float*>(p.sin) + at);
+            const float4 c0 = c[0], c1 = c[1], s0 = s[0], s1 = s[1];
+            cs[0] = pack_bf16x2(c0.x, c0.y), cs[1] = pack_bf16x2(c0.z, c0.w), cs[2] = pack_bf16x2(c1.x, c1.y), cs[3] = pack_bf16x2(c1.z, c1.w);
+            sn[0] = pack_bf16x2(s0.x, s0.y), sn[1] = pack_bf16x2(s0.z, s0.w), sn[2] = pack_bf16x2(s1.x, s1.y), sn[3] = pack_bf16x2(s1.z, s1.w);
+        }
+    }
+};
 
 __device__ __forceinline__ void load_weight(const uint16_t* weight, int i0, float w[8])
 {
@@ -162,58 +191,60 @@ __device__ __forceinline__ void prepare8(const KvAppendArgs& p, const float x[8]
     const int partner = lane + (first ? half / 8 : -(half / 8));
     const float ss = head_sum_squares<G>(x);
     const float rstd = 1.0f / __builtin_sqrtf(ss / (float)D + eps);
-    float n[8];
+    float n[8], cs[8], sn[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) n[e] = (x[e] * rstd) * w[e];
-    rotate8<G>(n, r.cs, r.sn, p.R == D, rot, first, partner, lane, o);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        cs[2 * e] = bf16_lo(r.cs[e]), cs[2 * e + 1] = bf16_hi(r.cs[e]);
+        sn[2 * e] = bf16_lo(r.sn[e]), sn[2 * e + 1] = bf16_hi(r.sn[e]);
+    }
+    rotate8<G>(n, cs, sn, p.R == D, rot, first, partner, lane, o);
 }
 
-// The queries of one token: each wave takes every fourth sweep of 64 lanes over its heads, four
-// sweeps' loads before their arithmetic.
+// The queries of one token, or the part of them that is wave `part`'s of `parts`: every parts-th sweep of 64
+// lanes over its heads, four sweeps' loads before their arithmetic.
 template <int D>
-__device__ __forceinline__ void prepare_query(const KvAppendArgs& p, int64_t token)
+__device__ __forceinline__ void prepare_query(const KvAppendArgs& p, int64_t token, int part, int parts)
 {
     constexpr int G = D / 8, kSweeps = 4;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int i0 = 8 * (lane % G), chunks = p.q_heads * G;
+    const int lane = threadIdx.x & 63;
+    const int i0 = 8 * (lane % G), chunks = p.q_heads * G, step = 64 * parts;
     float w[8];
     load_weight(p.weight_q, i0, w);
-    const Rotation r = load_rotation<D>(p, token, i0, i0 < p.R);
-    for (int base = wave * 64; base < chunks; base += 4 * 64 * kSweeps) {
-        float x[kSweeps][8];
+    Rotation r;
+    r.load(p, token, i0);
+    for (int base = part * 64; base < chunks; base += step * kSweeps) {
+        Chunk<VDN_FP8_DTYPE_BF16> v[kSweeps];
+#pragma unroll
+        for (int s = 0; s < kSweeps; ++s) v[s].load(p.query, token * p.ldq + 8 * min(base + s * step + lane, chunks - 1));
 #pragma unroll
         for (int s = 0; s < kSweeps; ++s) {
-            const int q = base + s * 256 + lane;
-            if (q < chunks) load8<VDN_FP8_DTYPE_BF16>(p.query, token * p.ldq + 8 * q, x[s]);
-            else
-#pragma unroll
-                for (int e = 0; e < 8; ++e) x[s][e] = 0.0f;
-        }
-#pragma unroll
-        for (int s = 0; s < kSweeps; ++s) {
-            const int q = base + s * 256 + lane;
-            if (base + s * 256 >= chunks) break;   // (wave-uniform)
-            float o[8];
-            prepare8<D>(p, x[s], w, p.eps_q, r, lane, o);
-            if (q < chunks) {
-                const uint4 v = make_uint4(pack_bf16x2(o[0], o[1]), pack_bf16x2(o[2], o[3]), pack_bf16x2(o[4], o[5]),
-                                           pack_bf16x2(o[6], o[7]));
-                *reinterpret_cast<uint4*>(p.out + token * p.ldo + 8 * q) = v;
-            }
+            const int q = base + s * step + lane;
+            if (base + s * step >= chunks) break;   // (wave-uniform)
+            float x[8], o[8];
+            v[s].get(x);
+            prepare8<D>(p, x, w, p.eps_q, r, lane, o);
+            if (q < chunks)
+                *reinterpret_cast<uint4*>(p.out + token * p.ldo + 8 * q) =
+                    make_uint4(pack_bf16x2(o[0], o[1]), pack_bf16x2(o[2], o[3]), pack_bf16x2(o[4], o[5]), pack_bf16x2(o[6], o[7]));
         }
     }
 }
 
+// One page of p.unit_heads heads, one after the other: the rows of the next head are read while one is stored,
+// and the tokens' rotations are kept.
 template <int D, int DTYPE, bool PREP>
 __device__ __forceinline__ void store_page(const KvAppendArgs& p, uint32_t unit, uint32_t* vt, float* part, uint32_t* top)
 {
     constexpr int CH = D / 8;               // chunks of a row: one lane each
-    constexpr int P = kPage * CH / kThreads;   // consecutive tokens of a thread: 2, 4, 8
+    constexpr int P = 2, kThreads = threads_of(D), kWaves = kThreads / 64;
     constexpr int kRow = 17;                // dwords of a v row in LDS (16 and one to spread the banks)
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int h = (int)(unit % (uint32_t)p.c.heads);
+    const uint32_t turns = (uint32_t)(p.c.heads + p.unit_heads - 1) / (uint32_t)p.unit_heads;
+    const int h0 = (int)(unit % turns) * p.unit_heads, h_end = min(h0 + p.unit_heads, p.c.heads);
     uint32_t at;
-    const int b = kv_locate(p.b, p.units, unit / (uint32_t)p.c.heads, at);
+    const int b = kv_locate(p.b, p.units, unit / turns, at);
     if (b == p.b.batch) return;   // behind the last sequence
     const KvSequence s = kv_sequence(p.b, b);
     const int64_t w64 = max(s.first, (int64_t)0) / kPage + at;
@@ -221,70 +252,81 @@ __device__ __forceinline__ void store_page(const KvAppendArgs& p, uint32_t unit,
     const int w = (int)w64;
     const int lo = (int)max(s.first - w64 * kPage, (int64_t)0), hi = (int)min((int64_t)s.length - w64 * kPage, (int64_t)kPage);
     if (lo >= hi) return;
-    const int page = kv_page(p.b, p.c, b, w);
-    if (page < 0) return;
-    const int64_t ph = (int64_t)page * p.c.heads + h;
     const int64_t row0 = s.start + w64 * kPage - s.first;   // the call's row of the page's token 0 (may lie before the call)
 
     const int ch = tid % CH, i0 = 8 * ch, t0 = (tid / CH) * P;
-    float kx[P][8], vx[P][8];
-#pragma unroll
-    for (int i = 0; i < P; ++i) {
-        const int t = t0 + i;
-        if (t >= lo && t < hi) {
-            load8<DTYPE>(p.key, (row0 + t) * p.ldk + h * D + i0, kx[i]);
-            load8<DTYPE>(p.value, (row0 + t) * p.ldv + h * D + i0, vx[i]);
-        } else {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) kx[i][e] = vx[i][e] = 0.0f;
-        }
-    }
-    if (PREP) {
-        float w8[8];
-        load_weight(p.weight_k, i0, w8);
+    Chunk<DTYPE> kc[P], vc[P];
+    auto read = [&](int h) {
 #pragma unroll
         for (int i = 0; i < P; ++i) {
-            const int t = t0 + i;
-            const bool on = t >= lo && t < hi;
-            const Rotation r = load_rotation<D>(p, on ? row0 + t : 0, i0, on && i0 < p.R);
-            float o[8];
-            prepare8<D>(p, kx[i], w8, p.eps_k, r, lane, o);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) kx[i][e] = on ? round_bf16(o[e]) : 0.0f;   // the bf16 key that k_qk_prep stores
+            // (rows that are not the call's are read as the nearest that is, and passed over)
+            const int64_t row = row0 + min(max(t0 + i, lo), hi - 1);
+            kc[i].load(p.key, row * p.ldk + h * D + i0);
+            vc[i].load(p.value, row * p.ldv + h * D + i0);
         }
+    };
+    read(h0);
+    const int page = kv_page(p.b, p.c, b, w);
+    if (page < 0) return;
+    Rotation rot[PREP ? P : 1];
+    uint4 w4 = make_uint4(0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u);   // ones
+    if (PREP) {
+        if (p.weight_k) w4 = *reinterpret_cast<const uint4*>(p.weight_k + i0);
+#pragma unroll
+        for (int i = 0; i < P; ++i) rot[i].load(p, row0 + min(max(t0 + i, lo), hi - 1), i0);
     }
-
+    for (int h = h0; h < h_end; ++h) {
+    const int64_t ph = (int64_t)page * p.c.heads + h;
+    const int own_k = p.c.k_scale[ph] - 127, own_v = p.c.v_scale[ph] - 127;
+    // This head's rows as they are to be stored, still packed: prepared keys as bf16, zeros where the row
+    // is not the call's.
+    Chunk<DTYPE> ks[P], vs[P];
     uint32_t ak = 0, av = 0;
 #pragma unroll
-    for (int i = 0; i < P; ++i)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            ak = max(ak, finite_magnitude(kx[i][e]));
-            av = max(av, finite_magnitude(vx[i][e]));
+    for (int i = 0; i < P; ++i) {
+        const bool on = t0 + i >= lo && t0 + i < hi;
+        ks[i] = kc[i], vs[i] = vc[i];
+        float x[8];
+        if (PREP) {
+            float o[8], w8[8];
+            ks[i].get(x);
+            asm volatile("" : "+v"(w4.x), "+v"(w4.y), "+v"(w4.z), "+v"(w4.w));
+            w8[0] = bf16_lo(w4.x), w8[1] = bf16_hi(w4.x), w8[2] = bf16_lo(w4.y), w8[3] = bf16_hi(w4.y);
+            w8[4] = bf16_lo(w4.z), w8[5] = bf16_hi(w4.z), w8[6] = bf16_lo(w4.w), w8[7] = bf16_hi(w4.w);
+            rot[i].hide();   // (unpacked for each head, not once for all in twice the registers)
+            prepare8<D>(p, x, w8, p.eps_k, rot[i], lane, o);
+            ks[i].v[0] = make_uint4(pack_bf16x2(o[0], o[1]), pack_bf16x2(o[2], o[3]), pack_bf16x2(o[4], o[5]), pack_bf16x2(o[6], o[7]));
         }
+        if (!on) ks[i].clear(), vs[i].clear();
+        ks[i].get(x);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) ak = max(ak, finite_magnitude(x[e]));
+        vs[i].get(x);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) av = max(av, finite_magnitude(x[e]));
+    }
+    if (h + 1 < h_end) read(h + 1);
+#pragma unroll
+    for (int i = 0; i < P; ++i) ks[i].hide(), vs[i].hide();
     ak = wave_max_u32(ak), av = wave_max_u32(av);
-    if (lane == 0) top[wave] = ak, top[4 + wave] = av;
-    const int own_k = p.c.k_scale[ph] - 127, own_v = p.c.v_scale[ph] - 127;
+    if (lane == 0) top[wave] = ak, top[kWaves + wave] = av;
     __syncthreads();
-    int ek = scale_exponent(max(max(top[0], top[1]), max(top[2], top[3])));
-    int ev = scale_exponent(max(max(top[4], top[5]), max(top[6], top[7])));
+#pragma unroll
+    for (int i = 0; i < kWaves; ++i) ak = max(ak, top[i]), av = max(av, top[kWaves + i]);
+    int ek = scale_exponent(ak), ev = scale_exponent(av);
     const bool keeps = lo > 0;
     if (keeps) ek = max(ek, own_k), ev = max(ev, own_v);
     const int dk = own_k - ek, dv = own_v - ev;   // used where the page keeps tokens: <= 0
     const float fk = power_of_two(-min(ek, 126)), fv = power_of_two(-min(ev, 126));
 
-    // v: one dword of four tokens' codes per element, to LDS
+    // v: the two tokens' codes of each element, to LDS
+    {
+        float x[P][8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        uint32_t* const at_e = vt + (i0 + e) * kRow;
-        if (P == 2) {
-            const uint32_t c2 = pack_e4m3x4(vx[0][e] * fv, vx[1][e] * fv, 0.0f, 0.0f);
-            reinterpret_cast<uint16_t*>(at_e)[t0 / 2] = (uint16_t)c2;
-        } else {
+        for (int i = 0; i < P; ++i) vs[i].get(x[i]);
 #pragma unroll
-            for (int i = 0; i + 3 < P; i += 4)
-                at_e[(t0 + i) / 4] = pack_e4m3x4(vx[i][e] * fv, vx[i + 1][e] * fv, vx[i + 2][e] * fv, vx[i + 3][e] * fv);
-        }
+        for (int e = 0; e < 8; ++e)
+            reinterpret_cast<uint16_t*>(vt + (i0 + e) * kRow)[t0 / 2] = (uint16_t)pack_e4m3x4(x[0][e] * fv, x[1][e] * fv, 0.0f, 0.0f);
     }
     // k: eight codes of a token, and their sums
     float sum[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
@@ -296,8 +338,9 @@ __device__ __forceinline__ void store_page(const KvAppendArgs& p, uint32_t unit,
         uint2* const dst = reinterpret_cast<uint2*>(p.c.k + (ph * kPage + t) * D + i0);
         uint2 c8;
         if (t >= lo) {
-            c8 = make_uint2(pack_e4m3x4(kx[i][0] * fk, kx[i][1] * fk, kx[i][2] * fk, kx[i][3] * fk),
-                            pack_e4m3x4(kx[i][4] * fk, kx[i][5] * fk, kx[i][6] * fk, kx[i][7] * fk));
+            float x[8];
+            ks[i].get(x);
+            c8 = make_uint2(pack_e4m3x4(x[0] * fk, x[1] * fk, x[2] * fk, x[3] * fk), pack_e4m3x4(x[4] * fk, x[5] * fk, x[6] * fk, x[7] * fk));
             *dst = c8;
         } else {
             c8 = *dst;
@@ -328,7 +371,7 @@ __device__ __forceinline__ void store_page(const KvAppendArgs& p, uint32_t unit,
             for (int e = 0; e < 2; ++e) {
                 float total = 0.0f;
 #pragma unroll
-                for (int g = 0; g < 4; ++g) total += part[g * D + 2 * i + e];
+                for (int g = 0; g < kWaves; ++g) total += part[g * D + 2 * i + e];
                 m[e] = (total / (float)hi) * power_of_two(ek);
             }
             reinterpret_cast<uint32_t*>(p.c.k_mean + ph * D)[i] = pack_bf16x2(m[0], m[1]);
@@ -339,59 +382,61 @@ __device__ __forceinline__ void store_page(const KvAppendArgs& p, uint32_t unit,
         const int d = u / 4, c = u % 4, first = 16 * c;
         const bool some = first < hi && first + 16 > lo, shift = keeps && dv < 0 && first < lo;
         if (!some && !shift) continue;
-        uint4* const dst = reinterpret_cast<uint4*>(p.c.v + (ph * D + d) * kPage) + c;
+        uint32_t* const dst = reinterpret_cast<uint32_t*>(p.c.v + (ph * D + d) * kPage) + 4 * c;
         const uint32_t* const src = vt + d * kRow + 4 * c;
-        uint32_t o[4] = {src[0], src[1], src[2], src[3]};
-        if (first < lo || first + 16 > hi) {
-            const uint4 old = *dst;
-            const uint32_t was[4] = {old.x, old.y, old.z, old.w};
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const uint32_t kept = shift ? rescale4(was[j], dv) : was[j];
-                uint32_t r = 0;
-#pragma unroll
-                for (int t = 0; t < 4; ++t) {
-                    const int token = first + 4 * j + t;
-                    const uint32_t from = token < lo ? kept : token < hi ? o[j] : was[j];
-                    r |= from & (0xffu << (8 * t));
-                }
-                o[j] = r;
-            }
+        if (first >= lo && first + 16 <= hi) {
+            *reinterpret_cast<uint4*>(dst) = make_uint4(src[0], src[1], src[2], src[3]);
+            continue;
         }
-        *dst = make_uint4(o[0], o[1], o[2], o[3]);
+#pragma unroll 1
+        for (int j = 0; j < 4; ++j) {   // (at a page's first and last call)
+            const uint32_t was = dst[j], kept = shift ? rescale4(was, dv) : was, now = src[j];
+            uint32_t r = 0;
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+                const int token = first + 4 * j + t;
+                r |= (token < lo ? kept : token < hi ? now : was) & (0xffu << (8 * t));
+            }
+            dst[j] = r;
+        }
     }
     if (tid == 0) {
         p.c.k_scale[ph] = (uint8_t)(ek + 127);
         p.c.v_scale[ph] = (uint8_t)(ev + 127);
     }
+    __syncthreads();   // before the next values overwrite LDS
+    }
 }
 
 template <int D, int DTYPE, bool PREP>
-__global__ __launch_bounds__(kThreads) void k_kv_append(KvAppendArgs p)
+__global__ __launch_bounds__(threads_of(D), 4) void k_kv_append(KvAppendArgs p)
 {
     __shared__ uint32_t vt[D * 17];
-    __shared__ float part[4 * D];
-    __shared__ uint32_t top[8];
+    __shared__ float part[threads_of(D) / 64 * D];
+    __shared__ uint32_t top[2 * threads_of(D) / 64];
     if ((int)blockIdx.x < p.page_groups) {
-        for (uint32_t u = blockIdx.x; u < p.page_units; u += p.page_groups) {
-            store_page<D, DTYPE, PREP>(p, u, vt, part, top);
-            __syncthreads();   // before the next page's values overwrite LDS
-        }
+        for (uint32_t u = blockIdx.x; u < p.page_units; u += p.page_groups) store_page<D, DTYPE, PREP>(p, u, vt, part, top);
     } else if (PREP) {
         const int64_t groups = gridDim.x - p.page_groups;
-        for (int64_t t = (int64_t)blockIdx.x - p.page_groups; t < p.b.tokens; t += groups) prepare_query<D>(p, t);
+        const int each = (int)(blockDim.x >> 6) / p.query_parts, wave = threadIdx.x >> 6;   // tokens of a workgroup
+        for (int64_t t = ((int64_t)blockIdx.x - p.page_groups) * each + wave / p.query_parts; t < p.b.tokens; t += groups * each)
+            prepare_query<D>(p, t, wave % p.query_parts, p.query_parts);
     }
 }
 
 template <int DTYPE, bool PREP>
 int launch(const KvAppendArgs& p, hipStream_t stream)
 {
-    const int64_t groups = p.page_groups + (PREP ? (p.b.tokens < kMostGroups ? p.b.tokens : kMostGroups) : 0);
-    const dim3 grid((unsigned)groups), block(kThreads);
+    const int threads = threads_of(p.c.d), waves = threads / 64;
+    KvAppendArgs q = p;
+    q.query_parts = p.b.tokens >= kFill / 2 ? 1 : waves;
+    const int64_t tokens = PREP ? (p.b.tokens * q.query_parts + waves - 1) / waves : 0;
+    const int64_t groups = p.page_groups + (tokens < kMostGroups ? tokens : kMostGroups);
+    const dim3 grid((unsigned)groups), block(threads);
     switch (p.c.d) {
-        case 64: hipLaunchKernelGGL((k_kv_append<64, DTYPE, PREP>), grid, block, 0, stream, p); break;
-        case 128: hipLaunchKernelGGL((k_kv_append<128, DTYPE, PREP>), grid, block, 0, stream, p); break;
-        default: hipLaunchKernelGGL((k_kv_append<256, DTYPE, PREP>), grid, block, 0, stream, p); break;
+        case 64: hipLaunchKernelGGL((k_kv_append<64, DTYPE, PREP>), grid, block, 0, stream, q); break;
+        case 128: hipLaunchKernelGGL((k_kv_append<128, DTYPE, PREP>), grid, block, 0, stream, q); break;
+        default: hipLaunchKernelGGL((k_kv_append<256, DTYPE, PREP>), grid, block, 0, stream, q); break;
     }
     return check_launch("kv_append");
 }
@@ -411,7 +456,12 @@ int append_arguments(const char* what, const vdn_fp8_kv_cache* cache, const vdn_
     // n tokens touch at most floor(n / 64) + 2 pages; none where they start at one's first token and end with it
     const int64_t n = p.b.q_start ? p.b.tokens : p.b.each;
     p.units = KvUnits{kPage, (uint32_t)((n + kPage - 2) / kPage + 1), 1, 2};
-    const int64_t units = kv_unit_count(p.b, p.units) * p.c.heads;
+    // Heads of a unit: several where the pages alone fill the part, for the rotations that they share (and
+    // the loads of the next that run beside the stores of one).
+    const int64_t pages = kv_unit_count(p.b, p.units);
+    p.unit_heads = 1;
+    while (p.unit_heads < kMostHeads && pages * p.c.heads / (2 * p.unit_heads) * (threads_of(p.c.d) / 64) >= kFill) p.unit_heads *= 2;
+    const int64_t units = pages * ((p.c.heads + p.unit_heads - 1) / p.unit_heads);
     if (units >= INT32_MAX) return set_error(VDN_FP8_EINVAL, "%s: %lld pages and heads, 2^31 at most", what, (long long)units);
     p.page_units = (uint32_t)units;
     p.page_groups = (int)(p.page_units < kMostGroups ? p.page_units : kMostGroups);

@@ -1048,9 +1048,9 @@ Plan make_plan(KvAttnArgs& p, int64_t max_query, int cus)
         groups = (kv_unit_count(p.b, p.units) + (p.b.q_start ? 1 : 0)) * p.c.heads;
     }
     // Splits where the workgroups alone leave compute units idle: enough for four workgroups (steps) or two
-    // (rows) on each, of at least eight pages, and none below 32: a page costs a wave of k_kv_attn_step about
+    // (rows) on each, of at least eight (four) pages, and none below 32: a page costs a wave of k_kv_attn_step about
     // 0.8 us where nothing else runs, the join and its launch 4 (13 pages of 8 heads: TODO us whole, TODO in four).
-    const int64_t want = (int64_t)cus * (plan.step ? 4 : 2), least = 8;
+    const int64_t want = (int64_t)cus * (plan.step ? 4 : 2), least = plan.step ? 8 : 4;
     int64_t splits = groups > 0 ? want / groups : 1;
     splits = pages < 32 ? 1 : splits < pages / least ? splits : pages / least;
     plan.splits = (int)(splits < 1 ? 1 : splits > kMostSplits ? kMostSplits : splits);

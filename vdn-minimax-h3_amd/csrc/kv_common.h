@@ -87,14 +87,18 @@ __device__ __forceinline__ int kv_locate(const KvBatchArgs& p, const KvUnits& u,
         at = unit - b * u.each;
         return (int)b;
     }
-    int lo = 0, hi = p.batch;   // the last sequence whose first unit is not behind this one
-    while (lo < hi) {
-        const int mid = (lo + hi + 1) >> 1;
-        if (kv_first_unit(p, u, mid) <= unit) lo = mid;
-        else hi = mid - 1;
+    // The sequences that do not begin behind the unit, counted 64 at a time by the wave (all of it is here).
+    const int lane = threadIdx.x & 63;
+    int n = 0;
+    for (int b0 = 0; b0 <= p.batch; b0 += 64) {
+        const int b = b0 + lane;
+        const uint64_t before = __ballot(b <= p.batch && kv_first_unit(p, u, min(b, p.batch)) <= unit);
+        n += __builtin_popcountll(before);
+        if (before != ~0ull) break;
     }
-    at = unit - kv_first_unit(p, u, lo);
-    return lo;
+    const int b = max(n - 1, 0);
+    at = unit - kv_first_unit(p, u, b);
+    return b;
 }
 
 inline int64_t kv_unit_count(const KvBatchArgs& p, const KvUnits& u)

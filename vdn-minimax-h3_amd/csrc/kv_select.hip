@@ -58,6 +58,28 @@ __device__ __forceinline__ bool block_of(const KvSelectArgs& p, int64_t row, int
     return true;
 }
 
+// Lane exchanges of binary64 within rows of 16 lanes.
+template <int CTRL>
+__device__ __forceinline__ double dpp_f64(double v)
+{
+    const uint64_t u = (uint64_t)__double_as_longlong(v);
+    const uint32_t lo = dpp_u32<CTRL>((uint32_t)u), hi = dpp_u32<CTRL>((uint32_t)(u >> 32));
+    return __longlong_as_double((int64_t)((uint64_t)hi << 32 | lo));
+}
+
+// Sum of the lanes up to and including this one, over the wave: within rows of 16 lanes by shifts, then the
+// last lanes of the rows before.
+__device__ __forceinline__ uint32_t wave_scan(uint32_t v)
+{
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x111, 0xf, 0xf, false);   // row_shr 1
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x112, 0xf, 0xf, false);   // 2
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x114, 0xf, 0xf, false);   // 4
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x118, 0xf, 0xf, false);   // 8
+    const uint32_t r0 = __builtin_amdgcn_readlane(v, 15), r1 = __builtin_amdgcn_readlane(v, 31), r2 = __builtin_amdgcn_readlane(v, 47);
+    const int row = (threadIdx.x & 63) / 16;
+    return v + (row > 0 ? r0 : 0) + (row > 1 ? r1 : 0) + (row > 2 ? r2 : 0);
+}
+
 // Adds eight elements.
 template <bool F16>
 __device__ __forceinline__ void add8(uint4 v, double sum[8])
@@ -165,7 +187,9 @@ __global__ __launch_bounds__(kThreads) void k_kv_scores_step(KvSelectArgs p)
     if (w0 - lane / L >= have) return;
     // (every load before any use, and none under a condition: each of its own would be a round trip to memory)
     const uint16_t* const src = p.q + (s.start + from) * p.ldq + (int64_t)h * p.group * D + i0;
-    const uint4 q0 = *reinterpret_cast<const uint4*>(src);
+    uint4 q0[8];
+#pragma unroll
+    for (int g = 0; g < 8; ++g) q0[g] = *reinterpret_cast<const uint4*>(src + (int64_t)min(g, p.group - 1) * D);
     int page[kSweeps];
 #pragma unroll
     for (int j = 0; j < kSweeps; ++j) page[j] = max(kv_page(p.b, p.c, b, min(w0 + j * kPages, have - 1)), 0);
@@ -174,9 +198,10 @@ __global__ __launch_bounds__(kThreads) void k_kv_scores_step(KvSelectArgs p)
     for (int j = 0; j < kSweeps; ++j)
         mean[j] = *reinterpret_cast<const uint4*>(p.c.k_mean + ((int64_t)page[j] * p.c.heads + h) * D + i0);
     double q[8] = {0.0, 0.0, 0.0, 0.0, 0.0, 0.0, 0.0, 0.0};
-    add8<F16>(q0, q);
-#pragma unroll 8
-    for (int g = 1; g < p.group; ++g) add8<F16>(*reinterpret_cast<const uint4*>(src + (int64_t)g * D), q);
+#pragma unroll
+    for (int g = 0; g < 8; ++g)
+        if (g < p.group) add8<F16>(q0[g], q);
+    for (int g = 8; g < p.group; ++g) add8<F16>(*reinterpret_cast<const uint4*>(src + (int64_t)g * D), q);
 #pragma unroll
     for (int e = 0; e < 8; ++e) q[e] = (double)(float)q[e];
 #pragma unroll
@@ -188,8 +213,11 @@ __global__ __launch_bounds__(kThreads) void k_kv_scores_step(KvSelectArgs p)
             sum = __builtin_fma(q[2 * e], (double)bf16_lo(m[e]), sum);
             sum = __builtin_fma(q[2 * e + 1], (double)bf16_hi(m[e]), sum);
         }
-#pragma unroll
-        for (int off = 1; off < L; off <<= 1) sum += __shfl_xor(sum, off, 64);
+        sum += dpp_f64<kDppXor1>(sum);
+        sum += dpp_f64<kDppXor2>(sum);
+        sum += dpp_f64<kDppHalfMirror>(sum);
+        if (L >= 16) sum += dpp_f64<kDppMirror>(sum);
+        if (L == 32) sum += __shfl_xor(sum, 16, 64);
         const int w = w0 + j * kPages;
         if (lane % L == 0 && w < have) p.score[(row * p.c.heads + h) * p.b.width + w] = sum;
     }
@@ -274,12 +302,7 @@ __global__ __launch_bounds__(kThreads) void k_kv_top(KvSelectArgs p)
             // lane l: digits 255 - 4 l and the three below it; what comes before them is what is larger
             const uint4 v = *reinterpret_cast<const uint4*>(&hist[pass][252 - 4 * lane]);
             const uint32_t n[4] = {v.w, v.z, v.y, v.x}, own = n[0] + n[1] + n[2] + n[3];
-            uint32_t run = own;
-#pragma unroll
-            for (int off = 1; off < 64; off <<= 1) {
-                const uint32_t t = __shfl_up(run, off, 64);
-                if (lane >= off) run += t;
-            }
+            const uint32_t run = wave_scan(own);
             uint32_t before = run - own;
             if (before < wanted && run >= wanted)
 #pragma unroll
@@ -328,34 +351,25 @@ __global__ __launch_bounds__(kThreads) void k_kv_top(KvSelectArgs p)
             uint32_t alike = same[lane], bits = above[lane], run = __builtin_popcount(alike);
             if (equal_left > 0) {   // (uniform)
                 const uint32_t own = run;
-#pragma unroll
-                for (int off = 1; off < 64; off <<= 1) {
-                    const uint32_t t = __shfl_up(run, off, 64);
-                    if (lane >= off) run += t;
-                }
+                run = wave_scan(own);
                 uint32_t room = equal_left > run - own ? equal_left - (run - own) : 0;   // of this word's
                 while (alike && room) {
                     bits |= alike & (0u - alike);
                     alike &= alike - 1;
                     --room;
                 }
-                const uint32_t all = __shfl(run, 63, 64);
+                const uint32_t all = __builtin_amdgcn_readlane(run, 63);
                 equal_left = equal_left > all ? equal_left - all : 0;
             }
             const uint32_t own = __builtin_popcount(bits);
-            run = own;
-#pragma unroll
-            for (int off = 1; off < 64; off <<= 1) {
-                const uint32_t t = __shfl_up(run, off, 64);
-                if (lane >= off) run += t;
-            }
+            run = wave_scan(own);
             uint32_t at = taken + run - own;
             while (bits) {
                 if (at < (uint32_t)p.top) out[at] = w0 + 32 * lane + __builtin_ctz(bits);
                 bits &= bits - 1;
                 ++at;
             }
-            taken += __shfl(run, 63, 64);
+            taken += __builtin_amdgcn_readlane(run, 63);
         }
     }
     if (wave == 0)
