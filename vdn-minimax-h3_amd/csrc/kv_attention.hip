@@ -29,12 +29,11 @@
 // that they read. Two kernels:
 //   k_kv_attn_rows    128 rows, 32 for each of four waves, which share the pages through LDS (copied
 //                     there asynchronously, two pages ahead). For chunks and prompts.
-//   k_kv_attn_step    up to 32 rows; each of the four waves takes every fourth page, straight from
+//   k_kv_attn_step    up to 16 rows; each of the four waves takes every fourth page, straight from
 //                     memory into the operands' registers, and they join at the end. For single tokens.
 // Both cut long key axes into splits where there are few rows, joined by k_kv_attn_join.
 #include <stdint.h>
 
-#include <atomic>
 
 #include "gemm_common.h"
 #include "kv_common.h"
@@ -44,7 +43,7 @@ namespace vdn {
 namespace {
 
 constexpr int kRows = 128, kWaveRows = 32;   // of k_kv_attn_rows
-constexpr int kStepRows = 32;                  // of k_kv_attn_step, at most
+constexpr int kStepRows = 16;                  // of k_kv_attn_step, at most
 constexpr int kInfo = 256;                     // pages that a workgroup looks up at a time
 constexpr int kMostSplits = 64;
 constexpr float kNoMax = -3.0e38f;      // the running maximum of no keys: finite, so that differences stay numbers
@@ -403,16 +402,17 @@ struct WaveRows {
     }
 };
 
-// One wave's rows of k_kv_attn_step, NT columns of 16: lane l holds row l % 16 of each, and the keys
-// 16 g .. 16 g + 15 of a page (g = l / 16), tile t of the scores standing for keys 16 g + 4 t + i.
-// (Half the accumulators and scores that 32 columns would take, at the group sizes that are usual.)
-template <int D, bool F16, int NT>
+// One wave's 16 rows of k_kv_attn_step: lane l holds row l % 16, and the keys 16 g .. 16 g + 15 of a page
+// (g = l / 16), tile t of the scores standing for keys 16 g + 4 t + i. (Half the accumulators and scores
+// that 32 columns would take. Two such sets to a wave spilled from d = 128 on: with groups of 8 and 4
+// queries 61 us against 58 for two workgroups that read the pages twice, 229 against 143 at d = 256.)
+template <int D, bool F16>
 struct StepRows {
     static constexpr int kSteps = D <= 128 ? 1 : D / 128, kTerms = F16 ? 3 : 2, kTiles = D / 16;
-    i32x8_t q[NT][kTerms][kSteps];
-    f32x4_t acc[NT][kTiles];
-    float m[NT], l[NT], c[NT];
-    int limit[NT];
+    i32x8_t q[kTerms][kSteps];
+    f32x4_t acc[kTiles];
+    float m, l, c;
+    int limit;
 
     // (a head of 64 fills half of the instruction's 128: the upper lanes repeat the keys against zeros)
     __device__ __forceinline__ static void read(RawQuery<kSteps>& raw, const uint16_t* row, int g)
@@ -422,97 +422,83 @@ struct StepRows {
         for (int s = 0; s < kSteps; ++s) at[s] = row && (D > 64 || g < 2) ? row + 128 * s + 32 * g : nullptr;
         raw.load(at);
     }
-    __device__ __forceinline__ void start(int n, const RawQuery<kSteps>& raw, float scale)
+    __device__ __forceinline__ void start(const RawQuery<kSteps>& raw, float scale)
     {
         const int e = split_query<F16>(raw, [](uint32_t v) {
             const auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
             v = max((uint32_t)r[0], (uint32_t)r[1]);
             const auto s = __builtin_amdgcn_permlane16_swap(v, v, false, false);
             return max((uint32_t)s[0], (uint32_t)s[1]);
-        }, q[n]);
-        c[n] = scale * exponent_f32(e);
+        }, q);
+        c = scale * exponent_f32(e);
     }
-    __device__ __forceinline__ void clear(int n)
+    __device__ __forceinline__ void clear()
     {
-        m[n] = kNoMax, l[n] = 0.0f;
+        m = kNoMax, l = 0.0f;
 #pragma unroll
-        for (int t = 0; t < kTiles; ++t) acc[n][t] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+        for (int t = 0; t < kTiles; ++t) acc[t] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
     }
 
     template <typename Key>
-    __device__ __forceinline__ void scores(Key key, f32x4_t s[NT][4]) const
+    __device__ __forceinline__ void scores(Key key, f32x4_t s[4]) const
     {
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
-#pragma unroll
-            for (int n = 0; n < NT; ++n) s[n][t] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+            s[t] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (int st = 0; st < kSteps; ++st) {
                 const i32x8_t a = key(t, st);
-#pragma unroll
-                for (int n = 0; n < NT; ++n) {
-                    s[n][t] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, q[n][0][st], s[n][t], 0, 0, 0, kOne, 0, kOne);
-                    s[n][t] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, q[n][1][st], s[n][t], 0, 0, 0, kOne, 0, kTerm1);
-                    if (kTerms == 3)
-                        s[n][t] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, q[n][kTerms - 1][st], s[n][t], 0, 0, 0, kOne, 0, kTerm2);
-                }
+                s[t] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, q[0][st], s[t], 0, 0, 0, kOne, 0, kOne);
+                s[t] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, q[1][st], s[t], 0, 0, 0, kOne, 0, kTerm1);
+                if (kTerms == 3)
+                    s[t] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, q[kTerms - 1][st], s[t], 0, 0, 0, kOne, 0, kTerm2);
             }
         }
     }
 
-    __device__ __forceinline__ void mask(f32x4_t s[NT][4], int key0, int g) const
+    __device__ __forceinline__ void mask(f32x4_t s[4], int key0, int g) const
     {
+        const int seen = limit - key0 - 16 * g;
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-            const int seen = limit[n] - key0 - 16 * g;
+        for (int t = 0; t < 4; ++t)
 #pragma unroll
-            for (int t = 0; t < 4; ++t)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) s[n][t][i] = 4 * t + i < seen ? s[n][t][i] : -__builtin_inff();
-        }
+            for (int i = 0; i < 4; ++i) s[t][i] = 4 * t + i < seen ? s[t][i] : -__builtin_inff();
     }
 
-    __device__ __forceinline__ void weights(const f32x4_t s[NT][4], int ek, int ev, f16x8_t w[NT][2])
+    __device__ __forceinline__ void weights(const f32x4_t s[4], int ek, int ev, f16x8_t w[2])
     {
-        const float shift = (float)ev;
+        const float shift = (float)ev, f = fmaxf(c * exponent_f32(ek), 1e-37f);
+        float top = s[0][0];
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-            const float f = fmaxf(c[n] * exponent_f32(ek), 1e-37f);
-            float top = s[n][0][0];
+        for (int i = 1; i < 16; ++i) top = larger(top, s[i / 4][i % 4]);
+        top = across16(across32(top, larger), larger) * f + shift;
+        if (__any(top > m + kSlack)) {
+            const float now = fmaxf(m, top), a = __builtin_amdgcn_exp2f(m - now);
+            m = now;
+            l *= a;
 #pragma unroll
-            for (int i = 1; i < 16; ++i) top = larger(top, s[n][i / 4][i % 4]);
-            top = across16(across32(top, larger), larger) * f + shift;
-            if (__any(top > m[n] + kSlack)) {
-                const float now = fmaxf(m[n], top), a = __builtin_amdgcn_exp2f(m[n] - now);
-                m[n] = now;
-                l[n] *= a;
-#pragma unroll
-                for (int t = 0; t < kTiles; ++t) acc[n][t] *= a;
-            }
-            const float base = shift - m[n];
-            float sum = 0.0f;
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][i / 4][i % 4], f, base));
-                sum += p;
-                w[n][i / 8][i % 8] = (_Float16)p;
-            }
-            l[n] = __builtin_fmaf(sum, exponent_f32(-ev), l[n]);
+            for (int t = 0; t < kTiles; ++t) acc[t] *= a;
         }
+        const float base = shift - m;
+        float sum = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i / 4][i % 4], f, base));
+            sum += p;
+            w[i / 8][i % 8] = (_Float16)p;
+        }
+        l = __builtin_fmaf(sum, exponent_f32(-ev), l);
     }
 
     // v[t]: the codes of 16 tokens, one element.
-    __device__ __forceinline__ void add_values(const uint4 v[kTiles], const f16x8_t w[NT][2])
+    __device__ __forceinline__ void add_values(const uint4 v[kTiles], const f16x8_t w[2])
     {
 #pragma unroll
         for (int t = 0; t < kTiles; ++t) {
             f16x8_t a[2];
             decode16(v[t], a);
-#pragma unroll
-            for (int n = 0; n < NT; ++n) {
-                acc[n][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a[0], w[n][0], acc[n][t], 0, 0, 0);
-                acc[n][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a[1], w[n][1], acc[n][t], 0, 0, 0);
-            }
+            acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a[0], w[0], acc[t], 0, 0, 0);
+            acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a[1], w[1], acc[t], 0, 0, 0);
         }
     }
 
@@ -535,15 +521,11 @@ struct StepRows {
             keep_tokens(v[t], 16, nan);
             f16x8_t is_nan[2];
             decode16(as_ones(nan), is_nan);
+            f32x4_t hit = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-            for (int n = 0; n < NT; ++n) {
-                f32x4_t hit = {0.0f, 0.0f, 0.0f, 0.0f};
+            for (int h = 0; h < 2; ++h) hit = __builtin_amdgcn_mfma_f32_16x16x32_f16(is_nan[h], seen_ones(key0 + 16 * g + 8 * h, limit), hit, 0, 0, 0);
 #pragma unroll
-                for (int h = 0; h < 2; ++h)
-                    hit = __builtin_amdgcn_mfma_f32_16x16x32_f16(is_nan[h], seen_ones(key0 + 16 * g + 8 * h, limit[n]), hit, 0, 0, 0);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) acc[n][t][i] = hit[i] > 0.0f ? __builtin_nanf("") : acc[n][t][i];
-            }
+            for (int i = 0; i < 4; ++i) acc[t][i] = hit[i] > 0.0f ? __builtin_nanf("") : acc[t][i];
             v[t] = without(v[t], nan);
         }
     }
@@ -606,10 +588,11 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_kv_attn_rows(KvAttnAr
         }
         return;
     }
-    const int at = __builtin_amdgcn_readfirstlane((int)at64);
     const KvSequence s = kv_sequence(p.b, b);
-    const int r0 = at * kRows, rows = s.n * p.group;   // (tokens * q_heads < 2^30)
-    if (at >= (rows + kRows - 1) / kRows) return;
+    const int rows = s.n * p.group, tiles = (rows + kRows - 1) / kRows;   // (tokens * q_heads < 2^30)
+    const int at = __builtin_amdgcn_readfirstlane((int)at64);
+    if (at >= tiles) return;
+    const int r0 = at * kRows;
     const int last = min(r0 + kRows, rows) - 1;
     auto limit_of = [&](int row) -> int {
         if (!p.causal) return s.length;
@@ -810,12 +793,14 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_kv_attn_rows(KvAttnAr
         p.lse[out_row] = l == 0.0f ? -__builtin_inff() : (rowset.m + __builtin_log2f(l)) * 0.6931471805599453f;
 }
 
-// Up to 16 NT rows of one sequence (or of one token, where each has its own pages) and key/value head.
-template <int D, bool F16, int NT>
+// Up to 16 rows of one sequence (or of one token, where each has its own pages) and key/value head.
+template <int D, bool F16>
 __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_kv_attn_step(KvAttnArgs p)
 {
-    constexpr int kTiles = D / 16, kSteps = StepRows<D, F16, NT>::kSteps;
-    extern __shared__ __attribute__((aligned(128))) uint8_t lds[];   // [4][rows][D], then the maxima and sums
+    constexpr int kTiles = D / 16, kSteps = StepRows<D, F16>::kSteps;
+    constexpr int kPart = D < 128 ? D : 128;
+    __shared__ __attribute__((aligned(16))) float acc[4][kStepRows][kPart];
+    __shared__ float2 sums[4][kStepRows];   // maximum, sum
     __shared__ __attribute__((aligned(16))) PageInfo info[kInfo];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int r = lane & 15, g = lane >> 4;
@@ -861,15 +846,14 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_kv_attn_step(KvAttnAr
         hi = min(lo + per, hi);
     }
 
-    StepRows<D, F16, NT> rowset;
-    RawQuery<kSteps> raw[NT];   // (on their way while the pages are looked up)
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
-        const int row = tile * kStepRows + 16 * n + r, own = at + row / p.group;
+    StepRows<D, F16> rowset;
+    RawQuery<kSteps> raw;   // (on its way while the pages are looked up)
+    {
+        const int row = tile * kStepRows + r, own = at + row / p.group;
         const bool valid = row < rows;
-        rowset.read(raw[n], valid ? p.q + (s.start + own) * p.ldq + (int64_t)(h * p.group + row % p.group) * D : nullptr, g);
-        rowset.clear(n);
-        rowset.limit[n] = valid ? limit_of(own) : 0;
+        rowset.read(raw, valid ? p.q + (s.start + own) * p.ldq + (int64_t)(h * p.group + row % p.group) * D : nullptr, g);
+        rowset.clear();
+        rowset.limit = valid ? limit_of(own) : 0;
     }
     const int least = limit_of(first_token), most = limit_of(last_token);
 
@@ -891,8 +875,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_kv_attn_step(KvAttnAr
     };
     look_up(p, b, h, s.length, list, lo, hi, info);
     __syncthreads();
-#pragma unroll
-    for (int n = 0; n < NT; ++n) rowset.start(n, raw[n], p.scale);
+    rowset.start(raw, p.scale);
     for (int first = lo; first < hi; first += kInfo) {
         const int count = min(hi - first, kInfo);
         if (first > lo) {
@@ -910,8 +893,8 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_kv_attn_step(KvAttnAr
         for (; i < count; i += 4) {
             const bool more = i + 4 < count;
             if (more) next = info_at(info, i + 4);
-            f32x4_t sc[NT][4];
-            f16x8_t w[NT][2];
+            f32x4_t sc[4];
+            f16x8_t w[2];
             rowset.scores([&](int t, int st) {
                 const uint4 x = kr[t][st][0], y = kr[t][st][1];
                 return i32x8_t{(int)x.x, (int)x.y, (int)x.z, (int)x.w, (int)y.x, (int)y.y, (int)y.z, (int)y.w};
@@ -930,46 +913,44 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_kv_attn_step(KvAttnAr
         }
     }
 
-    // The four waves' parts of each row, joined in LDS.
+    // The four waves' parts of each row, joined in LDS, 128 elements at a time.
     const int kept = min(rows - tile * kStepRows, kStepRows);
-    float* const acc = reinterpret_cast<float*>(lds);
-    float* const sums = acc + 4 * kept * D;
+    const float l = across16(across32(rowset.l, added), added);
+    if (g == 0) sums[wave][r] = make_float2(rowset.m, l);
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
-        const float l = across16(across32(rowset.l[n], added), added);
-        const int at_row = 16 * n + r;
-        if (at_row < kept) {
+    for (int d0 = 0; d0 < D; d0 += kPart) {
+        if (d0 > 0) __syncthreads();
 #pragma unroll
-            for (int t = 0; t < kTiles; ++t)
-                *reinterpret_cast<float4*>(acc + (wave * kept + at_row) * D + 16 * t + 4 * g) =
-                    make_float4(rowset.acc[n][t][0], rowset.acc[n][t][1], rowset.acc[n][t][2], rowset.acc[n][t][3]);
-            if (g == 0) sums[2 * (wave * kept + at_row)] = rowset.m[n], sums[2 * (wave * kept + at_row) + 1] = l;
+        for (int t = 0; t < kPart / 16; ++t) {
+            const f32x4_t v = rowset.acc[d0 / 16 + t];
+            *reinterpret_cast<float4*>(&acc[wave][r][16 * t + 4 * g]) = make_float4(v[0], v[1], v[2], v[3]);
         }
-    }
-    __syncthreads();
-    for (int e = tid; e < kept * (D / 4); e += 256) {
-        const int row_e = e / (D / 4), d = 4 * (e % (D / 4));
-        float m = kNoMax;
+        __syncthreads();
+        for (int e = tid; e < kept * (kPart / 4); e += 256) {
+            const int row_e = e / (kPart / 4), d = 4 * (e % (kPart / 4));
+            float m = kNoMax;
 #pragma unroll
-        for (int wv = 0; wv < 4; ++wv) m = fmaxf(m, sums[2 * (wv * kept + row_e)]);
-        float total = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            for (int wv = 0; wv < 4; ++wv) m = fmaxf(m, sums[wv][row_e].x);
+            float total = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-        for (int wv = 0; wv < 4; ++wv) {
-            const float f = __builtin_amdgcn_exp2f(sums[2 * (wv * kept + row_e)] - m);
-            const float4 a = *reinterpret_cast<const float4*>(acc + (wv * kept + row_e) * D + d);
-            total += f * sums[2 * (wv * kept + row_e) + 1];
-            o[0] += f * a.x, o[1] += f * a.y, o[2] += f * a.z, o[3] += f * a.w;
-        }
-        const int row_at = tile * kStepRows + row_e;
-        const int64_t out_row = (s.start + at + row_at / p.group) * p.q_heads + h * p.group + row_at % p.group;
-        if (p.splits > 1) {
-            *reinterpret_cast<float4*>(p.part + (out_row * p.splits + split) * D + d) = make_float4(o[0], o[1], o[2], o[3]);
-            if (d == 0) *reinterpret_cast<float2*>(part_sums(p) + 2 * (out_row * p.splits + split)) = make_float2(m, total);
-        } else {
-            const float inv = total == 0.0f ? 0.0f : 1.0f / total;
-            *reinterpret_cast<uint2*>(p.out + out_row * D + d) =
-                make_uint2(pack_out<F16>(o[0] * inv, o[1] * inv), pack_out<F16>(o[2] * inv, o[3] * inv));
-            if (p.lse && d == 0) p.lse[out_row] = total == 0.0f ? -__builtin_inff() : (m + __builtin_log2f(total)) * 0.6931471805599453f;
+            for (int wv = 0; wv < 4; ++wv) {
+                const float f = __builtin_amdgcn_exp2f(sums[wv][row_e].x - m);
+                const float4 a = *reinterpret_cast<const float4*>(&acc[wv][row_e][d]);
+                total += f * sums[wv][row_e].y;
+                o[0] += f * a.x, o[1] += f * a.y, o[2] += f * a.z, o[3] += f * a.w;
+            }
+            const int row_at = tile * kStepRows + row_e;
+            const int64_t out_row = (s.start + at + row_at / p.group) * p.q_heads + h * p.group + row_at % p.group;
+            if (p.splits > 1) {
+                *reinterpret_cast<float4*>(p.part + (out_row * p.splits + split) * D + d0 + d) = make_float4(o[0], o[1], o[2], o[3]);
+                if (d0 + d == 0) *reinterpret_cast<float2*>(part_sums(p) + 2 * (out_row * p.splits + split)) = make_float2(m, total);
+            } else {
+                const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+                *reinterpret_cast<uint2*>(p.out + out_row * D + d0 + d) =
+                    make_uint2(pack_out<F16>(o[0] * inv, o[1] * inv), pack_out<F16>(o[2] * inv, o[3] * inv));
+                if (p.lse && d0 + d == 0)
+                    p.lse[out_row] = total == 0.0f ? -__builtin_inff() : (m + __builtin_log2f(total)) * 0.6931471805599453f;
+            }
         }
     }
 }
@@ -1034,7 +1015,9 @@ Plan make_plan(KvAttnArgs& p, int64_t max_query, int cus)
     Plan plan{};
     const int64_t n = p.b.q_start ? (max_query > 0 && max_query < p.b.tokens ? max_query : p.b.tokens) : p.b.tokens / p.b.batch;
     const int64_t most = p.blocks ? p.query_block : n;   // tokens of a unit of the step kernel
-    plan.step = p.blocks ? p.query_block == 1 : n * p.group <= kStepRows;
+    // Steps up to 16 rows, at d = 256 up to 32 (4 queries in groups of 8 over 30000 tokens, eight sequences:
+    // d = 64 37 us in either kernel, 128 58 us in two tiles of k_kv_attn_step against 52, 256 143 against 172).
+    plan.step = p.blocks ? p.query_block == 1 : n * p.group <= (p.c.d == 256 ? 2 : 1) * kStepRows;
     const int64_t pages = p.blocks ? p.top : p.b.width;
     int64_t groups;
     if (plan.step) {
@@ -1059,31 +1042,13 @@ Plan make_plan(KvAttnArgs& p, int64_t max_query, int cus)
     return plan;
 }
 
-template <int D, bool F16, int NT>
-int launch_step(const KvAttnArgs& p, hipStream_t stream)
-{
-    const size_t bytes = (size_t)(4 * (p.step_rows < kStepRows ? p.step_rows : kStepRows)) * (D + 2) * 4;
-    if (bytes + kInfo * sizeof(PageInfo) > 65536) {   // (beyond what a launch may take unasked; once per device)
-        static std::atomic<bool> raised[64];
-        int dev = 0;
-        if (hipGetDevice(&dev) != hipSuccess) return set_error(VDN_FP8_ELAUNCH, "kv_attention: no device");
-        if (dev >= 64 || !raised[dev].load(std::memory_order_relaxed)) {
-            if (hipFuncSetAttribute((const void*)k_kv_attn_step<D, F16, NT>, hipFuncAttributeMaxDynamicSharedMemorySize,
-                                    4 * kStepRows * (D + 2) * 4) != hipSuccess)
-                return set_error(VDN_FP8_ELAUNCH, "kv_attention: the device refuses %zu bytes of LDS", bytes);
-            if (dev < 64) raised[dev].store(true, std::memory_order_relaxed);
-        }
-    }
-    hipLaunchKernelGGL((k_kv_attn_step<D, F16, NT>), dim3(p.items), dim3(256), bytes, stream, p);
-    return check_launch("kv_attention");
-}
-
 template <int D, bool F16>
 int launch(const KvAttnArgs& p, bool step, hipStream_t stream)
 {
     int st;
     if (step) {
-        st = p.step_rows <= 16 ? launch_step<D, F16, 1>(p, stream) : launch_step<D, F16, 2>(p, stream);
+        hipLaunchKernelGGL((k_kv_attn_step<D, F16>), dim3(p.items), dim3(256), 0, stream, p);
+        st = check_launch("kv_attention");
     } else {
         hipLaunchKernelGGL((k_kv_attn_rows<D, F16>), dim3(p.items), dim3(256), 0, stream, p);
         st = check_launch("kv_attention");
