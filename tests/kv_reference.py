@@ -137,9 +137,10 @@ def attend(cache, q, table, lengths, starts, scale, causal=False, blocks=None, b
                     # Weights are rounded to binary16: 2^-11 of each, and 2^-25 where it is below that
                     # type's normal range, next to a largest one of at least 1 (in units of the largest
                     # value times 2^e, so at most 2^-24 of the largest value for each token). Scores:
-                    # queries keep 2^-21 of their largest element, sums of products are good to 2^-22
-                    # of their magnitudes; both together stay below 2^-20 of |q|.|k|.
-                    es = scale * 2.0 ** -20 * ((x.abs().amax(1, keepdim=True) + x.abs()) @ k.abs().nan_to_num(0).T).amax(1)
+                    # products are exact; their sum is d / 16 sums one after another, at most 16, of 16
+                    # products each (four more levels), so at most 20 roundings (2^-23 each, should they
+                    # truncate) of the magnitudes' sum, and two more for the scale: below 2^-18 of |q|.|k|.
+                    es = scale * 2.0 ** -18 * (x.abs() @ k.abs().nan_to_num(0).T).amax(1)
                     a = p.nan_to_num(0) @ v.nan_to_num(0).abs()
                     tol[row + rows, gh] = (2.0 ** -11 + 2.0 ** -18 + 2 * es)[:, None] * a + len(place) * 2.0 ** -24 * float(v.abs().nan_to_num(0).max())
                     tol_lse[row + rows, gh] = 2 * es + 2.0 ** -20 + 2.0 ** -22 * z.abs().nan_to_num(0, 0, 0)

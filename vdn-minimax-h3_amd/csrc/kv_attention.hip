@@ -4,13 +4,11 @@
 //   x_j = log2(e) scale (q . k_j),  k_j = code 2^ek,   o = sum_j 2^(x_j) v_j / sum_j 2^(x_j)
 // in one pass over the pages with a running maximum. Three choices carry the arithmetic:
 //
-//   Scores on the fp8 matrix cores, without rounding the queries to 8 bits. A bf16 value has eight
-//   significant bits, so it is exactly hi + lo with hi = e4m3(q 2^-eq) and lo the e4m3 of the
-//   rest times 2^4 (eq: a power of two for each row that brings its largest element to [224, 448];
-//   elements 2^-11 below that one lose bits under 2^-21 of it). Two fp8 products cost what one bf16
-//   product does, and the keys, the larger operand, go to the matrix cores as they are stored. A
-//   binary16 query has eleven bits and takes a third term. The lower terms' factors are the
-//   instruction's own block scales.
+//   Scores in the queries' own type: e4m3 codes are bf16 and binary16 numbers, so keys are decoded exactly,
+//   products are exact and sums are binary32. (On the fp8 matrix cores, with a bf16 query as the sum of two
+//   e4m3 terms, a product costs the same and keys need no decoding; but those cores align the 64 or 128
+//   products of an instruction to the largest and drop what is below: scores were off by up to 2^-12 of the
+//   largest product, where these sums stay within 2^-18 of it, for 1.99 against 2.15 ms on 3120 tokens over 32760.)
 //
 //   Values in binary16: e4m3 codes are binary16 numbers, and weights in [0, 2^8] keep eleven bits
 //   (bf16 weights would leave eight, an error as large as the output's own rounding). The value's scale
@@ -27,13 +25,17 @@
 //
 // Rows are (token, head of a group) pairs of one key/value head, so grouped heads share the pages
 // that they read. Two kernels:
-//   k_kv_attn_rows    128 rows, 32 for each of four waves, which share the pages through LDS (copied
-//                     there asynchronously, two pages ahead). For chunks and prompts.
+//   k_kv_attn_rows    128 rows, 32 for each of four waves, which share the pages through LDS: keys as codes
+//                     (asynchronous copies, two pages ahead; each wave decodes what it reads), values decoded
+//                     once for all four. For chunks and prompts. 3120 tokens over 32760, 40 heads of 128:
+//                     2.15 ms, 0.97 PF/s; the card's power limit holds its clock at 1.9 of 2.4 GHz, where bare
+//                     chains of the same instructions reach 1.6 to 1.8 PF/s. Keys decoded once as well are
+//                     slower (2.28 ms: LDS reads, 32 KB a wave and page, take as long as the products).
 //   k_kv_attn_step    up to 16 rows; each of the four waves takes every fourth page, straight from
 //                     memory into the operands' registers, and they join at the end. For single tokens.
+//                     8 sequences of 71000 to 131072 tokens, 40 on 8 heads of 128: 0.29 ms, 5.6 TB/s.
 // Both cut long key axes into splits where there are few rows, joined by k_kv_attn_join.
 #include <stdint.h>
-
 
 #include "gemm_common.h"
 #include "kv_common.h"
@@ -52,6 +54,9 @@ constexpr int kAbsent = 1 << 30;        // first key of a page that is not there
 
 typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
+typedef float f32x4_t __attribute__((ext_vector_type(4)));
+typedef float f32x16_t __attribute__((ext_vector_type(16)));
 
 struct KvAttnArgs {
     KvCacheArgs c;
@@ -101,7 +106,7 @@ __device__ __forceinline__ float added(float a, float b) { return a + b; }
 
 __device__ __forceinline__ float exponent_f32(int e) { return __uint_as_float((uint32_t)(min(max(e, -126), 127) + 127) << 23); }
 
-// 16 codes of one operand row -> two operands of eight binary16 values (exact).
+// 16 codes of one operand row -> two operands of eight values (exact).
 __device__ __forceinline__ void decode16(uint4 w, f16x8_t o[2])
 {
     const uint32_t u[4] = {w.x, w.y, w.z, w.w};
@@ -113,80 +118,44 @@ __device__ __forceinline__ void decode16(uint4 w, f16x8_t o[2])
         o[i / 2][4 * (i % 2) + 2] = hi.x, o[i / 2][4 * (i % 2) + 3] = hi.y;
     }
 }
-
-// 32 elements of a query row for each step of the inner dimension, as they are (row[s] NULL: zeros).
-template <int STEPS>
-struct RawQuery {
-    uint4 v[STEPS][4];
-    __device__ __forceinline__ void load(const uint16_t* const (&row)[STEPS])
-    {
-#pragma unroll
-        for (int s = 0; s < STEPS; ++s)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                v[s][i] = make_uint4(0, 0, 0, 0);
-                if (row[s]) v[s][i] = *reinterpret_cast<const uint4*>(row[s] + 8 * i);
-            }
-    }
-};
-
-// Their fp8 terms, and the exponent e that they are scaled by: TERMS values whose sum is x 2^-e, term t
-// times 2^(5 t - 1) (t > 0). Every lane of a row passes its largest magnitude through `join`.
-template <bool F16, int STEPS, int TERMS, typename Join>
-__device__ __forceinline__ int split_query(const RawQuery<STEPS>& raw, Join join, i32x8_t (&q)[TERMS][STEPS])
+__device__ __forceinline__ void decode16(uint4 w, bf16x8_t o[2])
 {
-    float x[STEPS][32];
-    uint32_t top = 0;
+    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-    for (int s = 0; s < STEPS; ++s)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const uint4 v = raw.v[s][i];
-            const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                float lo, hi;
-                if (F16) {
-                    lo = (float)__builtin_bit_cast(_Float16, (uint16_t)w[e]);
-                    hi = (float)__builtin_bit_cast(_Float16, (uint16_t)(w[e] >> 16));
-                } else {
-                    lo = bf16_lo(w[e]), hi = bf16_hi(w[e]);
-                }
-                x[s][8 * i + 2 * e] = lo, x[s][8 * i + 2 * e + 1] = hi;
-                const uint32_t a = __float_as_uint(lo) & 0x7fffffffu, b = __float_as_uint(hi) & 0x7fffffffu;
-                top = max(top, max(a < 0x7f800000u ? a : 0u, b < 0x7f800000u ? b : 0u));
-            }
-        }
-    top = join(top);
-    int e = (int)(top >> 23) - 127 - 8 + ((top & 0x7fffffu) > 0x600000u ? 1 : 0);
-    e = top == 0 ? 0 : min(max(e, -120), 120);
-    const float f = exponent_f32(-e);
-#pragma unroll
-    for (int s = 0; s < STEPS; ++s)
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            float r[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) r[j] = x[s][4 * i + j] * f;
-#pragma unroll
-            for (int t = 0; t < TERMS; ++t) {
-                const uint32_t w = pack_e4m3x4(r[0], r[1], r[2], r[3]);
-                q[t][s][i] = (int)w;
-                // the rest, exact; times the next term's factor: 2^4, then 2^5
-                const float up = t == 0 ? 16.0f : 32.0f;
-                r[0] = (r[0] - __builtin_amdgcn_cvt_f32_fp8(w, 0)) * up;
-                r[1] = (r[1] - __builtin_amdgcn_cvt_f32_fp8(w, 1)) * up;
-                r[2] = (r[2] - __builtin_amdgcn_cvt_f32_fp8(w, 2)) * up;
-                r[3] = (r[3] - __builtin_amdgcn_cvt_f32_fp8(w, 3)) * up;
-            }
-        }
-    return e;
+    for (int i = 0; i < 4; ++i) {
+        const bf16x2_t lo = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(u[i], 1.0f, false);
+        const bf16x2_t hi = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(u[i], 1.0f, true);
+        o[i / 2][4 * (i % 2)] = lo.x, o[i / 2][4 * (i % 2) + 1] = lo.y;
+        o[i / 2][4 * (i % 2) + 2] = hi.x, o[i / 2][4 * (i % 2) + 3] = hi.y;
+    }
 }
 
-// The block scales of the terms, as the matrix instructions take them.
-constexpr int waitcnt_lgkm0() { return 15 | (7 << 4) | (0 << 8) | (3 << 14); }   // any vmcnt
+// The queries' type: its operand of eight values, and the products of 32 x 32 x 16 and 16 x 16 x 32.
+template <bool F16>
+struct Query;
+template <>
+struct Query<true> {
+    typedef f16x8_t Eight;
+    __device__ __forceinline__ static f32x16_t mma32(Eight a, Eight b, f32x16_t c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+    __device__ __forceinline__ static f32x4_t mma16(Eight a, Eight b, f32x4_t c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+};
+template <>
+struct Query<false> {
+    typedef bf16x8_t Eight;
+    __device__ __forceinline__ static f32x16_t mma32(Eight a, Eight b, f32x16_t c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+    __device__ __forceinline__ static f32x4_t mma16(Eight a, Eight b, f32x4_t c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+};
 
-constexpr int kOne = 0x7f7f7f7f, kTerm1 = 0x7b7b7b7b, kTerm2 = 0x76767676;
+// Eight query values at `row` (NULL: zeros).
+template <bool F16>
+__device__ __forceinline__ typename Query<F16>::Eight query8(const uint16_t* row)
+{
+    uint4 v = make_uint4(0, 0, 0, 0);
+    if (row) v = *reinterpret_cast<const uint4*>(row);
+    return __builtin_bit_cast(typename Query<F16>::Eight, v);
+}
+
+constexpr int waitcnt_lgkm0() { return 15 | (7 << 4) | (0 << 8) | (3 << 14); }   // any vmcnt
 
 // What the workgroup knows of a page: its number in the pool (-1: not there), its number in the
 // sequence, and its scales' exponents. Looked up by all threads at once, kInfo pages at a time, so
@@ -260,29 +229,18 @@ __device__ __forceinline__ f16x8_t seen_ones(int first, int limit)
 // Lane l: column l % 32 is the row of the problem, g = l / 32 its half of the keys.
 template <int D, bool F16>
 struct WaveRows {
-    static constexpr int kSteps = D / 64, kTerms = F16 ? 3 : 2, kTiles = D / 32;
-    i32x8_t q[kTerms][kSteps];
+    static constexpr int kSteps = D / 16, kTiles = D / 32;
+    typedef typename Query<F16>::Eight Eight;
+    Eight q[kSteps];
     f32x16_t acc[kTiles];
-    float m, l, c;     // running maximum and sum (of this half's keys), factor of the raw scores
+    float m, l;        // running maximum and sum (of this half's keys)
     int limit;         // keys below it are visible to the row
 
-    __device__ __forceinline__ static void read(RawQuery<kSteps>& raw, const uint16_t* row, int g)
+    // row: the row's values (NULL: none, zeros).
+    __device__ __forceinline__ void start(const uint16_t* row, int g)
     {
-        const uint16_t* at[kSteps];
 #pragma unroll
-        for (int s = 0; s < kSteps; ++s) at[s] = row ? row + 64 * s + 32 * g : nullptr;
-        raw.load(at);
-    }
-    __device__ __forceinline__ void start(const RawQuery<kSteps>& raw, float scale)
-    {
-        const int e = split_query<F16>(raw, [](uint32_t v) {
-            const auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
-            return max((uint32_t)r[0], (uint32_t)r[1]);
-        }, q);
-        c = scale * exponent_f32(e);
-    }
-    __device__ __forceinline__ void clear()
-    {
+        for (int s = 0; s < kSteps; ++s) q[s] = query8<F16>(row ? row + 64 * (s >> 2) + 32 * g + 8 * (s & 3) : nullptr);
         m = kNoMax, l = 0.0f;
 #pragma unroll
         for (int t = 0; t < kTiles; ++t)
@@ -290,7 +248,7 @@ struct WaveRows {
             for (int i = 0; i < 16; ++i) acc[t][i] = 0.0f;
     }
 
-    // Scores of 64 keys: key(kt, s) gives 32 codes of this lane's matrix row.
+    // Scores of 64 keys: key(kt, s) gives 16 codes, 64 (s / 2) + 32 g + 16 (s % 2) on, of this lane's matrix row.
     template <typename Key>
     __device__ __forceinline__ void scores(Key key, f32x16_t s[2]) const
     {
@@ -299,12 +257,11 @@ struct WaveRows {
 #pragma unroll
             for (int i = 0; i < 16; ++i) s[kt][i] = 0.0f;
 #pragma unroll
-            for (int st = 0; st < kSteps; ++st) {
-                const i32x8_t a = key(kt, st);
-                s[kt] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a, q[0][st], s[kt], 0, 0, 0, kOne, 0, kOne);
-                s[kt] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a, q[1][st], s[kt], 0, 0, 0, kOne, 0, kTerm1);
-                if (kTerms == 3)
-                    s[kt] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a, q[kTerms - 1][st], s[kt], 0, 0, 0, kOne, 0, kTerm2);
+            for (int st = 0; st < kSteps / 2; ++st) {
+                Eight k[2];
+                decode16(key(kt, st), k);
+                s[kt] = Query<F16>::mma32(k[0], q[2 * st], s[kt]);
+                s[kt] = Query<F16>::mma32(k[1], q[2 * st + 1], s[kt]);
             }
         }
     }
@@ -319,10 +276,10 @@ struct WaveRows {
             for (int i = 0; i < 16; ++i) s[kt][i] = 32 * kt + i < seen ? s[kt][i] : -__builtin_inff();
     }
 
-    // Scores -> weights in binary16, for a page whose scales are 2^ek and 2^ev.
-    __device__ __forceinline__ void weights(f32x16_t s[2], int ek, int ev, f16x8_t w[2][2])
+    // Scores -> weights in binary16, for a page whose scales are 2^ek and 2^ev; scale: of the scores.
+    __device__ __forceinline__ void weights(f32x16_t s[2], float scale, int ek, int ev, f16x8_t w[2][2])
     {
-        const float f = fmaxf(c * exponent_f32(ek), 1e-37f);   // (never 0: a masked score stays -inf)
+        const float f = fmaxf(scale * exponent_f32(ek), 1e-37f);   // (never 0: a masked score stays -inf)
         const float shift = (float)ev;
         float top = larger(s[0][0], s[1][0]);
 #pragma unroll
@@ -408,50 +365,35 @@ struct WaveRows {
 // queries 61 us against 58 for two workgroups that read the pages twice, 229 against 143 at d = 256.)
 template <int D, bool F16>
 struct StepRows {
-    static constexpr int kSteps = D <= 128 ? 1 : D / 128, kTerms = F16 ? 3 : 2, kTiles = D / 16;
-    i32x8_t q[kTerms][kSteps];
+    static constexpr int kSteps = D / 32, kTiles = D / 16;
+    typedef typename Query<F16>::Eight Eight;
+    Eight q[kSteps];
     f32x4_t acc[kTiles];
-    float m, l, c;
+    float m, l;
     int limit;
 
-    // (a head of 64 fills half of the instruction's 128: the upper lanes repeat the keys against zeros)
-    __device__ __forceinline__ static void read(RawQuery<kSteps>& raw, const uint16_t* row, int g)
+    // (the inner dimension of the scores: lane group g takes elements g D / 4 on, eight a step)
+    __device__ __forceinline__ void start(const uint16_t* row, int g)
     {
-        const uint16_t* at[kSteps];
 #pragma unroll
-        for (int s = 0; s < kSteps; ++s) at[s] = row && (D > 64 || g < 2) ? row + 128 * s + 32 * g : nullptr;
-        raw.load(at);
-    }
-    __device__ __forceinline__ void start(const RawQuery<kSteps>& raw, float scale)
-    {
-        const int e = split_query<F16>(raw, [](uint32_t v) {
-            const auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
-            v = max((uint32_t)r[0], (uint32_t)r[1]);
-            const auto s = __builtin_amdgcn_permlane16_swap(v, v, false, false);
-            return max((uint32_t)s[0], (uint32_t)s[1]);
-        }, q);
-        c = scale * exponent_f32(e);
-    }
-    __device__ __forceinline__ void clear()
-    {
+        for (int s = 0; s < kSteps; ++s) q[s] = query8<F16>(row ? row + D / 4 * g + 8 * s : nullptr);
         m = kNoMax, l = 0.0f;
 #pragma unroll
         for (int t = 0; t < kTiles; ++t) acc[t] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
     }
 
-    template <typename Key>
-    __device__ __forceinline__ void scores(Key key, f32x4_t s[4]) const
+    // k[t][j]: 16 codes of a key of tile t, of this lane's D / 4.
+    __device__ __forceinline__ void scores(const uint4 (&k)[4][D / 64], f32x4_t s[4]) const
     {
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
             s[t] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-            for (int st = 0; st < kSteps; ++st) {
-                const i32x8_t a = key(t, st);
-                s[t] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, q[0][st], s[t], 0, 0, 0, kOne, 0, kOne);
-                s[t] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, q[1][st], s[t], 0, 0, 0, kOne, 0, kTerm1);
-                if (kTerms == 3)
-                    s[t] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, q[kTerms - 1][st], s[t], 0, 0, 0, kOne, 0, kTerm2);
+            for (int j = 0; j < D / 64; ++j) {
+                Eight a[2];
+                decode16(k[t][j], a);
+                s[t] = Query<F16>::mma16(a[0], q[2 * j], s[t]);
+                s[t] = Query<F16>::mma16(a[1], q[2 * j + 1], s[t]);
             }
         }
     }
@@ -465,9 +407,9 @@ struct StepRows {
             for (int i = 0; i < 4; ++i) s[t][i] = 4 * t + i < seen ? s[t][i] : -__builtin_inff();
     }
 
-    __device__ __forceinline__ void weights(const f32x4_t s[4], int ek, int ev, f16x8_t w[2])
+    __device__ __forceinline__ void weights(const f32x4_t s[4], float scale, int ek, int ev, f16x8_t w[2])
     {
-        const float shift = (float)ev, f = fmaxf(c * exponent_f32(ek), 1e-37f);
+        const float shift = (float)ev, f = fmaxf(scale * exponent_f32(ek), 1e-37f);
         float top = s[0][0];
 #pragma unroll
         for (int i = 1; i < 16; ++i) top = larger(top, s[i / 4][i % 4]);
@@ -590,9 +532,8 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_kv_attn_rows(KvAttnAr
     }
     const KvSequence s = kv_sequence(p.b, b);
     const int rows = s.n * p.group, tiles = (rows + kRows - 1) / kRows;   // (tokens * q_heads < 2^30)
-    const int at = __builtin_amdgcn_readfirstlane((int)at64);
-    if (at >= tiles) return;
-    const int r0 = at * kRows;
+    if (at64 >= (uint32_t)tiles) return;
+    const int at = __builtin_amdgcn_readfirstlane((int)at64), r0 = at * kRows;
     const int last = min(r0 + kRows, rows) - 1;
     auto limit_of = [&](int row) -> int {
         if (!p.causal) return s.length;
@@ -622,8 +563,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_kv_attn_rows(KvAttnAr
     const bool valid = row < rows;
     const int64_t token = s.start + (uint32_t)row / (uint32_t)p.group;
     const int head = h * p.group + (uint32_t)row % (uint32_t)p.group;
-    RawQuery<WaveRows<D, F16>::kSteps> raw;   // (on its way while the pages are looked up)
-    rowset.read(raw, valid ? p.q + token * p.ldq + (int64_t)head * D : nullptr, g);
+    rowset.start(valid ? p.q + token * p.ldq + (int64_t)head * D : nullptr, g);
     rowset.limit = valid ? limit_of(row) : 0;
     const int least = limit_of(min(w0, last)), most = limit_of(min(w0 + kWaveRows - 1, last));
 
@@ -685,8 +625,6 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_kv_attn_rows(KvAttnAr
     look_up(p, b, h, s.length, list, lo, hi, info);
     if (tid < 2) nan_page[tid] = -1;
     __syncthreads();
-    rowset.start(raw, p.scale);
-    rowset.clear();
     for (int first = lo; first < hi; first += kInfo) {
         const int count = min(hi - first, kInfo);
         if (first > lo) {
@@ -729,12 +667,10 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_kv_attn_rows(KvAttnAr
             if (!idle && key0 < most) {
                 const uint8_t* const kb = lds_k + buffer * kPageBytes;
                 const uint8_t* const vb = lds_v + (i & 1) * (2 * kPageBytes) + r * 128;
-                auto key = [&](int kt, int st) {
-                    const uint8_t* const at_k = kb + k_line + (D == 64 ? kt * 2048 : kt * 4096 + (st >> 1) * 8192);
-                    const int c = D == 64 ? k_chunk : k_chunk + 4 * (st & 1);
-                    const uint4 x = *reinterpret_cast<const uint4*>(at_k + ((c ^ sw) * 16));
-                    const uint4 y = *reinterpret_cast<const uint4*>(at_k + (((c + 1) ^ sw) * 16));
-                    return i32x8_t{(int)x.x, (int)x.y, (int)x.z, (int)x.w, (int)y.x, (int)y.y, (int)y.z, (int)y.w};
+                auto key = [&](int kt, int st) {   // 16 codes: 64 (st / 2) + 32 g + 16 (st % 2) on
+                    const uint8_t* const at_k = kb + k_line + (D == 64 ? kt * 2048 : kt * 4096 + (st >> 2) * 8192);
+                    const int c = (D == 64 ? k_chunk : k_chunk + 4 * ((st >> 1) & 1)) + (st & 1);
+                    return *reinterpret_cast<const uint4*>(at_k + ((c ^ sw) * 16));
                 };
                 auto value = [&](int kt, int half, int t) {
                     return *reinterpret_cast<const f16x8_t*>(vb + t * 4096 + (((4 * kt + 2 * g + half) ^ sw) * 16));
@@ -755,7 +691,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_kv_attn_rows(KvAttnAr
                     for (int tt = 0; tt < D / 32; ++tt) v0[hf][tt] = value(0, hf, tt);
                 __builtin_amdgcn_sched_barrier(0);
                 if (masked) rowset.mask(sc, key0, g);
-                rowset.weights(sc, now.ek, now.ev, w);
+                rowset.weights(sc, p.scale, now.ek, now.ev, w);
                 rowset.add_values(v0, value, w);
             }
             now = next, next = after;
@@ -797,7 +733,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_kv_attn_rows(KvAttnAr
 template <int D, bool F16>
 __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_kv_attn_step(KvAttnArgs p)
 {
-    constexpr int kTiles = D / 16, kSteps = StepRows<D, F16>::kSteps;
+    constexpr int kTiles = D / 16;
     constexpr int kPart = D < 128 ? D : 128;
     __shared__ __attribute__((aligned(16))) float acc[4][kStepRows][kPart];
     __shared__ float2 sums[4][kStepRows];   // maximum, sum
@@ -847,26 +783,22 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_kv_attn_step(KvAttnAr
     }
 
     StepRows<D, F16> rowset;
-    RawQuery<kSteps> raw;   // (on its way while the pages are looked up)
     {
         const int row = tile * kStepRows + r, own = at + row / p.group;
         const bool valid = row < rows;
-        rowset.read(raw, valid ? p.q + (s.start + own) * p.ldq + (int64_t)(h * p.group + row % p.group) * D : nullptr, g);
-        rowset.clear();
+        rowset.start(valid ? p.q + (s.start + own) * p.ldq + (int64_t)(h * p.group + row % p.group) * D : nullptr, g);
         rowset.limit = valid ? limit_of(own) : 0;
     }
     const int least = limit_of(first_token), most = limit_of(last_token);
 
-    const int from_k = (16 * (r >> 2) + (r & 3)) * D + 32 * (D == 64 ? g & 1 : g), from_v = r * kPage + 16 * g;
-    uint4 kr[4][kSteps][2], vr[kTiles];
+    const int from_k = (16 * (r >> 2) + (r & 3)) * D + D / 4 * g, from_v = r * kPage + 16 * g;
+    uint4 kr[4][D / 64], vr[kTiles];
     auto load_k = [&](const PageInfo& a) {
         const uint8_t* const src = p.c.k + ((int64_t)max(a.page, 0) * p.c.heads + h) * (kPage * D);
 #pragma unroll
         for (int t = 0; t < 4; ++t)
 #pragma unroll
-            for (int st = 0; st < kSteps; ++st)
-#pragma unroll
-                for (int j = 0; j < 2; ++j) kr[t][st][j] = *reinterpret_cast<const uint4*>(src + from_k + t * 4 * D + st * 128 + j * 16);
+            for (int j = 0; j < D / 64; ++j) kr[t][j] = *reinterpret_cast<const uint4*>(src + from_k + t * 4 * D + j * 16);
     };
     auto load_v = [&](const PageInfo& a) {
         const uint8_t* const src = p.c.v + ((int64_t)max(a.page, 0) * p.c.heads + h) * (kPage * D);
@@ -875,7 +807,6 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_kv_attn_step(KvAttnAr
     };
     look_up(p, b, h, s.length, list, lo, hi, info);
     __syncthreads();
-    rowset.start(raw, p.scale);
     for (int first = lo; first < hi; first += kInfo) {
         const int count = min(hi - first, kInfo);
         if (first > lo) {
@@ -895,16 +826,13 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_kv_attn_step(KvAttnAr
             if (more) next = info_at(info, i + 4);
             f32x4_t sc[4];
             f16x8_t w[2];
-            rowset.scores([&](int t, int st) {
-                const uint4 x = kr[t][st][0], y = kr[t][st][1];
-                return i32x8_t{(int)x.x, (int)x.y, (int)x.z, (int)x.w, (int)y.x, (int)y.y, (int)y.z, (int)y.w};
-            }, sc);
+            rowset.scores(kr, sc);
             if (more) load_k(next);
             const int key0 = first_key(now);
             if (key0 < most) {
                 const bool masked = key0 + kPage > least;
                 if (masked) rowset.mask(sc, key0, g);
-                rowset.weights(sc, now.ek, now.ev, w);
+                rowset.weights(sc, p.scale, now.ek, now.ev, w);
                 if (masked) rowset.settle_values(vr, key0, s.length, g);
                 rowset.add_values(vr, w);
             }
@@ -1032,7 +960,7 @@ Plan make_plan(KvAttnArgs& p, int64_t max_query, int cus)
     }
     // Splits where the workgroups alone leave compute units idle: enough for four workgroups (steps) or two
     // (rows) on each, of at least eight (four) pages, and none below 32: a page costs a wave of k_kv_attn_step about
-    // 0.8 us where nothing else runs, the join and its launch 4 (13 pages of 8 heads: TODO us whole, TODO in four).
+    // 0.8 us where nothing else runs, the join and its launch 4 (13 pages of 8 heads: 10.1 us whole, 7.7 + 3.9 in four).
     const int64_t want = (int64_t)cus * (plan.step ? 4 : 2), least = plan.step ? 8 : 4;
     int64_t splits = groups > 0 ? want / groups : 1;
     splits = pages < 32 ? 1 : splits < pages / least ? splits : pages / least;
