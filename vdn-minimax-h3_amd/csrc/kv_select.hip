@@ -437,9 +437,9 @@ extern "C" int vdn_fp8_kv_select(const vdn_fp8_kv_cache* cache, const vdn_fp8_kv
     p.score = (double*)(p.sum + p.rows * p.c.heads * p.c.d);
     const dim3 block(kThreads), per_row((unsigned)(p.rows * p.c.heads));
     const bool f16 = dtype == VDN_FP8_DTYPE_F16;
-    if (p.b.width > 0 && p.query_block == 1 && p.rows <= 65535) {
-        const int64_t pages = 4 * 4 * (64 / (p.c.d / 8));   // of a workgroup
-        const dim3 grid((unsigned)((p.b.width + pages - 1) / pages), (unsigned)p.c.heads, (unsigned)p.rows);
+    const int64_t step_pages = 4 * 4 * (64 / (p.c.d / 8)), step_groups = (p.b.width + step_pages - 1) / step_pages;   // of k_kv_scores_step
+    if (p.b.width > 0 && p.query_block == 1 && p.rows <= 65535 && step_groups * p.c.heads * p.rows < (1 << 24)) {
+        const dim3 grid((unsigned)step_groups, (unsigned)p.c.heads, (unsigned)p.rows);
 #define VDN_STEP(n)                                                                                         \
     case n:                                                                                                 \
         if (f16) hipLaunchKernelGGL((k_kv_scores_step<n, true>), grid, block, 0, stream, p);                \
