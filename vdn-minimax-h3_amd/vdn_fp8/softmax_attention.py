@@ -9,6 +9,9 @@ it is a hand-written HIP kernel (`vdn_fp8_qk_prep`). Numerics follow the compile
 kernel: binary32 throughout, the cos/sin tables rounded to bf16 first
 (`cos.to(x.dtype)`), one rounding at the store -- not bitwise with the eager chain,
 which rounds after every op, exactly as the reference notes for its own kernel.
+
+`cached_attention` is the branch over tokens of earlier calls, kept in 8 bits
+(`vdn_fp8.kv_cache`).
 """
 import torch
 
@@ -60,6 +63,16 @@ def qk_prep(t, weight, eps, cos=None, sin=None):
 _qk_prep = qk_prep
 
 
+def _project(x, projections):
+    """Every projection of x; fp8 ones share one quantization of it."""
+    from .fp8_linear import Fp8Linear, quantize_activation
+
+    if all(isinstance(p, Fp8Linear) for p in projections):
+        x_fp8, x_scale = quantize_activation(x)
+        return [p.forward_quantized(x_fp8, x_scale, out_dtype=x.dtype) for p in projections]
+    return [p(x) for p in projections]
+
+
 def qkv(x, to_q, to_k, to_v, heads, norm_q, norm_k, rotary_emb=None):
     """The inference body of `HybridAttention._qkv` (hybrid_attention.py:108-137) on this
     library: with fp8 projections x is quantized ONCE and shared by the three GEMMs
@@ -70,16 +83,35 @@ def qkv(x, to_q, to_k, to_v, heads, norm_q, norm_k, rotary_emb=None):
     everything [T, heads, d] -- the raw q/k are the ones the linear branch consumes.
     Without rotary_emb the norms alone run (the same kernel with no rotation), as the
     reference's eager branch would apply them."""
-    from .fp8_linear import Fp8Linear, quantize_activation
-
-    projections = (to_q, to_k, to_v)
-    if all(isinstance(p, Fp8Linear) for p in projections):
-        x_fp8, x_scale = quantize_activation(x)
-        out = [p.forward_quantized(x_fp8, x_scale, out_dtype=x.dtype) for p in projections]
-    else:
-        out = [p(x) for p in projections]
+    out = _project(x, (to_q, to_k, to_v))
     query_raw, key_raw, value = (t.unflatten(-1, (heads, -1)) for t in out)
     cos, sin = (None, None) if rotary_emb is None else rotary_emb
     query = qk_prep(query_raw, norm_q.weight, norm_q.eps, cos, sin)
     key = qk_prep(key_raw, norm_k.weight, norm_k.eps, cos, sin)
     return query, key, value, (query_raw, key_raw, value)
+
+
+def cached_attention(x, to_q, to_k, to_v, norm_q, norm_k, cache, page_table, lengths, *, rotary_emb=None, causal=False,
+                     scale=None, q_start=None, max_query=None, top=None, query_block=None):
+    """`qkv` and the attention behind it where earlier tokens are kept in a `KvCache`: one quantization
+    of x for the three GEMMs, then QK-norm, rope and the store of k and v in one launch
+    (`qk_prep_append`), then `kv_attention` over each sequence's cache, its new tokens included. The cache's
+    shape gives the heads; to_q may have more of them (a multiple of the cache's). x [T, hidden] bf16;
+    projections, norms and rotary_emb as in `qkv`; page_table, lengths, q_start, max_query, causal and scale
+    as in `kv_attention`. With `top`, each block of `query_block` queries attends to the `top` pages
+    that `kv_select` finds for it. Returns [T, q_heads * d], what the output projection takes."""
+    from .kv_cache import kv_attention, kv_select, qk_prep_append
+
+    if (top is None) != (query_block is None):
+        raise ValueError("top and query_block go together")
+    d = cache.k.shape[-1]
+    query, key, value = (t.unflatten(-1, (-1, d)) for t in _project(x, (to_q, to_k, to_v)))
+    cos, sin = (None, None) if rotary_emb is None else rotary_emb
+    query = qk_prep_append(query, key, value, (norm_q.weight, norm_q.eps), (norm_k.weight, norm_k.eps), cache, page_table, lengths,
+                           cos=cos, sin=sin, q_start=q_start)
+    blocks = None
+    if top is not None:
+        blocks = kv_select(query, cache, page_table, lengths, top, query_block=query_block, causal=causal, q_start=q_start)
+    out = kv_attention(query, cache, page_table, lengths, scale=scale, causal=causal, q_start=q_start, max_query=max_query, blocks=blocks,
+                       query_block=query_block)
+    return out.flatten(1)
