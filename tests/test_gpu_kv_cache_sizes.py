@@ -133,6 +133,25 @@ def test_more_pages_than_a_workgroup_looks_up(device, n, B, H, group):
         assert bool(((z[rows].double().cpu() - wz).abs() <= tol_z).all())
 
 
+@pytest.mark.parametrize("rows", [1, 20, 150])
+@pytest.mark.parametrize("order", [[0, 1, 2, 3], [3, 2, 1, 0], [1, 3, 0, 2]])
+def test_scales_of_values_further_apart_than_a_float(device, rows, order):
+    """Pages of zeros and tiny values beside pages of enormous ones: the former take no less of the weight,
+    whichever come first, in one pass and where the keys are split."""
+    H, d = 1, 64
+    g = torch.Generator().manual_seed(14)
+    for pages in (4, 64):
+        sizes = [0.0, 1e-24, 1.0, 1e33] * (pages // 4)
+        value = torch.cat([torch.randn(PAGE, H, d, generator=g) * sizes[(w // 4) * 4 + order[w % 4]] for w in range(pages)]).to(BF16)
+        n = pages * PAGE
+        cache, table = R.Cache(pages, H, d, seed=2), [list(range(pages))]
+        R.append(cache, torch.randn(n, H, d, generator=g).to(BF16), value, table, [n], [0, n])
+        print(f"far apart rows={rows} pages={pages} {order}", flush=True)
+        q = torch.randn(rows, 2, d, generator=g).to(BF16)
+        attention_case(device, BF16, 2, H, d, [rows], [n], False, cache=cache, table=table, q=q)
+        attention_case(device, BF16, 2, H, d, [rows], [n], False, cache=cache, table=table, q=q, scale=2.0)
+
+
 @pytest.mark.parametrize("n", [1, 40])
 def test_a_table_without_columns(device, n):
     """No sequence has a page: nothing is stored, every row is zeros, every list empty."""

@@ -106,6 +106,24 @@ __device__ __forceinline__ float added(float a, float b) { return a + b; }
 
 __device__ __forceinline__ float exponent_f32(int e) { return __uint_as_float((uint32_t)(min(max(e, -126), 127) + 127) << 23); }
 
+// v 2^e, where 2^e alone may be below the least float.
+__device__ __forceinline__ float times_power(float v, float e)
+{
+    const float half = __builtin_amdgcn_exp2f(0.5f * e);
+    return v * half * half;
+}
+
+// A page whose values are smaller than others' by orders has weights P' that are as much smaller: nothing next to
+// what the accumulators hold, but 2^-ev times their sum counts. Where a row's largest, 2^(top - m), is below 2^-60, its
+// weights are lifted to that (still zeros in binary16) and their sum is brought down again.
+__device__ __forceinline__ float lift_of(float top, float m) { return __builtin_amdgcn_fmed3f(m - top - 60.0f, 0.0f, 400.0f); }
+__device__ __forceinline__ void add_sum(float& l, float sum, int ev, float lift)
+{
+    float part = sum * exponent_f32(-ev);
+    if (__any(lift > 0.0f)) part = times_power(part, -lift);
+    l += part;
+}
+
 // 16 codes of one operand row -> two operands of eight values (exact).
 __device__ __forceinline__ void decode16(uint4 w, f16x8_t o[2])
 {
@@ -287,14 +305,14 @@ struct WaveRows {
         top = across32(top, larger) * f + shift;
         if (__any(top > m + kSlack)) {
             const float now = fmaxf(m, top), a = __builtin_amdgcn_exp2f(m - now);
+            l = times_power(l, m - now);
             m = now;
-            l *= a;
 #pragma unroll
             for (int t = 0; t < kTiles; ++t)
 #pragma unroll
                 for (int i = 0; i < 16; ++i) acc[t][i] *= a;
         }
-        const float base = shift - m;
+        const float lift = lift_of(top, m), base = shift - m + lift;
         float sum = 0.0f;
 #pragma unroll
         for (int kt = 0; kt < 2; ++kt)
@@ -306,7 +324,7 @@ struct WaveRows {
                     sum += p;
                     w[kt][h][j] = (_Float16)p;
                 }
-        l = __builtin_fmaf(sum, exponent_f32(-ev), l);
+        add_sum(l, sum, ev, lift);
     }
 
     // Adds the weighted values of a page: value(kt, h, t) gives one element's values of the eight tokens from
@@ -416,12 +434,12 @@ struct StepRows {
         top = across16(across32(top, larger), larger) * f + shift;
         if (__any(top > m + kSlack)) {
             const float now = fmaxf(m, top), a = __builtin_amdgcn_exp2f(m - now);
+            l = times_power(l, m - now);
             m = now;
-            l *= a;
 #pragma unroll
             for (int t = 0; t < kTiles; ++t) acc[t] *= a;
         }
-        const float base = shift - m;
+        const float lift = lift_of(top, m), base = shift - m + lift;
         float sum = 0.0f;
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
@@ -429,7 +447,7 @@ struct StepRows {
             sum += p;
             w[i / 8][i % 8] = (_Float16)p;
         }
-        l = __builtin_fmaf(sum, exponent_f32(-ev), l);
+        add_sum(l, sum, ev, lift);
     }
 
     // v[t]: the codes of 16 tokens, one element.
@@ -862,9 +880,9 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_kv_attn_step(KvAttnAr
             float total = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (int wv = 0; wv < 4; ++wv) {
-                const float f = __builtin_amdgcn_exp2f(sums[wv][row_e].x - m);
+                const float e = sums[wv][row_e].x - m, f = __builtin_amdgcn_exp2f(e);
                 const float4 a = *reinterpret_cast<const float4*>(&acc[wv][row_e][d]);
-                total += f * sums[wv][row_e].y;
+                total += times_power(sums[wv][row_e].y, e);
                 o[0] += f * a.x, o[1] += f * a.y, o[2] += f * a.z, o[3] += f * a.w;
             }
             const int row_at = tile * kStepRows + row_e;
@@ -899,7 +917,7 @@ __global__ __launch_bounds__(256) void k_kv_attn_join(KvAttnArgs p)
 #pragma unroll
     for (int off = 1; off < 64; off <<= 1) m = fmaxf(m, __shfl_xor(m, off, 64));
     const float f = __builtin_amdgcn_exp2f(own.x - m);
-    float total = f * own.y;
+    float total = times_power(own.y, own.x - m);
 #pragma unroll
     for (int off = 1; off < 64; off <<= 1) total += __shfl_xor(total, off, 64);
     float o[E];

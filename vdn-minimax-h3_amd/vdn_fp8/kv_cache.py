@@ -140,7 +140,7 @@ def kv_append(key, value, cache, page_table, lengths, *, q_start=None):
     and no smaller than before where the page keeps earlier tokens (their codes then move to
     the new scale); each element is rounded once; infinities and NaN are stored as NaN. Positions
     below 0, beyond the table, or in a page that is not there are left out; a page may receive
-    tokens of one sequence only."""
+    tokens of one sequence only, at one place of its table."""
     d, heads = cache.k.shape[-1], cache.k.shape[1]
     key = _rows(key, heads, d, "key", tuple(_DTYPES))
     value = _rows(value, heads, d, "value", (key.dtype,))
