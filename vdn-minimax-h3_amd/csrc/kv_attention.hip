@@ -102,6 +102,7 @@ __device__ __forceinline__ float across16(float v, F f)
 }
 // (NaN wins: the row becomes NaN anyway, and one instruction takes two values without quieting them first)
 __device__ __forceinline__ float larger(float a, float b) { return __builtin_elementwise_maximum(a, b); }
+__device__ __forceinline__ float larger3(float a, float b, float c) { return larger(larger(a, b), c); }   // (one instruction)
 __device__ __forceinline__ float added(float a, float b) { return a + b; }
 
 __device__ __forceinline__ float exponent_f32(int e) { return __uint_as_float((uint32_t)(min(max(e, -126), 127) + 127) << 23); }
@@ -299,10 +300,14 @@ struct WaveRows {
     {
         const float f = fmaxf(scale * exponent_f32(ek), 1e-37f);   // (never 0: a masked score stays -inf)
         const float shift = (float)ev;
-        float top = larger(s[0][0], s[1][0]);
+        float four[4];   // (two new scores an instruction)
 #pragma unroll
-        for (int i = 1; i < 16; ++i) top = larger(top, larger(s[0][i], s[1][i]));
-        top = across32(top, larger) * f + shift;
+        for (int i = 0; i < 4; ++i) {
+            const f32x16_t& a = s[i / 2];
+            const int j = 8 * (i % 2);
+            four[i] = larger3(larger3(larger3(larger(a[j], a[j + 1]), a[j + 2], a[j + 3]), a[j + 4], a[j + 5]), a[j + 6], a[j + 7]);
+        }
+        const float top = across32(larger(larger3(four[0], four[1], four[2]), four[3]), larger) * f + shift;
         if (__any(top > m + kSlack)) {
             const float now = fmaxf(m, top), a = __builtin_amdgcn_exp2f(m - now);
             l = times_power(l, m - now);
@@ -428,10 +433,10 @@ struct StepRows {
     __device__ __forceinline__ void weights(const f32x4_t s[4], float scale, int ek, int ev, f16x8_t w[2])
     {
         const float shift = (float)ev, f = fmaxf(scale * exponent_f32(ek), 1e-37f);
-        float top = s[0][0];
+        float four[4];
 #pragma unroll
-        for (int i = 1; i < 16; ++i) top = larger(top, s[i / 4][i % 4]);
-        top = across16(across32(top, larger), larger) * f + shift;
+        for (int i = 0; i < 4; ++i) four[i] = larger(larger3(s[i][0], s[i][1], s[i][2]), s[i][3]);
+        const float top = across16(across32(larger(larger3(four[0], four[1], four[2]), four[3]), larger), larger) * f + shift;
         if (__any(top > m + kSlack)) {
             const float now = fmaxf(m, top), a = __builtin_amdgcn_exp2f(m - now);
             l = times_power(l, m - now);
