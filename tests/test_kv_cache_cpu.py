@@ -77,6 +77,7 @@ def select(c=None, b=None, q=FAKE, dtype=0, heads=4, ldq=512, top=4, first=1, la
     (lambda: attention(out=FAKE + 2), "misaligned"),
     (lambda: attention(scale=0.0), "scale"),
     (lambda: attention(scale=float("inf")), "scale"),
+    (lambda: attention(scale=3e38), "scale"),   # (times log2(e) it is beyond binary32)
     (lambda: attention(scale=float("nan")), "scale"),
     (lambda: attention(most=-1), "max_query"),
     (lambda: attention(b=batch(tokens=1 << 30)), "2^30"),
@@ -150,6 +151,20 @@ def test_cache_checks(change, needle):
     from vdn_fp8 import kv_cache as K
     with pytest.raises(ValueError, match=needle):
         K._cache(pool(**change), torch.device("cpu"))
+
+
+def test_the_branch_refuses_before_it_stores():
+    """What a later part of `cached_attention` would refuse is refused before anything is stored."""
+    from vdn_fp8.softmax_attention import cached_attention
+    x, table, lengths = torch.zeros(2, 8, dtype=torch.bfloat16), torch.zeros(1, 3, dtype=torch.int32), torch.zeros(1, dtype=torch.int32)
+    to = [torch.nn.Linear(8, n, dtype=torch.bfloat16) for n in (128, 128, 128)]
+    norm = torch.nn.RMSNorm(64, eps=1e-6, dtype=torch.bfloat16)
+    odd = torch.nn.Linear(8, 192, dtype=torch.bfloat16)
+    for args, more, needle in (((*to, norm, norm, pool()), dict(top=2), "query_block"), ((*to, norm, norm, pool()), dict(query_block=64), "query_block"),
+                               ((*to, norm, norm, pool(k_mean=None)), dict(top=2, query_block=64), "k_mean"),
+                               ((odd, *to[1:], norm, norm, pool()), {}, "query heads"), ((*to, norm, norm, pool()), {}, "GPU")):
+        with pytest.raises(ValueError, match=needle):
+            cached_attention(x, *args, table, lengths, **more)
 
 
 def test_batch_checks():

@@ -244,7 +244,7 @@ __device__ __forceinline__ f16x8_t seen_ones(int first, int limit)
     return o;
 }
 
-// One wave's 32 rows of k_kv_attn_rows: the queries' terms, the running softmax, the output's accumulators.
+// One wave's 32 rows of k_kv_attn_rows: the queries, the running softmax, the output's accumulators.
 // Lane l: column l % 32 is the row of the problem, g = l / 32 its half of the keys.
 template <int D, bool F16>
 struct WaveRows {
@@ -1066,7 +1066,7 @@ extern "C" int vdn_fp8_kv_attention(const vdn_fp8_kv_cache* cache, const vdn_fp8
     if (ldq % 8 || ldq < q_heads * p.c.d) return set_error(VDN_FP8_EINVAL, "kv_attention: need ldq a multiple of 8 and >= q_heads * head_dim");
     if (!aligned(query, 16) || !aligned(out, 16) || !aligned(lse, 4) || !aligned(blocks, 4) || !aligned(workspace, 16))
         return set_error(VDN_FP8_EINVAL, "kv_attention: misaligned pointer (query, out, workspace 16 B; lse, blocks 4 B)");
-    if (!(scale > 0.0f) || scale > 3e38f) return set_error(VDN_FP8_EINVAL, "kv_attention: scale must be positive and finite");
+    if (!(scale > 0.0f) || scale > 2e38f) return set_error(VDN_FP8_EINVAL, "kv_attention: scale must be positive and finite");
     const int cus = device_cus();
     if (cus == 0) return set_error(VDN_FP8_ELAUNCH, "kv_attention: the device cannot be queried");
     const Plan plan = make_plan(p, max_query, cus);

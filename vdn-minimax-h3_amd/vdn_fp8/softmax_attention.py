@@ -102,10 +102,15 @@ def cached_attention(x, to_q, to_k, to_v, norm_q, norm_k, cache, page_table, len
     that `kv_select` finds for it. Returns [T, q_heads * d], what the output projection takes."""
     from .kv_cache import kv_attention, kv_select, qk_prep_append
 
+    # (what only a later part would refuse is refused before the store)
     if (top is None) != (query_block is None):
         raise ValueError("top and query_block go together")
-    d = cache.k.shape[-1]
+    if top is not None and cache.k_mean is None:
+        raise ValueError("top needs a cache that keeps k_mean")
+    heads, d = cache.k.shape[1], cache.k.shape[-1]
     query, key, value = (t.unflatten(-1, (-1, d)) for t in _project(x, (to_q, to_k, to_v)))
+    if query.shape[1] % heads:
+        raise ValueError(f"{query.shape[1]} query heads for a cache of {heads}")
     cos, sin = (None, None) if rotary_emb is None else rotary_emb
     query = qk_prep_append(query, key, value, (norm_q.weight, norm_q.eps), (norm_k.weight, norm_k.eps), cache, page_table, lengths,
                            cos=cos, sin=sin, q_start=q_start)
