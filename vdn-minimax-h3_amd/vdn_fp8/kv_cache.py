@@ -57,23 +57,35 @@ class KvCache(NamedTuple):
 
 
 def _cache(cache, device):
-    """The C struct of a cache, checked."""
+    """The C struct of a cache, checked. (Each of a tensor's properties read once: 0.1 us a piece.)"""
     k, v, ks, vs, mean = cache
     shape = k.shape
-    if len(shape) != 4 or k.dtype != FP8_DTYPE or shape[2] != KV_PAGE:
+    if k.dtype is not FP8_DTYPE or len(shape) != 4 or shape[2] != KV_PAGE:
         raise ValueError(f"cache.k must be float8_e4m3fn [pages, heads, {KV_PAGE}, d] (got {k.dtype} {tuple(shape)})")
     P, H, _, d = shape
-    if v.shape != (P, H, d, KV_PAGE) or v.dtype != FP8_DTYPE:
+    if v.dtype is not FP8_DTYPE or v.shape != (P, H, d, KV_PAGE):
         raise ValueError(f"cache.v must be float8_e4m3fn [{P}, {H}, {d}, {KV_PAGE}] (got {v.dtype} {tuple(v.shape)})")
-    if ks.shape != (P, H) or vs.shape != (P, H) or ks.dtype != SCALE_DTYPE or vs.dtype != SCALE_DTYPE:
+    each = (P, H)
+    if ks.dtype is not SCALE_DTYPE or vs.dtype is not SCALE_DTYPE or ks.shape != each or vs.shape != each:
         raise ValueError(f"cache.k_scale and v_scale must be float8_e8m0fnu [{P}, {H}]")
-    if mean is not None and (mean.shape != (P, H, d) or mean.dtype != torch.bfloat16):
-        raise ValueError(f"cache.k_mean must be bfloat16 [{P}, {H}, {d}]")
     at = _index(device)
-    for t in (k, v, ks, vs, mean):
-        if t is not None and (t.get_device() != at or not t.is_contiguous()):
-            raise ValueError(f"the cache's tensors must be contiguous, on {device}")
-    return _lib.KvCacheStruct(k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr(), None if mean is None else mean.data_ptr(), P, H, d)
+    here = (k.get_device() == at and v.get_device() == at and ks.get_device() == at and vs.get_device() == at and
+            k.is_contiguous() and v.is_contiguous() and ks.is_contiguous() and vs.is_contiguous())
+    mean_ptr = None
+    if mean is not None:
+        if mean.dtype is not torch.bfloat16 or mean.shape != (P, H, d):
+            raise ValueError(f"cache.k_mean must be bfloat16 [{P}, {H}, {d}]")
+        here = here and mean.get_device() == at and mean.is_contiguous()
+        mean_ptr = mean.data_ptr()
+    if not here:
+        raise ValueError(f"the cache's tensors must be contiguous, on {device}")
+    return _lib.KvCacheStruct(k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr(), mean_ptr, P, H, d)
+
+
+def _heads(cache):
+    """Heads and their size (whatever else is wrong with the cache, `_cache` says)."""
+    shape = cache.k.shape
+    return (shape[1], shape[3]) if len(shape) == 4 else (1, 0)
 
 
 def _index(device):
@@ -84,25 +96,32 @@ def _index(device):
 def _batch(page_table, lengths, q_start, tokens, pages, device):
     """The C struct of a batch, checked (and what it points to, to be kept until the launch)."""
     shape = page_table.shape
-    if len(shape) != 2 or page_table.dtype != torch.int32 or (shape[1] > 1 and page_table.stride(1) != 1):
+    if page_table.dtype is not torch.int32 or len(shape) != 2:
         raise ValueError("page_table must be int32 [B, W] with unit column stride")
     B, W = shape
-    if lengths.shape != (B,) or lengths.dtype != torch.int32 or not lengths.is_contiguous():
+    ld, unit = page_table.stride()
+    if unit != 1 and W > 1:
+        raise ValueError("page_table must be int32 [B, W] with unit column stride")
+    if lengths.dtype is not torch.int32 or lengths.shape != (B,) or not lengths.is_contiguous():
         raise ValueError(f"lengths must be a contiguous int32 [{B}] tensor")
-    if q_start is not None and (q_start.shape != (B + 1,) or q_start.dtype != torch.int32 or not q_start.is_contiguous()):
-        raise ValueError(f"q_start must be a contiguous int32 [{B + 1}] tensor")
     at = _index(device)
-    if page_table.get_device() != at or lengths.get_device() != at or (q_start is not None and q_start.get_device() != at):
+    here = page_table.get_device() == at and lengths.get_device() == at
+    start = None
+    if q_start is not None:
+        if q_start.dtype is not torch.int32 or q_start.shape != (B + 1,) or not q_start.is_contiguous():
+            raise ValueError(f"q_start must be a contiguous int32 [{B + 1}] tensor")
+        here = here and q_start.get_device() == at
+        start = q_start.data_ptr()
+    if not here:
         raise ValueError(f"page_table, lengths and q_start must be on {device}")
     if tokens and not B:
         raise ValueError(f"{tokens} tokens of an empty batch")
-    if q_start is None and B and tokens % B:
+    if start is None and B and tokens % B:
         raise ValueError(f"{tokens} tokens do not divide among {B} sequences: pass q_start")
     check_index_range(lengths, W * KV_PAGE + 1, "lengths")
     if q_start is not None:
         check_index_range(q_start, tokens + 1, "q_start")
-    ld = page_table.stride(0) if B > 1 else W
-    return _lib.KvBatchStruct(page_table.data_ptr(), ld, W, lengths.data_ptr(), None if q_start is None else q_start.data_ptr(), B, tokens)
+    return _lib.KvBatchStruct(page_table.data_ptr(), ld if B > 1 else W, W, lengths.data_ptr(), start, B, tokens)
 
 
 def _rows(t, heads, d, name, dtypes):
@@ -121,7 +140,8 @@ def _rows(t, heads, d, name, dtypes):
 
 
 def _ld(t):
-    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1] * t.shape[2])
+    rows, heads, d = t.shape
+    return t.stride(0) if rows > 1 else max(t.stride(0), heads * d)
 
 
 _HERE = contextlib.nullcontext()
@@ -141,7 +161,7 @@ def kv_append(key, value, cache, page_table, lengths, *, q_start=None):
     the new scale); each element is rounded once; infinities and NaN are stored as NaN. Positions
     below 0, beyond the table, or in a page that is not there are left out; a page may receive
     tokens of one sequence only, at one place of its table."""
-    d, heads = cache.k.shape[-1], cache.k.shape[1]
+    heads, d = _heads(cache)
     key = _rows(key, heads, d, "key", tuple(_DTYPES))
     value = _rows(value, heads, d, "value", (key.dtype,))
     dev, T = key.device, key.shape[0]
@@ -170,7 +190,7 @@ def qk_prep_append(query, key, value, norm_q, norm_k, cache, page_table, lengths
     likewise, then the rotation by cos, sin [T, R] -- and `kv_append` of that key and the value, in one
     launch with the same bits. query bf16 [T, q_heads, d], key and value bf16 [T, heads, d] (column
     slices of one projection's output are fine). Returns the prepared query, a new [T, q_heads, d]."""
-    d, heads = cache.k.shape[-1], cache.k.shape[1]
+    heads, d = _heads(cache)
     bf16 = (torch.bfloat16,)
     query = _rows(query, None, d, "query", bf16)
     key, value = _rows(key, heads, d, "key", bf16), _rows(value, heads, d, "value", bf16)
@@ -186,13 +206,14 @@ def qk_prep_append(query, key, value, norm_q, norm_k, cache, page_table, lengths
         at = _index(dev)
         if cos.dim() != 2 or cos.get_device() != at or sin.dim() != 2 or sin.get_device() != at:
             cos, sin = cos.detach().to(dev).reshape(-1, cos.shape[-1]), sin.detach().to(dev).reshape(-1, sin.shape[-1])
-        if cos.shape != sin.shape or cos.shape[0] != T or cos.dtype != sin.dtype:
+        shape, kind = cos.shape, cos.dtype
+        if sin.shape != shape or shape[0] != T or sin.dtype is not kind:
             raise ValueError(f"cos/sin must both be [T={T}, R] of one dtype (got {tuple(cos.shape)}, {tuple(sin.shape)})")
-        if cos.dtype not in (torch.float32, torch.bfloat16):
+        if kind is not torch.float32 and kind is not torch.bfloat16:
             cos, sin = cos.float(), sin.float()
         cos, sin = _aligned16(cos.contiguous()), _aligned16(sin.contiguous())
-        R = ldcs = cos.shape[1]
-        bf16_table = int(cos.dtype == torch.bfloat16)
+        R = ldcs = shape[1]
+        bf16_table = int(kind is torch.bfloat16)
     c = _cache(cache, dev)
     b = _batch(page_table, lengths, q_start, T, c.pages, dev)
     out = torch.empty(T, q_heads, d, device=dev, dtype=torch.bfloat16)
@@ -242,9 +263,9 @@ def kv_attention(query, cache, page_table, lengths, *, scale=None, causal=False,
     sequence take another kernel (rows beyond it are not computed).
     blocks, query_block: int32 [rows, heads, top] from `kv_select` (or a caller's own list; entries
     outside the sequence are skipped, one listed twice counts twice): only those pages are read."""
-    d, heads = cache.k.shape[-1], cache.k.shape[1]
+    heads, d = _heads(cache)
     query = _rows(query, None, d, "query", _QUERY_DTYPES)
-    dev, T, q_heads = query.device, query.shape[0], query.shape[1]
+    dev, (T, q_heads, _) = query.device, query.shape
     if q_heads % heads or not q_heads:
         raise ValueError(f"{q_heads} query heads for a cache of {heads}")
     c = _cache(cache, dev)
@@ -280,9 +301,9 @@ def kv_select(query, cache, page_table, lengths, top, *, query_block, first=1, l
     a multiple of 128. rows: T for query_block = 1; B * ceil(T / B / query_block) without q_start,
     T // query_block + B with it (sequence b's blocks from q_start[b] // query_block + b on; rows that
     no block takes hold -1)."""
-    d, heads = cache.k.shape[-1], cache.k.shape[1]
+    heads, d = _heads(cache)
     query = _rows(query, None, d, "query", _QUERY_DTYPES)
-    dev, T, q_heads = query.device, query.shape[0], query.shape[1]
+    dev, (T, q_heads, _) = query.device, query.shape
     if q_heads % heads or not q_heads:
         raise ValueError(f"{q_heads} query heads for a cache of {heads}")
     if cache.k_mean is None:
