@@ -245,9 +245,9 @@ __device__ __forceinline__ void store_page(const KvAppendArgs& p, uint32_t unit,
     const uint32_t turns = (uint32_t)(p.c.heads + p.unit_heads - 1) / (uint32_t)p.unit_heads;
     const int h0 = (int)(unit % turns) * p.unit_heads, h_end = min(h0 + p.unit_heads, p.c.heads);
     uint32_t at;
-    const int b = kv_locate(p.b, p.units, unit / turns, at);
+    KvSequence s{};
+    const int b = kv_locate(p.b, p.units, unit / turns, at, s);
     if (b == p.b.batch) return;   // behind the last sequence
-    const KvSequence s = kv_sequence(p.b, b);
     const int64_t w64 = max(s.first, (int64_t)0) / kPage + at;
     if (w64 * kPage >= s.length) return;
     const int w = (int)w64;

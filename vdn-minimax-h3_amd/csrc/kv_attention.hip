@@ -543,7 +543,8 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_kv_attn_rows(KvAttnAr
     const int h = __builtin_amdgcn_readfirstlane((int)(item / units));
     uint32_t at64;
     // (the last units of a sequence first: with a causal mask they are the longest)
-    const int b = __builtin_amdgcn_readfirstlane(kv_locate(p.b, p.units, units - 1 - item % units, at64));
+    KvSequence s{};
+    const int b = __builtin_amdgcn_readfirstlane(kv_locate(p.b, p.units, units - 1 - item % units, at64, s));
     if (b == p.b.batch) {   // behind the last sequence
         if (split == 0) {
             const int64_t end = min(max((int64_t)p.b.q_start[b], (int64_t)0), p.b.tokens);
@@ -553,7 +554,6 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_kv_attn_rows(KvAttnAr
         }
         return;
     }
-    const KvSequence s = kv_sequence(p.b, b);
     const int rows = s.n * p.group, tiles = (rows + kRows - 1) / kRows;   // (tokens * q_heads < 2^30)
     if (at64 >= (uint32_t)tiles) return;
     const int at = __builtin_amdgcn_readfirstlane((int)at64), r0 = at * kRows;
@@ -772,15 +772,13 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_kv_attn_step(KvAttnAr
     const int h = __builtin_amdgcn_readfirstlane((int)(item % p.c.heads));
     const uint32_t unit = item / p.c.heads;
     int b = (int)unit;
+    KvSequence s{};
     if (p.blocks) {   // a unit is a token
-        if (p.b.q_start) {
-            uint32_t none;
-            b = kv_locate(p.b, KvUnits{1, 1, 1, 0}, unit, none);
-        } else {
-            b = (int)(unit / (uint32_t)p.b.each);
-        }
+        uint32_t at_token;
+        b = __builtin_amdgcn_readfirstlane(kv_locate(p.b, KvUnits{1, (uint32_t)p.b.each, 1, 0}, unit, at_token, s));
+    } else if (b < p.b.batch) {
+        s = kv_sequence(p.b, b);
     }
-    b = __builtin_amdgcn_readfirstlane(b);
     if (b == p.b.batch) {   // behind the last sequence
         if (split == 0 && tile == 0) {
             const int64_t end = min(max((int64_t)p.b.q_start[b], (int64_t)0), p.b.tokens);
@@ -788,7 +786,6 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_kv_attn_step(KvAttnAr
         }
         return;
     }
-    const KvSequence s = kv_sequence(p.b, b);
     const int at = p.blocks ? (int)((int64_t)unit - s.start) : 0;   // the unit's first token in its sequence
     if (at < 0 || at >= s.n) return;
     const int rows = min(p.blocks ? p.group : s.n * p.group, p.step_rows);

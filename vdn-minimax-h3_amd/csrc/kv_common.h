@@ -43,22 +43,19 @@ struct KvSequence {
     int n, length;
 };
 
+__device__ __forceinline__ KvSequence kv_sequence(const KvBatchArgs& p, int64_t start, int n, int length)
+{
+    const int64_t kept = max((int64_t)length, (int64_t)0);
+    return KvSequence{start, kept - n, n, (int)min(kept, (int64_t)p.width * kPage)};
+}
+
+__device__ __forceinline__ int kv_start(const KvBatchArgs& p, int b) { return min(max(p.q_start[b], 0), (int)p.tokens); }
+
 __device__ __forceinline__ KvSequence kv_sequence(const KvBatchArgs& p, int b)
 {
-    KvSequence s;
-    if (p.q_start) {
-        const int64_t lo = min(max((int64_t)p.q_start[b], (int64_t)0), p.tokens);
-        const int64_t hi = min(max((int64_t)p.q_start[b + 1], lo), p.tokens);
-        s.start = lo;
-        s.n = (int)(hi - lo);
-    } else {
-        s.n = p.each;
-        s.start = (int64_t)b * p.each;
-    }
-    const int64_t length = max((int64_t)p.lengths[b], (int64_t)0);
-    s.first = length - s.n;
-    s.length = (int)min(length, (int64_t)p.width * kPage);
-    return s;
+    if (!p.q_start) return kv_sequence(p, (int64_t)b * p.each, p.each, p.lengths[b]);
+    const int lo = kv_start(p, b), hi = max(kv_start(p, b + 1), lo);
+    return kv_sequence(p, lo, hi - lo, p.lengths[b]);
 }
 
 // Work is handed out in units of `size` rows of one sequence (`mult` rows a token), and the host
@@ -73,32 +70,39 @@ struct KvUnits {
     int mult, more;
 };
 
-__device__ __forceinline__ uint32_t kv_first_unit(const KvBatchArgs& p, const KvUnits& u, int b)
-{
-    return (uint32_t)(min(max(p.q_start[b], 0), (int)p.tokens) * u.mult) / u.size + (uint32_t)(u.more * b);
-}
+__device__ __forceinline__ uint32_t kv_first_unit(const KvUnits& u, int start, int b) { return (uint32_t)(start * u.mult) / u.size + (uint32_t)(u.more * b); }
 
-// The sequence that a unit belongs to, and its number `at` within it; with q_start, the batch's
-// size stands for the rows behind the last sequence.
-__device__ __forceinline__ int kv_locate(const KvBatchArgs& p, const KvUnits& u, uint32_t unit, uint32_t& at)
+__device__ __forceinline__ uint32_t kv_first_unit(const KvBatchArgs& p, const KvUnits& u, int b) { return kv_first_unit(u, kv_start(p, b), b); }
+
+// The sequence s that a unit belongs to, its number, and the unit's number `at` within it; with q_start, the
+// batch's size stands for the rows behind the last sequence (and s for none).
+__device__ __forceinline__ int kv_locate(const KvBatchArgs& p, const KvUnits& u, uint32_t unit, uint32_t& at, KvSequence& s)
 {
     if (!p.q_start) {
-        const uint32_t b = unit / u.each;
-        at = unit - b * u.each;
-        return (int)b;
+        const int b = (int)(unit / u.each);
+        at = unit - (uint32_t)b * u.each;
+        s = kv_sequence(p, b);
+        return b;
     }
-    // The sequences that do not begin behind the unit, counted 64 at a time by the wave (all of it is here).
+    // The sequences that do not begin behind the unit, counted 64 at a time by the wave (all of it is here). The
+    // last of them is at hand as a rule, its end in the next lane: one trip to memory instead of two.
     const int lane = threadIdx.x & 63;
-    int n = 0;
-    for (int b0 = 0; b0 <= p.batch; b0 += 64) {
-        const int b = b0 + lane;
-        const uint64_t before = __ballot(b <= p.batch && kv_first_unit(p, u, min(b, p.batch)) <= unit);
-        n += __builtin_popcountll(before);
-        if (before != ~0ull) break;
+    for (int b0 = 0;; b0 += 64) {
+        const int own = min(b0 + lane, p.batch), start = kv_start(p, own), length = p.lengths[min(own, p.batch - 1)];
+        const uint64_t before = __ballot(b0 + lane <= p.batch && kv_first_unit(u, start, own) <= unit);
+        const int count = __builtin_popcountll(before);
+        if (count == 64 && b0 + 64 <= p.batch) continue;
+        const int b = max(b0 + count - 1, 0);
+        if (count > 0 && count < 64) {
+            const int lo = __builtin_amdgcn_readlane(start, count - 1), hi = max(__builtin_amdgcn_readlane(start, count), lo);
+            at = unit - kv_first_unit(u, lo, b);
+            s = kv_sequence(p, lo, hi - lo, __builtin_amdgcn_readlane(length, count - 1));
+        } else {
+            at = unit - kv_first_unit(p, u, b);
+            if (b < p.batch) s = kv_sequence(p, b);
+        }
+        return b;
     }
-    const int b = max(n - 1, 0);
-    at = unit - kv_first_unit(p, u, b);
-    return b;
 }
 
 inline int64_t kv_unit_count(const KvBatchArgs& p, const KvUnits& u)

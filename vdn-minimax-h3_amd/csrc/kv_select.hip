@@ -51,9 +51,8 @@ struct KvSelectArgs {
 __device__ __forceinline__ bool block_of(const KvSelectArgs& p, int64_t row, int& b, KvSequence& s, int& from, int& to)
 {
     uint32_t at;
-    b = kv_locate(p.b, p.listed, (uint32_t)row, at);
+    b = kv_locate(p.b, p.listed, (uint32_t)row, at, s);
     if (b == p.b.batch) return false;
-    s = kv_sequence(p.b, b);
     if ((int64_t)at * p.query_block >= s.n) return false;
     from = (int)at * p.query_block;
     to = min(from + p.query_block, s.n);
