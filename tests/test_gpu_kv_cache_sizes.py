@@ -67,6 +67,40 @@ def test_select_of_many_sequences(device, block):
     assert np.array_equal(got.cpu().numpy(), want)
 
 
+@pytest.mark.parametrize("d,Hq,H,news,lengths", [(64, 24, 2, [1, 2], [300, 90]), (256, 12, 1, [1], [500]), (128, 9, 1, [3, 3], [700, 2]), (256, 2, 2, [1, 1, 1], [64, 0, 1000])])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("causal", [False, True])
+def test_single_queries_choose_and_attend(device, d, Hq, H, news, lengths, dtype, causal):
+    """Each query its own pages, groups above and below eight heads, every head size."""
+    print(f"single queries {dtype} d={d} {Hq}/{H} {news} of {lengths} causal={causal}", flush=True)
+    starts, ragged_ = starts_of(news), len(set(news)) != 1
+    pages = sum(-(-n // PAGE) for n in lengths) + 2
+    table, cache = tables(lengths, pages, 1), R.Cache(pages, H, d, seed=6)
+    g = torch.Generator().manual_seed(d + Hq)
+    key, value = (torch.randn(sum(lengths), H, d, generator=g).to(BF16) for _ in range(2))
+    R.append(cache, key, value, table, lengths, starts_of(lengths))
+    q = torch.randn(sum(news), Hq, d, generator=g).to(dtype)
+    want = R.select(cache, q, table, lengths, starts, 3, 1, 1, 1, causal, ragged_)
+    got = vdn_fp8.kv_select(q.to(device), vdn_fp8.KvCache(*cache.tensors(device)), i32(table, device), i32(lengths, device), 3, query_block=1,
+                            causal=causal, q_start=i32(starts, device) if ragged_ else None)
+    assert np.array_equal(got.cpu().numpy(), want)
+    attention_case(device, dtype, Hq, H, d, news, lengths, causal, cache=cache, table=table, q=q, blocks=want, block=1, max_query=max(news))
+
+
+def test_more_single_queries_than_a_launch_numbers(device):
+    """Past 65535 single queries the page scores take the way of the blocks; the choice is the same."""
+    n, H, d, length = 66000, 1, 64, 330
+    g = torch.Generator().manual_seed(15)
+    pages = -(-length // PAGE)
+    cache, table = R.Cache(pages, H, d, seed=6), [list(range(pages))]
+    q = torch.randn(n, H, d, generator=g).to(BF16)
+    got = vdn_fp8.kv_select(q.to(device), vdn_fp8.KvCache(*cache.tensors(device)), i32(table, device), i32([length], device), 3, query_block=1)
+    for rows in (slice(0, 40), slice(65510, 65560), slice(n - 30, n)):
+        part = q[rows]
+        want = R.select(cache, part, table, [length], [0, len(part)], 3, 1, 1, 1, False)
+        assert np.array_equal(got[rows].cpu().numpy(), want)
+
+
 # -- workgroups ------------------------------------------------------------------------------
 
 @pytest.mark.parametrize("H,d,T", [(10, 64, 9000), (9, 128, 7000), (6, 256, 6000)])
