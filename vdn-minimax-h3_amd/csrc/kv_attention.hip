@@ -37,6 +37,8 @@
 // Both cut long key axes into splits where there are few rows, joined by k_kv_attn_join.
 #include <stdint.h>
 
+#include <algorithm>
+
 #include "gemm_common.h"
 #include "kv_common.h"
 #include "vdn_common.h"
@@ -69,6 +71,7 @@ struct KvAttnArgs {
     int causal;
     const int32_t* blocks;  // [listed units, heads, top] pages that a query block attends to, or NULL
     int top, query_block;
+    int block_rows;         // rows of a query block of k_kv_attn_rows (2^30, more than a call has, where they are more)
     KvUnits listed;
     uint16_t* out;
     float* lse;
@@ -566,7 +569,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_kv_attn_rows(KvAttnAr
     int lo, hi;
     if (p.blocks) {
         // the query block's number, as p.listed counts them
-        const int64_t block = r0 / (p.query_block * p.group);
+        const int64_t block = r0 / p.block_rows;
         const int64_t unit = (p.b.q_start ? (int64_t)kv_first_unit(p.b, p.listed, b) : (int64_t)b * p.listed.each) + block;
         list = p.blocks + (unit * p.c.heads + h) * p.top;
         lo = 0, hi = p.b.width > 0 ? p.top : 0;   // (no pages, no list to look at)
@@ -1022,6 +1025,7 @@ int attn_arguments(const vdn_fp8_kv_cache* cache, const vdn_fp8_kv_batch* batch,
             return set_error(VDN_FP8_EINVAL, "kv_attention: query_block must be 1, or such that query_block * group is a multiple of %d "
                              "(got %lld with groups of %d)", kRows, (long long)query_block, p.group);
         p.top = (int)top, p.query_block = (int)query_block;
+        p.block_rows = (int)std::min(query_block * p.group, (int64_t)1 << 30);
         const int64_t n = p.b.batch > 0 ? p.b.tokens / p.b.batch : 0;
         p.listed = KvUnits{(uint32_t)query_block, (uint32_t)((n + query_block - 1) / query_block), 1, query_block == 1 ? 0 : 1};
         p.blocks = (const int32_t*)(uintptr_t)4;   // replaced by the call
