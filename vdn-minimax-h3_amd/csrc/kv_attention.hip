@@ -10,18 +10,24 @@
 //   products of an instruction to the largest and drop what is below: scores were off by up to 2^-12 of the
 //   largest product, where these sums stay within 2^-18 of it, for 1.99 against 2.15 ms on 3120 tokens over 32760.)
 //
-//   Values in binary16: e4m3 codes are binary16 numbers, and weights in [0, 2^8] keep eleven bits
-//   (bf16 weights would leave eight, an error as large as the output's own rounding). The value's scale
-//   2^ev never meets the codes: it joins the exponent of the weight, P' = 2^(x + ev - m), where m
-//   is the running maximum of x + ev, so that the product's sum is that of the real values, and a
-//   page's sum of weights is 2^-ev times its sum of P'. Sums, maxima and accumulators are binary32.
+//   Values in binary16: e4m3 codes are binary16 numbers, and weights keep eleven bits (bf16 weights would
+//   leave eight, an error as large as the output's own rounding). The value's scale 2^ev never meets the
+//   codes: it joins the exponent of the weight, P' = 2^(x + ev - m + 5), where 2^m is the unit of the row's
+//   accumulators, so that the product's sum is that of the real values. Sums, units and accumulators are
+//   binary32, and so is the sum of the weights 2^(x - t), which has a unit 2^t of its own.
 //
 //   The transposed scores S^T = K Q^T leave each lane 16 consecutive keys of one query (the key that
 //   a matrix row stands for is a matter of which row is loaded where), and those are the operand of
 //   O^T = V^T P^T as they are: P goes from one product to the next in registers.
 //
-// A running maximum is raised only when it would move by more than 8 (weights up to 2^8 stay in
-// binary16's range), so most pages rescale nothing.
+// binary16 has few exponents, and one maximum for all pages would leave them to the weights next to the row's
+// largest: behind a token 17 nats above the others, or one of little weight in a page of large values, the others would
+// be lost from the output, though not from the sum. So a row's unit follows its pages both ways: a page whose
+// largest x + ev lies more than 10 from m moves m to it, and the accumulators by that power of two, exactly. A page's
+// largest weight is then held as 2^-5 to 2^15 (2^5 where the unit moves), and each weight is off by 2^-11 of itself or
+// 2^-20 of its page's largest. A unit comes down by 2^60 at most, which binary32 accumulators leave room for: pages
+// further below a row's largest are zeros. On 3120 tokens over 32760, whose pages' largest scores spread by 2 in standard
+// deviation, 2.19 ms; with 9, 8 and 6 in place of 10 2.24, 2.29 and 2.33; with a unit that only rises, by more than 8, 2.17.
 //
 // Rows are (token, head of a group) pairs of one key/value head, so grouped heads share the pages
 // that they read. Two kernels:
@@ -50,8 +56,10 @@ constexpr int kRows = 128, kWaveRows = 32;   // of k_kv_attn_rows
 constexpr int kStepRows = 16;                  // of k_kv_attn_step, at most
 constexpr int kInfo = 256;                     // pages that a workgroup looks up at a time
 constexpr int kMostSplits = 64;
-constexpr float kNoMax = -3.0e38f;      // the running maximum of no keys: finite, so that differences stay numbers
-constexpr float kSlack = 8.0f;          // the maximum moves only past this
+constexpr float kNone = -3.0e38f;       // the exponent of a unit before any key: finite, so that differences stay numbers
+constexpr float kWindow = 10.0f;        // a unit moves when a page's largest weight is further from it than this,
+constexpr float kLargest = 5.0f;        // and weights are held times 2^5, so 2^15 at most
+constexpr float kRange = 60.0f;         // how far a unit comes down, and how far scores rise above the sum's unit
 constexpr int kAbsent = 1 << 30;        // first key of a page that is not there: behind every sequence
 
 typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
@@ -75,7 +83,7 @@ struct KvAttnArgs {
     KvUnits listed;
     uint16_t* out;
     float* lse;
-    float* part;            // splits > 1: [tokens * q_heads][splits][d], then the (maximum, sum) pairs
+    float* part;            // splits > 1: outputs [tokens * q_heads][splits][d], then (unit, sum) pairs of their weights
     int splits, column_tiles;
     int step_rows;          // rows of a unit of k_kv_attn_step at most
     uint32_t items;         // workgroups of k_kv_attn_rows
@@ -110,23 +118,40 @@ __device__ __forceinline__ float added(float a, float b) { return a + b; }
 
 __device__ __forceinline__ float exponent_f32(int e) { return __uint_as_float((uint32_t)(min(max(e, -126), 127) + 127) << 23); }
 
-// v 2^e, where 2^e alone may be below the least float.
+// v 2^e for a whole number e, exact within binary32's range. (What is further out than 1000 is 0, or was NaN.)
 __device__ __forceinline__ float times_power(float v, float e)
 {
-    const float half = __builtin_amdgcn_exp2f(0.5f * e);
-    return v * half * half;
+    return __builtin_ldexpf(v, (int)__builtin_amdgcn_fmed3f(e, -1000.0f, 1000.0f));
 }
 
-// A page whose values are smaller than others' by orders has weights P' that are as much smaller: nothing next to
-// what the accumulators hold, but 2^-ev times their sum counts. Where a row's largest, 2^(top - m), is below 2^-60, its
-// weights are lifted to that (still zeros in binary16) and their sum is brought down again.
-__device__ __forceinline__ float lift_of(float top, float m) { return __builtin_amdgcn_fmed3f(m - top - 60.0f, 0.0f, 400.0f); }
-__device__ __forceinline__ void add_sum(float& l, float sum, int ev, float lift)
-{
-    float part = sum * exponent_f32(-ev);
-    if (__any(lift > 0.0f)) part = times_power(part, -lift);
-    l += part;
-}
+// One row's softmax over the pages so far: accumulators hold sum P' v in units of 2^m, P' times 2^kLargest, and the
+// sum of weights (of the lane's keys) is l 2^t.
+struct Running {
+    float m, t;   // whole numbers
+    float low;    // m does not go below
+    float l;
+    __device__ __forceinline__ void start() { m = t = low = kNone, l = 0.0f; }
+
+    // A page whose largest score is x (-inf: none seen), values' scale 2^ev: true where the unit of some row of the wave
+    // moves, and then the accumulators are to be multiplied by 2^move.
+    __device__ __forceinline__ bool moves(float x, float ev, float& move)
+    {
+        const float to = fmaxf(x + ev, low);
+        if (!__any(fabsf(to - m) > kWindow || x > t + kRange)) return false;
+        const float now = __builtin_rintf(to), most = fmaxf(t, __builtin_rintf(x));
+        move = m - now;
+        l = times_power(l, t - most);
+        m = now, t = most, low = fmaxf(low, now - kRange);
+        return true;
+    }
+    // A page below the unit's reach adds nothing to the accumulators, but its weights count in l (values of zeros have the
+    // least scale): they are lifted to 2^-55, still zeros in binary16, so that their sum is one.
+    __device__ __forceinline__ float lift(float x, float ev) const { return __builtin_amdgcn_fmed3f(m - (x + ev) - kRange, 0.0f, 400.0f); }
+    // What joins a score in the exponent of P'.
+    __device__ __forceinline__ float base(float ev, float lift) const { return ev - m + (kLargest + lift); }
+    // The page's sum of P'.
+    __device__ __forceinline__ void add(float sum, float ev, float lift) { l += sum * __builtin_amdgcn_exp2f((m - t) - (ev + (kLargest + lift))); }
+};
 
 // 16 codes of one operand row -> two operands of eight values (exact).
 __device__ __forceinline__ void decode16(uint4 w, f16x8_t o[2])
@@ -255,7 +280,7 @@ struct WaveRows {
     typedef typename Query<F16>::Eight Eight;
     Eight q[kSteps];
     f32x16_t acc[kTiles];
-    float m, l;        // running maximum and sum (of this half's keys)
+    Running run;       // (l of this half's keys)
     int limit;         // keys below it are visible to the row
 
     // row: the row's values (NULL: none, zeros).
@@ -263,7 +288,7 @@ struct WaveRows {
     {
 #pragma unroll
         for (int s = 0; s < kSteps; ++s) q[s] = query8<F16>(row ? row + 64 * (s >> 2) + 32 * g + 8 * (s & 3) : nullptr);
-        m = kNoMax, l = 0.0f;
+        run.start();
 #pragma unroll
         for (int t = 0; t < kTiles; ++t)
 #pragma unroll
@@ -310,17 +335,16 @@ struct WaveRows {
             const int j = 8 * (i % 2);
             four[i] = larger3(larger3(larger3(larger(a[j], a[j + 1]), a[j + 2], a[j + 3]), a[j + 4], a[j + 5]), a[j + 6], a[j + 7]);
         }
-        const float top = across32(larger(larger3(four[0], four[1], four[2]), four[3]), larger) * f + shift;
-        if (__any(top > m + kSlack)) {
-            const float now = fmaxf(m, top), a = __builtin_amdgcn_exp2f(m - now);
-            l = times_power(l, m - now);
-            m = now;
+        const float x = across32(larger(larger3(four[0], four[1], four[2]), four[3]), larger) * f;
+        float move;
+        if (run.moves(x, shift, move)) {
+            const float a = times_power(1.0f, move);
 #pragma unroll
             for (int t = 0; t < kTiles; ++t)
 #pragma unroll
                 for (int i = 0; i < 16; ++i) acc[t][i] *= a;
         }
-        const float lift = lift_of(top, m), base = shift - m + lift;
+        const float lift = run.lift(x, shift), base = run.base(shift, lift);
         float sum = 0.0f;
 #pragma unroll
         for (int kt = 0; kt < 2; ++kt)
@@ -332,7 +356,7 @@ struct WaveRows {
                     sum += p;
                     w[kt][h][j] = (_Float16)p;
                 }
-        add_sum(l, sum, ev, lift);
+        run.add(sum, shift, lift);
     }
 
     // Adds the weighted values of a page: value(kt, h, t) gives one element's values of the eight tokens from
@@ -395,7 +419,7 @@ struct StepRows {
     typedef typename Query<F16>::Eight Eight;
     Eight q[kSteps];
     f32x4_t acc[kTiles];
-    float m, l;
+    Running run;
     int limit;
 
     // (the inner dimension of the scores: lane group g takes elements g D / 4 on, eight a step)
@@ -403,7 +427,7 @@ struct StepRows {
     {
 #pragma unroll
         for (int s = 0; s < kSteps; ++s) q[s] = query8<F16>(row ? row + D / 4 * g + 8 * s : nullptr);
-        m = kNoMax, l = 0.0f;
+        run.start();
 #pragma unroll
         for (int t = 0; t < kTiles; ++t) acc[t] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
     }
@@ -439,15 +463,14 @@ struct StepRows {
         float four[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) four[i] = larger(larger3(s[i][0], s[i][1], s[i][2]), s[i][3]);
-        const float top = across16(across32(larger(larger3(four[0], four[1], four[2]), four[3]), larger), larger) * f + shift;
-        if (__any(top > m + kSlack)) {
-            const float now = fmaxf(m, top), a = __builtin_amdgcn_exp2f(m - now);
-            l = times_power(l, m - now);
-            m = now;
+        const float x = across16(across32(larger(larger3(four[0], four[1], four[2]), four[3]), larger), larger) * f;
+        float move;
+        if (run.moves(x, shift, move)) {
+            const float a = times_power(1.0f, move);
 #pragma unroll
             for (int t = 0; t < kTiles; ++t) acc[t] *= a;
         }
-        const float lift = lift_of(top, m), base = shift - m + lift;
+        const float lift = run.lift(x, shift), base = run.base(shift, lift);
         float sum = 0.0f;
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
@@ -455,7 +478,7 @@ struct StepRows {
             sum += p;
             w[i / 8][i % 8] = (_Float16)p;
         }
-        add_sum(l, sum, ev, lift);
+        run.add(sum, shift, lift);
     }
 
     // v[t]: the codes of 16 tokens, one element.
@@ -498,6 +521,9 @@ struct StepRows {
         }
     }
 };
+
+// log(l 2^t)
+__device__ __forceinline__ float log_sum(float l, float t) { return l == 0.0f ? -__builtin_inff() : (t + __builtin_log2f(l)) * 0.6931471805599453f; }
 
 template <bool F16>
 __device__ __forceinline__ uint32_t pack_out(float lo, float hi)
@@ -726,7 +752,8 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_kv_attn_rows(KvAttnAr
     }
 
     if (!valid) return;
-    const float l = across32(rowset.l, added);
+    const float l = across32(rowset.run.l, added), inv = l == 0.0f ? 0.0f : 1.0f / l, power = rowset.run.m - rowset.run.t - kLargest;
+    auto out_at = [&](int t, int i) { return times_power(rowset.acc[t][i] * inv, power); };
     const int64_t out_row = token * p.q_heads + head;
     if (p.splits > 1) {
         float* const dst = p.part + (out_row * p.splits + split) * D + 16 * g;
@@ -734,25 +761,20 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_kv_attn_rows(KvAttnAr
 #pragma unroll
             for (int t = 0; t < D / 32; ++t)
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    *reinterpret_cast<float4*>(dst + 32 * t + 4 * i) = make_float4(rowset.acc[t][4 * i], rowset.acc[t][4 * i + 1],
-                                                                                 rowset.acc[t][4 * i + 2], rowset.acc[t][4 * i + 3]);
-        if (g == 0) *reinterpret_cast<float2*>(part_sums(p) + 2 * (out_row * p.splits + split)) = make_float2(rowset.m, l);
+                for (int i = 0; i < 16; i += 4)
+                    *reinterpret_cast<float4*>(dst + 32 * t + i) = make_float4(out_at(t, i), out_at(t, i + 1), out_at(t, i + 2), out_at(t, i + 3));
+        if (g == 0) *reinterpret_cast<float2*>(part_sums(p) + 2 * (out_row * p.splits + split)) = make_float2(rowset.run.t, l);
         return;
     }
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
     uint16_t* const dst = p.out + out_row * D + 16 * g;
 #pragma unroll
     for (int t = 0; t < D / 32; ++t)
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const f32x16_t& a = rowset.acc[t];
-            *reinterpret_cast<uint4*>(dst + 32 * t + 8 * i) =
-                make_uint4(pack_out<F16>(a[8 * i] * inv, a[8 * i + 1] * inv), pack_out<F16>(a[8 * i + 2] * inv, a[8 * i + 3] * inv),
-                           pack_out<F16>(a[8 * i + 4] * inv, a[8 * i + 5] * inv), pack_out<F16>(a[8 * i + 6] * inv, a[8 * i + 7] * inv));
-        }
-    if (p.lse && g == 0)
-        p.lse[out_row] = l == 0.0f ? -__builtin_inff() : (rowset.m + __builtin_log2f(l)) * 0.6931471805599453f;
+        for (int i = 0; i < 16; i += 8)
+            *reinterpret_cast<uint4*>(dst + 32 * t + i) =
+                make_uint4(pack_out<F16>(out_at(t, i), out_at(t, i + 1)), pack_out<F16>(out_at(t, i + 2), out_at(t, i + 3)),
+                           pack_out<F16>(out_at(t, i + 4), out_at(t, i + 5)), pack_out<F16>(out_at(t, i + 6), out_at(t, i + 7)));
+    if (p.lse && g == 0) p.lse[out_row] = log_sum(l, rowset.run.t);
 }
 
 // Up to 16 rows of one sequence (or of one token, where each has its own pages) and key/value head.
@@ -762,7 +784,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_kv_attn_step(KvAttnAr
     constexpr int kTiles = D / 16;
     constexpr int kPart = D < 128 ? D : 128;
     __shared__ __attribute__((aligned(16))) float acc[4][kStepRows][kPart];
-    __shared__ float2 sums[4][kStepRows];   // maximum, sum
+    __shared__ float2 sums[4][kStepRows];   // the sum's unit, the sum
     __shared__ __attribute__((aligned(16))) PageInfo info[kInfo];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int r = lane & 15, g = lane >> 4;
@@ -866,28 +888,32 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_kv_attn_step(KvAttnAr
 
     // The four waves' parts of each row, joined in LDS, 128 elements at a time.
     const int kept = min(rows - tile * kStepRows, kStepRows);
-    const float l = across16(across32(rowset.l, added), added);
-    if (g == 0) sums[wave][r] = make_float2(rowset.m, l);
+    const float l = across16(across32(rowset.run.l, added), added), own = l == 0.0f ? 0.0f : 1.0f / l;
+    const float power = rowset.run.m - rowset.run.t - kLargest;
+    if (g == 0) sums[wave][r] = make_float2(rowset.run.t, l);
 #pragma unroll
     for (int d0 = 0; d0 < D; d0 += kPart) {
         if (d0 > 0) __syncthreads();
 #pragma unroll
         for (int t = 0; t < kPart / 16; ++t) {
             const f32x4_t v = rowset.acc[d0 / 16 + t];
-            *reinterpret_cast<float4*>(&acc[wave][r][16 * t + 4 * g]) = make_float4(v[0], v[1], v[2], v[3]);
+            *reinterpret_cast<float4*>(&acc[wave][r][16 * t + 4 * g]) =
+                make_float4(times_power(v[0] * own, power), times_power(v[1] * own, power), times_power(v[2] * own, power), times_power(v[3] * own, power));
         }
         __syncthreads();
         for (int e = tid; e < kept * (kPart / 4); e += 256) {
             const int row_e = e / (kPart / 4), d = 4 * (e % (kPart / 4));
-            float m = kNoMax;
+            float m = kNone;
 #pragma unroll
             for (int wv = 0; wv < 4; ++wv) m = fmaxf(m, sums[wv][row_e].x);
-            float total = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            float total = 0.0f, part[4], o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int wv = 0; wv < 4; ++wv) part[wv] = times_power(sums[wv][row_e].y, sums[wv][row_e].x - m), total += part[wv];
+            const float inv = total == 0.0f ? 0.0f : 1.0f / total;
 #pragma unroll
             for (int wv = 0; wv < 4; ++wv) {
-                const float e = sums[wv][row_e].x - m, f = __builtin_amdgcn_exp2f(e);
+                const float f = part[wv] * inv;
                 const float4 a = *reinterpret_cast<const float4*>(&acc[wv][row_e][d]);
-                total += times_power(sums[wv][row_e].y, e);
                 o[0] += f * a.x, o[1] += f * a.y, o[2] += f * a.z, o[3] += f * a.w;
             }
             const int row_at = tile * kStepRows + row_e;
@@ -896,11 +922,8 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_kv_attn_step(KvAttnAr
                 *reinterpret_cast<float4*>(p.part + (out_row * p.splits + split) * D + d0 + d) = make_float4(o[0], o[1], o[2], o[3]);
                 if (d0 + d == 0) *reinterpret_cast<float2*>(part_sums(p) + 2 * (out_row * p.splits + split)) = make_float2(m, total);
             } else {
-                const float inv = total == 0.0f ? 0.0f : 1.0f / total;
-                *reinterpret_cast<uint2*>(p.out + out_row * D + d0 + d) =
-                    make_uint2(pack_out<F16>(o[0] * inv, o[1] * inv), pack_out<F16>(o[2] * inv, o[3] * inv));
-                if (p.lse && d0 + d == 0)
-                    p.lse[out_row] = total == 0.0f ? -__builtin_inff() : (m + __builtin_log2f(total)) * 0.6931471805599453f;
+                *reinterpret_cast<uint2*>(p.out + out_row * D + d0 + d) = make_uint2(pack_out<F16>(o[0], o[1]), pack_out<F16>(o[2], o[3]));
+                if (p.lse && d0 + d == 0) p.lse[out_row] = log_sum(total, m);
             }
         }
     }
@@ -916,15 +939,15 @@ __global__ __launch_bounds__(256) void k_kv_attn_join(KvAttnArgs p)
     if (row >= p.b.tokens * p.q_heads) return;
     if (p.b.q_start && row / p.q_heads >= p.b.q_start[p.b.batch]) return;   // behind the last sequence
     const float* const sums = part_sums(p) + 2 * row * p.splits;
-    float2 own = make_float2(kNoMax, 0.0f);
+    float2 own = make_float2(kNone, 0.0f);
     if (lane < p.splits) own = *reinterpret_cast<const float2*>(sums + 2 * lane);
     float m = own.x;
 #pragma unroll
     for (int off = 1; off < 64; off <<= 1) m = fmaxf(m, __shfl_xor(m, off, 64));
-    const float f = __builtin_amdgcn_exp2f(own.x - m);
-    float total = times_power(own.y, own.x - m);
+    float f = times_power(own.y, own.x - m), total = f;
 #pragma unroll
     for (int off = 1; off < 64; off <<= 1) total += __shfl_xor(total, off, 64);
+    f *= total == 0.0f ? 0.0f : 1.0f / total;
     float o[E];
 #pragma unroll
     for (int e = 0; e < E; ++e) o[e] = 0.0f;
@@ -937,20 +960,19 @@ __global__ __launch_bounds__(256) void k_kv_attn_join(KvAttnArgs p)
             for (int e = 0; e < E; ++e) v[i][e] = src[(int64_t)min(i0 + i, p.splits - 1) * D + e];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            // (a split without keys has not written its accumulators; lanes beyond the splits hold none)
+            // (a split without keys may not have written its outputs; lanes beyond the splits hold none)
             const bool some = __shfl(own.y, (i0 + i) & 63, 64) != 0.0f && i0 + i < p.splits;
             const float w = __shfl(f, (i0 + i) & 63, 64);
 #pragma unroll
             for (int e = 0; e < E; ++e) o[e] += some ? w * v[i][e] : 0.0f;
         }
     }
-    const float inv = total == 0.0f ? 0.0f : 1.0f / total;
     uint16_t* const dst = p.out + row * D + lane * E;
-    if (E == 1) dst[0] = (uint16_t)pack_out<F16>(o[0] * inv, 0.0f);
+    if (E == 1) dst[0] = (uint16_t)pack_out<F16>(o[0], 0.0f);
     else
 #pragma unroll
-        for (int e = 0; e + 1 < E; e += 2) *reinterpret_cast<uint32_t*>(dst + e) = pack_out<F16>(o[e] * inv, o[e + 1] * inv);
-    if (p.lse && lane == 0) p.lse[row] = total == 0.0f ? -__builtin_inff() : (m + __builtin_log2f(total)) * 0.6931471805599453f;
+        for (int e = 0; e + 1 < E; e += 2) *reinterpret_cast<uint32_t*>(dst + e) = pack_out<F16>(o[e], o[e + 1]);
+    if (p.lse && lane == 0) p.lse[row] = log_sum(total, m);
 }
 
 // Which kernel a call takes, its units and its splits.
