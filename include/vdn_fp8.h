@@ -421,7 +421,8 @@ int vdn_fp8_qk_prep_append(const vdn_fp8_kv_cache *cache, const vdn_fp8_kv_batch
  * twice. The block that holds token i of sequence b is row floor(q_start[b] / query_block) + b +
  * floor(i / query_block) with q_start and query_block > 1, b ceil(n / query_block) + floor(i /
  * query_block) without; with query_block = 1 the token's own row.
- * max_query: at least the rows of the longest sequence where q_start is given (0: unknown).
+ * max_query: the rows of the longest sequence where q_start is given (0: unknown). It chooses the kernel;
+ * sequences of more rows are attended to all the same, at some cost.
  * The workspace has the bytes that the size query gives for the same arguments (top = 0 without
  * blocks), 16-byte aligned; nothing in it needs to be set, and calls that overlap need their own.
  * Replaces: the attention of HybridAttention's softmax branch (src/models/softmax_attention/window.py:56,

@@ -1,5 +1,5 @@
 """The 8-bit key/value cache on the GPU at the edges of what its entry points allow: the largest blocks of
-queries, weights far below a row's largest."""
+queries, weights far below a row's largest, hints that are wrong."""
 import numpy as np
 import pytest
 import torch
@@ -155,3 +155,16 @@ def test_the_sum_of_many_pages_of_zeros(device):
     assert not bool(out.any())
     # one sum a page in binary32, and the logarithm's rounding
     assert bool(((z.double() - want).abs() <= pages * 2.0 ** -24 + 2.0 ** -20).all())
+
+
+# -- hints and empty batches -------------------------------------------------------------------
+
+@pytest.mark.parametrize("d,Hq,H", [(64, 3, 1), (128, 10, 2), (256, 4, 2)])
+@pytest.mark.parametrize("news,lengths", [([1, 5, 40], [90, 5, 700]), ([0, 17, 1], [70, 3000, 1]), ([33], [4100])])
+@pytest.mark.parametrize("causal", [False, True])
+def test_more_rows_than_max_query(device, d, Hq, H, news, lengths, causal):
+    """max_query chooses a kernel; rows beyond it are attended to all the same."""
+    for most in (1, 2):
+        print(f"max_query {most} of {news} d={d} {Hq}/{H} causal={causal}", flush=True)
+        torch.full((1 << 22,), float("nan"), device=device)   # (what an allocation of the call may find)
+        attention_case(device, BF16, Hq, H, d, news, lengths, causal, seed=43, ragged=True, max_query=most)

@@ -85,7 +85,7 @@ struct KvAttnArgs {
     float* lse;
     float* part;            // splits > 1: outputs [tokens * q_heads][splits][d], then (unit, sum) pairs of their weights
     int splits, column_tiles;
-    int step_rows;          // rows of a unit of k_kv_attn_step at most
+    bool turns;             // of k_kv_attn_step: sequences may have more rows than column_tiles hold
     uint32_t items;         // workgroups of k_kv_attn_rows
 };
 
@@ -778,7 +778,8 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_kv_attn_rows(KvAttnAr
 }
 
 // Up to 16 rows of one sequence (or of one token, where each has its own pages) and key/value head.
-template <int D, bool F16>
+// TURNS: max_query may be less than a sequence's rows.
+template <int D, bool F16, bool TURNS>
 __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_kv_attn_step(KvAttnArgs p)
 {
     constexpr int kTiles = D / 16;
@@ -792,7 +793,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_kv_attn_step(KvAttnAr
     uint32_t item = blockIdx.x;
     const int split = (int)(item % p.splits);
     item /= p.splits;
-    const int tile = (int)(item % p.column_tiles);
+    const int first_tile = (int)(item % p.column_tiles);
     item /= p.column_tiles;
     const int h = __builtin_amdgcn_readfirstlane((int)(item % p.c.heads));
     const uint32_t unit = item / p.c.heads;
@@ -805,7 +806,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_kv_attn_step(KvAttnAr
         s = kv_sequence(p.b, b);
     }
     if (b == p.b.batch) {   // behind the last sequence
-        if (split == 0 && tile == 0) {
+        if (split == 0 && first_tile == 0) {
             const int64_t end = min(max((int64_t)p.b.q_start[b], (int64_t)0), p.b.tokens);
             clear_rows(p, p.blocks ? unit : end, p.blocks ? unit + 1 : p.b.tokens, h);
         }
@@ -813,119 +814,125 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_kv_attn_step(KvAttnAr
     }
     const int at = p.blocks ? (int)((int64_t)unit - s.start) : 0;   // the unit's first token in its sequence
     if (at < 0 || at >= s.n) return;
-    const int rows = min(p.blocks ? p.group : s.n * p.group, p.step_rows);
-    if (tile * kStepRows >= rows) return;
-    const int first_token = at + tile * kStepRows / p.group, last_token = at + (min((tile + 1) * kStepRows, rows) - 1) / p.group;
-    auto limit_of = [&](int t) -> int {
-        return p.causal ? (int)min(max(s.first + t + 1, (int64_t)0), (int64_t)s.length) : s.length;
-    };
-    const int32_t* list = p.blocks ? p.blocks + ((int64_t)unit * p.c.heads + h) * p.top : nullptr;
-    int lo = 0, hi = list ? (p.b.width > 0 ? p.top : 0) : (limit_of(last_token) + kPage - 1) / kPage;
-    if (p.splits > 1) {
-        const int per = max((hi + p.splits - 1) / p.splits, 4);
-        lo = min(split * per, hi);
-        hi = min(lo + per, hi);
-    }
+    const int rows = p.blocks ? p.group : s.n * p.group;
+    // One tile, but for more rows than max_query said: the unit's workgroups then take turns (an instance of its own: the
+    // loop costs the others 0.4 us in 10).
+#pragma unroll 1
+    for (int tile = first_tile; tile * kStepRows < rows; tile += p.column_tiles) {
+        if (TURNS && tile != first_tile) __syncthreads();   // (the join before has been read)
+        const int first_token = at + tile * kStepRows / p.group, last_token = at + (min((tile + 1) * kStepRows, rows) - 1) / p.group;
+        auto limit_of = [&](int t) -> int {
+            return p.causal ? (int)min(max(s.first + t + 1, (int64_t)0), (int64_t)s.length) : s.length;
+        };
+        const int32_t* list = p.blocks ? p.blocks + ((int64_t)unit * p.c.heads + h) * p.top : nullptr;
+        int lo = 0, hi = list ? (p.b.width > 0 ? p.top : 0) : (limit_of(last_token) + kPage - 1) / kPage;
+        if (p.splits > 1) {
+            const int per = max((hi + p.splits - 1) / p.splits, 4);
+            lo = min(split * per, hi);
+            hi = min(lo + per, hi);
+        }
 
-    StepRows<D, F16> rowset;
-    {
-        const int row = tile * kStepRows + r, own = at + row / p.group;
-        const bool valid = row < rows;
-        rowset.start(valid ? p.q + (s.start + own) * p.ldq + (int64_t)(h * p.group + row % p.group) * D : nullptr, g);
-        rowset.limit = valid ? limit_of(own) : 0;
-    }
-    const int least = limit_of(first_token), most = limit_of(last_token);
+        StepRows<D, F16> rowset;
+        {
+            const int row = tile * kStepRows + r, own = at + row / p.group;
+            const bool valid = row < rows;
+            rowset.start(valid ? p.q + (s.start + own) * p.ldq + (int64_t)(h * p.group + row % p.group) * D : nullptr, g);
+            rowset.limit = valid ? limit_of(own) : 0;
+        }
+        const int least = limit_of(first_token), most = limit_of(last_token);
 
-    const int from_k = (16 * (r >> 2) + (r & 3)) * D + D / 4 * g, from_v = r * kPage + 16 * g;
-    uint4 kr[4][D / 64], vr[kTiles];
-    auto load_k = [&](const PageInfo& a) {
-        const uint8_t* const src = p.c.k + ((int64_t)max(a.page, 0) * p.c.heads + h) * (kPage * D);
+        const int from_k = (16 * (r >> 2) + (r & 3)) * D + D / 4 * g, from_v = r * kPage + 16 * g;
+        uint4 kr[4][D / 64], vr[kTiles];
+        auto load_k = [&](const PageInfo& a) {
+            const uint8_t* const src = p.c.k + ((int64_t)max(a.page, 0) * p.c.heads + h) * (kPage * D);
 #pragma unroll
-        for (int t = 0; t < 4; ++t)
+            for (int t = 0; t < 4; ++t)
 #pragma unroll
-            for (int j = 0; j < D / 64; ++j) kr[t][j] = *reinterpret_cast<const uint4*>(src + from_k + t * 4 * D + j * 16);
-    };
-    auto load_v = [&](const PageInfo& a) {
-        const uint8_t* const src = p.c.v + ((int64_t)max(a.page, 0) * p.c.heads + h) * (kPage * D);
+                for (int j = 0; j < D / 64; ++j) kr[t][j] = *reinterpret_cast<const uint4*>(src + from_k + t * 4 * D + j * 16);
+        };
+        auto load_v = [&](const PageInfo& a) {
+            const uint8_t* const src = p.c.v + ((int64_t)max(a.page, 0) * p.c.heads + h) * (kPage * D);
 #pragma unroll
-        for (int t = 0; t < kTiles; ++t) vr[t] = *reinterpret_cast<const uint4*>(src + from_v + t * 16 * kPage);
-    };
-    look_up(p, b, h, s.length, list, lo, hi, info);
-    __syncthreads();
-    for (int first = lo; first < hi; first += kInfo) {
-        const int count = min(hi - first, kInfo);
-        if (first > lo) {
-            __syncthreads();
-            look_up(p, b, h, s.length, list, first, hi, info);
-            __syncthreads();
-        }
-        PageInfo now{}, next{};
-        int i = wave;
-        if (i < count) {
-            now = info_at(info, i);
-            load_k(now);
-            load_v(now);
-        }
-        for (; i < count; i += 4) {
-            const bool more = i + 4 < count;
-            if (more) next = info_at(info, i + 4);
-            f32x4_t sc[4];
-            f16x8_t w[2];
-            rowset.scores(kr, sc);
-            if (more) load_k(next);
-            const int key0 = first_key(now);
-            if (key0 < most) {
-                const bool masked = key0 + kPage > least;
-                if (masked) rowset.mask(sc, key0, g);
-                rowset.weights(sc, p.scale, now.ek, now.ev, w);
-                if (masked) rowset.settle_values(vr, key0, s.length, g);
-                rowset.add_values(vr, w);
-            }
-            if (more) load_v(next);
-            now = next;
-        }
-    }
-
-    // The four waves' parts of each row, joined in LDS, 128 elements at a time.
-    const int kept = min(rows - tile * kStepRows, kStepRows);
-    const float l = across16(across32(rowset.run.l, added), added), own = l == 0.0f ? 0.0f : 1.0f / l;
-    const float power = rowset.run.m - rowset.run.t - kLargest;
-    if (g == 0) sums[wave][r] = make_float2(rowset.run.t, l);
-#pragma unroll
-    for (int d0 = 0; d0 < D; d0 += kPart) {
-        if (d0 > 0) __syncthreads();
-#pragma unroll
-        for (int t = 0; t < kPart / 16; ++t) {
-            const f32x4_t v = rowset.acc[d0 / 16 + t];
-            *reinterpret_cast<float4*>(&acc[wave][r][16 * t + 4 * g]) =
-                make_float4(times_power(v[0] * own, power), times_power(v[1] * own, power), times_power(v[2] * own, power), times_power(v[3] * own, power));
-        }
+            for (int t = 0; t < kTiles; ++t) vr[t] = *reinterpret_cast<const uint4*>(src + from_v + t * 16 * kPage);
+        };
+        look_up(p, b, h, s.length, list, lo, hi, info);
         __syncthreads();
-        for (int e = tid; e < kept * (kPart / 4); e += 256) {
-            const int row_e = e / (kPart / 4), d = 4 * (e % (kPart / 4));
-            float m = kNone;
-#pragma unroll
-            for (int wv = 0; wv < 4; ++wv) m = fmaxf(m, sums[wv][row_e].x);
-            float total = 0.0f, part[4], o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-            for (int wv = 0; wv < 4; ++wv) part[wv] = times_power(sums[wv][row_e].y, sums[wv][row_e].x - m), total += part[wv];
-            const float inv = total == 0.0f ? 0.0f : 1.0f / total;
-#pragma unroll
-            for (int wv = 0; wv < 4; ++wv) {
-                const float f = part[wv] * inv;
-                const float4 a = *reinterpret_cast<const float4*>(&acc[wv][row_e][d]);
-                o[0] += f * a.x, o[1] += f * a.y, o[2] += f * a.z, o[3] += f * a.w;
+        for (int first = lo; first < hi; first += kInfo) {
+            const int count = min(hi - first, kInfo);
+            if (first > lo) {
+                __syncthreads();
+                look_up(p, b, h, s.length, list, first, hi, info);
+                __syncthreads();
             }
-            const int row_at = tile * kStepRows + row_e;
-            const int64_t out_row = (s.start + at + row_at / p.group) * p.q_heads + h * p.group + row_at % p.group;
-            if (p.splits > 1) {
-                *reinterpret_cast<float4*>(p.part + (out_row * p.splits + split) * D + d0 + d) = make_float4(o[0], o[1], o[2], o[3]);
-                if (d0 + d == 0) *reinterpret_cast<float2*>(part_sums(p) + 2 * (out_row * p.splits + split)) = make_float2(m, total);
-            } else {
-                *reinterpret_cast<uint2*>(p.out + out_row * D + d0 + d) = make_uint2(pack_out<F16>(o[0], o[1]), pack_out<F16>(o[2], o[3]));
-                if (p.lse && d0 + d == 0) p.lse[out_row] = log_sum(total, m);
+            PageInfo now{}, next{};
+            int i = wave;
+            if (i < count) {
+                now = info_at(info, i);
+                load_k(now);
+                load_v(now);
+            }
+            for (; i < count; i += 4) {
+                const bool more = i + 4 < count;
+                if (more) next = info_at(info, i + 4);
+                f32x4_t sc[4];
+                f16x8_t w[2];
+                rowset.scores(kr, sc);
+                if (more) load_k(next);
+                const int key0 = first_key(now);
+                if (key0 < most) {
+                    const bool masked = key0 + kPage > least;
+                    if (masked) rowset.mask(sc, key0, g);
+                    rowset.weights(sc, p.scale, now.ek, now.ev, w);
+                    if (masked) rowset.settle_values(vr, key0, s.length, g);
+                    rowset.add_values(vr, w);
+                }
+                if (more) load_v(next);
+                now = next;
             }
         }
+
+        // The four waves' parts of each row, joined in LDS, 128 elements at a time.
+        const int kept = min(rows - tile * kStepRows, kStepRows);
+        const float l = across16(across32(rowset.run.l, added), added), own = l == 0.0f ? 0.0f : 1.0f / l;
+        const float power = rowset.run.m - rowset.run.t - kLargest;
+        if (g == 0) sums[wave][r] = make_float2(rowset.run.t, l);
+#pragma unroll
+        for (int d0 = 0; d0 < D; d0 += kPart) {
+            if (d0 > 0) __syncthreads();
+#pragma unroll
+            for (int t = 0; t < kPart / 16; ++t) {
+                const f32x4_t v = rowset.acc[d0 / 16 + t];
+                *reinterpret_cast<float4*>(&acc[wave][r][16 * t + 4 * g]) =
+                    make_float4(times_power(v[0] * own, power), times_power(v[1] * own, power), times_power(v[2] * own, power), times_power(v[3] * own, power));
+            }
+            __syncthreads();
+            for (int e = tid; e < kept * (kPart / 4); e += 256) {
+                const int row_e = e / (kPart / 4), d = 4 * (e % (kPart / 4));
+                float m = kNone;
+#pragma unroll
+                for (int wv = 0; wv < 4; ++wv) m = fmaxf(m, sums[wv][row_e].x);
+                float total = 0.0f, part[4], o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int wv = 0; wv < 4; ++wv) part[wv] = times_power(sums[wv][row_e].y, sums[wv][row_e].x - m), total += part[wv];
+                const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+#pragma unroll
+                for (int wv = 0; wv < 4; ++wv) {
+                    const float f = part[wv] * inv;
+                    const float4 a = *reinterpret_cast<const float4*>(&acc[wv][row_e][d]);
+                    o[0] += f * a.x, o[1] += f * a.y, o[2] += f * a.z, o[3] += f * a.w;
+                }
+                const int row_at = tile * kStepRows + row_e;
+                const int64_t out_row = (s.start + at + row_at / p.group) * p.q_heads + h * p.group + row_at % p.group;
+                if (p.splits > 1) {
+                    *reinterpret_cast<float4*>(p.part + (out_row * p.splits + split) * D + d0 + d) = make_float4(o[0], o[1], o[2], o[3]);
+                    if (d0 + d == 0) *reinterpret_cast<float2*>(part_sums(p) + 2 * (out_row * p.splits + split)) = make_float2(m, total);
+                } else {
+                    *reinterpret_cast<uint2*>(p.out + out_row * D + d0 + d) = make_uint2(pack_out<F16>(o[0], o[1]), pack_out<F16>(o[2], o[3]));
+                    if (p.lse && d0 + d == 0) p.lse[out_row] = log_sum(total, m);
+                }
+            }
+        }
+        if (!TURNS) break;
     }
 }
 
@@ -979,7 +986,7 @@ __global__ __launch_bounds__(256) void k_kv_attn_join(KvAttnArgs p)
 struct Plan {
     bool step;
     int64_t items;          // workgroups
-    int splits, column_tiles, step_rows;
+    int splits, column_tiles;
     int64_t bytes;          // of workspace
 };
 
@@ -994,8 +1001,7 @@ Plan make_plan(KvAttnArgs& p, int64_t max_query, int cus)
     const int64_t pages = p.blocks ? p.top : p.b.width;
     int64_t groups;
     if (plan.step) {
-        plan.step_rows = (int)(most * p.group);
-        plan.column_tiles = (plan.step_rows + kStepRows - 1) / kStepRows;
+        plan.column_tiles = (int)((most * p.group + kStepRows - 1) / kStepRows);
         // (and one unit that clears what is behind the last sequence)
         groups = (p.blocks ? p.b.tokens : (int64_t)p.b.batch + (p.b.q_start ? 1 : 0)) * p.c.heads * plan.column_tiles;
     } else {
@@ -1020,7 +1026,8 @@ int launch(const KvAttnArgs& p, bool step, hipStream_t stream)
 {
     int st;
     if (step) {
-        hipLaunchKernelGGL((k_kv_attn_step<D, F16>), dim3(p.items), dim3(256), 0, stream, p);
+        if (p.turns) hipLaunchKernelGGL((k_kv_attn_step<D, F16, true>), dim3(p.items), dim3(256), 0, stream, p);
+        else hipLaunchKernelGGL((k_kv_attn_step<D, F16, false>), dim3(p.items), dim3(256), 0, stream, p);
         st = check_launch("kv_attention");
     } else {
         hipLaunchKernelGGL((k_kv_attn_rows<D, F16>), dim3(p.items), dim3(256), 0, stream, p);
@@ -1098,7 +1105,8 @@ extern "C" int vdn_fp8_kv_attention(const vdn_fp8_kv_cache* cache, const vdn_fp8
         return set_error(VDN_FP8_EINVAL, "kv_attention: workspace of %lld bytes, %lld needed", (long long)workspace_bytes, (long long)plan.bytes);
     p.q = (const uint16_t*)query, p.ldq = ldq, p.scale = scale * 1.4426950408889634f, p.causal = causal != 0;
     p.blocks = blocks, p.out = (uint16_t*)out, p.lse = lse, p.part = (float*)workspace;
-    p.splits = plan.splits, p.column_tiles = plan.column_tiles, p.step_rows = plan.step_rows, p.items = (uint32_t)plan.items;
+    p.splits = plan.splits, p.column_tiles = plan.column_tiles, p.items = (uint32_t)plan.items;
+    p.turns = p.b.q_start && !blocks && max_query > 0 && max_query < p.b.tokens;
     const bool f16 = dtype == VDN_FP8_DTYPE_F16;
     switch (p.c.d) {
         case 64: return f16 ? launch<64, true>(p, plan.step, stream) : launch<64, false>(p, plan.step, stream);

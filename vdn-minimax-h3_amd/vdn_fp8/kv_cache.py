@@ -259,8 +259,8 @@ def kv_attention(query, cache, page_table, lengths, *, scale=None, causal=False,
 
     return_lse: also log(sum exp(scores)), float32 [T, q_heads] (-inf for such a row), by which
     results over different keys join.
-    max_query: with q_start, at least the rows of the longest sequence, if known: a few rows per
-    sequence take another kernel (rows beyond it are not computed).
+    max_query: with q_start, the rows of the longest sequence, if known: a few rows per sequence take
+    another kernel (in which a sequence of more rows than that takes longer).
     blocks, query_block: int32 [rows, heads, top] from `kv_select` (or a caller's own list; entries
     outside the sequence are skipped, one listed twice counts twice): only those pages are read."""
     heads, d = _heads(cache)
