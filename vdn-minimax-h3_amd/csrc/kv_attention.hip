@@ -83,15 +83,16 @@ struct KvAttnArgs {
     KvUnits listed;
     uint16_t* out;
     float* lse;
-    float* part;            // splits > 1: outputs [tokens * q_heads][splits][d], then (unit, sum) pairs of their weights
+    float* part;            // splits > 1: accumulators [tokens * q_heads][splits][d], then what part_sums holds
     int splits, column_tiles;
     bool turns;             // of k_kv_attn_step: sequences may have more rows than column_tiles hold
     uint32_t items;         // workgroups of k_kv_attn_rows
 };
 
-__device__ __forceinline__ float* part_sums(const KvAttnArgs& p)
+// Of a part of a row's keys: the accumulators' unit, the sum's unit and the sum (Running), and nothing.
+__device__ __forceinline__ float4* part_sums(const KvAttnArgs& p)
 {
-    return p.part + p.b.tokens * p.q_heads * p.splits * p.c.d;
+    return reinterpret_cast<float4*>(p.part + p.b.tokens * p.q_heads * p.splits * p.c.d);
 }
 
 // The key of each 32 that row r of the matrix stands for: lane group g = (r >> 2) & 1 of the output
@@ -281,7 +282,6 @@ struct WaveRows {
     Eight q[kSteps];
     f32x16_t acc[kTiles];
     Running run;       // (l of this half's keys)
-    int limit;         // keys below it are visible to the row
 
     // row: the row's values (NULL: none, zeros).
     __device__ __forceinline__ void start(const uint16_t* row, int g)
@@ -313,8 +313,8 @@ struct WaveRows {
         }
     }
 
-    // Keys from key0 on that the row does not see.
-    __device__ __forceinline__ void mask(f32x16_t s[2], int key0, int g) const
+    // Keys from key0 on that the row does not see: from `limit` on.
+    __device__ __forceinline__ void mask(f32x16_t s[2], int limit, int key0, int g) const
     {
         const int seen = limit - key0 - 16 * g;   // visible ones of this half's keys, counted from its first
 #pragma unroll
@@ -384,7 +384,7 @@ struct WaveRows {
     // A page in which some rows see NaN values that others do not (its NaN were stored as zeros): the rows
     // that see one become NaN, by a product of indicators. codes(kt, t): 16 tokens from 32 kt + 16 g on.
     template <typename Codes>
-    __device__ __forceinline__ void add_nan(Codes codes, int key0, int end, int g)
+    __device__ __forceinline__ void add_nan(Codes codes, int limit, int key0, int end, int g)
     {
 #pragma unroll
         for (int t = 0; t < kTiles; ++t) {
@@ -611,12 +611,24 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_kv_attn_rows(KvAttnAr
     WaveRows<D, F16> rowset;
     const int w0 = r0 + wave * kWaveRows;
     const bool idle = w0 >= rows;   // this wave copies only
-    const int row = w0 + r;
-    const bool valid = row < rows;
-    const int64_t token = s.start + (uint32_t)row / (uint32_t)p.group;
-    const int head = h * p.group + (uint32_t)row % (uint32_t)p.group;
-    rowset.start(valid ? p.q + token * p.ldq + (int64_t)head * D : nullptr, g);
-    rowset.limit = valid ? limit_of(row) : 0;
+    // The lane's row, from a value that the compiler does not know, so that what follows from it (a place, a limit) is
+    // computed where it is rarely needed: kept through the loop it takes registers that d = 256 lacks (the values under
+    // way are then waited for, to be moved: 0.79 against 0.73 ms on 3120 rows of 8 heads over 16000 tokens).
+    auto own_row = [&]() -> int {
+        int t = tid;
+        asm volatile("" : "+v"(t));
+        return w0 + (t & 31);
+    };
+    auto token_of = [&](int row) -> int64_t { return s.start + (uint32_t)row / (uint32_t)p.group; };
+    auto head_of = [&](int row) -> int { return h * p.group + (uint32_t)row % (uint32_t)p.group; };
+    auto own_limit = [&]() -> int {
+        const int row = own_row();
+        return row < rows ? limit_of(row) : 0;
+    };
+    {
+        const int row = own_row();
+        rowset.start(row < rows ? p.q + token_of(row) * p.ldq + (int64_t)head_of(row) * D : nullptr, g);
+    }
     const int least = limit_of(min(w0, last)), most = limit_of(min(w0 + kWaveRows - 1, last));
 
     // k goes to LDS as it is, by asynchronous copies of this thread's 16 bytes of each 4 KB; v passes through
@@ -729,7 +741,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_kv_attn_rows(KvAttnAr
                 };
                 if (key0 + kPage > least_all && nan_page[i & 1] == first + i) {   // (also where this wave sees the whole page)
                     const uint8_t* const src = p.c.v + ((int64_t)now.page * p.c.heads + h) * kPageBytes + row_key(r) * kPage + 16 * g;
-                    rowset.add_nan([&](int kt, int t) { return *reinterpret_cast<const uint4*>(src + t * 32 * kPage + 32 * kt); }, key0, s.length, g);
+                    rowset.add_nan([&](int kt, int t) { return *reinterpret_cast<const uint4*>(src + t * 32 * kPage + 32 * kt); }, own_limit(), key0, s.length, g);
                 }
                 f32x16_t sc[2];
                 f16x8_t w[2][2];
@@ -742,7 +754,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_kv_attn_rows(KvAttnAr
 #pragma unroll
                     for (int tt = 0; tt < D / 32; ++tt) v0[hf][tt] = value(0, hf, tt);
                 __builtin_amdgcn_sched_barrier(0);
-                if (masked) rowset.mask(sc, key0, g);
+                if (masked) rowset.mask(sc, own_limit(), key0, g);
                 rowset.weights(sc, p.scale, now.ek, now.ev, w);
                 rowset.add_values(v0, value, w);
             }
@@ -751,21 +763,24 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_kv_attn_rows(KvAttnAr
         }
     }
 
-    if (!valid) return;
-    const float l = across32(rowset.run.l, added), inv = l == 0.0f ? 0.0f : 1.0f / l, power = rowset.run.m - rowset.run.t - kLargest;
-    auto out_at = [&](int t, int i) { return times_power(rowset.acc[t][i] * inv, power); };
-    const int64_t out_row = token * p.q_heads + head;
+    const int row = own_row();
+    if (row >= rows) return;
+    const float l = across32(rowset.run.l, added);
+    const int64_t out_row = token_of(row) * p.q_heads + head_of(row);
     if (p.splits > 1) {
         float* const dst = p.part + (out_row * p.splits + split) * D + 16 * g;
         if (lo < hi)
 #pragma unroll
             for (int t = 0; t < D / 32; ++t)
 #pragma unroll
-                for (int i = 0; i < 16; i += 4)
-                    *reinterpret_cast<float4*>(dst + 32 * t + i) = make_float4(out_at(t, i), out_at(t, i + 1), out_at(t, i + 2), out_at(t, i + 3));
-        if (g == 0) *reinterpret_cast<float2*>(part_sums(p) + 2 * (out_row * p.splits + split)) = make_float2(rowset.run.t, l);
+                for (int i = 0; i < 4; ++i)
+                    *reinterpret_cast<float4*>(dst + 32 * t + 4 * i) = make_float4(rowset.acc[t][4 * i], rowset.acc[t][4 * i + 1],
+                                                                                 rowset.acc[t][4 * i + 2], rowset.acc[t][4 * i + 3]);
+        if (g == 0) part_sums(p)[out_row * p.splits + split] = make_float4(rowset.run.m, rowset.run.t, l, 0.0f);
         return;
     }
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l, power = rowset.run.m - rowset.run.t - kLargest;
+    auto out_at = [&](int t, int i) { return times_power(rowset.acc[t][i] * inv, power); };
     uint16_t* const dst = p.out + out_row * D + 16 * g;
 #pragma unroll
     for (int t = 0; t < D / 32; ++t)
@@ -785,7 +800,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_kv_attn_step(KvAttnAr
     constexpr int kTiles = D / 16;
     constexpr int kPart = D < 128 ? D : 128;
     __shared__ __attribute__((aligned(16))) float acc[4][kStepRows][kPart];
-    __shared__ float2 sums[4][kStepRows];   // the sum's unit, the sum
+    __shared__ float4 sums[4][kStepRows];   // as part_sums
     __shared__ __attribute__((aligned(16))) PageInfo info[kInfo];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int r = lane & 15, g = lane >> 4;
@@ -893,42 +908,42 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_kv_attn_step(KvAttnAr
 
         // The four waves' parts of each row, joined in LDS, 128 elements at a time.
         const int kept = min(rows - tile * kStepRows, kStepRows);
-        const float l = across16(across32(rowset.run.l, added), added), own = l == 0.0f ? 0.0f : 1.0f / l;
-        const float power = rowset.run.m - rowset.run.t - kLargest;
-        if (g == 0) sums[wave][r] = make_float2(rowset.run.t, l);
+        const float l = across16(across32(rowset.run.l, added), added);
+        if (g == 0) sums[wave][r] = make_float4(rowset.run.m, rowset.run.t, l, 0.0f);
 #pragma unroll
         for (int d0 = 0; d0 < D; d0 += kPart) {
             if (d0 > 0) __syncthreads();
 #pragma unroll
             for (int t = 0; t < kPart / 16; ++t) {
                 const f32x4_t v = rowset.acc[d0 / 16 + t];
-                *reinterpret_cast<float4*>(&acc[wave][r][16 * t + 4 * g]) =
-                    make_float4(times_power(v[0] * own, power), times_power(v[1] * own, power), times_power(v[2] * own, power), times_power(v[3] * own, power));
+                *reinterpret_cast<float4*>(&acc[wave][r][16 * t + 4 * g]) = make_float4(v[0], v[1], v[2], v[3]);
             }
             __syncthreads();
             for (int e = tid; e < kept * (kPart / 4); e += 256) {
                 const int row_e = e / (kPart / 4), d = 4 * (e % (kPart / 4));
-                float m = kNone;
+                float4 of[4];
+                float m = kNone, t = kNone;
 #pragma unroll
-                for (int wv = 0; wv < 4; ++wv) m = fmaxf(m, sums[wv][row_e].x);
-                float total = 0.0f, part[4], o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-                for (int wv = 0; wv < 4; ++wv) part[wv] = times_power(sums[wv][row_e].y, sums[wv][row_e].x - m), total += part[wv];
-                const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+                for (int wv = 0; wv < 4; ++wv) of[wv] = sums[wv][row_e], m = fmaxf(m, of[wv].x), t = fmaxf(t, of[wv].y);
+                float total = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
                 for (int wv = 0; wv < 4; ++wv) {
-                    const float f = part[wv] * inv;
+                    const float f = times_power(1.0f, of[wv].x - m);
                     const float4 a = *reinterpret_cast<const float4*>(&acc[wv][row_e][d]);
+                    total += times_power(of[wv].z, of[wv].y - t);
                     o[0] += f * a.x, o[1] += f * a.y, o[2] += f * a.z, o[3] += f * a.w;
                 }
                 const int row_at = tile * kStepRows + row_e;
                 const int64_t out_row = (s.start + at + row_at / p.group) * p.q_heads + h * p.group + row_at % p.group;
                 if (p.splits > 1) {
                     *reinterpret_cast<float4*>(p.part + (out_row * p.splits + split) * D + d0 + d) = make_float4(o[0], o[1], o[2], o[3]);
-                    if (d0 + d == 0) *reinterpret_cast<float2*>(part_sums(p) + 2 * (out_row * p.splits + split)) = make_float2(m, total);
+                    if (d0 + d == 0) part_sums(p)[out_row * p.splits + split] = make_float4(m, t, total, 0.0f);
                 } else {
-                    *reinterpret_cast<uint2*>(p.out + out_row * D + d0 + d) = make_uint2(pack_out<F16>(o[0], o[1]), pack_out<F16>(o[2], o[3]));
-                    if (p.lse && d0 + d == 0) p.lse[out_row] = log_sum(total, m);
+                    const float inv = total == 0.0f ? 0.0f : 1.0f / total, power = m - t - kLargest;
+                    *reinterpret_cast<uint2*>(p.out + out_row * D + d0 + d) =
+                        make_uint2(pack_out<F16>(times_power(o[0] * inv, power), times_power(o[1] * inv, power)),
+                                   pack_out<F16>(times_power(o[2] * inv, power), times_power(o[3] * inv, power)));
+                    if (p.lse && d0 + d == 0) p.lse[out_row] = log_sum(total, t);
                 }
             }
         }
@@ -945,16 +960,15 @@ __global__ __launch_bounds__(256) void k_kv_attn_join(KvAttnArgs p)
     const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
     if (row >= p.b.tokens * p.q_heads) return;
     if (p.b.q_start && row / p.q_heads >= p.b.q_start[p.b.batch]) return;   // behind the last sequence
-    const float* const sums = part_sums(p) + 2 * row * p.splits;
-    float2 own = make_float2(kNone, 0.0f);
-    if (lane < p.splits) own = *reinterpret_cast<const float2*>(sums + 2 * lane);
-    float m = own.x;
+    float4 own = make_float4(kNone, kNone, 0.0f, 0.0f);
+    if (lane < p.splits) own = part_sums(p)[row * p.splits + lane];
+    float m = own.x, t = own.y;
 #pragma unroll
-    for (int off = 1; off < 64; off <<= 1) m = fmaxf(m, __shfl_xor(m, off, 64));
-    float f = times_power(own.y, own.x - m), total = f;
+    for (int off = 1; off < 64; off <<= 1) m = fmaxf(m, __shfl_xor(m, off, 64)), t = fmaxf(t, __shfl_xor(t, off, 64));
+    const float f = times_power(1.0f, own.x - m);
+    float total = times_power(own.z, own.y - t);
 #pragma unroll
     for (int off = 1; off < 64; off <<= 1) total += __shfl_xor(total, off, 64);
-    f *= total == 0.0f ? 0.0f : 1.0f / total;
     float o[E];
 #pragma unroll
     for (int e = 0; e < E; ++e) o[e] = 0.0f;
@@ -967,19 +981,22 @@ __global__ __launch_bounds__(256) void k_kv_attn_join(KvAttnArgs p)
             for (int e = 0; e < E; ++e) v[i][e] = src[(int64_t)min(i0 + i, p.splits - 1) * D + e];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            // (a split without keys may not have written its outputs; lanes beyond the splits hold none)
-            const bool some = __shfl(own.y, (i0 + i) & 63, 64) != 0.0f && i0 + i < p.splits;
+            // (a split without keys has not written its accumulators; lanes beyond the splits hold none)
+            const bool some = __shfl(own.z, (i0 + i) & 63, 64) != 0.0f && i0 + i < p.splits;
             const float w = __shfl(f, (i0 + i) & 63, 64);
 #pragma unroll
             for (int e = 0; e < E; ++e) o[e] += some ? w * v[i][e] : 0.0f;
         }
     }
+    const float inv = total == 0.0f ? 0.0f : 1.0f / total, power = m - t - kLargest;
+#pragma unroll
+    for (int e = 0; e < E; ++e) o[e] = times_power(o[e] * inv, power);
     uint16_t* const dst = p.out + row * D + lane * E;
     if (E == 1) dst[0] = (uint16_t)pack_out<F16>(o[0], 0.0f);
     else
 #pragma unroll
         for (int e = 0; e + 1 < E; e += 2) *reinterpret_cast<uint32_t*>(dst + e) = pack_out<F16>(o[e], o[e + 1]);
-    if (p.lse && lane == 0) p.lse[row] = log_sum(total, m);
+    if (p.lse && lane == 0) p.lse[row] = log_sum(total, t);
 }
 
 // Which kernel a call takes, its units and its splits.
@@ -1017,7 +1034,7 @@ Plan make_plan(KvAttnArgs& p, int64_t max_query, int cus)
     splits = pages < 32 ? 1 : splits < pages / least ? splits : pages / least;
     plan.splits = (int)(splits < 1 ? 1 : splits > kMostSplits ? kMostSplits : splits);
     plan.items = groups * plan.splits;
-    plan.bytes = plan.splits > 1 ? p.b.tokens * p.q_heads * plan.splits * (int64_t)(p.c.d + 2) * 4 : 0;
+    plan.bytes = plan.splits > 1 ? p.b.tokens * p.q_heads * plan.splits * (int64_t)(p.c.d + 4) * 4 : 0;
     return plan;
 }
 
