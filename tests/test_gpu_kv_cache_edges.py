@@ -1,5 +1,5 @@
 """The 8-bit key/value cache on the GPU at the edges of what its entry points allow: the largest blocks of
-queries, weights far below a row's largest, hints that are wrong."""
+queries, weights far below a row's largest, hints that are wrong, batches without tokens."""
 import numpy as np
 import pytest
 import torch
@@ -168,3 +168,14 @@ def test_more_rows_than_max_query(device, d, Hq, H, news, lengths, causal):
         print(f"max_query {most} of {news} d={d} {Hq}/{H} causal={causal}", flush=True)
         torch.full((1 << 22,), float("nan"), device=device)   # (what an allocation of the call may find)
         attention_case(device, BF16, Hq, H, d, news, lengths, causal, seed=43, ragged=True, max_query=most)
+
+
+def test_choice_of_a_batch_without_tokens(device):
+    """No tokens, sequences with q_start: each has a row of the list that no block takes."""
+    H, d = 2, 128
+    kc = vdn_fp8.KvCache(*R.Cache(3, H, d, seed=1).tensors(device))
+    q, table, lengths = torch.zeros(0, 4, d, dtype=BF16, device=device), i32([[0, 1], [2, -1]], device), i32([100, 30], device)
+    for block, rows in ((128, 2), (1, 0)):
+        torch.full((rows * H * 3,), 7, dtype=torch.int32, device=device)   # (what the allocation may find)
+        lists = vdn_fp8.kv_select(q, kc, table, lengths, 3, query_block=block, q_start=i32([0, 0, 0], device))
+        assert lists.shape == (rows, H, 3) and bool((lists == -1).all())

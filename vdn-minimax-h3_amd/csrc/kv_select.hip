@@ -377,6 +377,12 @@ __global__ __launch_bounds__(kThreads) void k_kv_top(KvSelectArgs p)
         for (int i = (int)taken + lane; i < p.top; i += 64) out[i] = -1;
 }
 
+// The list of a call without tokens.
+__global__ __launch_bounds__(kThreads) void k_kv_no_blocks(KvSelectArgs p)
+{
+    for (int i = threadIdx.x; i < p.top; i += kThreads) p.blocks[(int64_t)blockIdx.x * p.top + i] = -1;
+}
+
 int select_arguments(const vdn_fp8_kv_cache* cache, const vdn_fp8_kv_batch* batch, int64_t q_heads, int64_t query_block, KvSelectArgs& p,
                      int64_t& bytes)
 {
@@ -392,11 +398,11 @@ int select_arguments(const vdn_fp8_kv_cache* cache, const vdn_fp8_kv_batch* batc
     p.query_block = (int)query_block;
     const int64_t n = p.b.batch > 0 ? p.b.tokens / p.b.batch : 0;
     p.listed = KvUnits{(uint32_t)query_block, (uint32_t)((n + query_block - 1) / query_block), 1, query_block == 1 ? 0 : 1};
-    p.rows = p.b.tokens == 0 ? 0 : kv_unit_count(p.b, p.listed);
+    p.rows = kv_unit_count(p.b, p.listed);   // (of a call without tokens too, where q_start gives each sequence one)
     if (p.rows * p.c.heads >= (1 << 24)) return set_error(VDN_FP8_EINVAL, "kv_select: %lld blocks of queries and heads, 2^24 at most", (long long)(p.rows * p.c.heads));
     if ((p.b.width + 63ll) / 64 * p.c.heads * p.b.batch >= (1 << 21))
         return set_error(VDN_FP8_EINVAL, "kv_select: 2^27 pages and heads of the page table at most");
-    bytes = p.rows * p.c.heads * (8 * (int64_t)p.b.width + 4 * p.c.d);
+    bytes = p.b.tokens == 0 ? 0 : p.rows * p.c.heads * (8 * (int64_t)p.b.width + 4 * p.c.d);
     return VDN_FP8_OK;
 }
 
@@ -423,7 +429,7 @@ extern "C" int vdn_fp8_kv_select(const vdn_fp8_kv_cache* cache, const vdn_fp8_kv
     if (dtype != VDN_FP8_DTYPE_BF16 && dtype != VDN_FP8_DTYPE_F16) return set_error(VDN_FP8_EINVAL, "kv_select: dtype must be bf16 or binary16");
     const int st = select_arguments(cache, batch, q_heads, query_block, p, bytes);
     if (st != VDN_FP8_OK || p.rows == 0) return st;
-    if (!query || !blocks) return set_error(VDN_FP8_EINVAL, "kv_select: null pointer");
+    if ((!query && p.b.tokens > 0) || !blocks) return set_error(VDN_FP8_EINVAL, "kv_select: null pointer");
     if (p.c.pages > 0 && !p.c.k_mean) return set_error(VDN_FP8_EINVAL, "kv_select: the cache keeps no k_mean");
     if (top < 1 || top > (1 << 24) || first < 0 || last < 0 || first + last > top)
         return set_error(VDN_FP8_EINVAL, "kv_select: need top >= 1, first and last >= 0, first + last <= top");
@@ -437,6 +443,10 @@ extern "C" int vdn_fp8_kv_select(const vdn_fp8_kv_cache* cache, const vdn_fp8_kv
     p.sum = (float*)workspace;   // (a multiple of 256 bytes)
     p.score = (double*)(p.sum + p.rows * p.c.heads * p.c.d);
     const dim3 block(kThreads), per_row((unsigned)(p.rows * p.c.heads));
+    if (p.b.tokens == 0) {
+        hipLaunchKernelGGL(k_kv_no_blocks, per_row, block, 0, stream, p);
+        return check_launch("kv_select");
+    }
     const bool f16 = dtype == VDN_FP8_DTYPE_F16;
     const int64_t step_pages = 4 * 4 * (64 / (p.c.d / 8)), step_groups = (p.b.width + step_pages - 1) / step_pages;   // of k_kv_scores_step
     if (p.b.width > 0 && p.query_block == 1 && p.rows <= 65535 && step_groups * p.c.heads * p.rows < (1 << 24)) {
