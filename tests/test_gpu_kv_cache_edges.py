@@ -179,3 +179,61 @@ def test_choice_of_a_batch_without_tokens(device):
         torch.full((rows * H * 3,), 7, dtype=torch.int32, device=device)   # (what the allocation may find)
         lists = vdn_fp8.kv_select(q, kc, table, lengths, 3, query_block=block, q_start=i32([0, 0, 0], device))
         assert lists.shape == (rows, H, 3) and bool((lists == -1).all())
+
+
+# -- the branch --------------------------------------------------------------------------------
+
+def branch(device, H, d, C, seed=51):
+    g = torch.Generator().manual_seed(seed)
+    to = [torch.nn.Linear(C, H * d, dtype=BF16) for _ in range(3)]
+    for m in to:
+        m.weight.data.copy_(0.1 * torch.randn(m.weight.shape, generator=g))
+    norm = torch.nn.RMSNorm(d, eps=1e-6, dtype=BF16).to(device)
+    return [m.to(device).requires_grad_(False) for m in to], norm.requires_grad_(False), g
+
+
+def test_the_branch_refuses_sizes_before_it_stores(device):
+    """What only the library knows to refuse: more sequences than a choice of pages numbers, more workgroups than a
+    launch holds."""
+    from vdn_fp8.softmax_attention import cached_attention
+    H, d, C, B = 1, 64, 16, 70000
+    to, norm, g = branch(device, H, d, C)
+    x = torch.randn(B, C, generator=g).to(BF16).to(device)
+    kc = vdn_fp8.KvCache.empty(2, H, d, device)
+    for t in kc:
+        t.view(torch.uint8).zero_()
+    table, lengths = i32([[0]], device).expand(B, 1), torch.zeros(B, dtype=torch.int32, device=device)
+    lengths[0] = 1
+    with pytest.raises(ValueError, match="65535"):
+        cached_attention(x, *to, norm, norm, kc, table, lengths, top=2, query_block=1)
+    assert not any(bool(t.view(torch.uint8).any()) for t in kc)
+    # (a head's units of rows and one behind the last sequence, 2^24 of them with 4096 heads of few tokens each)
+    heads = 4096
+    wide = vdn_fp8.KvCache.empty(1, heads, d, device)
+    rows = torch.zeros(5000, heads, d, dtype=BF16, device=device)
+    start, table = torch.arange(5001, dtype=torch.int32, device=device), i32([[0]], device).expand(5000, 1)
+    with pytest.raises(ValueError, match="2\\^24"):
+        vdn_fp8.kv_cache.check_attention(rows, wide, table, torch.ones(5000, dtype=torch.int32, device=device), q_start=start)
+
+
+def test_the_branch_over_one_page(device):
+    """top = 1: the newest page alone, or the best one."""
+    from vdn_fp8 import softmax_attention as SA
+    H, d, C, n = 2, 64, 48, 128
+    to, norm, g = branch(device, H, d, C)
+    table = i32([[4, 0, 2, 3]], device)
+    caches = []
+    for _ in range(2):
+        caches.append(vdn_fp8.KvCache.empty(5, H, d, device))
+        for t in caches[-1]:
+            t.view(torch.uint8).zero_()
+    lengths = i32([0], device)
+    for first, last in ((0, 1), (0, 0)):
+        x = torch.randn(n, C, generator=g).to(BF16).to(device)
+        lengths += n
+        out = SA.cached_attention(x, *to, norm, norm, caches[0], table, lengths, top=1, query_block=128, first=first, last=last)
+        q, k, v, _ = SA.qkv(x, *to, H, norm, norm)
+        vdn_fp8.kv_append(k, v, caches[1], table, lengths)
+        lists = vdn_fp8.kv_select(q, caches[1], table, lengths, 1, query_block=128, first=first, last=last)
+        assert torch.equal(out, vdn_fp8.kv_attention(q, caches[1], table, lengths, blocks=lists, query_block=128).flatten(1))
+        assert last == 0 or bool((lists == lengths.item() // PAGE - 1).all())

@@ -167,6 +167,25 @@ def test_the_branch_refuses_before_it_stores():
             cached_attention(x, *args, table, lengths, **more)
 
 
+@pytest.mark.parametrize("more,needle", [
+    (dict(top=1, query_block=128), "top must be"), (dict(top=0, query_block=128), "top must be"), (dict(top=4, query_block=128, first=3, last=2), "top must be"),
+    (dict(top=4, query_block=128, first=-1), "top must be"), (dict(top=4, query_block=65), "query_block must be"), (dict(top=4, query_block=0), "query_block must be"),
+    (dict(top=4, query_block=-128), "query_block must be"), (dict(scale=0.0), "scale"), (dict(scale=-1.0), "scale"), (dict(scale=float("nan")), "scale"),
+    (dict(scale=float("inf")), "scale"), (dict(scale=3e38), "scale"), (dict(max_query=-1), "max_query"),
+])
+def test_the_branch_stores_nothing_when_it_refuses(monkeypatch, more, needle):
+    from vdn_fp8 import kv_cache as K
+    from vdn_fp8.softmax_attention import cached_attention
+    stored = []
+    monkeypatch.setattr(K, "qk_prep_append", lambda query, *a, **kw: stored.append(query) or query)
+    x, table, lengths = torch.zeros(2, 8, dtype=torch.bfloat16), torch.zeros(1, 3, dtype=torch.int32), torch.zeros(1, dtype=torch.int32)
+    to = [torch.nn.Linear(8, 128, dtype=torch.bfloat16) for _ in range(3)]
+    norm = torch.nn.RMSNorm(64, eps=1e-6, dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match=needle):
+        cached_attention(x, *to, norm, norm, pool(), table, lengths, **more)
+    assert not stored
+
+
 def test_batch_checks():
     from vdn_fp8 import kv_cache as K
     cpu, table, lengths = torch.device("cpu"), torch.zeros(2, 3, dtype=torch.int32), torch.zeros(2, dtype=torch.int32)

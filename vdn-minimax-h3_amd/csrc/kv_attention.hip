@@ -1038,6 +1038,12 @@ Plan make_plan(KvAttnArgs& p, int64_t max_query, int cus)
     return plan;
 }
 
+int check_plan(const Plan& plan)
+{
+    if (plan.items < ((int64_t)1 << 24)) return VDN_FP8_OK;
+    return set_error(VDN_FP8_EINVAL, "kv_attention: %lld workgroups, 2^24 at most", (long long)plan.items);
+}
+
 template <int D, bool F16>
 int launch(const KvAttnArgs& p, bool step, hipStream_t stream)
 {
@@ -1096,8 +1102,9 @@ extern "C" int vdn_fp8_kv_attention_workspace_size(const vdn_fp8_kv_cache* cache
     if (st != VDN_FP8_OK || p.b.tokens == 0) return st;
     const int cus = device_cus();
     if (cus == 0) return set_error(VDN_FP8_ELAUNCH, "kv_attention_workspace_size: the device cannot be queried");
-    *bytes = make_plan(p, max_query, cus).bytes;
-    return VDN_FP8_OK;
+    const Plan plan = make_plan(p, max_query, cus);
+    *bytes = plan.bytes;
+    return check_plan(plan);
 }
 
 extern "C" int vdn_fp8_kv_attention(const vdn_fp8_kv_cache* cache, const vdn_fp8_kv_batch* batch, const void* query, int dtype,
@@ -1117,7 +1124,8 @@ extern "C" int vdn_fp8_kv_attention(const vdn_fp8_kv_cache* cache, const vdn_fp8
     const int cus = device_cus();
     if (cus == 0) return set_error(VDN_FP8_ELAUNCH, "kv_attention: the device cannot be queried");
     const Plan plan = make_plan(p, max_query, cus);
-    if (plan.items >= ((int64_t)1 << 24)) return set_error(VDN_FP8_EINVAL, "kv_attention: %lld workgroups, 2^24 at most", (long long)plan.items);
+    const int fits = check_plan(plan);
+    if (fits != VDN_FP8_OK) return fits;
     if (plan.bytes > 0 && (!workspace || workspace_bytes < plan.bytes))
         return set_error(VDN_FP8_EINVAL, "kv_attention: workspace of %lld bytes, %lld needed", (long long)workspace_bytes, (long long)plan.bytes);
     p.q = (const uint16_t*)query, p.ldq = ldq, p.scale = scale * 1.4426950408889634f, p.causal = causal != 0;

@@ -250,6 +250,47 @@ def _workspace(entry, c, b, args, dev):
     return got
 
 
+def _check_scale(scale, d):
+    scale = float(d ** -0.5 if scale is None else scale)
+    if not 0 < scale <= 2e38:   # (NaN too)
+        raise ValueError(f"scale must be positive, and 2e38 at most (got {scale})")
+    return scale
+
+
+def _check_choice(group, top, query_block, first, last):
+    if query_block < 1 or (query_block > 1 and query_block * group % 128):
+        raise ValueError(f"query_block must be 1, or such that query_block * {group} (heads of a group) is a multiple of 128 (got {query_block})")
+    if top < 1 or first < 0 or last < 0 or first + last > top:
+        raise ValueError(f"top must be at least 1 and hold the first {first} and last {last} pages (got {top})")
+
+
+def check_attention(query, cache, page_table, lengths, *, scale=None, q_start=None, max_query=None, top=None, query_block=None, first=1, last=1):
+    """Raises what `kv_attention` of these arguments would -- with `top`, over the pages of `kv_select` --
+    and launches nothing: for callers that store before they attend."""
+    dev, (T, q_heads, _) = query.device, query.shape
+    c = _cache(cache, dev)
+    heads, d = c.heads, c.head_dim
+    if q_heads % heads or not q_heads:
+        raise ValueError(f"{q_heads} query heads for a cache of {heads}")
+    if (top is None) != (query_block is None):
+        raise ValueError("top and query_block go together")
+    _check_scale(scale, d)
+    if top is not None:
+        if cache.k_mean is None:
+            raise ValueError("top needs a cache that keeps k_mean")
+        _check_choice(q_heads // heads, top, query_block, first, last)
+    if max_query is not None and max_query < 0:
+        raise ValueError(f"max_query must not be negative (got {max_query})")
+    if not query.is_cuda:
+        raise ValueError("the cache's kernels run on the GPU; query is a CPU tensor")
+    # what the library refuses by sizes
+    b = _batch(page_table, lengths, q_start, T, c.pages, dev)
+    with _on(dev):
+        _workspace("vdn_fp8_kv_attention_workspace_size", c, b, (q_heads, int(max_query or 0), top or 0, query_block or 0), dev)
+        if top is not None:
+            _workspace("vdn_fp8_kv_select_workspace_size", c, b, (q_heads, query_block), dev)
+
+
 def kv_attention(query, cache, page_table, lengths, *, scale=None, causal=False, q_start=None, max_query=None, blocks=None,
                  query_block=None, return_lse=False):
     """Softmax attention of query [T, q_heads, d] (bf16 or float16; any token stride) over the cached
@@ -286,7 +327,7 @@ def kv_attention(query, cache, page_table, lengths, *, scale=None, causal=False,
         n = _workspace("vdn_fp8_kv_attention_workspace_size", c, b, size, dev)
         ws = torch.empty(n, device=dev, dtype=torch.uint8) if n else None
         _lib.check(_lib.load().vdn_fp8_kv_attention(
-            c, b, query.data_ptr(), _DTYPES[query.dtype], q_heads, _ld(query), size[1], float(d ** -0.5 if scale is None else scale),
+            c, b, query.data_ptr(), _DTYPES[query.dtype], q_heads, _ld(query), size[1], _check_scale(scale, d),
             int(bool(causal)), _ptr(blocks), top, size[3], out.data_ptr(), _ptr(lse), _ptr(ws), n, _stream(query)), "kv_attention")
     return (out, lse) if return_lse else out
 
@@ -308,8 +349,7 @@ def kv_select(query, cache, page_table, lengths, top, *, query_block, first=1, l
         raise ValueError(f"{q_heads} query heads for a cache of {heads}")
     if cache.k_mean is None:
         raise ValueError("kv_select needs a cache that keeps k_mean")
-    if query_block < 1 or top < 1:
-        raise ValueError(f"query_block and top must be at least 1 (got {query_block}, {top})")
+    _check_choice(q_heads // heads, top, query_block, first, last)
     c = _cache(cache, dev)
     b = _batch(page_table, lengths, q_start, T, c.pages, dev)
     blocks = torch.empty(_block_rows(T, b.batch, query_block, q_start is not None), heads, top, device=dev, dtype=torch.int32)

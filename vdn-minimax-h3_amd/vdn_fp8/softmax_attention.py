@@ -92,31 +92,28 @@ def qkv(x, to_q, to_k, to_v, heads, norm_q, norm_k, rotary_emb=None):
 
 
 def cached_attention(x, to_q, to_k, to_v, norm_q, norm_k, cache, page_table, lengths, *, rotary_emb=None, causal=False,
-                     scale=None, q_start=None, max_query=None, top=None, query_block=None):
+                     scale=None, q_start=None, max_query=None, top=None, query_block=None, first=1, last=1):
     """`qkv` and the attention behind it where earlier tokens are kept in a `KvCache`: one quantization
     of x for the three GEMMs, then QK-norm, rope and the store of k and v in one launch
     (`qk_prep_append`), then `kv_attention` over each sequence's cache, its new tokens included. The cache's
     shape gives the heads; to_q may have more of them (a multiple of the cache's). x [T, hidden] bf16;
     projections, norms and rotary_emb as in `qkv`; page_table, lengths, q_start, max_query, causal and scale
     as in `kv_attention`. With `top`, each block of `query_block` queries attends to the `top` pages
-    that `kv_select` finds for it. Returns [T, q_heads * d], what the output projection takes."""
-    from .kv_cache import kv_attention, kv_select, qk_prep_append
+    that `kv_select` finds for it (`first` and `last` as there). What any part refuses is refused before
+    anything is stored. Returns [T, q_heads * d], what the output projection takes."""
+    from .kv_cache import check_attention, kv_attention, kv_select, qk_prep_append
 
-    # (what only a later part would refuse is refused before the store)
-    if (top is None) != (query_block is None):
-        raise ValueError("top and query_block go together")
-    if top is not None and cache.k_mean is None:
-        raise ValueError("top needs a cache that keeps k_mean")
-    heads, d = cache.k.shape[1], cache.k.shape[-1]
+    d = cache.k.shape[-1]
     query, key, value = (t.unflatten(-1, (-1, d)) for t in _project(x, (to_q, to_k, to_v)))
-    if query.shape[1] % heads:
-        raise ValueError(f"{query.shape[1]} query heads for a cache of {heads}")
+    check_attention(query, cache, page_table, lengths, scale=scale, q_start=q_start, max_query=max_query, top=top, query_block=query_block,
+                    first=first, last=last)
     cos, sin = (None, None) if rotary_emb is None else rotary_emb
     query = qk_prep_append(query, key, value, (norm_q.weight, norm_q.eps), (norm_k.weight, norm_k.eps), cache, page_table, lengths,
                            cos=cos, sin=sin, q_start=q_start)
     blocks = None
     if top is not None:
-        blocks = kv_select(query, cache, page_table, lengths, top, query_block=query_block, causal=causal, q_start=q_start)
+        blocks = kv_select(query, cache, page_table, lengths, top, query_block=query_block, first=first, last=last, causal=causal,
+                           q_start=q_start)
     out = kv_attention(query, cache, page_table, lengths, scale=scale, causal=causal, q_start=q_start, max_query=max_query, blocks=blocks,
                        query_block=query_block)
     return out.flatten(1)
