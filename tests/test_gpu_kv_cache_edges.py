@@ -237,3 +237,13 @@ def test_the_branch_over_one_page(device):
         lists = vdn_fp8.kv_select(q, caches[1], table, lengths, 1, query_block=128, first=first, last=last)
         assert torch.equal(out, vdn_fp8.kv_attention(q, caches[1], table, lengths, blocks=lists, query_block=128).flatten(1))
         assert last == 0 or bool((lists == lengths.item() // PAGE - 1).all())
+
+
+@pytest.mark.parametrize("block", [0, -64])
+def test_lists_of_no_queries_are_refused(device, block):
+    H, d = 2, 64
+    kc = vdn_fp8.KvCache.empty(2, H, d, device)
+    q, blocks = torch.zeros(3, H, d, dtype=BF16, device=device), torch.zeros(1, H, 1, dtype=torch.int32, device=device)
+    for start in (None, i32([0, 3], device)):
+        with pytest.raises(ValueError, match="query_block"):
+            vdn_fp8.kv_attention(q, kc, i32([[0]], device), i32([3], device), q_start=start, blocks=blocks, query_block=block)

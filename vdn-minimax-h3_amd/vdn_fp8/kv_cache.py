@@ -315,6 +315,8 @@ def kv_attention(query, cache, page_table, lengths, *, scale=None, causal=False,
     if blocks is not None:
         if query_block is None:
             raise ValueError("blocks need query_block, the queries that share a list")
+        if query_block < 1:
+            raise ValueError(f"query_block must be at least 1 (got {query_block})")
         rows = _block_rows(T, b.batch, query_block, q_start is not None)
         if blocks.dim() != 3 or blocks.shape[:2] != (rows, heads) or blocks.dtype != torch.int32 or blocks.device != dev or not blocks.shape[2]:
             raise ValueError(f"blocks must be int32 [{rows}, {heads}, top] on {dev} (got {blocks.dtype} {tuple(blocks.shape)})")
