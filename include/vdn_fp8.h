@@ -428,7 +428,8 @@ int vdn_fp8_qk_prep_append(const vdn_fp8_kv_cache *cache, const vdn_fp8_kv_batch
  * Replaces: the attention of HybridAttention's softmax branch (src/models/softmax_attention/window.py:56,
  *           decomposed.py:190) for keys and values held in a cache.
  * Requires: q_heads a multiple of heads; tokens * q_heads < 2^30; query_block 1 or query_block *
- *           q_heads / heads a multiple of 128; scale > 0; ldq % 8 == 0; query, out 16-byte aligned.
+ *           q_heads / heads a multiple of 128; scale in (0, 2e38]; fewer than 2^24 workgroups (128 rows, or single
+ *           queries up to 16, of a key/value head each); ldq % 8 == 0; query, out 16-byte aligned.
  */
 int vdn_fp8_kv_attention_workspace_size(const vdn_fp8_kv_cache *cache, const vdn_fp8_kv_batch *batch,
                                         int64_t q_heads, int64_t max_query, int64_t top,
@@ -450,7 +451,8 @@ int vdn_fp8_kv_attention(const vdn_fp8_kv_cache *cache, const vdn_fp8_kv_batch *
  * The workspace as above.
  * Replaces: nothing in the reference (its softmax branch attends to fixed windows,
  *           src/models/softmax_attention/window.py).
- * Requires: as vdn_fp8_kv_attention; k_mean; first, last >= 0; first + last <= top.
+ * Requires: as vdn_fp8_kv_attention; k_mean; first, last >= 0; first + last <= top; batch <= 65535; rows * heads < 2^24;
+ *           ceil(max_pages / 64) * heads * batch < 2^21.
  */
 int vdn_fp8_kv_select_workspace_size(const vdn_fp8_kv_cache *cache, const vdn_fp8_kv_batch *batch,
                                      int64_t q_heads, int64_t query_block, int64_t *bytes);

@@ -123,6 +123,14 @@ def test_select_workspace_holds_scores_and_sums():
     assert n.value == 4 * 2 * (3 * 8 + 128 * 4)
 
 
+def test_select_counts_rows_as_attention_does():
+    n, many = ctypes.c_int64(0), batch(batch=1, tokens=1 << 28)
+    for rows, ok in (((1 << 28) - 1, L.OK), (1 << 28, L.EINVAL)):
+        assert L.load().vdn_fp8_kv_select_workspace_size(cache(), batch(batch=1, tokens=rows), 4, 1 << 20, ctypes.byref(n)) == ok
+    assert "2^30" in L.load().vdn_fp8_last_error().decode()
+    assert attention(b=many) == L.EINVAL and "2^30" in L.load().vdn_fp8_last_error().decode()
+
+
 def pool(**kw):
     c = vdn_fp8.KvCache.empty(3, 2, 64, "cpu")
     return c._replace(**kw)

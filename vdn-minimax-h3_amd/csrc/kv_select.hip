@@ -391,6 +391,8 @@ int select_arguments(const vdn_fp8_kv_cache* cache, const vdn_fp8_kv_batch* batc
     if (q_heads < 1 || q_heads > (1 << 16) || q_heads % p.c.heads)
         return set_error(VDN_FP8_EINVAL, "kv_select: %lld query heads for %d key/value heads", (long long)q_heads, p.c.heads);
     p.group = (int)(q_heads / p.c.heads);
+    if (p.b.tokens * q_heads >= ((int64_t)1 << 30))
+        return set_error(VDN_FP8_EINVAL, "kv_select: %lld tokens of %lld heads, 2^30 rows at most", (long long)p.b.tokens, (long long)q_heads);
     if (query_block < 1 || query_block > (1 << 20) || (query_block > 1 && query_block * p.group % 128))
         return set_error(VDN_FP8_EINVAL, "kv_select: query_block must be 1, or such that query_block * group is a multiple of 128 "
                          "(got %lld with groups of %d)", (long long)query_block, p.group);
