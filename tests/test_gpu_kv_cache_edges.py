@@ -181,6 +181,29 @@ def test_choice_of_a_batch_without_tokens(device):
         assert lists.shape == (rows, H, 3) and bool((lists == -1).all())
 
 
+# -- splits of short key axes ------------------------------------------------------------------
+
+@pytest.mark.parametrize("d,Hq,H,B,n,pages,split", [
+    (128, 40, 8, 1, 1, 16, False), (128, 40, 8, 1, 1, 24, True), (256, 32, 4, 1, 1, 16, True), (64, 16, 2, 1, 1, 24, False),
+    (64, 12, 12, 3, 77, 8, False), (64, 12, 12, 3, 77, 12, True), (64, 12, 12, 3, 77, 31, True), (128, 8, 8, 4, 300, 14, False), (128, 8, 8, 4, 300, 24, True),
+])
+def test_short_key_axes_are_split_where_that_pays(device, d, Hq, H, B, n, pages, split):
+    """Below 32 pages too, where the pages spared outweigh the parts; the workspace tells which way a call goes."""
+    import ctypes
+
+    import vdn_fp8._lib as L
+    if torch.cuda.get_device_properties(device).multi_processor_count != 256:
+        pytest.skip("the sizes are those of 256 compute units")
+    size = ctypes.c_int64(-1)
+    c = L.KvCacheStruct(*[1 << 20] * 5, pages, H, d)
+    b = L.KvBatchStruct(1 << 20, pages, pages, 1 << 20, None, B, B * n)
+    assert L.load().vdn_fp8_kv_attention_workspace_size(c, b, Hq, 0, 0, 0, ctypes.byref(size)) == L.OK
+    assert (size.value > 0) == split
+    if B == 1 or n < 100:
+        print(f"split {pages} pages d={d} {Hq}/{H}", flush=True)
+        attention_case(device, BF16, Hq, H, d, [n] * B, [pages * PAGE - 5 * b for b in range(B)], True, seed=45, extra=0)
+
+
 # -- the branch --------------------------------------------------------------------------------
 
 def branch(device, H, d, C, seed=51):

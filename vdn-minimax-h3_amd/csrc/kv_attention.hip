@@ -1027,14 +1027,23 @@ Plan make_plan(KvAttnArgs& p, int64_t max_query, int cus)
         groups = (kv_unit_count(p.b, p.units) + (p.b.q_start ? 1 : 0)) * p.c.heads;
     }
     // Splits where the workgroups alone leave compute units idle: enough for four workgroups (steps) or two
-    // (rows) on each, of at least eight (four) pages, and none below 32: a page costs a wave of k_kv_attn_step about
-    // 0.8 us where nothing else runs, the join and its launch 4 (13 pages of 8 heads: 10.1 us whole, 7.7 + 3.9 in four).
-    const int64_t want = (int64_t)cus * (plan.step ? 4 : 2), least = plan.step ? 8 : 4;
+    // (rows) on each, of at least eight (four) pages, and only where the pages that a workgroup is spared take longer than
+    // the join and its launch (3.4 us) and the parts (a row's 0.13 + 0.0022 d ns, written and read). A page takes max(1, d / 100) us of
+    // k_kv_attn_rows, d / 400 of k_kv_attn_step, whose waves take four at once. Measured (us, whole and split): one token,
+    // d = 128, 20 pages 11.2 and 11.4, 24 12.6 and 10.9, 31 14.9 and 11.9; d = 256, 14 16.3 and 16.3, 16 17.6 and 15.5;
+    // d = 64, 22 7.7 and 8.6; 3 x 77 rows of 12 heads of 64, 8 11.6 and 11.7, 12 15.9 and 12.4, 31 35.3 and 15.1;
+    // 200 rows of 16 heads on 8 of 128, 8 15.4 and 16.9, 12 20.5 and 18.3; 4 x 300 rows of 8 heads of 128, 14 23.2 and 30.4,
+    // 24 36.0 and 32.2; 1000 rows of 16 heads of 64, 24 28.0 and 32.2, 32 35.9 and 34.8.
+    const int64_t want = (int64_t)cus * (plan.step ? 4 : 2), least = plan.step ? 8 : 4, rows = p.b.tokens * p.q_heads;
     int64_t splits = groups > 0 ? want / groups : 1;
-    splits = pages < 32 ? 1 : splits < pages / least ? splits : pages / least;
-    plan.splits = (int)(splits < 1 ? 1 : splits > kMostSplits ? kMostSplits : splits);
+    splits = std::min(std::min(splits, pages / least), (int64_t)kMostSplits);
+    if (splits > 1) {
+        const double page = plan.step ? p.c.d / 400.0 : std::max(1.0, p.c.d / 100.0), part = rows * (0.13 + 0.0022 * p.c.d) * 1e-3;
+        if ((pages - (pages + splits - 1) / splits) * page < 3.4 + splits * part) splits = 1;
+    }
+    plan.splits = (int)std::max(splits, (int64_t)1);
     plan.items = groups * plan.splits;
-    plan.bytes = plan.splits > 1 ? p.b.tokens * p.q_heads * plan.splits * (int64_t)(p.c.d + 4) * 4 : 0;
+    plan.bytes = plan.splits > 1 ? rows * plan.splits * (p.c.d + 4) * 4 : 0;
     return plan;
 }
 
