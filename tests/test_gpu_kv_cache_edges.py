@@ -32,8 +32,9 @@ def attend_by_channel(cache, q, table, length, scale, causal=False):
     as 2^5 where it moves the row's unit, which it does when it is more than 2^20 from every other page's (the unit
     is within 2^10 of the page before). Rounded to binary16 each is off by 2^-11 of itself or by 2^-25 there: 2^-20,
     or 2^-30, of the page's largest. A unit stays within 2^60 of the largest: 2^-90 of that at most. The products'
-    sum is N / 16 sums one after another of 16 products each (four more levels), and a few joins: N / 16 + 22 roundings
-    (2^-23, should they truncate) of the magnitudes. Scores as in kv_reference.attend."""
+    sum is N / 16 sums one after another of 16 products each (four more levels), a few joins, and a power and a product
+    for each page that moves the unit: N / 16 + N / 32 + 22 roundings (2^-23, should they truncate) of the magnitudes.
+    Scores as in kv_reference.attend."""
     n, Hq, d = q.shape
     pages = -(-length // PAGE)
     k = torch.cat([R.decode(cache.k[p, 0], cache.ek[p, 0]) for p in table[:pages]])[:length]
@@ -55,7 +56,7 @@ def attend_by_channel(cache, q, table, length, scale, causal=False):
     alone = (unit == first[:, None]) & (first > 2.0 ** 20 * second)[:, None]
     held = torch.where(alone, 2.0 ** -30, 2.0 ** -20) * unit + 2.0 ** -90 * first[:, None]
     es = scale * 2.0 ** -18 * (x.abs() @ k.abs().T).amax(1)
-    tol = (2.0 ** -11 + 2.0 ** -18 + 2.0 ** -23 * (length / 16 + 22) + 2 * es)[:, None] * a + held @ size
+    tol = (2.0 ** -11 + 2.0 ** -18 + 2.0 ** -23 * (length / 16 + length / 32 + 22) + 2 * es)[:, None] * a + held @ size
     return out.reshape(n, Hq, d), z.reshape(n, Hq), tol.reshape(n, Hq, d), (2 * es + 2.0 ** -20 + 2.0 ** -22 * z.abs()).reshape(n, Hq)
 
 
@@ -153,7 +154,7 @@ def test_the_sum_of_many_pages_of_zeros(device):
     top = float(R.decode(cache.k[1, 0], cache.ek[1, 0])[0, 0])
     want = top + np.log(64.0 * (pages - 1) + 64.0 * np.exp(-top))
     assert not bool(out.any())
-    # one sum a page in binary32, and the logarithm's rounding
+    # one sum a page in binary32, and the logarithm's rounding (the unit moves once)
     assert bool(((z.double() - want).abs() <= pages * 2.0 ** -24 + 2.0 ** -20).all())
 
 

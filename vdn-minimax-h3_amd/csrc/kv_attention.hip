@@ -23,9 +23,10 @@
 // binary16 has few exponents, and one maximum for all pages would leave them to the weights next to the row's
 // largest: behind a token 17 nats above the others, or one of little weight in a page of large values, the others would
 // be lost from the output, though not from the sum. So a row's unit follows its pages both ways: a page whose
-// largest x + ev lies more than 10 from m moves m to it, and the accumulators by that power of two, exactly. A page's
-// largest weight is then held as 2^-5 to 2^15 (2^5 where the unit moves), and each weight is off by 2^-11 of itself or
-// 2^-20 of its page's largest. A unit comes down by 2^60 at most, which binary32 accumulators leave room for: pages
+// largest x + ev lies more than 10 from m moves m to it, and the accumulators by that power. A page's
+// largest weight is then held as 2^-5 to 2^15 (as 2^5, without a rounding, where the unit moves: whole numbers for m would make
+// the moves exact but round that weight, and make 2.9e-4 of 2.7e-4 of error in binary16 outputs), and each weight is off by 2^-11
+// of itself or 2^-20 of its page's largest. A unit comes down by 2^60 at most, which binary32 accumulators leave room for: pages
 // further below a row's largest are zeros. On 3120 tokens over 32760, whose pages' largest scores spread by 2 in standard
 // deviation, 2.19 ms; with 9, 8 and 6 in place of 10 2.24, 2.29 and 2.33; with a unit that only rises, by more than 8, 2.17.
 //
@@ -119,16 +120,17 @@ __device__ __forceinline__ float added(float a, float b) { return a + b; }
 
 __device__ __forceinline__ float exponent_f32(int e) { return __uint_as_float((uint32_t)(min(max(e, -126), 127) + 127) << 23); }
 
-// v 2^e for a whole number e, exact within binary32's range. (What is further out than 1000 is 0, or was NaN.)
+// v 2^e, where 2^e alone may be out of binary32's range.
 __device__ __forceinline__ float times_power(float v, float e)
 {
-    return __builtin_ldexpf(v, (int)__builtin_amdgcn_fmed3f(e, -1000.0f, 1000.0f));
+    const float half = __builtin_amdgcn_exp2f(0.5f * e);
+    return v * half * half;
 }
 
 // One row's softmax over the pages so far: accumulators hold sum P' v in units of 2^m, P' times 2^kLargest, and the
 // sum of weights (of the lane's keys) is l 2^t.
 struct Running {
-    float m, t;   // whole numbers
+    float m, t;
     float low;    // m does not go below
     float l;
     __device__ __forceinline__ void start() { m = t = low = kNone, l = 0.0f; }
@@ -139,10 +141,10 @@ struct Running {
     {
         const float to = fmaxf(x + ev, low);
         if (!__any(fabsf(to - m) > kWindow || x > t + kRange)) return false;
-        const float now = __builtin_rintf(to), most = fmaxf(t, __builtin_rintf(x));
-        move = m - now;
-        l = times_power(l, t - most);
-        m = now, t = most, low = fmaxf(low, now - kRange);
+        const float most = fmaxf(t, x);
+        move = m - to;
+        l *= __builtin_amdgcn_exp2f(t - most);
+        m = to, t = most, low = fmaxf(low, to - kRange);
         return true;
     }
     // A page below the unit's reach adds nothing to the accumulators, but its weights count in l (values of zeros have the
@@ -338,7 +340,7 @@ struct WaveRows {
         const float x = across32(larger(larger3(four[0], four[1], four[2]), four[3]), larger) * f;
         float move;
         if (run.moves(x, shift, move)) {
-            const float a = times_power(1.0f, move);
+            const float a = __builtin_amdgcn_exp2f(move);
 #pragma unroll
             for (int t = 0; t < kTiles; ++t)
 #pragma unroll
@@ -466,7 +468,7 @@ struct StepRows {
         const float x = across16(across32(larger(larger3(four[0], four[1], four[2]), four[3]), larger), larger) * f;
         float move;
         if (run.moves(x, shift, move)) {
-            const float a = times_power(1.0f, move);
+            const float a = __builtin_amdgcn_exp2f(move);
 #pragma unroll
             for (int t = 0; t < kTiles; ++t) acc[t] *= a;
         }
@@ -928,9 +930,9 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_kv_attn_step(KvAttnAr
                 float total = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
                 for (int wv = 0; wv < 4; ++wv) {
-                    const float f = times_power(1.0f, of[wv].x - m);
+                    const float f = __builtin_amdgcn_exp2f(of[wv].x - m);
                     const float4 a = *reinterpret_cast<const float4*>(&acc[wv][row_e][d]);
-                    total += times_power(of[wv].z, of[wv].y - t);
+                    total += of[wv].z * __builtin_amdgcn_exp2f(of[wv].y - t);
                     o[0] += f * a.x, o[1] += f * a.y, o[2] += f * a.z, o[3] += f * a.w;
                 }
                 const int row_at = tile * kStepRows + row_e;
@@ -965,8 +967,8 @@ __global__ __launch_bounds__(256) void k_kv_attn_join(KvAttnArgs p)
     float m = own.x, t = own.y;
 #pragma unroll
     for (int off = 1; off < 64; off <<= 1) m = fmaxf(m, __shfl_xor(m, off, 64)), t = fmaxf(t, __shfl_xor(t, off, 64));
-    const float f = times_power(1.0f, own.x - m);
-    float total = times_power(own.z, own.y - t);
+    const float f = __builtin_amdgcn_exp2f(own.x - m);
+    float total = own.z * __builtin_amdgcn_exp2f(own.y - t);
 #pragma unroll
     for (int off = 1; off < 64; off <<= 1) total += __shfl_xor(total, off, 64);
     float o[E];
