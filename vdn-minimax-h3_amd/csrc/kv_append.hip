@@ -17,7 +17,7 @@
 // One workgroup takes a page of one head, so that the page's maximum needs no second pass over
 // memory: the rows stay in registers between the maximum and the cast. A thread holds two consecutive
 // tokens of one 8-element chunk, packed as they came (4 d threads a page; with four tokens and 256 threads
-// the registers left a compute unit 2.3 waves a SIMD: 67 us for 3120 tokens of 40 + 2 x 40 heads, 50 us now).
+// the registers left a compute unit 2.3 waves a SIMD: 67 us for 3120 tokens of 40 + 2 x 40 heads, 51 us now).
 // k is packed along the chunk, v along the tokens, so the transposition is a matter of which values one
 // conversion takes, and one pass through LDS makes whole 16-byte stores of it. Where pages alone fill the
 // part, a workgroup takes up to four heads of a page (1: 59 us): it reads the next head's rows while it

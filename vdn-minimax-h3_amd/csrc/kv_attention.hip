@@ -2,7 +2,7 @@
 //
 // For a query row q (one token, one head) over the visible tokens j of its sequence:
 //   x_j = log2(e) scale (q . k_j),  k_j = code 2^ek,   o = sum_j 2^(x_j) v_j / sum_j 2^(x_j)
-// in one pass over the pages with a running maximum. Three choices carry the arithmetic:
+// in one pass over the pages, in units that follow them. Three choices carry the arithmetic:
 //
 //   Scores in the queries' own type: e4m3 codes are bf16 and binary16 numbers, so keys are decoded exactly,
 //   products are exact and sums are binary32. (On the fp8 matrix cores, with a bf16 query as the sum of two
@@ -25,7 +25,7 @@
 // be lost from the output, though not from the sum. So a row's unit follows its pages both ways: a page whose
 // largest x + ev lies more than 10 from m moves m to it, and the accumulators by that power. A page's
 // largest weight is then held as 2^-5 to 2^15 (as 2^5, without a rounding, where the unit moves: whole numbers for m would make
-// the moves exact but round that weight, and make 2.9e-4 of 2.7e-4 of error in binary16 outputs), and each weight is off by 2^-11
+// the moves exact but round that weight: binary16 outputs 2.9e-4 off instead of 2.7e-4), and each weight is off by 2^-11
 // of itself or 2^-20 of its page's largest. A unit comes down by 2^60 at most, which binary32 accumulators leave room for: pages
 // further below a row's largest are zeros. On 3120 tokens over 32760, whose pages' largest scores spread by 2 in standard
 // deviation, 2.19 ms; with 9, 8 and 6 in place of 10 2.24, 2.29 and 2.33; with a unit that only rises, by more than 8, 2.17.
@@ -35,7 +35,7 @@
 //   k_kv_attn_rows    128 rows, 32 for each of four waves, which share the pages through LDS: keys as codes
 //                     (asynchronous copies, two pages ahead; each wave decodes what it reads), values decoded
 //                     once for all four. For chunks and prompts. 3120 tokens over 32760, 40 heads of 128:
-//                     2.15 ms, 0.97 PF/s; the card's power limit holds its clock at 1.9 of 2.4 GHz, where bare
+//                     2.15 to 2.23 ms, 0.94 to 0.97 PF/s; the card's power limit holds its clock at 1.9 of 2.4 GHz, where bare
 //                     chains of the same instructions reach 1.6 to 1.8 PF/s. Keys decoded once as well are
 //                     slower (2.28 ms: LDS reads, 32 KB a wave and page, take as long as the products).
 //   k_kv_attn_step    up to 16 rows; each of the four waves takes every fourth page, straight from

@@ -10,8 +10,7 @@ namespace vdn {
 
 constexpr int kPage = VDN_FP8_KV_PAGE;
 
-// Exponents of a page's scale. The least one is what a page of zeros gets: far enough below
-// every real scale, and such that 2^100 times a page's sum of weights stays in binary32.
+// Exponents of a page's scale. The least one is what a page of zeros gets: far enough below every real scale.
 constexpr int kLeastScale = -100, kMostScale = 120;
 
 struct KvCacheArgs {

@@ -13,8 +13,8 @@
 //
 // What bounds it: at many queries the query sum's bytes (each query read once); at single tokens the
 // page means' bytes (2 d a page and head, 1/64 of the cache) and the latency of two launches. 3120 queries in
-// blocks of 128 over 512 pages, 40 heads of 128: 8.2 + 8.2 + 8.0 us; eight single queries of 40 heads over
-// up to 2048 pages of 8: 9.2 + 6.8 us.
+// blocks of 128 over 512 pages, 40 heads of 128: 8.3 + 7.5 + 7.8 us; eight single queries of 40 heads over
+// up to 2048 pages of 8: 9.2 + 6.6 us.
 //   k_kv_query_sum   one workgroup per block and head
 //   k_kv_scores      one wave per 16 pages, all blocks of the sequence, 16 at a time
 //   k_kv_scores_step both of these where each query has its own pages
