@@ -413,7 +413,7 @@ int vdn_fp8_qk_prep_append(const vdn_fp8_kv_cache *cache, const vdn_fp8_kv_batch
  * receives log(sum_j exp(scale * query . k_j)). A row that sees no token gets zeros, and -inf in lse;
  * so do rows behind the last sequence. Scores, weights' sums and outputs are accumulated in binary32;
  * queries take part with all their bits. A weight times its page's value scale is off by 2^-11 of itself, or
- * by 2^-20 of the largest of its page where that is more (2^-90 of the row's largest at most counts as 0).
+ * by 2^-20 of the largest of its page where that is more (2^-80 of the row's largest at most counts as 0).
  * A NaN that is stored reaches the rows that attend to it and no others.
  * blocks (int32 [rows, heads, top], or NULL for all pages) lists, for each block of query_block
  * consecutive queries of a sequence and each key/value head, the pages (numbers within the

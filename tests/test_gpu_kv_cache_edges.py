@@ -31,7 +31,8 @@ def attend_by_channel(cache, q, table, length, scale, causal=False):
     A page's largest weight P' = p 2^ev (p the weight, 2^ev the page's value scale) is held as 2^-5 at least, and
     as 2^5 where it moves the row's unit, which it does when it is more than 2^20 from every other page's (the unit
     is within 2^10 of the page before). Rounded to binary16 each is off by 2^-11 of itself or by 2^-25 there: 2^-20,
-    or 2^-30, of the page's largest. A unit stays within 2^60 of the largest: 2^-90 of that at most. The products'
+    or 2^-30, of the page's largest. A unit comes down by 2^60 and stays where it is
+    within 2^10 of that: 2^-25 is then 2^-30 of a unit of 2^-50, 2^-80 of the row's largest at most. The products'
     sum is N / 16 sums one after another of 16 products each (four more levels), a few joins, and a power and a product
     for each page that moves the unit: N / 16 + N / 32 + 22 roundings (2^-23, should they truncate) of the magnitudes.
     Scores as in kv_reference.attend."""
@@ -54,7 +55,7 @@ def attend_by_channel(cache, q, table, length, scale, causal=False):
     unit = most * torch.exp2(ev)
     first, second = unit.topk(min(2, pages), 1).values.T[[0, -1]]
     alone = (unit == first[:, None]) & (first > 2.0 ** 20 * second)[:, None]
-    held = torch.where(alone, 2.0 ** -30, 2.0 ** -20) * unit + 2.0 ** -90 * first[:, None]
+    held = torch.where(alone, 2.0 ** -30, 2.0 ** -20) * unit + 2.0 ** -80 * first[:, None]
     es = scale * 2.0 ** -18 * (x.abs() @ k.abs().T).amax(1)
     tol = (2.0 ** -11 + 2.0 ** -18 + 2.0 ** -23 * (length / 16 + length / 32 + 22) + 2 * es)[:, None] * a + held @ size
     return out.reshape(n, Hq, d), z.reshape(n, Hq), tol.reshape(n, Hq, d), (2 * es + 2.0 ** -20 + 2.0 ** -22 * z.abs()).reshape(n, Hq)
