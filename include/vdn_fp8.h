@@ -37,7 +37,7 @@
 extern "C" {
 #endif
 
-#define VDN_FP8_ABI_VERSION 7
+#define VDN_FP8_ABI_VERSION 8
 
 /* status codes */
 #define VDN_FP8_OK 0
@@ -55,6 +55,11 @@ extern "C" {
 #define VDN_FP8_DTYPE_BF16 0
 #define VDN_FP8_DTYPE_F16 1
 #define VDN_FP8_DTYPE_F32 2
+
+/* Types of rotary positions (vdn_fp8_qk_prep_axes). */
+#define VDN_FP8_POSITION_I32 0
+#define VDN_FP8_POSITION_I64 1
+#define VDN_FP8_POSITION_F32 2
 
 /*
  * Per-token activation quantization: for each row m of x (bf16 [M, K]),
@@ -460,6 +465,75 @@ int vdn_fp8_kv_select(const vdn_fp8_kv_cache *cache, const vdn_fp8_kv_batch *bat
                       int dtype, int64_t q_heads, int64_t ldq, int causal, int64_t top, int64_t first,
                       int64_t last, int64_t query_block, int32_t *blocks, void *workspace,
                       int64_t workspace_bytes, hipStream_t stream);
+
+/*
+ * The residual's addition, the root-mean-square norm with its affine, and the codes of the next
+ * projection's input, one launch:
+ *   hidden[m][k] = S(residual[m][k] + gate[i][k] * branch[m][k])    (one rounding to the stream's
+ *                                       type S; residual + branch without a gate)
+ *   rstd         = 1 / sqrt(sum_k hidden[m][k]^2 / K + eps)         (binary32)
+ *   n[m][k]      = hidden * rstd * weight[k] * (1 + mod_scale[i][k]) + mod_shift[i][k]   (binary32)
+ *   y_scale[m]   = max(max_k |n| / 448, 1e-12),  y[m][k] = e4m3(n / y_scale[m])
+ *   normed[m][k] = B(n)                                             (if normed is not NULL)
+ * with i = index[m] (row 0 if NULL), clamped into [0, rows). n is not rounded before the codes.
+ * stream_type: VDN_FP8_DTYPE_* of residual and hidden; dtype: of branch, gate, weight, mod_scale,
+ * mod_shift and normed. gate, weight, mod_scale with mod_shift, index and normed may be NULL. hidden
+ * may be residual or branch itself (with its stride); nothing else may overlap.
+ * Replaces: nothing in one call; `post`, then `pre`, then quantize_rows
+ *           (src/models/ops/fused_block.py:41-49, fp8_linear.py:110-117), which round n to bf16 between.
+ * Requires: stream_type = dtype, or VDN_FP8_DTYPE_F32; K % 8 == 0, 8 <= K <= 16384; strides
+ *           multiples of 8 and >= K (a table of one row needs none); y 8-byte aligned, the other
+ *           rows, weight and tables 16-byte, index and y_scale 4-byte.
+ */
+int vdn_fp8_add_norm_quantize(const void *residual, int stream_type, int64_t ldr, const void *branch, int dtype,
+                              int64_t ldb, int64_t M, int64_t K, const void *gate, int64_t ldgate,
+                              const void *weight, float eps, const void *mod_scale, const void *mod_shift,
+                              int64_t ldmod, const int32_t *index, int64_t rows, void *hidden, int64_t ldh,
+                              void *y, int64_t ldy, float *y_scale, void *normed, int64_t ldn, hipStream_t stream);
+
+/*
+ * Low-rank adapters of many requests beside a shared projection (two launches):
+ *   out[t][n] = T(base[t][n] + scale[i] * sum_r (sum_k x[t][k] a[i][r][k]) b[i][n][r]),  i = index[t]
+ *   out[t][n] = base[t][n] where index[t] is outside [0, L)
+ * x [T, K], base and out [T, N], a [L, R, K], b [L, N, R] of dtype (bf16 or binary16), scale
+ * binary32 [L], index [T]. The first product is accumulated and kept in binary32, and enters the
+ * second as two 16-bit parts (2^-17 of it or less is left out). out may be base itself (with its stride);
+ * nothing else may overlap. The same inputs give the same bits, and a token's do not depend on the
+ * others' values. workspace: device memory, 16-byte aligned, of the size asked for with the same T, K,
+ * N, L, R; it need not be zeroed, and calls that overlap need one each.
+ * Replaces: nothing in the reference, which merges its one adapter into the weight (`merge_lora_state`,
+ *           src/inference/utils/lora.py:80-94).
+ * Requires: K and N multiples of 8, 8 to 2^17; R a multiple of 16, 16 to 128 (an adapter of another rank
+ *           is padded with zeros); T, L <= 2^23; strides multiples of 8, at most 2^23; x, base, out, a, b
+ *           16-byte aligned, scale and index 4-byte.
+ */
+int vdn_fp8_adapter_add_workspace_size(int64_t T, int64_t K, int64_t N, int64_t L, int64_t R, int64_t *bytes);
+int vdn_fp8_adapter_add(const void *x, int dtype, int64_t ldx, const void *base, int64_t ldbase, int64_t T,
+                        int64_t K, int64_t N, const void *a, const void *b, const float *scale, int64_t L,
+                        int64_t R, const int32_t *index, void *out, int64_t ldo, void *workspace,
+                        int64_t workspace_bytes, hipStream_t stream);
+
+/*
+ * QK preparation with rotary positions of several axes (time, height, width), q and k in one launch:
+ * per-head RMSNorm (norm_q / norm_k nonzero; weight NULL: ones), then a rotation by angles that are
+ * computed from each token's positions:
+ *   angle[t][j] = positions[t][axis[j]] * inv_freq[j],  j < rotary_dim / 2      (radians, in binary64)
+ *   lo, hi      = elements j and j + rotary_dim / 2 of the head, or with pairs 2 j and 2 j + 1
+ *   out[lo] = n[lo] cos - n[hi] sin,  out[hi] = n[hi] cos + n[lo] sin           (cos, sin binary32)
+ *   out[i]  = n[i] for i >= rotary_dim
+ * query [T, q_heads, d], key [T, k_heads, d], their outputs and weights [d] of dtype; positions
+ * [T, axes] of position_type, row stride ldpos; inv_freq binary64 and axis (clamped into [0, axes))
+ * [rotary_dim / 2]. Either side may have no heads. An output may be its input itself (with its stride).
+ * Replaces: `_qk_prep` of q and of k (src/models/softmax_attention/kernels.py:8-45) and the tables of
+ *           the caller's rotary embedding, whose bf16 rounding (`cos.to(x.dtype)`) is not taken over.
+ * Requires: d in {64, 128, 256}; heads * d <= 65536; rotary_dim in [0, d], a multiple of 16 (pairs: 8); 1 to 8 axes;
+ *           row strides multiples of 8; rows and weights 16-byte aligned.
+ */
+int vdn_fp8_qk_prep_axes(const void *query, int64_t q_heads, int64_t ldq, const void *key, int64_t k_heads,
+                         int64_t ldk, int64_t T, int64_t d, int dtype, int norm_q, const void *weight_q, float eps_q,
+                         int norm_k, const void *weight_k, float eps_k, const double *inv_freq, const int32_t *axis,
+                         int64_t rotary_dim, int pairs, const void *positions, int position_type, int64_t axes,
+                         int64_t ldpos, void *out_q, int64_t ldoq, void *out_k, int64_t ldok, hipStream_t stream);
 
 /* The message of the last failed call on this host thread ("" if none). */
 const char *vdn_fp8_last_error(void);

@@ -1,0 +1,193 @@
+"""The residual's addition, the norm and the codes in one pass (`add_norm_quantize`) against the formulas in 64 bits.
+
+The new stream is compared exactly: a product of two 16-bit values and its sum with a third are formed by one fma,
+that is as the 64-bit sum rounded to binary32, then rounded to the stream's type (a binary32 stream's product
+of binary32 values is exact to 2^-53 in 64 bits: one step of binary32 is allowed there).
+
+The normed rows' bound. With u = 2^-24: the sum of squares takes at most 8 * 8 fused steps of a lane, 6 of a wave and 16
+of the waves (relative error 90 u, all terms positive), the quotient by K, eps, root and reciprocal 4 u: rstd is off by
+45 u + 4 u. h rstd, w (1 + scale), their product and the shift's sum round 5 times. So n is off by no more than
+ERR = 56 u of |h rstd w (1 + scale)| + |shift|."""
+import pytest
+import torch
+
+import vdn_fp8
+
+pytestmark = pytest.mark.gpu
+
+BF16, F16, F32 = torch.bfloat16, torch.float16, torch.float32
+E4M3 = torch.float8_e4m3fn
+ERR = 56 * 2.0 ** -24
+TYPES = [(BF16, BF16), (F16, F16), (F32, BF16), (F32, F16), (F32, F32)]
+
+
+def inputs(device, M, K, stream, dtype, rows, seed):
+    g = torch.Generator().manual_seed(seed)
+    channel = torch.exp(0.5 * torch.randn(K, generator=g))
+    r = (3 * torch.randn(M, K, generator=g) * channel).to(stream)
+    b = torch.randn(M, K, generator=g).to(dtype)
+    w = (1 / channel + 0.05 * torch.randn(K, generator=g)).to(dtype)
+    gate, sc, sh = ((0.5 * torch.randn(rows, K, generator=g)).to(dtype) for _ in range(3))
+    index = torch.randint(0, rows, (M,), generator=g).to(torch.int32)
+    return [t.to(device) for t in (r, b, w, gate, sc, sh, index)]
+
+
+def formula(r, b, w, eps, gate=None, scale=None, shift=None, index=None):
+    """hidden (its type), n and the bound of n in 64 bits."""
+    i = torch.zeros(r.shape[0], dtype=torch.long, device=r.device) if index is None else index.long()
+    total = r.double() + (b.double() if gate is None else gate.double()[i] * b.double())
+    hidden = total.float().to(r.dtype)
+    h = hidden.double()
+    n = h / (h.square().mean(1, keepdim=True) + eps).sqrt()
+    if w is not None:
+        n = n * w.double()
+    size = n.abs()
+    if scale is not None:
+        n = n * (1 + scale.double()[i])
+        size = n.abs() + shift.double()[i].abs()
+        n = n + shift.double()[i]
+    return hidden, n, ERR * size
+
+
+def check(got, want, dtype):
+    hidden, n, err = want
+    out, codes, s = got[:3]
+    assert out.dtype == hidden.dtype and codes.dtype == E4M3 and s.shape == (n.shape[0], 1)
+    if hidden.dtype == F32:
+        assert torch.all((out.double() - hidden.double()).abs() <= 2.0 ** -23 * hidden.double().abs())
+    else:
+        assert torch.equal(out, hidden)
+    size = (n.abs().amax(1, keepdim=True) / 448).clamp_min(1e-12)
+    assert torch.all((s.double() - size).abs() <= err.amax(1, keepdim=True) / 448 + 2.0 ** -23 * size)
+    # a code is that of a value within the bound of n, over the scale that came back (its quotient rounds once more)
+    quotient, slack = n / s.double(), (err / s.double()) + 2.0 ** -23 * (n / s.double()).abs()
+    low = (quotient - slack).clamp(-448, 448).float().to(E4M3).float()
+    high = (quotient + slack).clamp(-448, 448).float().to(E4M3).float()
+    c = codes.float()
+    assert torch.all((low <= c) & (c <= high))
+    if len(got) == 4:
+        assert got[3].dtype == dtype
+        room = err + torch.finfo(dtype).eps / 2 * (n.abs() + err) + (2.0 ** -25 if dtype == F16 else 0.0)   # (float16 below 2^-14)
+        assert torch.all((got[3].double() - n).abs() <= room)
+
+
+@pytest.mark.parametrize("M,K", [(1, 8), (3, 72), (2, 512), (5, 1024), (7, 1032), (1, 4104), (16, 5120), (33, 5376), (9, 7168), (2, 16384), (700, 2056),
+                                 (515, 8200)])
+@pytest.mark.parametrize("stream,dtype", TYPES)
+def test_sizes_and_types(device, M, K, stream, dtype):
+    print(f"add_norm {M} x {K} {stream} {dtype}", flush=True)
+    r, b, w, gate, sc, sh, index = inputs(device, M, K, stream, dtype, 5, M * K)
+    got = vdn_fp8.add_norm_quantize(r, b, w, 1e-6, gate=gate, scale=sc, shift=sh, indices=index, return_normed=True)
+    check(got, formula(r, b, w, 1e-6, gate, sc, sh, index), dtype)
+    got = vdn_fp8.add_norm_quantize(r, b, None, 1e-5)
+    check(got, formula(r, b, None, 1e-5), dtype)
+
+
+@pytest.mark.parametrize("gate,table,index,weight", [(True, False, True, True), (False, True, True, False), (True, True, False, True),
+                                                     (False, True, False, True), (True, False, False, False)])
+def test_forms(device, gate, table, index, weight):
+    r, b, w, g, sc, sh, i = inputs(device, 37, 1288, F32, BF16, 1 if not index else 4, 3)
+    kw = dict(gate=g if gate else None, scale=sc if table else None, shift=sh if table else None)
+    got = vdn_fp8.add_norm_quantize(r, b, w if weight else None, 1e-6, indices=i if index else None, return_normed=True, **kw)
+    want = formula(r, b, w if weight else None, 1e-6, kw["gate"], kw["scale"], kw["shift"], i if index else None)
+    check(got, want, BF16)
+    # without the normed rows the others have the same bits
+    again = vdn_fp8.add_norm_quantize(r, b, w if weight else None, 1e-6, indices=i if index else None, **kw)
+    for x, y in zip(got, again):
+        assert torch.equal(x.view(torch.uint8), y.view(torch.uint8))
+
+
+def test_shapes_strides_and_indices(device):
+    r, b, w, gate, sc, sh, index = inputs(device, 24, 256, BF16, BF16, 6, 5)
+    want = vdn_fp8.add_norm_quantize(r, b, w, 1e-6, gate=gate, scale=sc, shift=sh, indices=index)
+    wide = torch.randn(24, 640, device=device).to(BF16)
+    wide[:, 8:264], wide[:, 304:560] = r, b
+    odd = torch.randn(24, 259, device=device).to(BF16)
+    odd[:, 1:257] = b
+    forms = {"column slices": (wide[:, 8:264], wide[:, 304:560]), "odd strides": (r, odd[:, 1:257]),
+             "transposed": (r.T.contiguous().T, b), "three dimensions": (r.view(2, 12, 256), b.view(2, 12, 256))}
+    for name, (x, y) in forms.items():
+        got = vdn_fp8.add_norm_quantize(x, y, w, 1e-6, gate=gate, scale=sc, shift=sh, indices=index)
+        assert got[0].shape == x.shape and got[1].shape == (24, 256), name
+        for p, q in zip(got, want):
+            assert torch.equal(p.reshape(q.shape).view(torch.uint8), q.view(torch.uint8)), name
+    # indices of other integer types, and outside the tables: clamped
+    out = index.long() * 0 + torch.tensor([-3, 0, 7, 1 << 40, 5, -(1 << 40)] * 4, device=device)
+    a = vdn_fp8.add_norm_quantize(r, b, w, 1e-6, gate=gate, scale=sc, shift=sh, indices=out)
+    c = vdn_fp8.add_norm_quantize(r, b, w, 1e-6, gate=gate, scale=sc, shift=sh, indices=out.clamp(0, 5).int())
+    assert all(torch.equal(p.view(torch.uint8), q.view(torch.uint8)) for p, q in zip(a, c))
+    empty = vdn_fp8.add_norm_quantize(r[:0], b[:0], w, 1e-6, return_normed=True)
+    assert [t.shape[0] for t in empty] == [0] * 4
+
+
+@pytest.mark.parametrize("K", [64, 5120])
+@pytest.mark.parametrize("stream,dtype", TYPES)
+def test_edge_rows(device, K, stream, dtype):
+    """Rows of zeros (codes of zero at the least scale), one value in a row, infinities and NaN, that reach their own
+    row alone; eps of zero."""
+    M = 8
+    r, b = torch.zeros(M, K, device=device, dtype=stream), torch.zeros(M, K, device=device, dtype=dtype)
+    w = torch.ones(K, device=device, dtype=dtype)
+    g = torch.Generator(device).manual_seed(1)
+    r[1:] = torch.randn(M - 1, K, device=device, generator=g).to(stream)
+    r[2] = 0
+    r[2, K // 3] = 5.0
+    r[3, 7], r[4, 0], b[5, K - 1] = float("inf"), float("nan"), float("-inf")
+    r[6] *= 1e-3
+    for eps in (1e-6, 0.0):
+        hidden, codes, s, normed = vdn_fp8.add_norm_quantize(r, b, w, eps, return_normed=True)
+        total = r.float() + b.float()
+        assert torch.equal(torch.nan_to_num(hidden.float(), 77.0), torch.nan_to_num(total.to(stream).float(), 77.0))
+        for row in (3, 4, 5):
+            assert s[row].isnan().all() and codes[row].float().isnan().all()
+        if eps:
+            assert torch.all(codes[0].float() == 0) and abs(float(s[0]) - 1e-12) < 1e-18
+            keep = [0, 1, 2, 6, 7]
+        else:
+            assert normed[0].isnan().all() and s[0].isnan().all()
+            keep = [1, 2, 6, 7]
+        want = formula(r[keep], b[keep], w, eps)
+        check((hidden[keep], codes[keep], s[keep], normed[keep]), want, dtype)
+
+
+def test_graphs_and_streams(device):
+    """Captured and replayed with other rows, with eager calls between; on a stream that is not the default one."""
+    sets = [inputs(device, 40, 5120, BF16, BF16, 3, s) for s in (11, 12, 13)]
+    static = [t.clone() for t in sets[0]]
+
+    def call(r, b, w, gate, sc, sh, index):
+        return vdn_fp8.add_norm_quantize(r, b, w, 1e-6, gate=gate, scale=sc, shift=sh, indices=index, return_normed=True)
+
+    want = [call(*s) for s in sets]
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = call(*static)
+    for k in (1, 2, 0, 1):
+        for t, u in zip(static, sets[k]):
+            t.copy_(u)
+        graph.replay()
+        call(*sets[0])
+        torch.cuda.synchronize()
+        assert all(torch.equal(p.view(torch.uint8), q.view(torch.uint8)) for p, q in zip(out, want[k])), k
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        got = call(*sets[2])
+    side.synchronize()
+    assert all(torch.equal(p.view(torch.uint8), q.view(torch.uint8)) for p, q in zip(got, want[2]))
+
+
+def test_codes_feed_the_next_projection(device):
+    """The codes and scales are what `Fp8Linear.forward_quantized` takes: its product is the one of the dequantized rows."""
+    r, b, w, gate, sc, sh, index = inputs(device, 50, 512, BF16, BF16, 3, 9)
+    hidden, codes, s = vdn_fp8.add_norm_quantize(r, b, w, 1e-6, gate=gate, scale=sc, shift=sh, indices=index)
+    lin = torch.nn.Linear(512, 256, bias=False, device=device, dtype=BF16)
+    f = vdn_fp8.Fp8Linear(lin)
+    got = f.forward_quantized(codes, s).double()
+    x = codes.double() * s.double()
+    q = f.weight_fp8.double() * f.weight_scale.double().T
+    want, size = x @ q.T, x.abs() @ q.abs().T
+    # the product's rounding to bf16, half a step of 2^-7 (it has 8 significant bits), and 512 sums and two scales in binary32
+    # (2^-23 each, should the matrix cores truncate)
+    room = 514 * 2.0 ** -23 * size
+    assert torch.all((got - want).abs() <= 2.0 ** -8 * (want.abs() + room) + room)

@@ -1,0 +1,239 @@
+// QK preparation with positions of several axes: per-head RMSNorm (or none) of q and of k, then the rotary
+// embedding whose angles come from each token's positions, in one launch.
+//
+//   rstd     = 1 / sqrt(sum_i x[i]^2 / d + eps),   n[i] = (x[i] rstd) w[i]        (binary32)
+//   angle_j  = positions[t][axis[j]] * inv_freq[j]                                (j < R / 2)
+//   halves:    pair j is elements (j, j + R/2);  pairs: elements (2j, 2j + 1)
+//   out[lo]  = n[lo] cos(angle_j) - n[hi] sin(angle_j),   out[hi] = n[hi] cos(angle_j) + n[lo] sin(angle_j)
+//   out[i]   = n[i] for i >= R
+// rounded once, at the store. Cosines and sines are binary32 (a table of bf16 values, as k_qk_prep takes,
+// is off by 2^-9 of a turn's radius).
+//
+// Angles. What matters of an angle is its fraction of a turn, and at far positions binary32 has none of it
+// left (position 10^6 at frequency 1: half a unit in the last place is 2^-5 rad). So the turns p f / 2 pi are
+// formed in binary64, the nearest whole number is taken off by an exact fma, and a quarter turn's remainder,
+// |g| <= pi / 4, goes to binary32, where Taylor's series to g^9 and g^10 have errors below 2^-28.
+//
+// Layout. A wave takes a token's chunks (eight elements a lane) of q or of k; a head is d / 8 consecutive
+// lanes, as in k_qk_prep. The lanes first compute one angle each (R / 2 <= 128 of them), leave cosine and sine
+// in the wave's own LDS, and read those of their chunk from there: an angle costs its wave about 60
+// operations once, and not once for each of the lanes that need it.
+#include <stdint.h>
+
+#include "eight.h"
+#include "qk_prep.h"
+#include "vdn_common.h"
+
+namespace vdn {
+namespace {
+
+constexpr int kLanes = 64;
+constexpr int kWaves = 4;            // of a workgroup
+constexpr int kMostAxes = 8;
+constexpr int kMostPairs = 128;      // R / 2 at d = 256
+
+struct RopeSide {
+    const void* x;        // [T, heads, d], row stride ld
+    int64_t ld;
+    int heads, spans;     // spans: waves that share a token
+    int norm;
+    const void* weight;   // [d] or NULL
+    float eps;
+    void* out;
+    int64_t ldo;
+};
+
+struct RopeArgs {
+    RopeSide side[2];
+    int64_t T;
+    int d, R;
+    const double* inv_freq;   // [R / 2]
+    const int32_t* axis;      // [R / 2]
+    const void* positions;    // [T, axes]
+    int64_t ldpos;
+    int axes, position_type;
+};
+
+__device__ __forceinline__ double position_at(const RopeArgs& p, int64_t at)
+{
+    if (p.position_type == VDN_FP8_POSITION_I32) return (double)static_cast<const int32_t*>(p.positions)[at];
+    if (p.position_type == VDN_FP8_POSITION_I64) return (double)static_cast<const int64_t*>(p.positions)[at];
+    return (double)static_cast<const float*>(p.positions)[at];
+}
+
+// Cosine and sine of 2 pi p f, f in turns.
+__device__ __forceinline__ void turn(double p, double f, float& cosine, float& sine)
+{
+    // p f less its nearest whole number; once more where p f is so large that the first leaves a few turns
+    double r = __builtin_fma(p, f, -__builtin_rint(p * f));
+    r -= __builtin_rint(r);
+    const double quarter = __builtin_rint(4.0 * r);
+    const float g = (float)((r - 0.25 * quarter) * 6.283185307179586477);
+    const float z = g * g;
+    // sin g = g - g^3/3! + ... + g^9/9!, cos g = 1 - g^2/2! + ... - g^10/10!
+    const float s = __builtin_fmaf(g * z, __builtin_fmaf(z, __builtin_fmaf(z, __builtin_fmaf(z, 1.0f / 362880, -1.0f / 5040), 1.0f / 120), -1.0f / 6), g);
+    const float c = __builtin_fmaf(z, __builtin_fmaf(z, __builtin_fmaf(z, __builtin_fmaf(z, __builtin_fmaf(z, -1.0f / 3628800, 1.0f / 40320), -1.0f / 720), 1.0f / 24), -0.5f), 1.0f);
+    const int q = (int)quarter & 3;
+    const float a = q & 1 ? s : c, b = q & 1 ? c : s;
+    cosine = q == 1 || q == 2 ? -a : a;
+    sine = q & 2 ? -b : b;
+}
+
+// G = d / 8 lanes of a head; CPL chunks a lane; PAIRS: which elements a pair is.
+template <int TYPE, int G, int CPL, bool PAIRS, bool NT>
+__global__ __launch_bounds__(kWaves * kLanes) void k_rope_axes(RopeArgs p, int64_t first_token)
+{
+    __shared__ float turned[kWaves][2][kMostPairs];
+    const int lane = threadIdx.x & (kLanes - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kLanes);
+    const int spans = p.side[0].spans + p.side[1].spans;
+    const uint32_t unit = blockIdx.x * kWaves + wave;
+    const int64_t t = first_token + unit / (uint32_t)spans;
+    if (t >= p.T) return;
+    const int place = (int)(unit % (uint32_t)spans);
+    const bool is_key = place >= p.side[0].spans;
+    const RopeSide s = is_key ? p.side[1] : p.side[0];
+    const int base = (place - (is_key ? p.side[0].spans : 0)) * kLanes * CPL;   // first chunk: whole heads, 64 being a multiple of G
+    const int nch = s.heads * G;
+    const int j = lane % G, i0 = 8 * j;
+
+    const __amdgpu_buffer_rsrc_t xr = row_buffer((const uint8_t*)s.x + t * s.ld * element_bytes(TYPE), (int64_t)nch * 8 * element_bytes(TYPE));
+    Eight<TYPE> v[CPL];
+#pragma unroll
+    for (int c = 0; c < CPL; ++c) v[c] = load8<TYPE, kBufferLoadOnce>(xr, (uint32_t)(base + lane + kLanes * c));
+    const __amdgpu_buffer_rsrc_t wr = row_buffer(s.weight ? s.weight : s.x, s.weight ? p.d * element_bytes(TYPE) : 0);
+    const Eight<TYPE> raw_weight = load8<TYPE, 0>(wr, (uint32_t)j);
+
+    const int half = p.R / 2;
+    const double mine = lane < p.axes ? position_at(p, t * p.ldpos + lane) : 0.0;
+    for (int a = lane; a < (half + kLanes - 1) / kLanes * kLanes; a += kLanes) {
+        const bool real = a < half;
+        const int axis = real ? min(max(p.axis[a], 0), p.axes - 1) : 0;
+        const double f = real ? p.inv_freq[a] * 0.15915494309189533577 : 0.0;
+        const double at = __shfl(mine, axis, kLanes);
+        float c, sn;
+        turn(at, f, c, sn);
+        if (real) {
+            turned[wave][0][a] = c;
+            turned[wave][1][a] = sn;
+        }
+    }
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+
+    const bool rot = i0 < p.R;
+    const bool first = i0 < half;                                     // (halves)
+    const int partner = lane + (first ? half / 8 : -(half / 8));      // (halves: the chunk R / 2 elements away)
+    float cs[8], sn[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        const int pair = PAIRS ? i0 / 2 + e / 2 : (first ? i0 : i0 - half) + e;
+        cs[e] = rot ? turned[wave][0][pair] : 1.0f;
+        sn[e] = rot ? turned[wave][1][pair] : 0.0f;
+    }
+    float w[8];
+    decode8<TYPE>(raw_weight, w);
+    if (!s.weight)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) w[e] = 1.0f;
+
+    const __amdgpu_buffer_rsrc_t outr = row_buffer((uint8_t*)s.out + t * s.ldo * element_bytes(TYPE), (int64_t)nch * 8 * element_bytes(TYPE));
+#pragma unroll
+    for (int c = 0; c < CPL; ++c) {
+        float n[8], o[8];
+        decode8<TYPE>(v[c], n);
+        if (s.norm) {
+            const float ss = head_sum_squares<G>(n);
+            const float rstd = 1.0f / __builtin_sqrtf(ss / (float)p.d + s.eps);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) n[e] = (n[e] * rstd) * w[e];
+        }
+        if (PAIRS) {
+#pragma unroll
+            for (int e = 0; e < 8; e += 2) {
+                o[e] = rot ? n[e] * cs[e] - n[e + 1] * sn[e] : n[e];
+                o[e + 1] = rot ? n[e + 1] * cs[e] + n[e] * sn[e] : n[e + 1];
+            }
+        } else {
+            rotate8<G>(n, cs, sn, p.R == p.d, rot, first, partner, lane, o);
+        }
+        store8<TYPE, NT ? kBufferLoadOnce : 0>(encode8<TYPE>(o), outr, (uint32_t)(base + lane + kLanes * c));
+    }
+}
+
+// Outputs of at least this many bytes are stored non-temporally: beyond what the last-level cache holds,
+// cached stores only evict each other.
+constexpr int64_t kNtStoreBytes = 256ll << 20;
+
+template <int TYPE, int G, int CPL, bool PAIRS>
+int launch_cpl(RopeArgs p, hipStream_t stream)
+{
+    for (RopeSide& s : p.side) s.spans = (s.heads * G + kLanes * CPL - 1) / (kLanes * CPL);
+    const int64_t spans = p.side[0].spans + p.side[1].spans;
+    const bool nt = p.T * (p.side[0].heads + p.side[1].heads) * p.d * element_bytes(TYPE) >= kNtStoreBytes;
+    const int64_t slab = kLaunchRows * kWaves / spans;   // tokens of a launch
+    return in_slabs(p.T, slab, [&](int64_t t, int64_t tokens) {
+        const dim3 grid((unsigned)((tokens * spans + kWaves - 1) / kWaves)), block(kWaves * kLanes);
+        RopeArgs q = p;
+        q.T = t + tokens;
+        if (nt) hipLaunchKernelGGL((k_rope_axes<TYPE, G, CPL, PAIRS, true>), grid, block, 0, stream, q, t);
+        else hipLaunchKernelGGL((k_rope_axes<TYPE, G, CPL, PAIRS, false>), grid, block, 0, stream, q, t);
+        return check_launch("qk_prep_axes");
+    });
+}
+
+template <int TYPE, int G>
+int launch(const RopeArgs& p, bool pairs, hipStream_t stream)
+{
+    const bool many = p.T >= 1024;
+    if (pairs) return many ? launch_cpl<TYPE, G, 5, true>(p, stream) : launch_cpl<TYPE, G, 1, true>(p, stream);
+    return many ? launch_cpl<TYPE, G, 5, false>(p, stream) : launch_cpl<TYPE, G, 1, false>(p, stream);
+}
+
+template <int TYPE>
+int launch_type(const RopeArgs& p, bool pairs, hipStream_t stream)
+{
+    return p.d == 64 ? launch<TYPE, 8>(p, pairs, stream) : p.d == 128 ? launch<TYPE, 16>(p, pairs, stream) : launch<TYPE, 32>(p, pairs, stream);
+}
+
+}  // namespace
+}  // namespace vdn
+
+using namespace vdn;
+
+extern "C" int vdn_fp8_qk_prep_axes(const void* query, int64_t q_heads, int64_t ldq, const void* key, int64_t k_heads, int64_t ldk,
+                                    int64_t T, int64_t d, int dtype, int norm_q, const void* weight_q, float eps_q, int norm_k,
+                                    const void* weight_k, float eps_k, const double* inv_freq, const int32_t* axis, int64_t rotary_dim,
+                                    int pairs, const void* positions, int position_type, int64_t axes, int64_t ldpos, void* out_q,
+                                    int64_t ldoq, void* out_k, int64_t ldok, hipStream_t stream)
+{
+    const char* what = "qk_prep_axes";
+    if (T < 0 || q_heads < 0 || k_heads < 0) return set_error(VDN_FP8_EINVAL, "%s: negative shape", what);
+    if (dtype < kBf16 || dtype > kF32) return set_error(VDN_FP8_EINVAL, "%s: unknown dtype %d", what, dtype);
+    if (d != 64 && d != 128 && d != 256) return set_error(VDN_FP8_EINVAL, "%s: head dim %lld not in {64, 128, 256}", what, (long long)d);
+    if (q_heads * d > 65536 || k_heads * d > 65536) return set_error(VDN_FP8_EINVAL, "%s: more than 65536 elements a token", what);
+    if (T == 0 || q_heads + k_heads == 0) return VDN_FP8_OK;
+    const int64_t unit = pairs ? 8 : 16;
+    if (rotary_dim < 0 || rotary_dim > d || rotary_dim % unit)
+        return set_error(VDN_FP8_EINVAL, "%s: the rotary dim %lld must be a multiple of %lld in [0, d]", what, (long long)rotary_dim, (long long)unit);
+    if (rotary_dim > 0) {
+        if (!inv_freq || !axis || !positions) return set_error(VDN_FP8_EINVAL, "%s: null pointer (frequencies, axes or positions)", what);
+        if (axes < 1 || axes > kMostAxes || ldpos < axes) return set_error(VDN_FP8_EINVAL, "%s: 1 to %d axes, and positions' row stride >= that (got %lld, %lld)", what, kMostAxes, (long long)axes, (long long)ldpos);
+        if (position_type < VDN_FP8_POSITION_I32 || position_type > VDN_FP8_POSITION_F32) return set_error(VDN_FP8_EINVAL, "%s: unknown type of positions %d", what, position_type);
+        const uintptr_t wide = position_type == VDN_FP8_POSITION_I64 ? 8 : 4;
+        if (!aligned(inv_freq, 8) || !aligned(axis, 4) || !aligned(positions, wide)) return set_error(VDN_FP8_EINVAL, "%s: misaligned pointer (frequencies, axes or positions)", what);
+    }
+    if (!(eps_q >= 0.0f) || !(eps_k >= 0.0f)) return set_error(VDN_FP8_EINVAL, "%s: eps must be >= 0", what);
+    auto bad = [&](const void* x, int64_t heads, int64_t ld, const void* out, int64_t ldo) {
+        return heads && (!x || !out || ld % 8 || ldo % 8 || ld < heads * d || ldo < heads * d || !aligned(x, 16) || !aligned(out, 16));
+    };
+    if (bad(query, q_heads, ldq, out_q, ldoq) || bad(key, k_heads, ldk, out_k, ldok))
+        return set_error(VDN_FP8_EINVAL, "%s: rows must be given, 16-byte aligned, with strides multiples of 8 and >= heads * d", what);
+    if (!aligned(weight_q, 16) || !aligned(weight_k, 16)) return set_error(VDN_FP8_EINVAL, "%s: misaligned pointer (weights 16 B)", what);
+    const RopeArgs p{{{query, ldq, (int)q_heads, 0, norm_q != 0, weight_q, eps_q, out_q, ldoq},
+                      {key, ldk, (int)k_heads, 0, norm_k != 0, weight_k, eps_k, out_k, ldok}},
+                     T, (int)d, (int)rotary_dim, inv_freq, axis, positions, ldpos, rotary_dim > 0 ? (int)axes : 0, position_type};
+    return dtype == kBf16 ? launch_type<kBf16>(p, pairs != 0, stream)
+         : dtype == kF16  ? launch_type<kF16>(p, pairs != 0, stream)
+                          : launch_type<kF32>(p, pairs != 0, stream);
+}

@@ -177,6 +177,21 @@ __device__ __forceinline__ uint32_t wave_max_u32(uint32_t v)
     return max(max(r0, r1), max(r2, r3));
 }
 
+// Sum over the 64 lanes of a wavefront, wave-uniform, in one order.
+__device__ __forceinline__ float wave_sum_f32(float v)
+{
+    // pairwise within the rows (both lanes of each exchange form the same sum), then
+    // (row 0 + row 1) + (row 2 + row 3), wave-uniform
+    v += __uint_as_float(dpp_u32<kDppXor1>(__float_as_uint(v)));
+    v += __uint_as_float(dpp_u32<kDppXor2>(__float_as_uint(v)));
+    v += __uint_as_float(dpp_u32<kDppHalfMirror>(__float_as_uint(v)));
+    v += __uint_as_float(dpp_u32<kDppMirror>(__float_as_uint(v)));
+    const uint32_t u = __float_as_uint(v);
+    const float r0 = __uint_as_float(__builtin_amdgcn_readlane(u, 0)), r1 = __uint_as_float(__builtin_amdgcn_readlane(u, 16)),
+                r2 = __uint_as_float(__builtin_amdgcn_readlane(u, 32)), r3 = __uint_as_float(__builtin_amdgcn_readlane(u, 48));
+    return (r0 + r1) + (r2 + r3);
+}
+
 // The per-row scale of the reference: max(amax / 448, 1e-12) with IEEE
 // binary32 division; NaN propagates (torch's clamp_min keeps NaN).
 __device__ __forceinline__ float row_scale(float amax)

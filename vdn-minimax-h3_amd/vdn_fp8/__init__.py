@@ -12,10 +12,10 @@ from .fp8_linear import (FP8_DTYPE, MIN_WIDTH, SKIP_END_BLOCKS, _FP8_MAX, Fp8Lin
                          convert_linear_to_fp8, gelu_quantize, per_tensor_gemm, quantize_activation,
                          quantize_rows, quantize_rows_reference, requantize_weight,
                          set_index_checks, swiglu_quantize, swiglu_quantize_activation)
-from .fused_block import fast_block_forward, fast_ff_forward, post, pre, pre_quantize
+from .fused_block import add_norm_quantize, fast_block_forward, fast_ff_forward, post, pre, pre_quantize
 from .kv_cache import KV_PAGE, KvCache, kv_append, kv_attention, kv_select, qk_prep_append
-from .lora import load_external_lora, merge_lora_and_convert, merge_lora_state
-from .softmax_attention import qk_prep
+from .lora import Adapters, adapter_add, load_external_lora, merge_lora_and_convert, merge_lora_state
+from .softmax_attention import RopeAxes, qk_prep, qk_prep_axes
 
 __all__ = [
     "FP8_DTYPE", "MIN_WIDTH", "SKIP_END_BLOCKS", "_FP8_MAX", "Fp8Linear", "convert_linear_to_fp8", "gelu_quantize",
@@ -24,4 +24,5 @@ __all__ = [
     "merge_lora_and_convert", "merge_lora_state", "pre_quantize", "qk_prep", "pre", "post",
     "fast_ff_forward", "fast_block_forward", "set_index_checks",
     "KV_PAGE", "KvCache", "kv_append", "kv_attention", "kv_select", "qk_prep_append",
+    "Adapters", "RopeAxes", "adapter_add", "add_norm_quantize", "qk_prep_axes",
 ]

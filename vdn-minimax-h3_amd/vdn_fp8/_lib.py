@@ -12,11 +12,12 @@ import os
 
 from .build import CSRC, INCLUDE, LIB_PATH, compiler_id, source_manifest
 
-ABI_VERSION = 7
+ABI_VERSION = 8
 
 OK, EINVAL, ELAUNCH = 0, 1, 2
 EPI_NONE, EPI_GELU_TANH, EPI_GATE, EPI_F32 = 0, 1, 2, 3
 DTYPE_BF16, DTYPE_F16, DTYPE_F32 = 0, 1, 2
+POSITION_I32, POSITION_I64, POSITION_F32 = 0, 1, 2
 
 _lib = None
 _build_info = None
@@ -67,6 +68,13 @@ EXPORTS = (
                                     _I64, _P]),
     ("vdn_fp8_kv_select_workspace_size", _I32, [_CACHE, _BATCH, _I64, _I64, _P]),
     ("vdn_fp8_kv_select", _I32, [_CACHE, _BATCH, _P, _I32, _I64, _I64, _I32, _I64, _I64, _I64, _I64, _P, _P, _I64, _P]),
+    ("vdn_fp8_add_norm_quantize", _I32, [_P, _I32, _I64, _P, _I32, _I64, _I64, _I64, _P, _I64, _P, _F32, _P, _P, _I64, _P,
+                                         _I64, _P, _I64, _P, _I64, _P, _P, _I64, _P]),
+    ("vdn_fp8_adapter_add_workspace_size", _I32, [_I64, _I64, _I64, _I64, _I64, _P]),
+    ("vdn_fp8_adapter_add", _I32, [_P, _I32, _I64, _P, _I64, _I64, _I64, _I64, _P, _P, _P, _I64, _I64, _P, _P, _I64, _P,
+                                   _I64, _P]),
+    ("vdn_fp8_qk_prep_axes", _I32, [_P, _I64, _I64, _P, _I64, _I64, _I64, _I64, _I32, _I32, _P, _F32, _I32, _P, _F32, _P, _P,
+                                    _I64, _I32, _P, _I32, _I64, _I64, _P, _I64, _P, _I64, _P]),
     ("vdn_fp8_last_error", ctypes.c_char_p, []),
     ("vdn_fp8_abi_version", _I32, []),
     ("vdn_fp8_build_info", ctypes.c_char_p, []),

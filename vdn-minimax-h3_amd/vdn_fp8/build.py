@@ -33,8 +33,8 @@ PROBE_SOURCES = ["stream_probe.hip", "mfma_probe.hip"]
 PROBE_PATH = os.path.join(_PKG, "libvdnprobe.so")
 
 SOURCES = ["capi.hip", "quantize.hip", "lora_requant.hip", "gemm.hip", "gemm_tile.hip", "qk_prep.hip", "block_ops.hip",
-           "kv_append.hip", "kv_attention.hip", "kv_select.hip"]
-HEADERS = ["vdn_common.h", "gemm_common.h", "qk_prep.h", "kv_common.h"]   # in csrc/
+           "kv_append.hip", "kv_attention.hip", "kv_select.hip", "add_norm.hip", "adapters.hip", "rope_axes.hip"]
+HEADERS = ["vdn_common.h", "gemm_common.h", "qk_prep.h", "kv_common.h", "eight.h"]   # in csrc/
 PUBLIC_HEADERS = ["vdn_fp8.h"]         # in include/
 
 # -ffp-contract=off: the quantizers' binary32 arithmetic is bit-exact only as
@@ -96,6 +96,9 @@ KERNEL_FILES = {
     "qk_prep": ["qk_prep.hip", "qk_prep.h", "vdn_common.h", "vdn_fp8.h"],
     "kv": ["kv_append.hip", "kv_attention.hip", "kv_select.hip", "kv_common.h", "qk_prep.h", "gemm_common.h",
            "vdn_common.h", "vdn_fp8.h"],
+    "add_norm": ["add_norm.hip", "eight.h", "vdn_common.h", "vdn_fp8.h"],
+    "adapters": ["adapters.hip", "eight.h", "vdn_common.h", "vdn_fp8.h"],
+    "rope_axes": ["rope_axes.hip", "eight.h", "qk_prep.h", "vdn_common.h", "vdn_fp8.h"],
     "lora_requant": ["lora_requant.hip", "quantize.hip", "vdn_common.h", "vdn_fp8.h"],
 }
 

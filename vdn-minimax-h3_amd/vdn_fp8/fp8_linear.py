@@ -482,7 +482,15 @@ class Fp8Linear(nn.Module):
                    "fp8 gemm")
         return out if late_bias is None else out + late_bias
 
-    def forward(self, x, **epilogue):
+    def forward(self, x, *, adapters=None, index=None, **epilogue):
+        """x [..., K] -> [..., N]. adapters, index: a bank of low-rank adapters (`vdn_fp8.lora.Adapters`) and each
+        row's own, added to the output (`vdn_fp8.lora.adapter_add`; bf16 or float16, without an epilogue)."""
+        if adapters is not None or index is not None:
+            if adapters is None or index is None or epilogue:
+                raise ValueError("adapters and index go together, without an epilogue")
+            from .lora import adapter_add
+            out = self.forward(x)
+            return adapter_add(x, out, adapters, index, out=out)
         shape = x.shape
         flat = x.dim() == 2   # already rows
         rows = x if flat else x.reshape(-1, shape[-1])

@@ -18,6 +18,9 @@ output is ever written. Numerics follow the compiled reference: binary32 inside 
 stretch, one rounding at its store (the reference's own caveat: not bitwise with the eager
 bodies, which round after every op).
 
+`add_norm_quantize` is the residual's addition, the norm and the quantization in one kernel, for streams
+whose next projection reads codes (bf16, float16 or float32).
+
 The eager bodies `_pre_ref`, `_post_ref`, `_swiglu_ref` are kept with the reference's names
 and meaning for callers that import them; nothing on the fast path uses them (a bf16
 feed-forward uses `_swiglu_one_rounding`, the compiled body's arithmetic).
@@ -26,8 +29,9 @@ import torch
 import torch.nn.functional as F
 
 from . import _lib
-from .fp8_linear import (FP8_DTYPE, Fp8Linear, _aligned16, _ptr, _rows, _stream, check_index_range,
+from .fp8_linear import (_DTYPES, FP8_DTYPE, Fp8Linear, _aligned16, _ptr, _rows, _stream, check_index_range,
                          swiglu_quantize_activation)
+from .kv_cache import _on
 
 
 # --------------------------------------------------------------------------------------
@@ -160,6 +164,89 @@ def post(residual, gate, indices, branch_out):
     _lib.check(lib.vdn_fp8_gated_residual(_ptr(r), r.stride(0), _ptr(g), N, _ptr(idx), g.shape[0], _ptr(b),
                                           b.stride(0), _ptr(out), N, M, N, _stream(r)), "post")
     return out.reshape(shape)
+
+
+def _typed_rows(x, width, name):
+    """x [..., K] as rows with unit column stride, 16-byte aligned, and their stride (a copy where they are not)."""
+    rows = x if x.dim() == 2 else x.reshape(-1, width)
+    ld, unit = rows.stride()
+    if unit != 1 or ld % 8 or ld < width or rows.data_ptr() % 16:
+        rows = rows.clone(memory_format=torch.contiguous_format)
+        ld = width
+    return rows, max(ld, width)
+
+
+def _table(t, width, dtype, dev, name):
+    """A modulation table [T, K] (or [K]) and its rows."""
+    if t.dtype != dtype or t.shape[-1:] != (width,) or t.dim() > 2 or t.device != dev:
+        raise ValueError(f"{name} must be a {str(dtype).replace('torch.', '')} [T, {width}] table (or [{width}]) on {dev} "
+                         f"(got {t.dtype} {tuple(t.shape)} on {t.device})")
+    return _aligned16(t.detach().reshape(-1, width).contiguous())
+
+
+def add_norm_quantize(residual, branch, weight, eps, *, gate=None, scale=None, shift=None, indices=None, return_normed=False):
+    """The residual's addition, the norm of the new stream and its quantization, in one pass:
+
+      hidden = residual + branch                          (+ gate[indices] * branch with a gate), the residual's type
+      n      = RMSNorm(hidden; weight, eps) * (1 + scale[indices]) + shift[indices]     in binary32
+      codes  = n per token as in `quantize_rows`, without a rounding of n in between
+
+    residual, branch [..., K]: both bf16, float16 or float32, or a float32 residual with a branch of 16 bits.
+    weight [K] (or None), gate, scale and shift [T, K] (or [K], or None) are of the branch's type; indices int [M] (None:
+    row 0; out-of-range ones are clamped). K is a multiple of 8, at most 16384. Returns hidden (a new tensor, the
+    residual's shape), codes e4m3 [M, K], scales fp32 [M, 1], and with return_normed n in the branch's type and shape.
+
+    (`post` and `pre_quantize` are the reference's two steps, with its rounding of n to bf16 before the codes.)"""
+    if not residual.is_cuda:
+        raise ValueError("add_norm_quantize runs on the GPU (a HIP kernel); residual is a CPU tensor")
+    dtype, stream, dev, shape = branch.dtype, residual.dtype, residual.device, residual.shape
+    if dtype not in _DTYPES or stream not in _DTYPES or (stream != dtype and stream != torch.float32):
+        raise ValueError("residual and branch must be bfloat16, float16 or float32 of one type, or residual float32 "
+                         f"(got {stream} and {dtype})")
+    if branch.shape != shape or branch.device != dev or not shape:
+        raise ValueError(f"branch must have the residual's shape {tuple(shape)} on {dev} (got {tuple(branch.shape)} on {branch.device})")
+    K = shape[-1]
+    if not 8 <= K <= 16384 or K % 8:
+        raise ValueError(f"add_norm_quantize takes widths that are multiples of 8, from 8 to 16384 (got {K})")
+    if (scale is None) != (shift is None):
+        raise ValueError("scale and shift go together")
+    r, ldr = _typed_rows(residual.detach(), K, "residual")
+    b, ldb = _typed_rows(branch.detach(), K, "branch")
+    M = r.shape[0]
+    if weight is not None:
+        if weight.dtype != dtype or weight.numel() != K or weight.device != dev:
+            raise ValueError(f"weight must be a {str(dtype).replace('torch.', '')} [{K}] tensor on {dev} (got {weight.dtype} {tuple(weight.shape)})")
+        weight = _aligned16(weight.detach().reshape(K).contiguous())
+    rows = 0
+    if gate is not None:
+        gate = _table(gate, K, dtype, dev, "gate")
+        rows = gate.shape[0]
+    if scale is not None:
+        scale, shift = _table(scale, K, dtype, dev, "scale"), _table(shift, K, dtype, dev, "shift")
+        if scale.shape != shift.shape or (gate is not None and scale.shape[0] != rows):
+            raise ValueError("gate, scale and shift must be tables of the same rows")
+        rows = scale.shape[0]
+    if (gate is not None or scale is not None) and not rows:
+        raise ValueError("a table needs at least 1 row")
+    if indices is not None:
+        if not rows:
+            raise ValueError("indices need a gate or a scale/shift table")
+        if indices.numel() != M or indices.is_floating_point():
+            raise ValueError("indices must hold one table row per token")
+        check_index_range(indices, rows, "add_norm_quantize: indices")
+        if indices.dtype != torch.int32 or indices.device != dev or not indices.is_contiguous():
+            # (a wider index is clamped before it is narrowed)
+            indices = indices.to(dev).clamp(0, rows - 1).to(torch.int32).contiguous()
+    hidden = torch.empty(shape, device=dev, dtype=stream)
+    y = torch.empty(M, K, device=dev, dtype=FP8_DTYPE)
+    s = torch.empty(M, 1, device=dev, dtype=torch.float32)
+    normed = torch.empty(shape, device=dev, dtype=dtype) if return_normed else None
+    with _on(dev):
+        _lib.check(_lib.load().vdn_fp8_add_norm_quantize(
+            r.data_ptr(), _DTYPES[stream], ldr, b.data_ptr(), _DTYPES[dtype], ldb, M, K, _ptr(gate), K, _ptr(weight), float(eps),
+            _ptr(scale), _ptr(shift), K, _ptr(indices), rows, hidden.data_ptr(), K, y.data_ptr(), K, s.data_ptr(), _ptr(normed), K,
+            _stream(r)), "add_norm_quantize")
+    return (hidden, y, s, normed) if return_normed else (hidden, y, s)
 
 
 # --------------------------------------------------------------------------------------

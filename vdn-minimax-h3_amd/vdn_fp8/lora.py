@@ -13,17 +13,23 @@ that `convert_linear_to_fp8` would swap, W + scale * B @ A is quantized directly
 place -- the reference's "merge LoRA, then convert" order (assemble.py:116-175) in
 one pass over each weight.
 
+`Adapters` and `adapter_add` serve adapters that are not merged: many requests of one batch, each with its own
+(or none), beside one shared projection.
+
 Adapter files: `load_external_lora` and `_translate_original_layout` read peft-named
 safetensors and the original (non-diffusers) key layout, as lora.py:25-117 does.
 """
+import ctypes
 import re
+from typing import NamedTuple
 
 import torch
 import torch.nn as nn
 
 from . import _lib
-from .fp8_linear import (MIN_WIDTH, SKIP_END_BLOCKS, Fp8Linear, _aligned16, _blocks_to_skip, _ptr,
+from .fp8_linear import (_DTYPES, MIN_WIDTH, SKIP_END_BLOCKS, Fp8Linear, _aligned16, _blocks_to_skip, _ptr,
                          _stream, lora_delta, lora_in_kernel)
+from .kv_cache import _on
 
 # Original-layout module names -> diffusers names (lora.py:22-30).
 _ORIGINAL_RENAMES = (
@@ -187,3 +193,133 @@ def load_external_lora(path, alpha=None):
         alpha = float(meta["alpha"]) if alpha is None else float(alpha)
         scale = alpha / ranks[0]
     return state, scale, ranks
+
+
+# --------------------------------------------------------------------------------------
+# Adapters of many requests at once
+# --------------------------------------------------------------------------------------
+
+RANK_UNIT = 16      # ranks of a bank are multiples of this
+_ADAPTER_DTYPES = (torch.bfloat16, torch.float16)
+
+
+class Adapters(NamedTuple):
+    """L adapters of one projection [N, K]: a [L, R, K] and b [L, N, R], bf16 or float16, scale float32 [L]. R is a
+    multiple of 16, at most 128; adapters of smaller rank are padded with zeros (`Adapters.pack`)."""
+    a: torch.Tensor
+    b: torch.Tensor
+    scale: torch.Tensor
+
+    @classmethod
+    def pack(cls, pairs, *, dtype=torch.bfloat16, device="cuda"):
+        """A bank of `pairs`, (A [r, K], B [N, r], scale) each, of any ranks up to 128: the largest, rounded up to
+        a multiple of 16, is the bank's. The factors are rounded to `dtype`."""
+        pairs = list(pairs)
+        if not pairs:
+            raise ValueError("a bank needs at least one adapter")
+        if dtype not in _ADAPTER_DTYPES:
+            raise ValueError(f"adapters are bfloat16 or float16 (got {dtype})")
+        K, N = pairs[0][0].shape[-1], pairs[0][1].shape[0]
+        for a, b, _ in pairs:
+            if a.dim() != 2 or b.dim() != 2 or a.shape[1] != K or b.shape[0] != N or b.shape[1] != a.shape[0]:
+                raise ValueError(f"LoRA shapes {tuple(a.shape)} / {tuple(b.shape)} do not fit a [{N}, {K}] weight")
+        rank = max(RANK_UNIT, *(-(-a.shape[0] // RANK_UNIT) * RANK_UNIT for a, _, _ in pairs))
+        if rank > 128:
+            raise ValueError(f"adapters of rank 128 at most (got {rank})")
+        bank = cls(torch.zeros(len(pairs), rank, K, device=device, dtype=dtype),
+                   torch.zeros(len(pairs), N, rank, device=device, dtype=dtype),
+                   torch.tensor([float(s) for _, _, s in pairs], dtype=torch.float32).to(device))
+        for i, (a, b, _) in enumerate(pairs):
+            bank.a[i, :a.shape[0]] = a.detach().to(device=device, dtype=dtype)
+            bank.b[i, :, :a.shape[0]] = b.detach().to(device=device, dtype=dtype)
+        return bank
+
+    @classmethod
+    def of_states(cls, states, target, **kinds):
+        """The bank of one Linear from adapter files: `states` is a list of (state, scale), as `load_external_lora`
+        returns them, `target` the Linear's name in them; each state holds the pair "<target>.lora_A. / .lora_B."."""
+        pairs = []
+        for state, scale in states:
+            found = [(a, b, scale) for name, a, b in _pairs(state) if name == target + ".weight"]
+            if len(found) != 1:
+                raise KeyError(f"{len(found)} LoRA pairs for {target!r}")
+            pairs += found
+        return cls.pack(pairs, **kinds)
+
+
+_ADAPTER_BYTES = {}
+
+
+def _adapter_workspace(T, K, N, L, R):
+    """Bytes of workspace of a call, asked of the library once per shape."""
+    key = (T, K, N, L, R)
+    got = _ADAPTER_BYTES.get(key)
+    if got is None:
+        if len(_ADAPTER_BYTES) >= 4096:
+            _ADAPTER_BYTES.clear()
+        size = ctypes.c_int64(0)
+        _lib.check(_lib.load().vdn_fp8_adapter_add_workspace_size(*key, ctypes.byref(size)), "adapter_add")
+        got = _ADAPTER_BYTES[key] = size.value
+    return got
+
+
+def _adapter_rows(t, width, dtype, dev, name):
+    if t.dtype != dtype or t.shape[-1:] != (width,) or t.device != dev:
+        raise ValueError(f"{name} must be {str(dtype).replace('torch.', '')} [..., {width}] on {dev} (got {t.dtype} {tuple(t.shape)} on {t.device})")
+    rows = t if t.dim() == 2 else t.reshape(-1, width)
+    ld, unit = rows.stride()
+    if unit != 1 or ld % 8 or ld < width or rows.data_ptr() % 16:
+        rows = rows.clone(memory_format=torch.contiguous_format)
+        ld = width
+    return rows, max(ld, width)
+
+
+def adapter_add(x, base, adapters, index, *, out=None):
+    """base + scale[i] * (x @ a[i].T) @ b[i].T, row by row with i = index[row]: the low-rank adapters of many requests
+    beside the projection that they share.
+
+    x [..., K], base [..., N] (that projection's output) and the adapters are of one type, bf16 or float16; index
+    int32 [T] names each row's adapter (-1, or any number outside [0, L): none, base's row as it is). Rows of one
+    request next to each other are read best; any order is right. out: base itself, to add in place
+    (a new tensor otherwise). Products are summed in binary32, x @ a.T is not rounded between, the
+    sum is rounded once."""
+    if not x.is_cuda:
+        raise ValueError("adapter_add runs on the GPU (HIP kernels); x is a CPU tensor")
+    a, b, scale = adapters
+    dtype, dev = x.dtype, x.device
+    if dtype not in _ADAPTER_DTYPES:
+        raise ValueError(f"adapter_add takes bfloat16 or float16 rows (got {dtype})")
+    if a.dim() != 3 or b.dim() != 3 or b.shape != (a.shape[0], b.shape[1], a.shape[1]):
+        raise ValueError(f"adapters must be a [L, R, K] and b [L, N, R] (got {tuple(a.shape)} and {tuple(b.shape)})")
+    L, R, K = a.shape
+    N = b.shape[1]
+    if a.dtype != dtype or b.dtype != dtype or scale.dtype != torch.float32 or scale.shape != (L,):
+        raise ValueError(f"adapters must be {str(dtype).replace('torch.', '')}, as the rows, and their scale float32 [{L}] "
+                         f"(got {a.dtype}, {b.dtype}, {scale.dtype} {tuple(scale.shape)})")
+    if a.device != dev or b.device != dev or scale.device != dev or index.device != dev:
+        raise ValueError(f"the adapters and index must be on {dev}")
+    if not a.is_contiguous() or not b.is_contiguous() or not scale.is_contiguous():
+        raise ValueError("the adapters must be contiguous")
+    if x.shape[:-1] != base.shape[:-1]:
+        raise ValueError(f"x {tuple(x.shape)} and base {tuple(base.shape)} must have the same rows")
+    rows, ldx = _adapter_rows(x.detach(), K, dtype, dev, "x")
+    T = rows.shape[0]
+    if index.dtype != torch.int32 or index.shape != (T,) or not index.is_contiguous():
+        raise ValueError(f"index must be a contiguous int32 [{T}] tensor (got {index.dtype} {tuple(index.shape)})")
+    if out is not None and out is not base:
+        raise ValueError("out must be base itself, or None for a new tensor")
+    given, ldbase = _adapter_rows(base.detach(), N, dtype, dev, "base")
+    if out is None:
+        result = torch.empty(base.shape, device=dev, dtype=dtype)
+        to, ldo = result, N
+    else:
+        if given.data_ptr() != base.data_ptr():
+            raise ValueError("base cannot be added to in place: its rows need unit stride, 16-byte alignment and row strides of multiples of 8")
+        result, to, ldo = base, given, ldbase
+    with _on(dev):
+        n = _adapter_workspace(T, K, N, L, R)
+        ws = torch.empty(n, device=dev, dtype=torch.uint8) if n else None
+        _lib.check(_lib.load().vdn_fp8_adapter_add(
+            rows.data_ptr(), _DTYPES[dtype], ldx, given.data_ptr(), ldbase, T, K, N, a.data_ptr(), b.data_ptr(), scale.data_ptr(), L, R,
+            index.data_ptr(), to.data_ptr(), ldo, _ptr(ws), n, _stream(rows)), "adapter_add")
+    return result

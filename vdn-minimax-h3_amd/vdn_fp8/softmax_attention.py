@@ -10,13 +10,19 @@ kernel: binary32 throughout, the cos/sin tables rounded to bf16 first
 (`cos.to(x.dtype)`), one rounding at the store -- not bitwise with the eager chain,
 which rounds after every op, exactly as the reference notes for its own kernel.
 
+`qk_prep_axes` is the same preparation of q and k at positions of several axes (time, height, width), the
+angles computed in the kernel.
+
 `cached_attention` is the branch over tokens of earlier calls, kept in 8 bits
 (`vdn_fp8.kv_cache`).
 """
+from typing import NamedTuple
+
 import torch
 
 from . import _lib
-from .fp8_linear import _aligned16, _ptr, _stream
+from .fp8_linear import _DTYPES, _aligned16, _ptr, _stream
+from .kv_cache import _ld, _on, _rows
 
 
 def qk_prep(t, weight, eps, cos=None, sin=None):
@@ -63,6 +69,91 @@ def qk_prep(t, weight, eps, cos=None, sin=None):
 _qk_prep = qk_prep
 
 
+class RopeAxes(NamedTuple):
+    """A rotary embedding over positions of several axes: pair j of a head turns by positions[axis[j]] *
+    inv_freq[j]. inv_freq float64 [R / 2] (radians a position), axis int32 [R / 2]; pairs: pair j is elements
+    (2 j, 2 j + 1) of the head, else (j, j + R / 2). Elements from R on pass through."""
+    inv_freq: torch.Tensor
+    axis: torch.Tensor
+    pairs: bool = False
+
+    @classmethod
+    def make(cls, sections, *, theta=10000.0, shared=False, pairs=False, device="cuda"):
+        """`sections` pairs for each axis in turn. Each axis has frequencies of its own, theta ** -(i / n) for its
+        n pairs, or with `shared` all take the one sequence theta ** -(j / sum(sections))."""
+        sections = [int(n) for n in sections]
+        if not sections or min(sections) < 0 or not sum(sections):
+            raise ValueError(f"sections must be pairs for each axis (got {sections})")
+        at = torch.arange(sum(sections), dtype=torch.float64) / sum(sections) if shared else \
+            torch.cat([torch.arange(n, dtype=torch.float64) / max(n, 1) for n in sections])
+        axis = torch.repeat_interleave(torch.arange(len(sections), dtype=torch.int32), torch.tensor(sections))
+        return cls((float(theta) ** -at).to(device), axis.to(device), bool(pairs))
+
+
+_POSITIONS = {torch.int32: _lib.POSITION_I32, torch.int64: _lib.POSITION_I64, torch.float32: _lib.POSITION_F32}
+_MOST_AXES = 8
+
+
+def _axes_norm(norm, d, dtype, dev, name):
+    """(normed, weight, eps) of a norm (weight or None, eps) or None."""
+    if norm is None:
+        return 0, None, 0.0
+    weight, eps = norm
+    if weight is None:
+        return 1, None, float(eps)
+    if weight.numel() != d or weight.dtype != dtype or weight.device != dev:
+        raise ValueError(f"{name}'s weight must be a {str(dtype).replace('torch.', '')} [{d}] tensor on {dev} (got {weight.dtype} {tuple(weight.shape)})")
+    return 1, _aligned16(weight.detach().reshape(d).contiguous()), float(eps)
+
+
+def qk_prep_axes(query, key, norm_q, norm_k, rope, positions):
+    """RMSNorm over each head, then the rotation of `rope` (`RopeAxes`) at `positions` int32, int64 or float32
+    [T, axes] (up to 8 axes, or [T] for one), of query [T, q_heads, d] and key [T, heads, d] in one launch. norm_q and
+    norm_k are (weight or None, eps), or None for no norm. bf16, float16 or float32 (weights of the same type), d 64,
+    128 or 256; heads contiguous, any token stride (column slices of one projection's output are fine).
+
+    Angles are formed in binary64, so that far positions keep their fraction of a turn; cosine and sine are
+    binary32, and the result is rounded once. Returns new contiguous query and key."""
+    dtype = query.dtype
+    if dtype not in _DTYPES:
+        raise ValueError(f"qk_prep_axes takes bfloat16, float16 or float32 (got {dtype})")
+    if query.dim() != 3 or query.shape[2] not in (64, 128, 256):
+        raise ValueError(f"query must be [T, heads, 64, 128 or 256] (got {tuple(query.shape)})")
+    T, q_heads, d = query.shape
+    query, key = _rows(query, None, d, "query", (dtype,)), _rows(key, None, d, "key", (dtype,))
+    dev, k_heads = query.device, key.shape[1]
+    if key.device != dev or key.shape[0] != T:
+        raise ValueError("query and key must have the same rows on one device")
+    inv_freq, axis, pairs = rope
+    half = inv_freq.numel()
+    if inv_freq.dtype != torch.float64 or axis.dtype != torch.int32 or inv_freq.dim() != 1 or axis.shape != (half,):
+        raise ValueError(f"rope must hold float64 inv_freq [R / 2] and int32 axis [R / 2] (got {inv_freq.dtype} {tuple(inv_freq.shape)}, "
+                         f"{axis.dtype} {tuple(axis.shape)})")
+    if 2 * half > d or half % (4 if pairs else 8):
+        raise ValueError(f"rope must turn at most {d // 2} pairs, a multiple of {4 if pairs else 8} (got {half})")
+    if positions.dtype not in _POSITIONS or positions.dim() not in (1, 2) or positions.shape[0] != T:
+        raise ValueError(f"positions must be int32, int64 or float32 [{T}, axes] (got {positions.dtype} {tuple(positions.shape)})")
+    if positions.dim() == 1:
+        positions = positions[:, None]
+    axes = positions.shape[1]
+    if not 1 <= axes <= _MOST_AXES:
+        raise ValueError(f"positions of 1 to {_MOST_AXES} axes (got {axes})")
+    if positions.device != dev or inv_freq.device != dev or axis.device != dev:
+        raise ValueError(f"positions and rope must be on {dev}")
+    positions, inv_freq, axis = positions.contiguous(), inv_freq.contiguous(), axis.contiguous()
+    nq, wq, eps_q = _axes_norm(norm_q, d, dtype, dev, "norm_q")
+    nk, wk, eps_k = _axes_norm(norm_k, d, dtype, dev, "norm_k")
+    out_q = torch.empty(T, q_heads, d, device=dev, dtype=dtype)
+    out_k = torch.empty(T, k_heads, d, device=dev, dtype=dtype)
+    with _on(dev):
+        _lib.check(_lib.load().vdn_fp8_qk_prep_axes(
+            query.data_ptr(), q_heads, _ld(query), key.data_ptr(), k_heads, _ld(key), T, d, _DTYPES[dtype], nq, _ptr(wq), eps_q, nk, _ptr(wk),
+            eps_k, inv_freq.data_ptr(), axis.data_ptr(), 2 * half, int(bool(pairs)), positions.data_ptr(),
+            _POSITIONS[positions.dtype], axes, axes, out_q.data_ptr(), q_heads * d, out_k.data_ptr(), k_heads * d, _stream(query)),
+            "qk_prep_axes")
+    return out_q, out_k
+
+
 def _project(x, projections):
     """Every projection of x; fp8 ones share one quantization of it."""
     from .fp8_linear import Fp8Linear, quantize_activation
@@ -92,7 +183,8 @@ def qkv(x, to_q, to_k, to_v, heads, norm_q, norm_k, rotary_emb=None):
 
 
 def cached_attention(x, to_q, to_k, to_v, norm_q, norm_k, cache, page_table, lengths, *, rotary_emb=None, causal=False,
-                     scale=None, q_start=None, max_query=None, top=None, query_block=None, first=1, last=1):
+                     scale=None, q_start=None, max_query=None, top=None, query_block=None, first=1, last=1, rope=None, positions=None,
+                     adapters=None, index=None):
     """`qkv` and the attention behind it where earlier tokens are kept in a `KvCache`: one quantization
     of x for the three GEMMs, then QK-norm, rope and the store of k and v in one launch
     (`qk_prep_append`), then `kv_attention` over each sequence's cache, its new tokens included. The cache's
@@ -100,16 +192,36 @@ def cached_attention(x, to_q, to_k, to_v, norm_q, norm_k, cache, page_table, len
     projections, norms and rotary_emb as in `qkv`; page_table, lengths, q_start, max_query, causal and scale
     as in `kv_attention`. With `top`, each block of `query_block` queries attends to the `top` pages
     that `kv_select` finds for it (`first` and `last` as there). What any part refuses is refused before
-    anything is stored. Returns [T, q_heads * d], what the output projection takes."""
-    from .kv_cache import check_attention, kv_attention, kv_select, qk_prep_append
+    anything is stored. Returns [T, q_heads * d], what the output projection takes.
+
+    rope, positions: a `RopeAxes` and each token's positions, in place of rotary_emb (`qk_prep_axes`, then the store).
+    adapters, index: the low-rank adapters of to_q, to_k and to_v (three `Adapters`, or None for one without) and
+    each token's own (`adapter_add`)."""
+    from .kv_cache import check_attention, kv_append, kv_attention, kv_select, qk_prep_append
 
     d = cache.k.shape[-1]
-    query, key, value = (t.unflatten(-1, (-1, d)) for t in _project(x, (to_q, to_k, to_v)))
+    if (rope is None) != (positions is None) or (rope is not None and rotary_emb is not None):
+        raise ValueError("rope and positions go together, in place of rotary_emb")
+    if (adapters is None) != (index is None) or (adapters is not None and len(adapters) != 3):
+        raise ValueError("adapters (of to_q, to_k and to_v) and index go together")
+    out = _project(x, (to_q, to_k, to_v))
+    if adapters is not None:
+        from .fp8_linear import Fp8Linear
+        from .lora import adapter_add
+
+        # in place where the output is a new tensor for certain (another callable may return x, or a buffer of its own)
+        out = [t if bank is None else adapter_add(x, t, bank, index, out=t if isinstance(p, Fp8Linear) else None)
+               for t, p, bank in zip(out, (to_q, to_k, to_v), adapters)]
+    query, key, value = (t.unflatten(-1, (-1, d)) for t in out)
     check_attention(query, cache, page_table, lengths, scale=scale, q_start=q_start, max_query=max_query, top=top, query_block=query_block,
                     first=first, last=last)
-    cos, sin = (None, None) if rotary_emb is None else rotary_emb
-    query = qk_prep_append(query, key, value, (norm_q.weight, norm_q.eps), (norm_k.weight, norm_k.eps), cache, page_table, lengths,
-                           cos=cos, sin=sin, q_start=q_start)
+    if rope is not None:
+        query, key = qk_prep_axes(query, key, (norm_q.weight, norm_q.eps), (norm_k.weight, norm_k.eps), rope, positions)
+        kv_append(key, value, cache, page_table, lengths, q_start=q_start)
+    else:
+        cos, sin = (None, None) if rotary_emb is None else rotary_emb
+        query = qk_prep_append(query, key, value, (norm_q.weight, norm_q.eps), (norm_k.weight, norm_k.eps), cache, page_table, lengths,
+                               cos=cos, sin=sin, q_start=q_start)
     blocks = None
     if top is not None:
         blocks = kv_select(query, cache, page_table, lengths, top, query_block=query_block, first=first, last=last, causal=causal,
