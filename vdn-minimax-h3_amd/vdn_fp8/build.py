@@ -49,7 +49,8 @@ HIPCC_FLAGS = [
 
 # Per-source additions. The LoRA kernels read every MFMA result with VALU code:
 # accumulating in VGPRs (rather than AGPRs) saves one copy per element.
-EXTRA_FLAGS = {"lora_requant.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"]}
+EXTRA_FLAGS = {"lora_requant.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
+               "adapters.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"]}
 
 
 def _sha256(path):

@@ -166,22 +166,29 @@ def post(residual, gate, indices, branch_out):
     return out.reshape(shape)
 
 
-def _typed_rows(x, width, name):
+def _typed_rows(x, width):
     """x [..., K] as rows with unit column stride, 16-byte aligned, and their stride (a copy where they are not)."""
     rows = x if x.dim() == 2 else x.reshape(-1, width)
     ld, unit = rows.stride()
     if unit != 1 or ld % 8 or ld < width or rows.data_ptr() % 16:
         rows = rows.clone(memory_format=torch.contiguous_format)
         ld = width
-    return rows, max(ld, width)
+    return rows, ld if ld > width else width
 
 
-def _table(t, width, dtype, dev, name):
-    """A modulation table [T, K] (or [K]) and its rows."""
-    if t.dtype != dtype or t.shape[-1:] != (width,) or t.dim() > 2 or t.device != dev:
-        raise ValueError(f"{name} must be a {str(dtype).replace('torch.', '')} [T, {width}] table (or [{width}]) on {dev} "
-                         f"(got {t.dtype} {tuple(t.shape)} on {t.device})")
-    return _aligned16(t.detach().reshape(-1, width).contiguous())
+def _name(dtype):
+    return str(dtype).replace("torch.", "")
+
+
+def _table(t, width, dtype, at, name):
+    """A modulation table [T, K] (or [K]), contiguous, and its rows."""
+    shape = t.shape
+    if t.dtype is not dtype or t.get_device() != at or len(shape) not in (1, 2) or shape[-1] != width:
+        raise ValueError(f"{name} must be a {_name(dtype)} [T, {width}] table (or [{width}]) on the rows' device "
+                         f"(got {t.dtype} {tuple(shape)} on {t.device})")
+    if not t.is_contiguous() or t.data_ptr() % 16:
+        t = t.clone(memory_format=torch.contiguous_format)
+    return t, shape[0] if len(shape) == 2 else 1
 
 
 def add_norm_quantize(residual, branch, weight, eps, *, gate=None, scale=None, shift=None, indices=None, return_normed=False):
@@ -199,34 +206,35 @@ def add_norm_quantize(residual, branch, weight, eps, *, gate=None, scale=None, s
     (`post` and `pre_quantize` are the reference's two steps, with its rounding of n to bf16 before the codes.)"""
     if not residual.is_cuda:
         raise ValueError("add_norm_quantize runs on the GPU (a HIP kernel); residual is a CPU tensor")
-    dtype, stream, dev, shape = branch.dtype, residual.dtype, residual.device, residual.shape
-    if dtype not in _DTYPES or stream not in _DTYPES or (stream != dtype and stream != torch.float32):
+    # (this call is short for few rows: each of a tensor's properties is read once)
+    dtype, stream, shape, at = branch.dtype, residual.dtype, residual.shape, residual.get_device()
+    if dtype not in _DTYPES or stream not in _DTYPES or (stream is not dtype and stream is not torch.float32):
         raise ValueError("residual and branch must be bfloat16, float16 or float32 of one type, or residual float32 "
                          f"(got {stream} and {dtype})")
-    if branch.shape != shape or branch.device != dev or not shape:
-        raise ValueError(f"branch must have the residual's shape {tuple(shape)} on {dev} (got {tuple(branch.shape)} on {branch.device})")
+    if branch.shape != shape or branch.get_device() != at or not shape:
+        raise ValueError(f"branch must have the residual's shape {tuple(shape)} on {residual.device} (got {tuple(branch.shape)} on {branch.device})")
     K = shape[-1]
     if not 8 <= K <= 16384 or K % 8:
         raise ValueError(f"add_norm_quantize takes widths that are multiples of 8, from 8 to 16384 (got {K})")
     if (scale is None) != (shift is None):
         raise ValueError("scale and shift go together")
-    r, ldr = _typed_rows(residual.detach(), K, "residual")
-    b, ldb = _typed_rows(branch.detach(), K, "branch")
-    M = r.shape[0]
+    r, ldr = _typed_rows(residual, K)
+    b, ldb = _typed_rows(branch, K)
+    M, dev = r.shape[0], r.device
     if weight is not None:
-        if weight.dtype != dtype or weight.numel() != K or weight.device != dev:
-            raise ValueError(f"weight must be a {str(dtype).replace('torch.', '')} [{K}] tensor on {dev} (got {weight.dtype} {tuple(weight.shape)})")
-        weight = _aligned16(weight.detach().reshape(K).contiguous())
+        if weight.dtype is not dtype or weight.numel() != K or weight.get_device() != at:
+            raise ValueError(f"weight must be a {_name(dtype)} [{K}] tensor on {dev} (got {weight.dtype} {tuple(weight.shape)})")
+        if not weight.is_contiguous() or weight.data_ptr() % 16:
+            weight = weight.clone(memory_format=torch.contiguous_format)
     rows = 0
     if gate is not None:
-        gate = _table(gate, K, dtype, dev, "gate")
-        rows = gate.shape[0]
+        gate, rows = _table(gate, K, dtype, at, "gate")
     if scale is not None:
-        scale, shift = _table(scale, K, dtype, dev, "scale"), _table(shift, K, dtype, dev, "shift")
-        if scale.shape != shift.shape or (gate is not None and scale.shape[0] != rows):
+        (scale, of_scale), (shift, of_shift) = _table(scale, K, dtype, at, "scale"), _table(shift, K, dtype, at, "shift")
+        if of_scale != of_shift or (gate is not None and of_scale != rows):
             raise ValueError("gate, scale and shift must be tables of the same rows")
-        rows = scale.shape[0]
-    if (gate is not None or scale is not None) and not rows:
+        rows = of_scale
+    if not rows and (gate is not None or scale is not None):
         raise ValueError("a table needs at least 1 row")
     if indices is not None:
         if not rows:
@@ -234,18 +242,24 @@ def add_norm_quantize(residual, branch, weight, eps, *, gate=None, scale=None, s
         if indices.numel() != M or indices.is_floating_point():
             raise ValueError("indices must hold one table row per token")
         check_index_range(indices, rows, "add_norm_quantize: indices")
-        if indices.dtype != torch.int32 or indices.device != dev or not indices.is_contiguous():
+        if indices.dtype is not torch.int32 or indices.get_device() != at or not indices.is_contiguous():
             # (a wider index is clamped before it is narrowed)
             indices = indices.to(dev).clamp(0, rows - 1).to(torch.int32).contiguous()
-    hidden = torch.empty(shape, device=dev, dtype=stream)
-    y = torch.empty(M, K, device=dev, dtype=FP8_DTYPE)
+    # (empty_like takes half the time of empty with a shape)
+    like = r if ldr == K and r.is_contiguous() else torch.empty(M, K, device=dev, dtype=stream)
+    flat = len(shape) == 2
+    hidden = torch.empty_like(like)
+    y = torch.empty_like(like, dtype=FP8_DTYPE)
     s = torch.empty(M, 1, device=dev, dtype=torch.float32)
-    normed = torch.empty(shape, device=dev, dtype=dtype) if return_normed else None
+    normed = torch.empty_like(like, dtype=dtype) if return_normed else None
     with _on(dev):
         _lib.check(_lib.load().vdn_fp8_add_norm_quantize(
-            r.data_ptr(), _DTYPES[stream], ldr, b.data_ptr(), _DTYPES[dtype], ldb, M, K, _ptr(gate), K, _ptr(weight), float(eps),
+            r.data_ptr(), _DTYPES[stream], ldr, b.data_ptr(), _DTYPES[dtype], ldb, M, K, _ptr(gate), K, _ptr(weight), eps,
             _ptr(scale), _ptr(shift), K, _ptr(indices), rows, hidden.data_ptr(), K, y.data_ptr(), K, s.data_ptr(), _ptr(normed), K,
             _stream(r)), "add_norm_quantize")
+    if not flat:
+        hidden = hidden.view(shape)
+        normed = normed.view(shape) if return_normed else None
     return (hidden, y, s, normed) if return_normed else (hidden, y, s)
 
 

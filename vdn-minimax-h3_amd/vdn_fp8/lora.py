@@ -263,15 +263,21 @@ def _adapter_workspace(T, K, N, L, R):
     return got
 
 
-def _adapter_rows(t, width, dtype, dev, name):
-    if t.dtype != dtype or t.shape[-1:] != (width,) or t.device != dev:
-        raise ValueError(f"{name} must be {str(dtype).replace('torch.', '')} [..., {width}] on {dev} (got {t.dtype} {tuple(t.shape)} on {t.device})")
-    rows = t if t.dim() == 2 else t.reshape(-1, width)
+def _name(dtype):
+    return str(dtype).replace("torch.", "")
+
+
+def _adapter_rows(t, width, dtype, at, name):
+    """t [..., width] as rows with unit column stride, 16-byte aligned, and their stride (a copy where they are not)."""
+    shape = t.shape
+    if t.dtype is not dtype or not shape or shape[-1] != width or t.get_device() != at:
+        raise ValueError(f"{name} must be {_name(dtype)} [..., {width}] on the rows' device (got {t.dtype} {tuple(shape)} on {t.device})")
+    rows = t if len(shape) == 2 else t.reshape(-1, width)
     ld, unit = rows.stride()
     if unit != 1 or ld % 8 or ld < width or rows.data_ptr() % 16:
         rows = rows.clone(memory_format=torch.contiguous_format)
         ld = width
-    return rows, max(ld, width)
+    return rows, ld if ld > width else width
 
 
 def adapter_add(x, base, adapters, index, *, out=None):
@@ -285,41 +291,44 @@ def adapter_add(x, base, adapters, index, *, out=None):
     sum is rounded once."""
     if not x.is_cuda:
         raise ValueError("adapter_add runs on the GPU (HIP kernels); x is a CPU tensor")
+    # (this call is short for few rows: each of a tensor's properties is read once)
     a, b, scale = adapters
-    dtype, dev = x.dtype, x.device
+    dtype, at, of_a, of_b = x.dtype, x.get_device(), a.shape, b.shape
     if dtype not in _ADAPTER_DTYPES:
         raise ValueError(f"adapter_add takes bfloat16 or float16 rows (got {dtype})")
-    if a.dim() != 3 or b.dim() != 3 or b.shape != (a.shape[0], b.shape[1], a.shape[1]):
-        raise ValueError(f"adapters must be a [L, R, K] and b [L, N, R] (got {tuple(a.shape)} and {tuple(b.shape)})")
-    L, R, K = a.shape
-    N = b.shape[1]
-    if a.dtype != dtype or b.dtype != dtype or scale.dtype != torch.float32 or scale.shape != (L,):
-        raise ValueError(f"adapters must be {str(dtype).replace('torch.', '')}, as the rows, and their scale float32 [{L}] "
+    if len(of_a) != 3 or len(of_b) != 3 or of_b[0] != of_a[0] or of_b[2] != of_a[1]:
+        raise ValueError(f"adapters must be a [L, R, K] and b [L, N, R] (got {tuple(of_a)} and {tuple(of_b)})")
+    L, R, K = of_a
+    N = of_b[1]
+    if a.dtype is not dtype or b.dtype is not dtype or scale.dtype is not torch.float32 or scale.shape != (L,):
+        raise ValueError(f"adapters must be {_name(dtype)}, as the rows, and their scale float32 [{L}] "
                          f"(got {a.dtype}, {b.dtype}, {scale.dtype} {tuple(scale.shape)})")
-    if a.device != dev or b.device != dev or scale.device != dev or index.device != dev:
-        raise ValueError(f"the adapters and index must be on {dev}")
+    if a.get_device() != at or b.get_device() != at or scale.get_device() != at or index.get_device() != at:
+        raise ValueError(f"the adapters and index must be on {x.device}")
     if not a.is_contiguous() or not b.is_contiguous() or not scale.is_contiguous():
         raise ValueError("the adapters must be contiguous")
     if x.shape[:-1] != base.shape[:-1]:
         raise ValueError(f"x {tuple(x.shape)} and base {tuple(base.shape)} must have the same rows")
-    rows, ldx = _adapter_rows(x.detach(), K, dtype, dev, "x")
-    T = rows.shape[0]
-    if index.dtype != torch.int32 or index.shape != (T,) or not index.is_contiguous():
+    rows, ldx = _adapter_rows(x, K, dtype, at, "x")
+    T, dev = rows.shape[0], rows.device
+    if index.dtype is not torch.int32 or index.shape != (T,) or not index.is_contiguous():
         raise ValueError(f"index must be a contiguous int32 [{T}] tensor (got {index.dtype} {tuple(index.shape)})")
-    if out is not None and out is not base:
-        raise ValueError("out must be base itself, or None for a new tensor")
-    given, ldbase = _adapter_rows(base.detach(), N, dtype, dev, "base")
+    given, ldbase = _adapter_rows(base, N, dtype, at, "base")
     if out is None:
-        result = torch.empty(base.shape, device=dev, dtype=dtype)
+        result = torch.empty_like(given) if ldbase == N and given.is_contiguous() else torch.empty(T, N, device=dev, dtype=dtype)
         to, ldo = result, N
+        if base.dim() != 2:
+            result = result.view(base.shape)
     else:
+        if out is not base:
+            raise ValueError("out must be base itself, or None for a new tensor")
         if given.data_ptr() != base.data_ptr():
             raise ValueError("base cannot be added to in place: its rows need unit stride, 16-byte alignment and row strides of multiples of 8")
         result, to, ldo = base, given, ldbase
+    n = _adapter_workspace(T, K, N, L, R)
+    ws = torch.empty(n, device=dev, dtype=torch.uint8) if n else None
     with _on(dev):
-        n = _adapter_workspace(T, K, N, L, R)
-        ws = torch.empty(n, device=dev, dtype=torch.uint8) if n else None
         _lib.check(_lib.load().vdn_fp8_adapter_add(
             rows.data_ptr(), _DTYPES[dtype], ldx, given.data_ptr(), ldbase, T, K, N, a.data_ptr(), b.data_ptr(), scale.data_ptr(), L, R,
-            index.data_ptr(), to.data_ptr(), ldo, _ptr(ws), n, _stream(rows)), "adapter_add")
+            index.data_ptr(), to.data_ptr(), ldo, None if ws is None else ws.data_ptr(), n, _stream(rows)), "adapter_add")
     return result

@@ -94,16 +94,19 @@ _POSITIONS = {torch.int32: _lib.POSITION_I32, torch.int64: _lib.POSITION_I64, to
 _MOST_AXES = 8
 
 
-def _axes_norm(norm, d, dtype, dev, name):
+def _axes_norm(norm, d, dtype, at, name):
     """(normed, weight, eps) of a norm (weight or None, eps) or None."""
     if norm is None:
         return 0, None, 0.0
     weight, eps = norm
     if weight is None:
-        return 1, None, float(eps)
-    if weight.numel() != d or weight.dtype != dtype or weight.device != dev:
-        raise ValueError(f"{name}'s weight must be a {str(dtype).replace('torch.', '')} [{d}] tensor on {dev} (got {weight.dtype} {tuple(weight.shape)})")
-    return 1, _aligned16(weight.detach().reshape(d).contiguous()), float(eps)
+        return 1, None, eps
+    if weight.numel() != d or weight.dtype is not dtype or weight.get_device() != at:
+        raise ValueError(f"{name}'s weight must be a {str(dtype).replace('torch.', '')} [{d}] tensor on the rows' device "
+                         f"(got {weight.dtype} {tuple(weight.shape)} on {weight.device})")
+    if not weight.is_contiguous() or weight.data_ptr() % 16:
+        weight = weight.clone(memory_format=torch.contiguous_format)
+    return 1, weight, eps
 
 
 def qk_prep_axes(query, key, norm_q, norm_k, rope, positions):
@@ -114,43 +117,45 @@ def qk_prep_axes(query, key, norm_q, norm_k, rope, positions):
 
     Angles are formed in binary64, so that far positions keep their fraction of a turn; cosine and sine are
     binary32, and the result is rounded once. Returns new contiguous query and key."""
-    dtype = query.dtype
+    # (this call is short for few tokens: each of a tensor's properties is read once)
+    dtype, shape = query.dtype, query.shape
     if dtype not in _DTYPES:
         raise ValueError(f"qk_prep_axes takes bfloat16, float16 or float32 (got {dtype})")
-    if query.dim() != 3 or query.shape[2] not in (64, 128, 256):
-        raise ValueError(f"query must be [T, heads, 64, 128 or 256] (got {tuple(query.shape)})")
-    T, q_heads, d = query.shape
-    query, key = _rows(query, None, d, "query", (dtype,)), _rows(key, None, d, "key", (dtype,))
-    dev, k_heads = query.device, key.shape[1]
-    if key.device != dev or key.shape[0] != T:
+    if len(shape) != 3 or shape[2] not in (64, 128, 256):
+        raise ValueError(f"query must be [T, heads, 64, 128 or 256] (got {tuple(shape)})")
+    T, q_heads, d = shape
+    kinds = (dtype,)
+    query, key = _rows(query, None, d, "query", kinds), _rows(key, None, d, "key", kinds)
+    at, of_key = query.get_device(), key.shape
+    if key.get_device() != at or of_key[0] != T:
         raise ValueError("query and key must have the same rows on one device")
+    k_heads, dev = of_key[1], query.device
     inv_freq, axis, pairs = rope
-    half = inv_freq.numel()
-    if inv_freq.dtype != torch.float64 or axis.dtype != torch.int32 or inv_freq.dim() != 1 or axis.shape != (half,):
-        raise ValueError(f"rope must hold float64 inv_freq [R / 2] and int32 axis [R / 2] (got {inv_freq.dtype} {tuple(inv_freq.shape)}, "
+    of_freq = inv_freq.shape
+    if inv_freq.dtype is not torch.float64 or axis.dtype is not torch.int32 or len(of_freq) != 1 or axis.shape != of_freq:
+        raise ValueError(f"rope must hold float64 inv_freq [R / 2] and int32 axis [R / 2] (got {inv_freq.dtype} {tuple(of_freq)}, "
                          f"{axis.dtype} {tuple(axis.shape)})")
+    half = of_freq[0]
     if 2 * half > d or half % (4 if pairs else 8):
         raise ValueError(f"rope must turn at most {d // 2} pairs, a multiple of {4 if pairs else 8} (got {half})")
-    if positions.dtype not in _POSITIONS or positions.dim() not in (1, 2) or positions.shape[0] != T:
-        raise ValueError(f"positions must be int32, int64 or float32 [{T}, axes] (got {positions.dtype} {tuple(positions.shape)})")
-    if positions.dim() == 1:
-        positions = positions[:, None]
-    axes = positions.shape[1]
+    kind, of_positions = positions.dtype, positions.shape
+    if kind not in _POSITIONS or len(of_positions) not in (1, 2) or of_positions[0] != T:
+        raise ValueError(f"positions must be int32, int64 or float32 [{T}, axes] (got {kind} {tuple(of_positions)})")
+    axes = of_positions[1] if len(of_positions) == 2 else 1
     if not 1 <= axes <= _MOST_AXES:
         raise ValueError(f"positions of 1 to {_MOST_AXES} axes (got {axes})")
-    if positions.device != dev or inv_freq.device != dev or axis.device != dev:
+    if positions.get_device() != at or inv_freq.get_device() != at or axis.get_device() != at:
         raise ValueError(f"positions and rope must be on {dev}")
     positions, inv_freq, axis = positions.contiguous(), inv_freq.contiguous(), axis.contiguous()
-    nq, wq, eps_q = _axes_norm(norm_q, d, dtype, dev, "norm_q")
-    nk, wk, eps_k = _axes_norm(norm_k, d, dtype, dev, "norm_k")
+    nq, wq, eps_q = _axes_norm(norm_q, d, dtype, at, "norm_q")
+    nk, wk, eps_k = _axes_norm(norm_k, d, dtype, at, "norm_k")
     out_q = torch.empty(T, q_heads, d, device=dev, dtype=dtype)
     out_k = torch.empty(T, k_heads, d, device=dev, dtype=dtype)
     with _on(dev):
         _lib.check(_lib.load().vdn_fp8_qk_prep_axes(
             query.data_ptr(), q_heads, _ld(query), key.data_ptr(), k_heads, _ld(key), T, d, _DTYPES[dtype], nq, _ptr(wq), eps_q, nk, _ptr(wk),
-            eps_k, inv_freq.data_ptr(), axis.data_ptr(), 2 * half, int(bool(pairs)), positions.data_ptr(),
-            _POSITIONS[positions.dtype], axes, axes, out_q.data_ptr(), q_heads * d, out_k.data_ptr(), k_heads * d, _stream(query)),
-            "qk_prep_axes")
+            eps_k, inv_freq.data_ptr(), axis.data_ptr(), 2 * half, 1 if pairs else 0, positions.data_ptr(), _POSITIONS[kind], axes, axes,
+            out_q.data_ptr(), q_heads * d, out_k.data_ptr(), k_heads * d, _stream(query)), "qk_prep_axes")
     return out_q, out_k
 
 
