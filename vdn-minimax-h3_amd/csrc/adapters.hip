@@ -24,6 +24,7 @@ namespace {
 constexpr int kLanes = 64;
 constexpr int kTile = 64;         // tokens of a tile: a lane's each
 constexpr int kMostRank = 128;
+constexpr uint32_t kDies = 8;     // of the card, each with an L2 of its own
 constexpr uint32_t kOutside = 0xfffffff0u;   // an offset outside every buffer: reads zero, stores nothing
 
 typedef float f32x4_t __attribute__((ext_vector_type(4)));
@@ -60,17 +61,19 @@ struct AdapterArgs {
     const int32_t* index;      // [T]
     int64_t T;
     int K, N, L, R;
-    float* part;               // [S, T, R]
+    float* part;               // [tiles, S, 64, R]
     int S;                     // parts of h
     int slots;                 // workgroups that the adapters of a tile are dealt out to
     int blocks;                // ranges of k (k_shrink) or of n (k_expand) of a tile
     int span;                  // k of a part (k_shrink), or columns of a workgroup (k_expand)
     int copy;                  // out is not base: tokens without an adapter are copied
+    int once;                  // out is so large that it only passes through the caches
 };
 
+template <int POL = 0>
 __device__ __forceinline__ uint4 load16(__amdgpu_buffer_rsrc_t buffer, uint32_t off)
 {
-    return __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(buffer, off, 0, 0));
+    return __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(buffer, off, 0, POL));
 }
 
 // The adapters of a tile, one after the other, as the masks of their tokens.
@@ -226,7 +229,7 @@ __global__ __launch_bounds__(WK * kLanes) void k_shrink_step(AdapterArgs p)
             for (int t = 0; t < 2; ++t) {
                 const int at = 16 * (f + t) + col;
                 if (at >= count) continue;
-                float* h = p.part + ((int64_t)part * p.T + tile * kTile + list[at]) * p.R + rank + 4 * quad;
+                float* h = p.part + ((tile * p.S + part) * kTile + list[at]) * p.R + rank + 4 * quad;
 #pragma unroll
                 for (int r = 0; r < RF; ++r)
                     if (rank + 16 * r < p.R) *reinterpret_cast<f32x4_t*>(h + 16 * r) = acc[r][t];
@@ -277,7 +280,7 @@ __global__ __launch_bounds__(kWaves * kLanes) void k_shrink_tile(AdapterArgs p)
         auto load = [&](int step) {
             const int k = k0 + step * kBk + 8 * mine;
 #pragma unroll
-            for (int i = 0; i < kEach; ++i) held[i] = load16(16 * i < kTile ? xr : ar, k < end && from[i] != kOutside ? from[i] + 2u * k : kOutside);
+            for (int i = 0; i < kEach; ++i) held[i] = 16 * i < kTile ? load16<2>(xr, k < end && from[i] != kOutside ? from[i] + 2u * k : kOutside) : load16(ar, k < end && from[i] != kOutside ? from[i] + 2u * k : kOutside);
         };
         auto store = [&]() {
 #pragma unroll
@@ -306,7 +309,7 @@ __global__ __launch_bounds__(kWaves * kLanes) void k_shrink_tile(AdapterArgs p)
         }
         const int at = 16 * wave + col;
         if (at < count) {
-            float* h = p.part + ((int64_t)part * p.T + tile * kTile + list[at]) * p.R + 4 * quad;
+            float* h = p.part + ((tile * p.S + part) * kTile + list[at]) * p.R + 4 * quad;
 #pragma unroll
             for (int r = 0; r < RF; ++r) *reinterpret_cast<f32x4_t*>(h + 16 * r) = acc[r];
         }
@@ -376,7 +379,7 @@ __device__ __forceinline__ void split_h(const float (&h)[RK][8], uint4 (&high)[R
 // Part s of the h of a tile's tokens.
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t part_buffer(const AdapterArgs& p, int64_t tile, int s)
 {
-    return row_buffer(p.part + ((int64_t)s * p.T + tile * kTile) * p.R, min(p.T - tile * kTile, (int64_t)kTile) * p.R * 4);
+    return row_buffer(p.part + (tile * p.S + s) * kTile * p.R, (int64_t)kTile * p.R * 4);
 }
 
 // The same of a tile's token (-1: zeros) from memory, its parts added.
@@ -393,19 +396,29 @@ __device__ __forceinline__ void load_h(const AdapterArgs& p, int64_t tile, int t
 #pragma unroll
         for (int e = 0; e < 8; ++e) h[r][e] = 0.0f;
     }
-#pragma unroll 4
-    for (int s = 0; s < p.S; ++s) {
-        const __amdgpu_buffer_rsrc_t part = part_buffer(p, tile, s);
+    // (two parts at a time, all their loads ahead of the first sum)
+    for (int s = 0; s < p.S; s += 2) {
+        const __amdgpu_buffer_rsrc_t part[2] = {part_buffer(p, tile, s), part_buffer(p, tile, s + 1 < p.S ? s + 1 : s)};
+        uint4 v[2][RK][2];
 #pragma unroll
-        for (int r = 0; r < RK; ++r) {
-            const f32x4_t lo = __builtin_bit_cast(f32x4_t, load16(part, from[r]));
-            const f32x4_t hi = __builtin_bit_cast(f32x4_t, load16(part, from[r] != kOutside ? from[r] + 16u : kOutside));
+        for (int i = 0; i < 2; ++i)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                h[r][e] += lo[e];
-                h[r][4 + e] += hi[e];
+            for (int r = 0; r < RK; ++r) {
+                const bool in = from[r] != kOutside && s + i < p.S;
+                v[i][r][0] = load16(part[i], in ? from[r] : kOutside);
+                v[i][r][1] = load16(part[i], in ? from[r] + 16u : kOutside);
             }
-        }
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int r = 0; r < RK; ++r)
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    const f32x4_t u = __builtin_bit_cast(f32x4_t, v[i][r][half]);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) h[r][4 * half + e] += u[e];
+                }
     }
     split_h<TYPE, RK>(h, high, low, up);
 }
@@ -546,6 +559,8 @@ __global__ __launch_bounds__(kWaves * kLanes) void k_expand_step(AdapterArgs p)
 // lines one step ahead: chunk c of row n lies at 17 (n % 8) + n / 8 of the plane of chunk c, the order in which product n % 8 reads it,
 // planes being spaced so that the writes, rows of neighbouring lanes, spread over the banks as well.
 constexpr int kBn = 128;
+// An out of at least this many bytes, the last-level cache's, is stored non-temporally (32760 x 15360: 367 us of k_expand_tile against 394).
+constexpr int64_t kOnceBytes = 256ll << 20;
 
 // h of 16 tokens of a wave, its parts added, rows of neighbouring lanes: binary32, a row padded by a chunk.
 template <int RF>
@@ -561,11 +576,21 @@ __device__ __forceinline__ void gather_h(const AdapterArgs& p, int64_t tile, con
         sum[i] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
         from[i] = row0 + row < count ? ((uint32_t)list[row0 + row] * (uint32_t)p.R + 4u * c) * 4u : kOutside;
     }
-#pragma unroll 2
-    for (int s = 0; s < p.S; ++s) {
-        const __amdgpu_buffer_rsrc_t part = part_buffer(p, tile, s);
+    // (two parts at a time, all their loads ahead of the first sum: left to itself the compiler waits for each, 2 us a part)
+    for (int s = 0; s < p.S; s += 2) {
+        const __amdgpu_buffer_rsrc_t part = part_buffer(p, tile, s), other = part_buffer(p, tile, s + 1 < p.S ? s + 1 : s);
+        uint4 v[2][RF];
 #pragma unroll
-        for (int i = 0; i < RF; ++i) sum[i] += __builtin_bit_cast(f32x4_t, load16(part, from[i]));
+        for (int i = 0; i < RF; ++i) {
+            v[0][i] = load16(part, from[i]);
+            v[1][i] = load16(other, s + 1 < p.S ? from[i] : kOutside);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int i = 0; i < RF; ++i) {
+            sum[i] += __builtin_bit_cast(f32x4_t, v[0][i]);
+            sum[i] += __builtin_bit_cast(f32x4_t, v[1][i]);
+        }
     }
 #pragma unroll
     for (int i = 0; i < RF; ++i) to[(lane + kLanes * i) / kChunks * (kChunks + 1) + (lane + kLanes * i) % kChunks] = sum[i];
@@ -588,8 +613,11 @@ __global__ __launch_bounds__(kWaves * kLanes) void k_expand_tile(AdapterArgs p)
     __shared__ uint4 buffer[kSize];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kLanes);
     const int lane = threadIdx.x & (kLanes - 1), col = lane & 15, quad = lane >> 4;
-    const int64_t tile = blockIdx.x / (uint32_t)p.blocks;
-    const int n0 = (int)(blockIdx.x % (uint32_t)p.blocks) * p.span, end = min(p.N, n0 + p.span);
+    // workgroups go to the eight dies in turn: those of one tile to the same die, whose L2 then reads the tile's h once
+    const uint32_t turn = blockIdx.x / kDies;
+    const int64_t tile = (int64_t)(turn / (uint32_t)p.blocks) * kDies + blockIdx.x % kDies;
+    const int n0 = (int)(turn % (uint32_t)p.blocks) * p.span, end = min(p.N, n0 + p.span);
+    if (tile * kTile >= p.T) return;
     const int steps = (end - n0 + kBn - 1) / kBn;
     int* list = lists[wave];
     const int64_t rows = min(p.T - tile * kTile, (int64_t)kTile);
@@ -627,7 +655,7 @@ __global__ __launch_bounds__(kWaves * kLanes) void k_expand_tile(AdapterArgs p)
         auto load_base = [&](int n) {
             const bool in = n + 8 * col < end;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) base[e] = load16(baser, in && brow[e] != kOutside ? brow[e] + 2u * n : kOutside);
+            for (int e = 0; e < 4; ++e) base[e] = load16<kBufferLoadOnce>(baser, in && brow[e] != kOutside ? brow[e] + 2u * n : kOutside);
         };
         load_b(n0);
         load_base(n0);
@@ -665,19 +693,15 @@ __global__ __launch_bounds__(kWaves * kLanes) void k_expand_tile(AdapterArgs p)
 #pragma unroll
                 for (int f = 0; f < 8; ++f) acc[f] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-                for (int r = 0; r < RK; ++r) {
-                    const bool in = 4 * r + quad < kChunks;   // (constant but for the last product of an odd number of 16 ranks: zeros beside zeros)
-                    uint4 v[8];
+                for (int f = 0; f < 8; ++f)
 #pragma unroll
-                    for (int f = 0; f < 8; ++f) {
-                        v[f] = buffer[(in ? 4 * r + quad : 0) * kPlane + f * 17 + col];
-                        if (RF % 2 && r == RK - 1 && !in) v[f] = make_uint4(0, 0, 0, 0);
+                    for (int r = 0; r < RK; ++r) {
+                        const bool in = 4 * r + quad < kChunks;   // (constant but for the last product of an odd number of 16 ranks: zeros beside zeros)
+                        uint4 v = buffer[(in ? 4 * r + quad : 0) * kPlane + f * 17 + col];
+                        if (RF % 2 && r == RK - 1 && !in) v = make_uint4(0, 0, 0, 0);
+                        acc[f] = Mma<TYPE>::mma(high[r], v, acc[f]);
+                        acc[f] = Mma<TYPE>::mma(low[r], v, acc[f]);
                     }
-#pragma unroll
-                    for (int f = 0; f < 8; ++f) acc[f] = Mma<TYPE>::mma(high[r], v[f], acc[f]);
-#pragma unroll
-                    for (int f = 0; f < 8; ++f) acc[f] = Mma<TYPE>::mma(low[r], v[f], acc[f]);
-                }
                 i32x4_t o[4];
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
@@ -691,9 +715,15 @@ __global__ __launch_bounds__(kWaves * kLanes) void k_expand_tile(AdapterArgs p)
                 }
                 load_base(n + kBn);
                 const bool in = n + 8 * col < end;
+                uint32_t to[4];
 #pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    __builtin_amdgcn_raw_buffer_store_b128(o[e], outr, in && orow[e] != kOutside ? orow[e] + 2u * n : kOutside, 0, 0);
+                for (int e = 0; e < 4; ++e) to[e] = in && orow[e] != kOutside ? orow[e] + 2u * n : kOutside;
+                if (p.once)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) __builtin_amdgcn_raw_buffer_store_b128(o[e], outr, to[e], 0, kBufferLoadOnce);
+                else
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) __builtin_amdgcn_raw_buffer_store_b128(o[e], outr, to[e], 0, 0);
                 settle_stores();
             }
             __syncthreads();
@@ -719,7 +749,6 @@ __global__ __launch_bounds__(kWaves * kLanes) void k_expand_tile(AdapterArgs p)
 constexpr int kFewWaves = 16, kFewColumns = 512;
 constexpr int kFewRank = 64, kFewK = 7168;              // (LDS: 8 tokens' x and 512 rows of B of 32 ranks, or 4 tokens' and 64)
 constexpr int few_tokens(int rank_frags) { return rank_frags <= 2 ? 8 : 4; }
-constexpr uint32_t kDies = 8;
 
 // acc + the products of eight elements.
 template <int TYPE>
@@ -924,11 +953,12 @@ Plan plan_of(int64_t T, int64_t K, int64_t N, int64_t L, int64_t R)
         p.rank_frags = (int)(R / 16);
         // workgroups to fill the card, and two (k) or four (n) of each tile even so: a workgroup's first steps wait for memory
         int64_t parts = ceil_div(kFill, p.tiles), blocks = kFill / p.tiles;
+        const int64_t eighths = ceil_div(columns, 8);
         if (parts < 2) parts = 2;
         if (parts > ceil_div(steps, 4)) parts = ceil_div(steps, 4);
         p.span_k = (int)(kBk * ceil_div(steps, parts));
         p.parts = (int)ceil_div(K, p.span_k);
-        if (blocks < 4) blocks = 4;
+        if (blocks < eighths) blocks = eighths;
         if (blocks > columns) blocks = columns;
         p.span_n = (int)(kBn * ceil_div(columns, blocks));
         // (a tile that holds the border between two requests takes twice as long: where few tiles are, its adapters go apart)
@@ -961,7 +991,8 @@ int launch_shrink(const AdapterArgs& p, const Plan& plan, hipStream_t stream)
 template <int TYPE, int RF>
 int launch_expand(const AdapterArgs& p, const Plan& plan, hipStream_t stream)
 {
-    const dim3 block(kWaves * kLanes), grid((unsigned)(plan.tiles * plan.expand_blocks * (plan.step ? plan.slots : 1)), (unsigned)(plan.step ? 1 : plan.slots));
+    const dim3 block(kWaves * kLanes), grid((unsigned)(plan.step ? plan.tiles * plan.expand_blocks * plan.slots : ceil_div(plan.tiles, kDies) * kDies * plan.expand_blocks),
+                                            (unsigned)(plan.step ? 1 : plan.slots));
     if (plan.step) hipLaunchKernelGGL((k_expand_step<TYPE, (RF + 1) / 2>), grid, block, 0, stream, p);
     else hipLaunchKernelGGL((k_expand_tile<TYPE, RF>), grid, block, 0, stream, p);
     return check_launch("adapter_add");
@@ -1008,6 +1039,9 @@ int launch(AdapterArgs p, const Plan& plan, hipStream_t stream)
     }
 }
 
+// h's parts, tile by tile: those that a workgroup adds lie next to each other.
+int64_t workspace_bytes_of(const Plan& plan, int64_t R) { return plan.tiles * plan.parts * kTile * R * 4; }
+
 int check_sizes(int64_t T, int64_t K, int64_t N, int64_t L, int64_t R)
 {
     const char* what = "adapter_add";
@@ -1028,7 +1062,7 @@ extern "C" int vdn_fp8_adapter_add_workspace_size(int64_t T, int64_t K, int64_t 
     if (!bytes) return set_error(VDN_FP8_EINVAL, "adapter_add: null pointer");
     const int st = check_sizes(T, K, N, L, R);
     if (st != VDN_FP8_OK) return st;
-    *bytes = T && L ? plan_of(T, K, N, L, R).parts * T * R * 4 : 0;
+    *bytes = T && L ? workspace_bytes_of(plan_of(T, K, N, L, R), R) : 0;
     return VDN_FP8_OK;
 }
 
@@ -1047,8 +1081,9 @@ extern "C" int vdn_fp8_adapter_add(const void* x, int dtype, int64_t ldx, const 
     if (!aligned(x, 16) || !aligned(base, 16) || !aligned(out, 16) || !aligned(a, 16) || !aligned(b, 16) || !aligned(scale, 4) || !aligned(index, 4))
         return set_error(VDN_FP8_EINVAL, "%s: misaligned pointer (x, base, out, A, B 16 B)", what);
     const Plan plan = plan_of(T, K, N, L ? L : 1, R);
-    if (plan.parts && L && (!workspace || !aligned(workspace, 16) || workspace_bytes < plan.parts * T * R * 4))
-        return set_error(VDN_FP8_EINVAL, "%s: the workspace must be 16-byte aligned and hold %lld bytes", what, (long long)(plan.parts * T * R * 4));
+    const int64_t need = L ? workspace_bytes_of(plan, R) : 0;
+    if (need && (!workspace || !aligned(workspace, 16) || workspace_bytes < need))
+        return set_error(VDN_FP8_EINVAL, "%s: the workspace must be 16-byte aligned and hold %lld bytes", what, (long long)need);
     AdapterArgs p{};
     p.x = (const uint8_t*)x; p.ldx = ldx;
     p.base = (const uint8_t*)base; p.ldbase = ldbase;
@@ -1058,5 +1093,6 @@ extern "C" int vdn_fp8_adapter_add(const void* x, int dtype, int64_t ldx, const 
     p.T = T; p.K = (int)K; p.N = (int)N; p.L = (int)L; p.R = (int)R;
     p.part = (float*)workspace;
     p.copy = out != base;
+    p.once = T * N * 2 >= kOnceBytes;
     return dtype == kBf16 ? launch<kBf16>(p, plan, stream) : launch<kF16>(p, plan, stream);
 }
