@@ -2,7 +2,7 @@
 // projection's input, in one pass over the rows:
 //   h[k]    = S(fma(g[i][k], b[k], r[k]))                (r[k] + b[k] without a gate; S the stream's type)
 //   rstd    = 1 / sqrt(sum_k h[k]^2 / K + eps)           (binary32)
-//   n[k]    = fma(h[k] * rstd, w[k] (1 + sc[i][k]), sh[i][k])      ((h rstd) w without a table)
+//   n[k]    = fma(h[k] * rstd, w[k] (1 + sc[i][k]), sh[i][k])
 //   scale   = max(max_k |n[k]| / 448, 1e-12),  code[k] = e4m3(n[k] / scale),  normed[k] = B(n[k])
 // with i = index[row], clamped into the tables. The stream is rounded where it is stored, and the
 // stored row is the one that is normed, as if a later call read it. n is not rounded before the
@@ -17,6 +17,8 @@ namespace vdn {
 namespace {
 
 constexpr int kLanes = 64;
+constexpr int kMostWaves = 16;   // of a workgroup
+constexpr int64_t kFewRows = 512; // one chunk a thread up to here
 
 struct AddNormArgs {
     const void* residual;
@@ -42,34 +44,50 @@ struct AddNormArgs {
     int64_t ldn;
 };
 
-// A value's code from its scale s and r = RN(1 / s); EXACT: the IEEE quotient, for scales that are not finite.
+// Codes of eight values: times R + R_low = 1 / scale before the scale's rounding, with the product's remainder, so that a quotient
+// is rounded once; the codes that n's own rounding moves are those of values at a border between two. EXACT: the IEEE quotient, for scales
+// that are not finite.
 template <bool EXACT>
-__device__ __forceinline__ uint2 codes8(const float (&n)[8], float s, float r)
+__device__ __forceinline__ uint2 codes8(const float (&n)[8], float scale, float R, float R_low)
 {
     float q[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) q[e] = EXACT ? n[e] / s : div_by_scale(n[e], s, r);
+    for (int e = 0; e < 8; ++e) {
+        if (EXACT) {
+            q[e] = n[e] / scale;
+        } else {
+            const float q0 = n[e] * R;
+            q[e] = q0 + __builtin_fmaf(n[e], R_low, __builtin_fmaf(n[e], R, -q0));
+        }
+    }
     return make_uint2(pack_e4m3x4(q[0], q[1], q[2], q[3]), pack_e4m3x4(q[4], q[5], q[6], q[7]));
 }
 
-// A workgroup of WPR waves per row: wave w holds chunks 64 w + lane + 64 WPR c of it, as binary32 in
-// registers from the addition to the codes; the partial sums of squares and the maxima meet in LDS.
-// S, B: the types of the stream, and of the branch and its parameters.
-template <int S, int B, int WPR, int CPL>
-__global__ __launch_bounds__(WPR * kLanes) void k_add_norm(AddNormArgs p, int64_t first)
+// Streams of at least this many bytes are stored non-temporally: they only pass through the last-level cache.
+constexpr int64_t kOnceBytes = 256ll << 20;
+
+// A workgroup per row, of as many waves as its chunks fill: thread t holds chunk t, or t and t + threads, as binary32 in
+// registers from the addition to the codes, and the partial sums of squares and the maxima meet in LDS. One chunk a thread makes a row short
+// for the few of a step (16 of 5120: 4.3 us on the card); two halve what every wave does once, which costs time where there are
+// many (32760 of 5376, gated and modulated: 226 us and 5.5 TB/s, where one takes 239 and three 231). All loads go out
+// before the first of them is used, the tables' as soon as the row's index is there; a table that is absent is a
+// descriptor of no bytes, which reads zeros. S, B: the types of the stream, and of the branch and its parameters.
+template <int S, int B, int CPL, bool ONCE>
+__global__ __launch_bounds__(kMostWaves * kLanes) void k_add_norm(AddNormArgs p, int waves, int64_t first)
 {
-    __shared__ float ssum[WPR];
-    __shared__ uint32_t smax[WPR];
+    __shared__ float ssum[kMostWaves];
+    __shared__ uint32_t smax[kMostWaves];
     const int64_t row = first + blockIdx.x;
     const int lane = threadIdx.x & (kLanes - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kLanes);
     const int nch = (int)(p.K >> 3);
     const int64_t sbytes = p.K * element_bytes(S), bbytes = p.K * element_bytes(B);
-    auto chunk = [&](int c) { return (uint32_t)(wave * kLanes + lane + kLanes * WPR * c); };
+    auto chunk = [&](int c) { return (uint32_t)threadIdx.x + (uint32_t)(kLanes * waves * c); };
+    auto table = [&](const void* t, int64_t at) { return row_buffer(t ? (const uint8_t*)t + at * element_bytes(B) : (const uint8_t*)p.branch, t ? bbytes : 0); };
 
     const __amdgpu_buffer_rsrc_t rr = row_buffer((const uint8_t*)p.residual + row * p.ldr * element_bytes(S), sbytes);
     const __amdgpu_buffer_rsrc_t br = row_buffer((const uint8_t*)p.branch + row * p.ldb * element_bytes(B), bbytes);
     Eight<S> r[CPL];
-    Eight<B> b[CPL], g[CPL];
+    Eight<B> b[CPL], g[CPL], w[CPL], sc[CPL], sh[CPL];
 #pragma unroll
     for (int c = 0; c < CPL; ++c) {
         r[c] = load8<S, kBufferLoadOnce>(rr, chunk(c));
@@ -77,80 +95,77 @@ __global__ __launch_bounds__(WPR * kLanes) void k_add_norm(AddNormArgs p, int64_
     }
     int64_t ti = 0;
     if (p.index) ti = min(max((int64_t)p.index[row], (int64_t)0), p.rows - 1);
-    if (p.gate) {
-        const __amdgpu_buffer_rsrc_t gr = row_buffer((const uint8_t*)p.gate + ti * p.ldgate * element_bytes(B), bbytes);
+    const __amdgpu_buffer_rsrc_t gr = table(p.gate, ti * p.ldgate), wr = table(p.weight, 0), scr = table(p.scale, ti * p.ldmod),
+                                 shr = table(p.shift, ti * p.ldmod);
 #pragma unroll
-        for (int c = 0; c < CPL; ++c) g[c] = load8<B, 0>(gr, chunk(c));
+    for (int c = 0; c < CPL; ++c) {
+        g[c] = load8<B, 0>(gr, chunk(c));
+        w[c] = load8<B, 0>(wr, chunk(c));
     }
+#pragma unroll
+    for (int c = 0; c < CPL; ++c) {
+        sc[c] = load8<B, 0>(scr, chunk(c));
+        sh[c] = load8<B, 0>(shr, chunk(c));
+    }
+    __builtin_amdgcn_sched_barrier(0);
 
     const __amdgpu_buffer_rsrc_t hr = row_buffer((uint8_t*)p.hidden + row * p.ldh * element_bytes(S), sbytes);
     float n[CPL][8], ss = 0.0f;
 #pragma unroll
     for (int c = 0; c < CPL; ++c) {
-        float x[8], y[8];
+        float x[8], y[8], f[8];
         decode8<S>(r[c], x);
         decode8<B>(b[c], y);
-        if (p.gate) {
-            float f[8];
-            decode8<B>(g[c], f);
+        decode8<B>(g[c], f);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) x[e] = __builtin_fmaf(f[e], y[e], x[e]);
-        } else {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) x[e] += y[e];
+        for (int e = 0; e < 8; ++e) {
+            x[e] = __builtin_fmaf(p.gate ? f[e] : 1.0f, y[e], x[e]);
+            if (S == kF16) asm volatile("" : "+v"(x[e]));   // a binary32 value first, not one fma that rounds to binary16
         }
         const Eight<S> h = encode8<S>(x);
-        store8<S, 0>(h, hr, chunk(c));
+        store8<S, ONCE ? kBufferLoadOnce : 0>(h, hr, chunk(c));
         decode8<S>(h, n[c]);
 #pragma unroll
         for (int e = 0; e < 8; ++e) ss = __builtin_fmaf(n[c][e], n[c][e], ss);
     }
     ss = wave_sum_f32(ss);
-    if (WPR > 1) {
-        if (lane == 0) ssum[wave] = ss;
-        __syncthreads();
-        ss = ssum[0];
-#pragma unroll
-        for (int w = 1; w < WPR; ++w) ss += ssum[w];
-    }
+    // (a lane of each 16 takes a wave's, and the 16 add them up by exchanges)
+    if (lane == 0) ssum[wave] = ss;
+    __syncthreads();
+    ss = lane % kMostWaves < waves ? ssum[lane % kMostWaves] : 0.0f;
+    ss += __uint_as_float(dpp_u32<kDppXor1>(__float_as_uint(ss)));
+    ss += __uint_as_float(dpp_u32<kDppXor2>(__float_as_uint(ss)));
+    ss += __uint_as_float(dpp_u32<kDppHalfMirror>(__float_as_uint(ss)));
+    ss += __uint_as_float(dpp_u32<kDppMirror>(__float_as_uint(ss)));
     const float rstd = 1.0f / __builtin_sqrtf(ss / (float)p.K + p.eps);
 
-    const __amdgpu_buffer_rsrc_t wr = row_buffer(p.weight ? p.weight : p.branch, p.weight ? bbytes : 0);
-    const __amdgpu_buffer_rsrc_t scr = row_buffer(p.scale ? (const uint8_t*)p.scale + ti * p.ldmod * element_bytes(B) : p.branch, p.scale ? bbytes : 0);
-    const __amdgpu_buffer_rsrc_t shr = row_buffer(p.shift ? (const uint8_t*)p.shift + ti * p.ldmod * element_bytes(B) : p.branch, p.shift ? bbytes : 0);
     float top = 0.0f;
 #pragma unroll
     for (int c = 0; c < CPL; ++c) {
-        float w[8];
-        decode8<B>(load8<B, 0>(wr, chunk(c)), w);
-        if (!p.weight)
-#pragma unroll
-            for (int e = 0; e < 8; ++e) w[e] = 1.0f;
-        if (p.scale) {
-            float sc[8], sh[8];
-            decode8<B>(load8<B, 0>(scr, chunk(c)), sc);
-            decode8<B>(load8<B, 0>(shr, chunk(c)), sh);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) n[c][e] = __builtin_fmaf(n[c][e] * rstd, w[e] * (1.0f + sc[e]), sh[e]);
-        } else {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) n[c][e] = (n[c][e] * rstd) * w[e];
-        }
+        float f[8], u[8], v[8];
+        decode8<B>(w[c], f);
+        decode8<B>(sc[c], u);
+        decode8<B>(sh[c], v);
         float most = 0.0f;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) most = __builtin_elementwise_maximum(most, __builtin_fabsf(n[c][e]));
+        for (int e = 0; e < 8; ++e) {
+            // h rstd f + shift, f = w (1 + scale); absent factors are 1, an absent shift 0
+            const float factor = (p.weight ? f[e] : 1.0f) * (1.0f + u[e]), t = n[c][e] * rstd;
+            n[c][e] = __builtin_fmaf(t, factor, v[e]);
+            most = __builtin_elementwise_maximum(most, __builtin_fabsf(n[c][e]));
+        }
         if (chunk(c) < (uint32_t)nch) top = __builtin_elementwise_maximum(top, most);   // (0 times an infinite rstd, past the row)
     }
     uint32_t bits = wave_max_u32(__float_as_uint(top) & 0x7fffffffu);
-    if (WPR > 1) {
-        if (lane == 0) smax[wave] = bits;
-        __syncthreads();
-#pragma unroll
-        for (int w = 0; w < WPR; ++w) bits = max(bits, smax[w]);
-    }
-    const float scale = row_scale(__uint_as_float(bits));
+    if (lane == 0) smax[wave] = bits;
+    __syncthreads();
+    bits = wave_max_u32(lane % kMostWaves < waves ? smax[lane % kMostWaves] : 0u);
+    const float most = __uint_as_float(bits), scale = row_scale(most);
     if (threadIdx.x == 0) p.y_scale[row] = scale;
-    const float inverse = 1.0f / scale;
+    // 1 / scale in two parts: 448 / most, or 1 / scale at the floor
+    const bool floor = most / 448.0f < 1e-12f;
+    const float over = floor ? 1.0f : 448.0f, under = floor ? scale : most;
+    const float R = over / under, R_low = __builtin_fmaf(-R, under, over) / under;
     const bool finite = __builtin_isfinite(scale);
     const __amdgpu_buffer_rsrc_t yr = row_buffer(p.y + row * p.ldy, p.K);
     const __amdgpu_buffer_rsrc_t nr = row_buffer(p.normed ? (uint8_t*)p.normed + row * p.ldn * element_bytes(B) : p.y, p.normed ? bbytes : 0);
@@ -158,7 +173,7 @@ __global__ __launch_bounds__(WPR * kLanes) void k_add_norm(AddNormArgs p, int64_
 #pragma unroll
     for (int c = 0; c < CPL; ++c) {
         if (p.normed) store8<B, 0>(encode8<B>(n[c]), nr, chunk(c));
-        const uint2 q = finite ? codes8<false>(n[c], scale, inverse) : codes8<true>(n[c], scale, inverse);
+        const uint2 q = finite ? codes8<false>(n[c], scale, R, R_low) : codes8<true>(n[c], scale, R, R_low);
         __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(i32x2_t, q), yr, chunk(c) * 8u, 0, 0);
     }
 }
@@ -167,18 +182,18 @@ template <int S, int B>
 int launch(const AddNormArgs& p, hipStream_t stream)
 {
     const int64_t nch = p.K / 8;
+    const bool once = p.M * p.K * element_bytes(S) >= kOnceBytes;
     return in_slabs(p.M, kLaunchRows / 4, [&](int64_t m, int64_t rows) {
         // (a workgroup has 1024 threads at most, and a launch fewer than 2^32 work-items)
-#define VDN_CASE(w, n)                                                                                             \
-        if (nch <= (int64_t)w * n * kLanes) {                                                                      \
-            hipLaunchKernelGGL((k_add_norm<S, B, w, n>), dim3((unsigned)rows), dim3(w * kLanes), 0, stream, p, m); \
-            return check_launch("add_norm_quantize");                                                              \
-        }
-        VDN_CASE(1, 1) VDN_CASE(1, 2)
-        if (p.M <= 512) { VDN_CASE(4, 1) VDN_CASE(8, 1) VDN_CASE(16, 1) VDN_CASE(16, 2) }
-        VDN_CASE(4, 1) VDN_CASE(4, 2) VDN_CASE(4, 3) VDN_CASE(4, 4) VDN_CASE(4, 6) VDN_CASE(4, 8)
-#undef VDN_CASE
-        return set_error(VDN_FP8_EINVAL, "add_norm_quantize: unsupported K");
+        const bool two = nch > kMostWaves * kLanes || (nch > 256 && p.M > kFewRows);
+        const int waves = (int)((nch + kLanes * (two ? 2 : 1) - 1) / (kLanes * (two ? 2 : 1)));
+#define VDN_LAUNCH(n, o) hipLaunchKernelGGL((k_add_norm<S, B, n, o>), dim3((unsigned)rows), dim3(waves * kLanes), 0, stream, p, waves, m)
+        if (two && once) VDN_LAUNCH(2, true);
+        else if (two) VDN_LAUNCH(2, false);
+        else if (once) VDN_LAUNCH(1, true);
+        else VDN_LAUNCH(1, false);
+#undef VDN_LAUNCH
+        return check_launch("add_norm_quantize");
     });
 }
 
