@@ -14,10 +14,11 @@
 // formed in binary64, the nearest whole number is taken off by an exact fma, and a quarter turn's remainder,
 // |g| <= pi / 4, goes to binary32, where Taylor's series to g^9 and g^10 have errors below 2^-28.
 //
-// Layout. A wave takes a token's chunks (eight elements a lane) of q or of k; a head is d / 8 consecutive
-// lanes, as in k_qk_prep. The lanes first compute one angle each (R / 2 <= 128 of them), leave cosine and sine
-// in the wave's own LDS, and read those of their chunk from there: an angle costs its wave about 60
-// operations once, and not once for each of the lanes that need it.
+// Layout. Chunks are eight elements, a lane's; a head is d / 8 consecutive lanes, as in k_qk_prep; a slot is 64 chunks of q or of k
+// of a token, and a wave takes up to CPL slots of one token, the last of q and the first of k among them. Its lanes first compute one angle
+// each (R / 2 <= 128 of them), leave cosine and sine in the wave's own LDS, and read those of their chunks from there: an angle costs
+// its wave about 60 operations once, and not once for each of the lanes that need it. The little that the angles need is fetched ahead of
+// the slots (loads come back in order), so that they are ready when those are.
 #include <stdint.h>
 
 #include "eight.h"
@@ -35,7 +36,7 @@ constexpr int kMostPairs = 128;      // R / 2 at d = 256
 struct RopeSide {
     const void* x;        // [T, heads, d], row stride ld
     int64_t ld;
-    int heads, spans;     // spans: waves that share a token
+    int heads, slots;
     int norm;
     const void* weight;   // [d] or NULL
     float eps;
@@ -52,6 +53,8 @@ struct RopeArgs {
     const void* positions;    // [T, axes]
     int64_t ldpos;
     int axes, position_type;
+    int spans, per;           // waves of a token, and slots of a wave
+    int once;                 // the outputs only pass through the last-level cache
 };
 
 __device__ __forceinline__ double position_at(const RopeArgs& p, int64_t at)
@@ -79,47 +82,68 @@ __device__ __forceinline__ void turn(double p, double f, float& cosine, float& s
     sine = q & 2 ? -b : b;
 }
 
-// G = d / 8 lanes of a head; CPL chunks a lane; PAIRS: which elements a pair is.
-template <int TYPE, int G, int CPL, bool PAIRS, bool NT>
+// G = d / 8 lanes of a head; CPL slots a wave at most; PAIRS: which elements a pair is.
+template <int TYPE, int G, int CPL, bool PAIRS>
 __global__ __launch_bounds__(kWaves * kLanes) void k_rope_axes(RopeArgs p, int64_t first_token)
 {
     __shared__ float turned[kWaves][2][kMostPairs];
     const int lane = threadIdx.x & (kLanes - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kLanes);
-    const int spans = p.side[0].spans + p.side[1].spans;
     const uint32_t unit = blockIdx.x * kWaves + wave;
-    const int64_t t = first_token + unit / (uint32_t)spans;
+    const int64_t t = first_token + unit / (uint32_t)p.spans;
     if (t >= p.T) return;
-    const int place = (int)(unit % (uint32_t)spans);
-    const bool is_key = place >= p.side[0].spans;
-    const RopeSide s = is_key ? p.side[1] : p.side[0];
-    const int base = (place - (is_key ? p.side[0].spans : 0)) * kLanes * CPL;   // first chunk: whole heads, 64 being a multiple of G
-    const int nch = s.heads * G;
-    const int j = lane % G, i0 = 8 * j;
+    const int first_slot = (int)(unit % (uint32_t)p.spans) * p.per, slots = min(p.side[0].slots + p.side[1].slots - first_slot, p.per);
+    const int j = lane % G, i0 = 8 * j, half = p.R / 2;
+    const int esize = element_bytes(TYPE);
 
-    const __amdgpu_buffer_rsrc_t xr = row_buffer((const uint8_t*)s.x + t * s.ld * element_bytes(TYPE), (int64_t)nch * 8 * element_bytes(TYPE));
-    Eight<TYPE> v[CPL];
-#pragma unroll
-    for (int c = 0; c < CPL; ++c) v[c] = load8<TYPE, kBufferLoadOnce>(xr, (uint32_t)(base + lane + kLanes * c));
-    const __amdgpu_buffer_rsrc_t wr = row_buffer(s.weight ? s.weight : s.x, s.weight ? p.d * element_bytes(TYPE) : 0);
-    const Eight<TYPE> raw_weight = load8<TYPE, 0>(wr, (uint32_t)j);
-
-    const int half = p.R / 2;
+    // what the angles need, then the weights, then the slots
+    const int a0 = min(lane, half - 1), a1 = min(lane + kLanes, half - 1);   // (-1 without any)
     const double mine = lane < p.axes ? position_at(p, t * p.ldpos + lane) : 0.0;
-    for (int a = lane; a < (half + kLanes - 1) / kLanes * kLanes; a += kLanes) {
-        const bool real = a < half;
-        const int axis = real ? min(max(p.axis[a], 0), p.axes - 1) : 0;
-        const double f = real ? p.inv_freq[a] * 0.15915494309189533577 : 0.0;
-        const double at = __shfl(mine, axis, kLanes);
-        float c, sn;
-        turn(at, f, c, sn);
-        if (real) {
-            turned[wave][0][a] = c;
-            turned[wave][1][a] = sn;
+    int axis[2] = {0, 0};
+    double f[2] = {0.0, 0.0};
+    if (half > 0) {
+        axis[0] = p.axis[a0];
+        f[0] = p.inv_freq[a0];
+        if (half > kLanes) {
+            axis[1] = p.axis[a1];
+            f[1] = p.inv_freq[a1];
         }
     }
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    Eight<TYPE> raw_weight[2];
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+        const void* w = p.side[s].weight;
+        raw_weight[s] = load8<TYPE, 0>(row_buffer(w ? w : (const void*)p.positions, w ? p.d * esize : 0), (uint32_t)j);
+    }
+    // slot c of the wave: its side, its row and this lane's chunk of it
+    auto is_key = [&](int c) { return first_slot + c >= p.side[0].slots; };
+    auto chunk = [&](int c) { return (uint32_t)((first_slot + c - (is_key(c) ? p.side[0].slots : 0)) * kLanes + lane); };
+    auto row = [&](int c, const void* x0, int64_t ld0, const void* x1, int64_t ld1) {
+        const bool key = is_key(c);
+        const int64_t bytes = (int64_t)(key ? p.side[1].heads : p.side[0].heads) * p.d * esize;
+        return row_buffer((const uint8_t*)(key ? x1 : x0) + t * (key ? ld1 : ld0) * esize, c < slots ? bytes : 0);
+    };
+    Eight<TYPE> v[CPL];
+#pragma unroll
+    for (int c = 0; c < CPL; ++c) v[c] = load8<TYPE, kBufferLoadOnce>(row(c, p.side[0].x, p.side[0].ld, p.side[1].x, p.side[1].ld), chunk(c));
+    __builtin_amdgcn_sched_barrier(0);
+
+    if (half > 0) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int a = lane + kLanes * i;
+            if (kLanes * i < half) {
+                float c, s;
+                turn(__shfl(mine, min(max(axis[i], 0), p.axes - 1), kLanes), f[i] * 0.15915494309189533577, c, s);
+                if (a < half) {
+                    turned[wave][0][a] = c;
+                    turned[wave][1][a] = s;
+                }
+            }
+        }
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    }
 
     const bool rot = i0 < p.R;
     const bool first = i0 < half;                                     // (halves)
@@ -131,22 +155,20 @@ __global__ __launch_bounds__(kWaves * kLanes) void k_rope_axes(RopeArgs p, int64
         cs[e] = rot ? turned[wave][0][pair] : 1.0f;
         sn[e] = rot ? turned[wave][1][pair] : 0.0f;
     }
-    float w[8];
-    decode8<TYPE>(raw_weight, w);
-    if (!s.weight)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) w[e] = 1.0f;
-
-    const __amdgpu_buffer_rsrc_t outr = row_buffer((uint8_t*)s.out + t * s.ldo * element_bytes(TYPE), (int64_t)nch * 8 * element_bytes(TYPE));
 #pragma unroll
     for (int c = 0; c < CPL; ++c) {
+        if (c >= slots) break;
+        const bool key = is_key(c);
         float n[8], o[8];
         decode8<TYPE>(v[c], n);
-        if (s.norm) {
+        if (key ? p.side[1].norm : p.side[0].norm) {
+            float w[8];
+            decode8<TYPE>(key ? raw_weight[1] : raw_weight[0], w);
+            const bool weight = key ? p.side[1].weight != nullptr : p.side[0].weight != nullptr;
             const float ss = head_sum_squares<G>(n);
-            const float rstd = 1.0f / __builtin_sqrtf(ss / (float)p.d + s.eps);
+            const float rstd = 1.0f / __builtin_sqrtf(ss / (float)p.d + (key ? p.side[1].eps : p.side[0].eps));
 #pragma unroll
-            for (int e = 0; e < 8; ++e) n[e] = (n[e] * rstd) * w[e];
+            for (int e = 0; e < 8; ++e) n[e] = (n[e] * rstd) * (weight ? w[e] : 1.0f);
         }
         if (PAIRS) {
 #pragma unroll
@@ -157,27 +179,36 @@ __global__ __launch_bounds__(kWaves * kLanes) void k_rope_axes(RopeArgs p, int64
         } else {
             rotate8<G>(n, cs, sn, p.R == p.d, rot, first, partner, lane, o);
         }
-        store8<TYPE, NT ? kBufferLoadOnce : 0>(encode8<TYPE>(o), outr, (uint32_t)(base + lane + kLanes * c));
+        const __amdgpu_buffer_rsrc_t outr = row(c, p.side[0].out, p.side[0].ldo, p.side[1].out, p.side[1].ldo);
+        if (p.once) store8<TYPE, kBufferLoadOnce>(encode8<TYPE>(o), outr, chunk(c));
+        else store8<TYPE, 0>(encode8<TYPE>(o), outr, chunk(c));
     }
 }
 
 // Outputs of at least this many bytes are stored non-temporally: beyond what the last-level cache holds,
 // cached stores only evict each other.
-constexpr int64_t kNtStoreBytes = 256ll << 20;
+constexpr int64_t kOnceBytes = 256ll << 20;
+constexpr int64_t kFewTokens = 1024;   // a slot a wave below this
 
-template <int TYPE, int G, int CPL, bool PAIRS>
-int launch_cpl(RopeArgs p, hipStream_t stream)
+template <int TYPE, int G, bool PAIRS>
+int launch(RopeArgs p, hipStream_t stream)
 {
-    for (RopeSide& s : p.side) s.spans = (s.heads * G + kLanes * CPL - 1) / (kLanes * CPL);
-    const int64_t spans = p.side[0].spans + p.side[1].spans;
-    const bool nt = p.T * (p.side[0].heads + p.side[1].heads) * p.d * element_bytes(TYPE) >= kNtStoreBytes;
-    const int64_t slab = kLaunchRows * kWaves / spans;   // tokens of a launch
-    return in_slabs(p.T, slab, [&](int64_t t, int64_t tokens) {
-        const dim3 grid((unsigned)((tokens * spans + kWaves - 1) / kWaves)), block(kWaves * kLanes);
-        RopeArgs q = p;
-        q.T = t + tokens;
-        if (nt) hipLaunchKernelGGL((k_rope_axes<TYPE, G, CPL, PAIRS, true>), grid, block, 0, stream, q, t);
-        else hipLaunchKernelGGL((k_rope_axes<TYPE, G, CPL, PAIRS, false>), grid, block, 0, stream, q, t);
+    int slots = 0;
+    for (RopeSide& s : p.side) slots += s.slots = (s.heads * G + kLanes - 1) / kLanes;
+    // up to six slots a wave, alike
+    const int most = p.T < kFewTokens ? 1 : 6;
+    p.spans = (slots + most - 1) / most;
+    p.per = (slots + p.spans - 1) / p.spans;
+    p.spans = (slots + p.per - 1) / p.per;
+    p.once = p.T * (p.side[0].heads + p.side[1].heads) * p.d * element_bytes(TYPE) >= kOnceBytes;
+    const int64_t slab = kLaunchRows * kWaves / p.spans, T = p.T;   // tokens of a launch
+    return in_slabs(T, slab, [&](int64_t t, int64_t tokens) {
+        const dim3 grid((unsigned)((tokens * p.spans + kWaves - 1) / kWaves)), block(kWaves * kLanes);
+        p.T = t + tokens;
+        if (p.per <= 1) hipLaunchKernelGGL((k_rope_axes<TYPE, G, 1, PAIRS>), grid, block, 0, stream, p, t);
+        else if (p.per <= 2) hipLaunchKernelGGL((k_rope_axes<TYPE, G, 2, PAIRS>), grid, block, 0, stream, p, t);
+        else if (p.per <= 4) hipLaunchKernelGGL((k_rope_axes<TYPE, G, 4, PAIRS>), grid, block, 0, stream, p, t);
+        else hipLaunchKernelGGL((k_rope_axes<TYPE, G, 6, PAIRS>), grid, block, 0, stream, p, t);
         return check_launch("qk_prep_axes");
     });
 }
@@ -185,9 +216,7 @@ int launch_cpl(RopeArgs p, hipStream_t stream)
 template <int TYPE, int G>
 int launch(const RopeArgs& p, bool pairs, hipStream_t stream)
 {
-    const bool many = p.T >= 1024;
-    if (pairs) return many ? launch_cpl<TYPE, G, 5, true>(p, stream) : launch_cpl<TYPE, G, 1, true>(p, stream);
-    return many ? launch_cpl<TYPE, G, 5, false>(p, stream) : launch_cpl<TYPE, G, 1, false>(p, stream);
+    return pairs ? launch<TYPE, G, true>(p, stream) : launch<TYPE, G, false>(p, stream);
 }
 
 template <int TYPE>
@@ -232,7 +261,7 @@ extern "C" int vdn_fp8_qk_prep_axes(const void* query, int64_t q_heads, int64_t 
     if (!aligned(weight_q, 16) || !aligned(weight_k, 16)) return set_error(VDN_FP8_EINVAL, "%s: misaligned pointer (weights 16 B)", what);
     const RopeArgs p{{{query, ldq, (int)q_heads, 0, norm_q != 0, weight_q, eps_q, out_q, ldoq},
                       {key, ldk, (int)k_heads, 0, norm_k != 0, weight_k, eps_k, out_k, ldok}},
-                     T, (int)d, (int)rotary_dim, inv_freq, axis, positions, ldpos, rotary_dim > 0 ? (int)axes : 0, position_type};
+                     T, (int)d, (int)rotary_dim, inv_freq, axis, positions, ldpos, rotary_dim > 0 ? (int)axes : 0, position_type, 0, 0, 0};
     return dtype == kBf16 ? launch_type<kBf16>(p, pairs != 0, stream)
          : dtype == kF16  ? launch_type<kF16>(p, pairs != 0, stream)
                           : launch_type<kF32>(p, pairs != 0, stream);
