@@ -44,35 +44,41 @@ struct AddNormArgs {
     int64_t ldn;
 };
 
-// Codes of eight values: times R + R_low = 1 / scale before the scale's rounding, with the product's remainder, so that a quotient
-// is rounded once; the codes that n's own rounding moves are those of values at a border between two. EXACT: the IEEE quotient, for scales
-// that are not finite.
+// Codes of eight values n + low: (n + low) (R + R_low), R + R_low = 1 / scale before the scale's rounding; the
+// product and its corrections are rounded once. EXACT: the IEEE quotient, for scales that are not finite.
 template <bool EXACT>
-__device__ __forceinline__ uint2 codes8(const float (&n)[8], float scale, float R, float R_low)
+__device__ __forceinline__ uint2 codes8(const float (&n)[8], const float (&low)[8], float scale, float R, float R_low)
 {
     float q[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        if (EXACT) {
-            q[e] = n[e] / scale;
-        } else {
-            const float q0 = n[e] * R;
-            q[e] = q0 + __builtin_fmaf(n[e], R_low, __builtin_fmaf(n[e], R, -q0));
-        }
-    }
+    for (int e = 0; e < 8; ++e) q[e] = EXACT ? n[e] / scale : __builtin_fmaf(n[e], R, __builtin_fmaf(low[e], R, n[e] * R_low));
     return make_uint2(pack_e4m3x4(q[0], q[1], q[2], q[3]), pack_e4m3x4(q[4], q[5], q[6], q[7]));
+}
+
+// v, or eight ones where it is absent.
+template <int TYPE>
+__device__ __forceinline__ Eight<TYPE> or_ones(const Eight<TYPE>& v, bool present)
+{
+    constexpr uint32_t one = TYPE == kBf16 ? 0x3f803f80u : TYPE == kF16 ? 0x3c003c00u : 0x3f800000u;
+    if (present) return v;
+    Eight<TYPE> u = v;
+    u.w[0] = make_uint4(one, one, one, one);
+    if (TYPE == kF32) u.w[TYPE == kF32] = u.w[0];
+    return u;
 }
 
 // Streams of at least this many bytes are stored non-temporally: they only pass through the last-level cache.
 constexpr int64_t kOnceBytes = 256ll << 20;
 
-// A workgroup per row, of as many waves as its chunks fill: thread t holds chunk t, or t and t + threads, as binary32 in
-// registers from the addition to the codes, and the partial sums of squares and the maxima meet in LDS. One chunk a thread makes a row short
-// for the few of a step (16 of 5120: 4.3 us on the card); two halve what every wave does once, which costs time where there are
-// many (32760 of 5376, gated and modulated: 226 us and 5.5 TB/s, where one takes 239 and three 231). All loads go out
-// before the first of them is used, the tables' as soon as the row's index is there; a table that is absent is a
-// descriptor of no bytes, which reads zeros. S, B: the types of the stream, and of the branch and its parameters.
-template <int S, int B, int CPL, bool ONCE>
+// A workgroup per row, of as many waves as its chunks fill: thread t holds chunk t, or t and t + threads, as
+// binary32 in registers from the addition to the codes, and the partial sums of squares and the maxima meet in
+// LDS. One chunk a thread makes a row short for the few of a step (16 of 5120: 4.1 us on the card); two halve what
+// every wave does once, which costs time where there are many (32760 of 5376, gated and modulated: 237 us and
+// 5.2 TB/s, as fast as a copy of those bytes; 243 with one chunk a thread). All loads go out before the first of
+// them is used, the tables' as soon as the row's index is there; a table that is absent is a descriptor of no
+// bytes, which reads zeros. S, B: the types of the stream, and of the branch and its parameters; AFFINE: scale and
+// shift are there; ONCE: hidden is stored non-temporally.
+template <int S, int B, int CPL, bool AFFINE, bool ONCE>
 __global__ __launch_bounds__(kMostWaves * kLanes) void k_add_norm(AddNormArgs p, int waves, int64_t first)
 {
     __shared__ float ssum[kMostWaves];
@@ -102,24 +108,25 @@ __global__ __launch_bounds__(kMostWaves * kLanes) void k_add_norm(AddNormArgs p,
         g[c] = load8<B, 0>(gr, chunk(c));
         w[c] = load8<B, 0>(wr, chunk(c));
     }
+    if (AFFINE)
 #pragma unroll
-    for (int c = 0; c < CPL; ++c) {
-        sc[c] = load8<B, 0>(scr, chunk(c));
-        sh[c] = load8<B, 0>(shr, chunk(c));
-    }
+        for (int c = 0; c < CPL; ++c) {
+            sc[c] = load8<B, 0>(scr, chunk(c));
+            sh[c] = load8<B, 0>(shr, chunk(c));
+        }
     __builtin_amdgcn_sched_barrier(0);
 
     const __amdgpu_buffer_rsrc_t hr = row_buffer((uint8_t*)p.hidden + row * p.ldh * element_bytes(S), sbytes);
-    float n[CPL][8], ss = 0.0f;
+    float n[CPL][8], low[CPL][8], ss = 0.0f;
 #pragma unroll
     for (int c = 0; c < CPL; ++c) {
         float x[8], y[8], f[8];
         decode8<S>(r[c], x);
         decode8<B>(b[c], y);
-        decode8<B>(g[c], f);
+        decode8<B>(or_ones<B>(g[c], p.gate), f);
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            x[e] = __builtin_fmaf(p.gate ? f[e] : 1.0f, y[e], x[e]);
+            x[e] = __builtin_fmaf(f[e], y[e], x[e]);
             if (S == kF16) asm volatile("" : "+v"(x[e]));   // a binary32 value first, not one fma that rounds to binary16
         }
         const Eight<S> h = encode8<S>(x);
@@ -143,15 +150,26 @@ __global__ __launch_bounds__(kMostWaves * kLanes) void k_add_norm(AddNormArgs p,
 #pragma unroll
     for (int c = 0; c < CPL; ++c) {
         float f[8], u[8], v[8];
-        decode8<B>(w[c], f);
-        decode8<B>(sc[c], u);
-        decode8<B>(sh[c], v);
+        decode8<B>(or_ones<B>(w[c], p.weight), f);
+        if (AFFINE) {
+            decode8<B>(sc[c], u);
+            decode8<B>(sh[c], v);
+        }
         float most = 0.0f;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            // h rstd f + shift, f = w (1 + scale); absent factors are 1, an absent shift 0
-            const float factor = (p.weight ? f[e] : 1.0f) * (1.0f + u[e]), t = n[c][e] * rstd;
-            n[c][e] = __builtin_fmaf(t, factor, v[e]);
+            // n + low: low is what the rounding of h rstd, and without a shift that of its product with w, leaves out of
+            // n. A code moves where such errors carry a value across a border between two: of the 176 million codes of
+            // 32760 x 5376 172 do, 281 where n, the scale and the quotient are each rounded to binary32.
+            const float t = n[c][e] * rstd, t_low = __builtin_fmaf(n[c][e], rstd, -t);
+            if (AFFINE) {
+                const float factor = f[e] * (1.0f + u[e]);
+                low[c][e] = t_low * factor;
+                n[c][e] = __builtin_fmaf(t, factor, v[e]);
+            } else {
+                n[c][e] = t * f[e];
+                low[c][e] = __builtin_fmaf(t_low, f[e], __builtin_fmaf(t, f[e], -n[c][e]));
+            }
             most = __builtin_elementwise_maximum(most, __builtin_fabsf(n[c][e]));
         }
         if (chunk(c) < (uint32_t)nch) top = __builtin_elementwise_maximum(top, most);   // (0 times an infinite rstd, past the row)
@@ -173,7 +191,7 @@ __global__ __launch_bounds__(kMostWaves * kLanes) void k_add_norm(AddNormArgs p,
 #pragma unroll
     for (int c = 0; c < CPL; ++c) {
         if (p.normed) store8<B, 0>(encode8<B>(n[c]), nr, chunk(c));
-        const uint2 q = finite ? codes8<false>(n[c], scale, R, R_low) : codes8<true>(n[c], scale, R, R_low);
+        const uint2 q = finite ? codes8<false>(n[c], low[c], scale, R, R_low) : codes8<true>(n[c], low[c], scale, R, R_low);
         __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(i32x2_t, q), yr, chunk(c) * 8u, 0, 0);
     }
 }
@@ -187,11 +205,14 @@ int launch(const AddNormArgs& p, hipStream_t stream)
         // (a workgroup has 1024 threads at most, and a launch fewer than 2^32 work-items)
         const bool two = nch > kMostWaves * kLanes || (nch > 256 && p.M > kFewRows);
         const int waves = (int)((nch + kLanes * (two ? 2 : 1) - 1) / (kLanes * (two ? 2 : 1)));
-#define VDN_LAUNCH(n, o) hipLaunchKernelGGL((k_add_norm<S, B, n, o>), dim3((unsigned)rows), dim3(waves * kLanes), 0, stream, p, waves, m)
-        if (two && once) VDN_LAUNCH(2, true);
-        else if (two) VDN_LAUNCH(2, false);
-        else if (once) VDN_LAUNCH(1, true);
-        else VDN_LAUNCH(1, false);
+#define VDN_LAUNCH(n, a, o) hipLaunchKernelGGL((k_add_norm<S, B, n, a, o>), dim3((unsigned)rows), dim3(waves * kLanes), 0, stream, p, waves, m)
+#define VDN_FORM(n)                                            \
+        if (p.scale && once) VDN_LAUNCH(n, true, true);        \
+        else if (p.scale) VDN_LAUNCH(n, true, false);          \
+        else if (once) VDN_LAUNCH(n, false, true);             \
+        else VDN_LAUNCH(n, false, false);
+        if (two) { VDN_FORM(2) } else { VDN_FORM(1) }
+#undef VDN_FORM
 #undef VDN_LAUNCH
         return check_launch("add_norm_quantize");
     });

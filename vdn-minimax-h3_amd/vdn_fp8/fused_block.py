@@ -254,7 +254,7 @@ def add_norm_quantize(residual, branch, weight, eps, *, gate=None, scale=None, s
     normed = torch.empty_like(like, dtype=dtype) if return_normed else None
     with _on(dev):
         _lib.check(_lib.load().vdn_fp8_add_norm_quantize(
-            r.data_ptr(), _DTYPES[stream], ldr, b.data_ptr(), _DTYPES[dtype], ldb, M, K, _ptr(gate), K, _ptr(weight), eps,
+            r.data_ptr(), _DTYPES[stream], ldr, b.data_ptr(), _DTYPES[dtype], ldb, M, K, _ptr(gate), K, _ptr(weight), float(eps),
             _ptr(scale), _ptr(shift), K, _ptr(indices), rows, hidden.data_ptr(), K, y.data_ptr(), K, s.data_ptr(), _ptr(normed), K,
             _stream(r)), "add_norm_quantize")
     if not flat:

@@ -100,13 +100,13 @@ def _axes_norm(norm, d, dtype, at, name):
         return 0, None, 0.0
     weight, eps = norm
     if weight is None:
-        return 1, None, eps
+        return 1, None, float(eps)
     if weight.numel() != d or weight.dtype is not dtype or weight.get_device() != at:
         raise ValueError(f"{name}'s weight must be a {str(dtype).replace('torch.', '')} [{d}] tensor on the rows' device "
                          f"(got {weight.dtype} {tuple(weight.shape)} on {weight.device})")
     if not weight.is_contiguous() or weight.data_ptr() % 16:
         weight = weight.clone(memory_format=torch.contiguous_format)
-    return 1, weight, eps
+    return 1, weight, float(eps)
 
 
 def qk_prep_axes(query, key, norm_q, norm_k, rope, positions):
