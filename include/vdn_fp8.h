@@ -492,15 +492,17 @@ int vdn_fp8_add_norm_quantize(const void *residual, int stream_type, int64_t ldr
                               void *y, int64_t ldy, float *y_scale, void *normed, int64_t ldn, hipStream_t stream);
 
 /*
- * Low-rank adapters of many requests beside a shared projection (two launches):
+ * Low-rank adapters of many requests beside a shared projection (two launches, or one for few tokens of
+ * up to 64 ranks):
  *   out[t][n] = T(base[t][n] + scale[i] * sum_r (sum_k x[t][k] a[i][r][k]) b[i][n][r]),  i = index[t]
  *   out[t][n] = base[t][n] where index[t] is outside [0, L)
  * x [T, K], base and out [T, N], a [L, R, K], b [L, N, R] of dtype (bf16 or binary16), scale
  * binary32 [L], index [T]. The first product is accumulated and kept in binary32, and enters the
- * second as two 16-bit parts (2^-17 of it or less is left out). out may be base itself (with its stride);
- * nothing else may overlap. The same inputs give the same bits, and a token's do not depend on the
- * others' values. workspace: device memory, 16-byte aligned, of the size asked for with the same T, K,
- * N, L, R; it need not be zeroed, and calls that overlap need one each.
+ * second so (one launch) or as two 16-bit parts (2^-17 of it or less is left out). out may be base itself
+ * (with its stride); nothing else may overlap (out over x, or over part of base, is VDN_FP8_EINVAL). The same
+ * inputs give the same bits, and a token's do not depend on the others' values. workspace: device memory,
+ * 16-byte aligned, of the size asked for with the same T, K, N, L, R (0: none is needed, NULL will do); it need
+ * not be zeroed, and calls that run at the same time need one each.
  * Replaces: nothing in the reference, which merges its one adapter into the weight (`merge_lora_state`,
  *           src/inference/utils/lora.py:80-94).
  * Requires: K and N multiples of 8, 8 to 2^17; R a multiple of 16, 16 to 128 (an adapter of another rank

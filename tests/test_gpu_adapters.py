@@ -258,3 +258,61 @@ def test_banks_from_adapter_files(device):
         a, b = state["blk.to_q.lora_A.weight"].to(BF16), state["blk.to_q.lora_B.weight"].to(BF16)
         assert torch.equal(ad.a[i, :a.shape[0]].cpu(), a) and torch.equal(ad.b[i, :, :a.shape[0]].cpu(), b)
         assert not ad.a[i, a.shape[0]:].any() and not ad.b[i, :, a.shape[0]:].any()
+
+
+@pytest.mark.parametrize("R", [16, 32, 48, 64])
+@pytest.mark.parametrize("form", ["one", "random", "runs", "each"])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_one_launch_at_its_limits(device, R, form, dtype):
+    """64 tokens, up to all of one adapter, and the widest rows that one launch takes; columns that end inside a workgroup's."""
+    T, K, N = 64, 7168, 1544
+    x, base = rows(device, T, K, N, dtype, R)
+    ad = bank(device, 16, R, K, N, dtype, R + 1)
+    index = choose(device, T, 16, form, R + 2)
+    got = adapter_add(x, base, ad, index)
+    check(got, x, base, ad, index)
+    mine = base.clone()
+    adapter_add(x, mine, ad, index, out=mine)
+    assert torch.equal(mine, got)
+
+
+@pytest.mark.parametrize("T", [9, 200, 1200])
+def test_shared_memory(device, T):
+    """out over x is refused (others still read those rows); x itself as the base, with a new out, is not."""
+    x, _ = rows(device, T, 64, 64, BF16, 1)
+    ad = bank(device, 4, 16, 64, 64, BF16, 2)
+    index = choose(device, T, 4, "random", 3)
+    kept = x.clone()
+    with pytest.raises(ValueError, match="overlap x"):
+        adapter_add(x, x, ad, index, out=x)
+    wide = torch.zeros(T, 96, device=device, dtype=BF16)
+    with pytest.raises(ValueError, match="overlap x"):
+        part = wide[:, 32:]
+        adapter_add(wide[:, :64], part, ad, index, out=part)
+    assert torch.equal(x, kept) and not wide.any()
+    check(adapter_add(x, x, ad, index), x, x, ad, index)
+
+
+def test_offsets_beyond_32_bits(device):
+    """33000 rows of 65544 columns, 4.3 GB: the last tokens' are what they are alone."""
+    T, K, N = 33000, 64, 65544
+    ad = bank(device, 2, 16, K, N, BF16, 2)
+    x = rows(device, T, K, 8, BF16, 1)[0]
+    base = torch.empty(T, N, device=device, dtype=BF16)
+    base.fill_(0.5)
+    tail = slice(T - 1300, T)
+    base[tail] = rows(device, 1300, 8, N, BF16, 3)[1]
+    index = choose(device, T, 2, "each", 0)
+    want = adapter_add(x[tail], base[tail].clone(), ad, index[tail])
+    check(want[-64:], x[-64:], base[-64:], ad, index[-64:])
+    got = adapter_add(x, base, ad, index)
+    assert torch.equal(got[tail], want)
+    adapter_add(x, base, ad, index, out=base)
+    assert torch.equal(base, got)
+
+
+def test_rows_of_float32_are_refused(device):
+    f = vdn_fp8.Fp8Linear(torch.nn.Linear(512, 384, device=device, dtype=torch.float32).requires_grad_(False))
+    with pytest.raises(ValueError, match="bfloat16 or float16"):
+        f(torch.randn(4, 512, device=device), adapters=bank(device, 2, 16, 512, 384, BF16, 2),
+          index=torch.zeros(4, device=device, dtype=torch.int32))

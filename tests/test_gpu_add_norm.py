@@ -191,3 +191,18 @@ def test_codes_feed_the_next_projection(device):
     # (2^-23 each, should the matrix cores truncate)
     room = 514 * 2.0 ** -23 * size
     assert torch.all((got - want).abs() <= 2.0 ** -8 * (want.abs() + room) + room)
+
+
+def test_offsets_beyond_32_bits(device):
+    """300000 rows of 8192, 4.9 GB a tensor, the last of them. (Their bits are not those of a call of 40 rows, whose waves sum squares
+    in another order.)"""
+    M, K = 300000, 8192
+    r, b, w, gate, sc, sh, index = inputs(device, 40, K, BF16, BF16, 3, 1)
+    residual, branch = (torch.empty(M, K, device=device, dtype=BF16) for _ in range(2))
+    residual.fill_(1.0)
+    branch.fill_(0.25)
+    residual[-40:], branch[-40:] = r, b
+    far = torch.zeros(M, device=device, dtype=torch.int32)
+    far[-40:] = index
+    got = vdn_fp8.add_norm_quantize(residual, branch, w, 1e-6, gate=gate, scale=sc, shift=sh, indices=far)
+    check([t[-40:] for t in got], formula(r, b, w, 1e-6, gate, sc, sh, index), BF16)

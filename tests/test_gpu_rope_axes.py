@@ -160,3 +160,17 @@ def test_graph_with_other_positions(device):
         want = vdn_fp8.qk_prep_axes(q, k, nq, nk, rope, pos)
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(out, want))
+
+
+def test_offsets_beyond_32_bits(device):
+    """300000 tokens of 64 + 1 heads of 128, 4.9 GB of queries: the last tokens' results are what they are alone."""
+    T, d, rope = 300000, 128, RopeAxes.make((24, 20, 20), device=device)
+    q, k, nq, nk = heads(device, 40, 64, 1, d, BF16, 1)
+    query, key = torch.empty(T, 64, d, device=device, dtype=BF16), torch.empty(T, 1, d, device=device, dtype=BF16)
+    query.fill_(1.0)
+    key.fill_(1.0)
+    query[-40:], key[-40:] = q, k
+    positions = torch.arange(3 * T, device=device, dtype=torch.int32).view(T, 3)
+    got = vdn_fp8.qk_prep_axes(query, key, nq, nk, rope, positions)
+    for out, x, norm in zip(got, (q, k), (nq, nk)):
+        check(out[-40:], x, norm, rope, positions[-40:])

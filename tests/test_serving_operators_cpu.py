@@ -9,6 +9,7 @@ import vdn_fp8._lib as L
 from vdn_fp8 import Adapters, RopeAxes
 
 FAKE = 1 << 20        # never dereferenced: every call below fails its checks first
+OTHER = 1 << 30
 
 
 def norm(r=FAKE, stream=0, ldr=64, b=FAKE, dtype=0, ldb=64, M=4, K=64, gate=None, ldgate=64, w=None, eps=1e-6, sc=None, sh=None, ldmod=64,
@@ -17,7 +18,7 @@ def norm(r=FAKE, stream=0, ldr=64, b=FAKE, dtype=0, ldb=64, M=4, K=64, gate=None
                                               s, n, ldn, None)
 
 
-def adapt(x=FAKE, dtype=0, ldx=64, base=FAKE, ldbase=32, T=4, K=64, N=32, a=FAKE, b=FAKE, scale=FAKE, banks=2, R=16, index=FAKE, out=FAKE, ldo=32,
+def adapt(x=FAKE, dtype=0, ldx=64, base=FAKE, ldbase=32, T=4, K=64, N=32, a=FAKE, b=FAKE, scale=FAKE, banks=2, R=16, index=FAKE, out=OTHER, ldo=32,
           ws=FAKE, n=1 << 40):
     return L.load().vdn_fp8_adapter_add(x, dtype, ldx, base, ldbase, T, K, N, a, b, scale, banks, R, index, out, ldo, ws, n, None)
 
@@ -42,8 +43,15 @@ def rope(q=FAKE, hq=4, ldq=512, k=FAKE, hk=2, ldk=256, T=4, d=128, dtype=0, wq=N
     (lambda: adapt(R=8), "rank"), (lambda: adapt(R=24), "rank"), (lambda: adapt(R=144), "rank"), (lambda: adapt(dtype=2), "dtype"),
     (lambda: adapt(x=None), "null"), (lambda: adapt(index=None), "null"), (lambda: adapt(b=None), "null"), (lambda: adapt(ldx=56), "strides"),
     (lambda: adapt(ldbase=36), "strides"), (lambda: adapt(ldo=(1 << 23) + 8), "strides"), (lambda: adapt(x=FAKE + 8), "misaligned"),
-    (lambda: adapt(index=FAKE + 2), "misaligned"), (lambda: adapt(ws=None), "workspace"), (lambda: adapt(n=16), "workspace"),
-    (lambda: adapt(ws=FAKE + 8), "workspace"),
+    (lambda: adapt(index=FAKE + 2), "misaligned"),
+    # (a call of few tokens has no workspace)
+    (lambda: adapt(T=9, ws=None), "workspace"), (lambda: adapt(T=9, n=16), "workspace"), (lambda: adapt(T=9, ws=FAKE + 8), "workspace"),
+    # out over x: the same rows, rows of another stride, one that begins in x's last row, columns that meet in it, that wrap into it
+    (lambda: adapt(N=64, ldbase=64, ldo=64, out=FAKE), "overlap x"), (lambda: adapt(out=FAKE + 3 * 128), "overlap x"),
+    (lambda: adapt(x=OTHER, out=OTHER - 3 * 64), "overlap x"), (lambda: adapt(ldx=96, ldo=96, x=OTHER, out=OTHER + 112), "overlap x"),
+    (lambda: adapt(ldx=96, ldo=96, x=OTHER + 96, out=OTHER + 64), "overlap x"),
+    (lambda: adapt(ldo=64, out=FAKE + (1 << 16), base=FAKE + (1 << 16)), "base itself"),
+    (lambda: adapt(base=FAKE + (1 << 16), out=FAKE + (1 << 16) + 64), "base itself"),
     (lambda: rope(T=-1), "negative"), (lambda: rope(dtype=3), "dtype"), (lambda: rope(d=96), "head dim"), (lambda: rope(hq=513, ldq=1 << 17), "65536"),
     (lambda: rope(R=136), "multiple of 16"), (lambda: rope(R=24), "multiple of 16"), (lambda: rope(R=12, pairs=1), "multiple of 8"),
     (lambda: rope(R=-16), "multiple of 16"), (lambda: rope(freq=None), "null"), (lambda: rope(pos=None), "null"), (lambda: rope(axes=0), "axes"),
@@ -69,10 +77,14 @@ def test_adapter_workspace_sizes():
     ask = lambda *a: lib.vdn_fp8_adapter_add_workspace_size(*a, ctypes.byref(size))   # noqa: E731
     assert ask(0, 64, 64, 2, 16) == L.OK and size.value == 0
     assert ask(5, 64, 64, 0, 16) == L.OK and size.value == 0
-    for T in (1, 64, 1024, 1025, 32760):
+    for T in (17, 64, 1024, 1025, 32760):
         for R in (16, 48, 128):
             assert ask(T, 5120, 5120, 4, R) == L.OK
-            assert size.value > 0 and size.value % (T * R * 4) == 0 and size.value // (T * R * 4) <= 32
+            whole = -(-T // 64) * 64 * R * 4       # h of whole tiles, in up to 32 parts
+            assert size.value > 0 and size.value % whole == 0 and size.value // whole <= 32
+    # few tokens of an adapter, ranks and widths that one launch takes: none
+    for T, R, K, none in ((1, 64, 7168, True), (16, 64, 5120, True), (16, 80, 5120, False), (16, 64, 7176, False), (17, 16, 64, False)):
+        assert ask(T, K, 5120, 4, R) == L.OK and (size.value == 0) == none
     assert ask(5, 64, 64, 2, 17) == L.EINVAL
     assert lib.vdn_fp8_adapter_add_workspace_size(5, 64, 64, 2, 16, None) == L.EINVAL
 
