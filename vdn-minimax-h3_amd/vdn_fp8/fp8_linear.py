@@ -72,6 +72,24 @@ def _aligned16(t):
     return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
+def _strided_rows(x, width):
+    """x [..., width] as rows with unit column stride, 16-byte aligned (a copy where they are not), their address
+    and their stride."""
+    rows = x if x.dim() == 2 else x.reshape(-1, width)
+    start = rows.data_ptr()
+    if start % 16 == 0 and rows.is_contiguous():
+        return rows, start, width
+    ld, unit = rows.stride()
+    if unit != 1 or ld % 8 or ld < width or start % 16:
+        rows = rows.clone(memory_format=torch.contiguous_format)
+        return rows, rows.data_ptr(), width
+    return rows, start, ld
+
+
+def _name(dtype):
+    return str(dtype).replace("torch.", "")
+
+
 # Element types the quantizers and the GEMM's output take, with their C ABI codes. The
 # reference's Triton kernels load any float type and compute in binary32 (fp8_linear.py:72);
 # float64 is refused here (its rows would be rounded to binary32 first).

@@ -29,9 +29,8 @@ import torch
 import torch.nn.functional as F
 
 from . import _lib
-from .fp8_linear import (_DTYPES, FP8_DTYPE, Fp8Linear, _aligned16, _ptr, _rows, _stream, check_index_range,
-                         swiglu_quantize_activation)
-from .kv_cache import _on
+from .fp8_linear import (_DTYPES, FP8_DTYPE, Fp8Linear, _aligned16, _name, _ptr, _rows, _stream, _strided_rows,
+                         check_index_range, swiglu_quantize_activation)
 
 
 # --------------------------------------------------------------------------------------
@@ -166,20 +165,6 @@ def post(residual, gate, indices, branch_out):
     return out.reshape(shape)
 
 
-def _typed_rows(x, width):
-    """x [..., K] as rows with unit column stride, 16-byte aligned, and their stride (a copy where they are not)."""
-    rows = x if x.dim() == 2 else x.reshape(-1, width)
-    ld, unit = rows.stride()
-    if unit != 1 or ld % 8 or ld < width or rows.data_ptr() % 16:
-        rows = rows.clone(memory_format=torch.contiguous_format)
-        ld = width
-    return rows, ld if ld > width else width
-
-
-def _name(dtype):
-    return str(dtype).replace("torch.", "")
-
-
 def _table(t, width, dtype, at, name):
     """A modulation table [T, K] (or [K]), contiguous, and its rows."""
     shape = t.shape
@@ -206,8 +191,12 @@ def add_norm_quantize(residual, branch, weight, eps, *, gate=None, scale=None, s
     (`post` and `pre_quantize` are the reference's two steps, with its rounding of n to bf16 before the codes.)"""
     if not residual.is_cuda:
         raise ValueError("add_norm_quantize runs on the GPU (a HIP kernel); residual is a CPU tensor")
-    # (this call is short for few rows: each of a tensor's properties is read once)
+    # (the kernel is short for few rows: each of a tensor's properties is read once, and nothing is called that can be done without)
     dtype, stream, shape, at = branch.dtype, residual.dtype, residual.shape, residual.get_device()
+    if torch._C._cuda_getDevice() != at:
+        with torch.cuda.device(at):
+            return add_norm_quantize(residual, branch, weight, eps, gate=gate, scale=scale, shift=shift, indices=indices,
+                                     return_normed=return_normed)
     if dtype not in _DTYPES or stream not in _DTYPES or (stream is not dtype and stream is not torch.float32):
         raise ValueError("residual and branch must be bfloat16, float16 or float32 of one type, or residual float32 "
                          f"(got {stream} and {dtype})")
@@ -218,22 +207,26 @@ def add_norm_quantize(residual, branch, weight, eps, *, gate=None, scale=None, s
         raise ValueError(f"add_norm_quantize takes widths that are multiples of 8, from 8 to 16384 (got {K})")
     if (scale is None) != (shift is None):
         raise ValueError("scale and shift go together")
-    r, ldr = _typed_rows(residual, K)
-    b, ldb = _typed_rows(branch, K)
-    M, dev = r.shape[0], r.device
+    r, of_r, ldr = _strided_rows(residual, K)
+    b, of_b, ldb = _strided_rows(branch, K)
+    M = r.shape[0]
+    of_weight = of_gate = of_scale = of_shift = of_indices = None
+    rows = 0
     if weight is not None:
         if weight.dtype is not dtype or weight.numel() != K or weight.get_device() != at:
-            raise ValueError(f"weight must be a {_name(dtype)} [{K}] tensor on {dev} (got {weight.dtype} {tuple(weight.shape)})")
-        if not weight.is_contiguous() or weight.data_ptr() % 16:
+            raise ValueError(f"weight must be a {_name(dtype)} [{K}] tensor on {r.device} (got {weight.dtype} {tuple(weight.shape)})")
+        of_weight = weight.data_ptr()
+        if of_weight % 16 or not weight.is_contiguous():
             weight = weight.clone(memory_format=torch.contiguous_format)
-    rows = 0
+            of_weight = weight.data_ptr()
     if gate is not None:
         gate, rows = _table(gate, K, dtype, at, "gate")
+        of_gate = gate.data_ptr()
     if scale is not None:
-        (scale, of_scale), (shift, of_shift) = _table(scale, K, dtype, at, "scale"), _table(shift, K, dtype, at, "shift")
-        if of_scale != of_shift or (gate is not None and of_scale != rows):
+        (scale, rows_scale), (shift, rows_shift) = _table(scale, K, dtype, at, "scale"), _table(shift, K, dtype, at, "shift")
+        if rows_scale != rows_shift or (gate is not None and rows_scale != rows):
             raise ValueError("gate, scale and shift must be tables of the same rows")
-        rows = of_scale
+        rows, of_scale, of_shift = rows_scale, scale.data_ptr(), shift.data_ptr()
     if not rows and (gate is not None or scale is not None):
         raise ValueError("a table needs at least 1 row")
     if indices is not None:
@@ -244,20 +237,21 @@ def add_norm_quantize(residual, branch, weight, eps, *, gate=None, scale=None, s
         check_index_range(indices, rows, "add_norm_quantize: indices")
         if indices.dtype is not torch.int32 or indices.get_device() != at or not indices.is_contiguous():
             # (a wider index is clamped before it is narrowed)
-            indices = indices.to(dev).clamp(0, rows - 1).to(torch.int32).contiguous()
-    # (empty_like takes half the time of empty with a shape)
-    like = r if ldr == K and r.is_contiguous() else torch.empty(M, K, device=dev, dtype=stream)
-    flat = len(shape) == 2
+            indices = indices.to(r.device).clamp(0, rows - 1).to(torch.int32).contiguous()
+        of_indices = indices.data_ptr()
+    # (empty_like is the shortest way to a new tensor: 1.1 us)
+    like = r if ldr == K and r.is_contiguous() else torch.empty(M, K, device=r.device, dtype=stream)
     hidden = torch.empty_like(like)
     y = torch.empty_like(like, dtype=FP8_DTYPE)
-    s = torch.empty(M, 1, device=dev, dtype=torch.float32)
+    s = torch.empty(M, 1, device=r.device, dtype=torch.float32)
     normed = torch.empty_like(like, dtype=dtype) if return_normed else None
-    with _on(dev):
-        _lib.check(_lib.load().vdn_fp8_add_norm_quantize(
-            r.data_ptr(), _DTYPES[stream], ldr, b.data_ptr(), _DTYPES[dtype], ldb, M, K, _ptr(gate), K, _ptr(weight), float(eps),
-            _ptr(scale), _ptr(shift), K, _ptr(indices), rows, hidden.data_ptr(), K, y.data_ptr(), K, s.data_ptr(), _ptr(normed), K,
-            _stream(r)), "add_norm_quantize")
-    if not flat:
+    status = _lib.load().vdn_fp8_add_norm_quantize(
+        of_r, _DTYPES[stream], ldr, of_b, _DTYPES[dtype], ldb, M, K, of_gate, K, of_weight, float(eps), of_scale, of_shift, K, of_indices,
+        rows, hidden.data_ptr(), K, y.data_ptr(), K, s.data_ptr(), normed.data_ptr() if return_normed else None, K,
+        torch._C._cuda_getCurrentRawStream(at))
+    if status:
+        _lib.check(status, "add_norm_quantize")
+    if len(shape) != 2:
         hidden = hidden.view(shape)
         normed = normed.view(shape) if return_normed else None
     return (hidden, y, s, normed) if return_normed else (hidden, y, s)

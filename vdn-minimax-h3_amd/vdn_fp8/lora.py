@@ -27,9 +27,8 @@ import torch
 import torch.nn as nn
 
 from . import _lib
-from .fp8_linear import (_DTYPES, MIN_WIDTH, SKIP_END_BLOCKS, Fp8Linear, _aligned16, _blocks_to_skip, _ptr,
-                         _stream, lora_delta, lora_in_kernel)
-from .kv_cache import _on
+from .fp8_linear import (_DTYPES, MIN_WIDTH, SKIP_END_BLOCKS, Fp8Linear, _aligned16, _blocks_to_skip, _name, _ptr,
+                         _stream, _strided_rows, lora_delta, lora_in_kernel)
 
 # Original-layout module names -> diffusers names (lora.py:22-30).
 _ORIGINAL_RENAMES = (
@@ -263,23 +262,6 @@ def _adapter_workspace(T, K, N, L, R):
     return got
 
 
-def _name(dtype):
-    return str(dtype).replace("torch.", "")
-
-
-def _adapter_rows(t, width, dtype, at, name):
-    """t [..., width] as rows with unit column stride, 16-byte aligned, and their stride (a copy where they are not)."""
-    shape = t.shape
-    if t.dtype is not dtype or not shape or shape[-1] != width or t.get_device() != at:
-        raise ValueError(f"{name} must be {_name(dtype)} [..., {width}] on the rows' device (got {t.dtype} {tuple(shape)} on {t.device})")
-    rows = t if len(shape) == 2 else t.reshape(-1, width)
-    ld, unit = rows.stride()
-    if unit != 1 or ld % 8 or ld < width or rows.data_ptr() % 16:
-        rows = rows.clone(memory_format=torch.contiguous_format)
-        ld = width
-    return rows, ld if ld > width else width
-
-
 def adapter_add(x, base, adapters, index, *, out=None):
     """base + scale[i] * (x @ a[i].T) @ b[i].T, row by row with i = index[row]: the low-rank adapters of many requests
     beside the projection that they share.
@@ -291,9 +273,12 @@ def adapter_add(x, base, adapters, index, *, out=None):
     sum is rounded once."""
     if not x.is_cuda:
         raise ValueError("adapter_add runs on the GPU (HIP kernels); x is a CPU tensor")
-    # (this call is short for few rows: each of a tensor's properties is read once)
+    # (the kernel is short for few rows: each of a tensor's properties is read once, and nothing is called that can be done without)
     a, b, scale = adapters
-    dtype, at, of_a, of_b = x.dtype, x.get_device(), a.shape, b.shape
+    dtype, at, of_x, of_base, of_a, of_b = x.dtype, x.get_device(), x.shape, base.shape, a.shape, b.shape
+    if torch._C._cuda_getDevice() != at:
+        with torch.cuda.device(at):
+            return adapter_add(x, base, adapters, index, out=out)
     if dtype not in _ADAPTER_DTYPES:
         raise ValueError(f"adapter_add takes bfloat16 or float16 rows (got {dtype})")
     if len(of_a) != 3 or len(of_b) != 3 or of_b[0] != of_a[0] or of_b[2] != of_a[1]:
@@ -307,28 +292,33 @@ def adapter_add(x, base, adapters, index, *, out=None):
         raise ValueError(f"the adapters and index must be on {x.device}")
     if not a.is_contiguous() or not b.is_contiguous() or not scale.is_contiguous():
         raise ValueError("the adapters must be contiguous")
-    if x.shape[:-1] != base.shape[:-1]:
-        raise ValueError(f"x {tuple(x.shape)} and base {tuple(base.shape)} must have the same rows")
-    rows, ldx = _adapter_rows(x, K, dtype, at, "x")
-    T, dev = rows.shape[0], rows.device
+    if not of_x or of_x[-1] != K:
+        raise ValueError(f"x must be [..., {K}], as the adapters (got {tuple(of_x)})")
+    if base.dtype is not dtype or not of_base or of_base[-1] != N or base.get_device() != at:
+        raise ValueError(f"base must be {_name(dtype)} [..., {N}] on {x.device} (got {base.dtype} {tuple(of_base)} on {base.device})")
+    if of_x[:-1] != of_base[:-1]:
+        raise ValueError(f"x {tuple(of_x)} and base {tuple(of_base)} must have the same rows")
+    rows, x_at, ldx = _strided_rows(x, K)
+    T = rows.shape[0]
     if index.dtype is not torch.int32 or index.shape != (T,) or not index.is_contiguous():
         raise ValueError(f"index must be a contiguous int32 [{T}] tensor (got {index.dtype} {tuple(index.shape)})")
-    given, ldbase = _adapter_rows(base, N, dtype, at, "base")
+    given, base_at, ldbase = _strided_rows(base, N)
     if out is None:
-        result = torch.empty_like(given) if ldbase == N and given.is_contiguous() else torch.empty(T, N, device=dev, dtype=dtype)
-        to, ldo = result, N
-        if base.dim() != 2:
-            result = result.view(base.shape)
+        result = torch.empty_like(given) if ldbase == N and given.is_contiguous() else torch.empty(T, N, device=rows.device, dtype=dtype)
+        out_at, ldo = result.data_ptr(), N
+        if len(of_base) != 2:
+            result = result.view(of_base)
     else:
         if out is not base:
             raise ValueError("out must be base itself, or None for a new tensor")
-        if given.data_ptr() != base.data_ptr():
+        if base_at != base.data_ptr():
             raise ValueError("base cannot be added to in place: its rows need unit stride, 16-byte alignment and row strides of multiples of 8")
-        result, to, ldo = base, given, ldbase
+        result, out_at, ldo = base, base_at, ldbase
     n = _adapter_workspace(T, K, N, L, R)
-    ws = torch.empty(n, device=dev, dtype=torch.uint8) if n else None
-    with _on(dev):
-        _lib.check(_lib.load().vdn_fp8_adapter_add(
-            rows.data_ptr(), _DTYPES[dtype], ldx, given.data_ptr(), ldbase, T, K, N, a.data_ptr(), b.data_ptr(), scale.data_ptr(), L, R,
-            index.data_ptr(), to.data_ptr(), ldo, None if ws is None else ws.data_ptr(), n, _stream(rows)), "adapter_add")
+    ws = torch.empty(n, device=rows.device, dtype=torch.uint8) if n else None
+    status = _lib.load().vdn_fp8_adapter_add(
+        x_at, _DTYPES[dtype], ldx, base_at, ldbase, T, K, N, a.data_ptr(), b.data_ptr(), scale.data_ptr(), L, R, index.data_ptr(), out_at, ldo,
+        None if ws is None else ws.data_ptr(), n, torch._C._cuda_getCurrentRawStream(at))
+    if status:
+        _lib.check(status, "adapter_add")
     return result

@@ -22,7 +22,7 @@ import torch
 
 from . import _lib
 from .fp8_linear import _DTYPES, _aligned16, _ptr, _stream
-from .kv_cache import _ld, _on, _rows
+from .kv_cache import _rows
 
 
 def qk_prep(t, weight, eps, cos=None, sin=None):
@@ -117,8 +117,11 @@ def qk_prep_axes(query, key, norm_q, norm_k, rope, positions):
 
     Angles are formed in binary64, so that far positions keep their fraction of a turn; cosine and sine are
     binary32, and the result is rounded once. Returns new contiguous query and key."""
-    # (this call is short for few tokens: each of a tensor's properties is read once)
-    dtype, shape = query.dtype, query.shape
+    # (the kernel is short for few tokens: each of a tensor's properties is read once, and nothing is called that can be done without)
+    dtype, shape, at = query.dtype, query.shape, query.get_device()
+    if at >= 0 and torch._C._cuda_getDevice() != at:
+        with torch.cuda.device(at):
+            return qk_prep_axes(query, key, norm_q, norm_k, rope, positions)
     if dtype not in _DTYPES:
         raise ValueError(f"qk_prep_axes takes bfloat16, float16 or float32 (got {dtype})")
     if len(shape) != 3 or shape[2] not in (64, 128, 256):
@@ -126,10 +129,10 @@ def qk_prep_axes(query, key, norm_q, norm_k, rope, positions):
     T, q_heads, d = shape
     kinds = (dtype,)
     query, key = _rows(query, None, d, "query", kinds), _rows(key, None, d, "key", kinds)
-    at, of_key = query.get_device(), key.shape
+    of_key = key.shape
     if key.get_device() != at or of_key[0] != T:
         raise ValueError("query and key must have the same rows on one device")
-    k_heads, dev = of_key[1], query.device
+    k_heads = of_key[1]
     inv_freq, axis, pairs = rope
     of_freq = inv_freq.shape
     if inv_freq.dtype is not torch.float64 or axis.dtype is not torch.int32 or len(of_freq) != 1 or axis.shape != of_freq:
@@ -145,17 +148,20 @@ def qk_prep_axes(query, key, norm_q, norm_k, rope, positions):
     if not 1 <= axes <= _MOST_AXES:
         raise ValueError(f"positions of 1 to {_MOST_AXES} axes (got {axes})")
     if positions.get_device() != at or inv_freq.get_device() != at or axis.get_device() != at:
-        raise ValueError(f"positions and rope must be on {dev}")
+        raise ValueError(f"positions and rope must be on {query.device}")
     positions, inv_freq, axis = positions.contiguous(), inv_freq.contiguous(), axis.contiguous()
     nq, wq, eps_q = _axes_norm(norm_q, d, dtype, at, "norm_q")
     nk, wk, eps_k = _axes_norm(norm_k, d, dtype, at, "norm_k")
-    out_q = torch.empty(T, q_heads, d, device=dev, dtype=dtype)
-    out_k = torch.empty(T, k_heads, d, device=dev, dtype=dtype)
-    with _on(dev):
-        _lib.check(_lib.load().vdn_fp8_qk_prep_axes(
-            query.data_ptr(), q_heads, _ld(query), key.data_ptr(), k_heads, _ld(key), T, d, _DTYPES[dtype], nq, _ptr(wq), eps_q, nk, _ptr(wk),
-            eps_k, inv_freq.data_ptr(), axis.data_ptr(), 2 * half, 1 if pairs else 0, positions.data_ptr(), _POSITIONS[kind], axes, axes,
-            out_q.data_ptr(), q_heads * d, out_k.data_ptr(), k_heads * d, _stream(query)), "qk_prep_axes")
+    # (empty_like is the shortest way to a new tensor, 1.1 us; of rows that lie apart it makes a contiguous one)
+    out_q, out_k = torch.empty_like(query), torch.empty_like(key)
+    of_q, of_k = q_heads * d, k_heads * d
+    status = _lib.load().vdn_fp8_qk_prep_axes(
+        query.data_ptr(), q_heads, query.stride(0) if T > 1 else of_q, key.data_ptr(), k_heads, key.stride(0) if T > 1 else of_k, T, d,
+        _DTYPES[dtype], nq, None if wq is None else wq.data_ptr(), eps_q, nk, None if wk is None else wk.data_ptr(), eps_k,
+        inv_freq.data_ptr(), axis.data_ptr(), 2 * half, 1 if pairs else 0, positions.data_ptr(), _POSITIONS[kind], axes, axes,
+        out_q.data_ptr(), of_q, out_k.data_ptr(), of_k, torch._C._cuda_getCurrentRawStream(at))
+    if status:
+        _lib.check(status, "qk_prep_axes")
     return out_q, out_k
 
 
