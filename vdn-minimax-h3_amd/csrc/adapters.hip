@@ -692,16 +692,28 @@ __global__ __launch_bounds__(kWaves * kLanes) void k_expand_tile(AdapterArgs p)
                 f32x4_t acc[8];
 #pragma unroll
                 for (int f = 0; f < 8; ++f) acc[f] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-                for (int f = 0; f < 8; ++f)
+                // (columns of the next product under this one's: left to itself the compiler reads all eight ahead, 69 us against 66
+                // at 6470 tokens of rank 128)
+                uint4 v[2][RK];
+                auto read = [&](uint4 (&to)[RK], int f) {
 #pragma unroll
                     for (int r = 0; r < RK; ++r) {
                         const bool in = 4 * r + quad < kChunks;   // (constant but for the last product of an odd number of 16 ranks: zeros beside zeros)
-                        uint4 v = buffer[(in ? 4 * r + quad : 0) * kPlane + f * 17 + col];
-                        if (RF % 2 && r == RK - 1 && !in) v = make_uint4(0, 0, 0, 0);
-                        acc[f] = Mma<TYPE>::mma(high[r], v, acc[f]);
-                        acc[f] = Mma<TYPE>::mma(low[r], v, acc[f]);
+                        to[r] = buffer[(in ? 4 * r + quad : 0) * kPlane + f * 17 + col];
+                        if (RF % 2 && r == RK - 1 && !in) to[r] = make_uint4(0, 0, 0, 0);
                     }
+                };
+                read(v[0], 0);
+#pragma unroll
+                for (int f = 0; f < 8; ++f) {
+                    if (f < 7) read(v[(f + 1) % 2], f + 1);
+#pragma unroll
+                    for (int r = 0; r < RK; ++r) {
+                        acc[f] = Mma<TYPE>::mma(high[r], v[f % 2][r], acc[f]);
+                        acc[f] = Mma<TYPE>::mma(low[r], v[f % 2][r], acc[f]);
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
+                }
                 i32x4_t o[4];
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
@@ -958,7 +970,12 @@ Plan plan_of(int64_t T, int64_t K, int64_t N, int64_t L, int64_t R)
         if (parts > ceil_div(steps, 4)) parts = ceil_div(steps, 4);
         p.span_k = (int)(kBk * ceil_div(steps, parts));
         p.parts = (int)ceil_div(K, p.span_k);
-        if (blocks < eighths) blocks = eighths;
+        // Above 64 ranks two workgroups of k_expand_tile are all that a compute unit has registers for, and where four or more of a tile are
+        // one round of them, an eighth left to tiles of two adapters, more would be two (6470 x 7168, rank 128: 61 us with four, 66 with
+        // seven; 3200 tokens 41 and 49. At rank 64 three go on a compute unit: 58 with four, 53 with seven).
+        const int64_t round = kFill * 7 / 8 / p.tiles;
+        if (R > 64 && round >= 4) blocks = round;
+        else if (blocks < eighths) blocks = eighths;
         if (blocks > columns) blocks = columns;
         p.span_n = (int)(kBn * ceil_div(columns, blocks));
         // (a tile that holds the border between two requests takes twice as long: where few tiles are, its adapters go apart)
