@@ -3,10 +3,15 @@
 //   out[t][n] = round(base[t][n] + scale[i] * sum_r h[t][r] B[i][n][r]),   h[t][r] = sum_k x[t][k] A[i][r][k],   i = index[t]
 //   out[t]    = base[t] where index[t] is outside [0, L)
 //
-// in two launches: k_shrink writes h, binary32, in S parts summed over disjoint ranges of k; k_expand
-// adds the parts and the second product to the base. Both are bound by memory (2 R operations for each element of x and of base,
-// R <= 128), so the matrix cores have time to spare: h is not rounded to 16 bits between the products but goes in as two
-// of them, a high and a low part, which keeps 2^-17 of it and costs the second product twice over.
+// in two launches: k_shrink_* write h, binary32, in S parts summed over disjoint ranges of k; k_expand_* add the parts and
+// the second product to the base. A step of few tokens is one launch (k_few). All are bound by memory (2 R operations for
+// each element of x and of base, R <= 128), so the matrix cores have time to spare: h is not rounded to 16 bits between the
+// products but goes in as two of them, a high and a low part, which keeps 2^-17 of it and costs the second product twice over
+// (1.5 us of 61 at 6470 tokens of rank 128).
+//
+// On the card: 32760 tokens, 5120 -> 15360, rank 64: 70 + 374 us, 5.2 TB/s of the bytes that it cannot do without (a large copy
+// reaches 5.1); 6470 tokens of six requests, 5376 -> 7168, rank 128: 31 + 53 us, 3.3 TB/s; 32 tokens of 12 adapters, 5120 -> 7168, rank 32:
+// 14 us; one token of rank 16, 5120 -> 5120: 4.6 us.
 //
 // Which tokens share an adapter. A tile is 64 consecutive tokens; a wave holds their adapters one a lane and finds the distinct
 // ones by ballots, so nothing is sorted, nothing is read back to the host, and a call can be captured into a graph and replayed

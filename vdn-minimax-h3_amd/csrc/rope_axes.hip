@@ -19,6 +19,10 @@
 // each (R / 2 <= 128 of them), leave cosine and sine in the wave's own LDS, and read those of their chunks from there: an angle costs
 // its wave about 60 operations once, and not once for each of the lanes that need it. The little that the angles need is fetched ahead of
 // the slots (loads come back in order), so that they are ready when those are.
+//
+// On the card: 32760 tokens of 40 + 40 heads of 128 224 us, 6.0 TB/s read and written, with the VALU busy 0.9 of the time (235 with what
+// the angles need fetched behind the rows); 5329 tokens of 16 + 16 heads of 64 10.9; 6405 float32 tokens of 32 + 8 heads of 128 52,
+// 5.1 TB/s; 16 tokens of 40 + 8 heads 3.8, a chain of the positions' load, the angles and the store.
 #include <stdint.h>
 
 #include "eight.h"
