@@ -239,6 +239,7 @@ __global__ __launch_bounds__(WK * kLanes) void k_shrink_step(AdapterArgs p)
                 for (int r = 0; r < RF; ++r)
                     if (rank + 16 * r < p.R) *reinterpret_cast<f32x4_t*>(h + 16 * r) = acc[r][t];
             }
+            settle_stores();
         }
     }
 }
@@ -318,6 +319,7 @@ __global__ __launch_bounds__(kWaves * kLanes) void k_shrink_tile(AdapterArgs p)
 #pragma unroll
             for (int r = 0; r < RF; ++r) *reinterpret_cast<f32x4_t*>(h + 16 * r) = acc[r];
         }
+        settle_stores();
     }
 }
 
