@@ -206,3 +206,35 @@ def test_offsets_beyond_32_bits(device):
     far[-40:] = index
     got = vdn_fp8.add_norm_quantize(residual, branch, w, 1e-6, gate=gate, scale=sc, shift=sh, indices=far)
     check([t[-40:] for t in got], formula(r, b, w, 1e-6, gate, sc, sh, index), BF16)
+
+
+@pytest.mark.parametrize("K", [64, 5120])
+def test_squares_beyond_binary32(device, K):
+    """Sums of squares that overflow (1 / inf: n is the shift itself) or are subnormal (no accuracy is left, but no NaN either)."""
+    g = torch.Generator(device).manual_seed(1)
+    r = torch.randn(6, K, device=device, generator=g)
+    r[:3] *= 1e25
+    r[3:] *= 1e-22
+    b, w, sc = torch.zeros(6, K, device=device, dtype=BF16), torch.ones(K, device=device, dtype=BF16), torch.zeros(K, device=device, dtype=BF16)
+    sh = torch.randn(K, device=device, generator=g).to(BF16)
+    hidden, codes, s, normed = vdn_fp8.add_norm_quantize(r, b, w, 0.0, scale=sc, shift=sh, return_normed=True)
+    assert torch.equal(hidden, r)
+    assert torch.equal(normed[:3], sh.expand(3, K))
+    alone, s_alone = vdn_fp8.quantize_rows(sh[None])
+    assert torch.equal(s[:3], s_alone.expand(3, 1)) and torch.equal(codes[:3].float(), alone.float().expand(3, K))
+    assert normed[3:].isfinite().all() and codes[3:].float().isfinite().all() and s[3:].isfinite().all()
+
+
+def test_equal_maxima(device):
+    """Rows in which many elements are the largest, in other waves: the same bits in every call, and the formula's."""
+    g = torch.Generator(device).manual_seed(1)
+    r = torch.randint(-2, 3, (600, 5120), device=device, generator=g).to(BF16)
+    b = torch.zeros_like(r)
+    w = (1 + torch.randint(0, 2, (5120,), device=device, generator=g).float() / 128).to(BF16)
+    sc, sh = (torch.randint(0, 2, (5120,), device=device, generator=g).float() / 64).to(BF16), torch.zeros(5120, device=device, dtype=BF16)
+    for tables in ({}, {"scale": sc, "shift": sh}):
+        first = vdn_fp8.add_norm_quantize(r, b, w, 1e-6, return_normed=True, **tables)
+        check(first, formula(r, b, w, 1e-6, scale=sc[None] if tables else None, shift=sh[None] if tables else None), BF16)
+        for _ in range(20):
+            again = vdn_fp8.add_norm_quantize(r, b, w, 1e-6, return_normed=True, **tables)
+            assert all(torch.equal(p.view(torch.uint8), q.view(torch.uint8)) for p, q in zip(first, again))

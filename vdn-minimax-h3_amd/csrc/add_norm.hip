@@ -44,7 +44,7 @@ struct AddNormArgs {
     int64_t ldn;
 };
 
-// Codes of eight values n + low: (n + low) (R + R_low), R + R_low = 1 / scale before the scale's rounding; the
+// Codes of eight values n + low: (n + low) (R + R_low), R + R_low = 1 / scale before the scale's roundings; the
 // product and its corrections are rounded once. EXACT: the IEEE quotient, for scales that are not finite.
 template <bool EXACT>
 __device__ __forceinline__ uint2 codes8(const float (&n)[8], const float (&low)[8], float scale, float R, float R_low)
@@ -73,8 +73,8 @@ constexpr int64_t kOnceBytes = 256ll << 20;
 // A workgroup per row, of as many waves as its chunks fill: thread t holds chunk t, or t and t + threads, as
 // binary32 in registers from the addition to the codes, and the partial sums of squares and the maxima meet in
 // LDS. One chunk a thread makes a row short for the few of a step (16 of 5120: 4.1 us on the card); two halve what
-// every wave does once, which costs time where there are many (32760 of 5376, gated and modulated: 237 us and
-// 5.2 TB/s, as fast as a copy of those bytes; 243 with one chunk a thread). All loads go out before the first of
+// every wave does once, which costs time where there are many (32760 of 5376, gated and modulated: 243 us and
+// 5.1 TB/s, as fast as a copy of those bytes; with one chunk a thread 3% slower). All loads go out before the first of
 // them is used, the tables' as soon as the row's index is there; a table that is absent is a descriptor of no
 // bytes, which reads zeros. S, B: the types of the stream, and of the branch and its parameters; AFFINE: scale and
 // shift are there; ONCE: hidden is stored non-temporally.
@@ -83,6 +83,7 @@ __global__ __launch_bounds__(kMostWaves * kLanes) void k_add_norm(AddNormArgs p,
 {
     __shared__ float ssum[kMostWaves];
     __shared__ uint32_t smax[kMostWaves];
+    __shared__ int32_t slow;
     const int64_t row = first + blockIdx.x;
     const int lane = threadIdx.x & (kLanes - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kLanes);
     const int nch = (int)(p.K >> 3);
@@ -144,7 +145,10 @@ __global__ __launch_bounds__(kMostWaves * kLanes) void k_add_norm(AddNormArgs p,
     ss += __uint_as_float(dpp_u32<kDppXor2>(__float_as_uint(ss)));
     ss += __uint_as_float(dpp_u32<kDppHalfMirror>(__float_as_uint(ss)));
     ss += __uint_as_float(dpp_u32<kDppMirror>(__float_as_uint(ss)));
-    const float rstd = 1.0f / __builtin_sqrtf(ss / (float)p.K + p.eps);
+    // rstd + rstd_low = 1 / sqrt(square), the second a step of Newton's method (none where square is 0 or not finite)
+    const float square = ss / (float)p.K + p.eps, rstd = 1.0f / __builtin_sqrtf(square), root = square * rstd;
+    const float off = __builtin_fmaf(-root, rstd, 1.0f) - __builtin_fmaf(square, rstd, -root) * rstd;
+    const float rstd_low = __builtin_fabsf(off) < 0x1p-20f ? 0.5f * rstd * off : 0.0f;
 
     float top = 0.0f;
 #pragma unroll
@@ -158,10 +162,12 @@ __global__ __launch_bounds__(kMostWaves * kLanes) void k_add_norm(AddNormArgs p,
         float most = 0.0f;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            // n + low: low is what the rounding of h rstd, and without a shift that of its product with w, leaves out of
-            // n. A code moves where such errors carry a value across a border between two: of the 176 million codes of
-            // 32760 x 5376 172 do, 281 where n, the scale and the quotient are each rounded to binary32.
-            const float t = n[c][e] * rstd, t_low = __builtin_fmaf(n[c][e], rstd, -t);
+            // n + low: low is what the rounding of h rstd leaves out of n, and with a shift that of rstd (without one it cancels
+            // against the scale's), without a shift that of the product with w. A code moves where such errors carry a value across a
+            // border between two, the largest's (below) for a whole row: 150 of the 176 million codes of 32760 x 5376 do and none
+            // of 16 x 5120 without a shift; 292 and 8 where n, the scale and the quotient are each rounded to binary32.
+            const float t = n[c][e] * rstd, left = __builtin_fmaf(n[c][e], rstd, -t);
+            const float t_low = AFFINE ? __builtin_fmaf(n[c][e], rstd_low, left) : left;
             if (AFFINE) {
                 const float factor = f[e] * (1.0f + u[e]);
                 low[c][e] = t_low * factor;
@@ -176,14 +182,29 @@ __global__ __launch_bounds__(kMostWaves * kLanes) void k_add_norm(AddNormArgs p,
     }
     uint32_t bits = wave_max_u32(__float_as_uint(top) & 0x7fffffffu);
     if (lane == 0) smax[wave] = bits;
+    if (threadIdx.x == 0) slow = 0x80000000;
     __syncthreads();
     bits = wave_max_u32(lane % kMostWaves < waves ? smax[lane % kMostWaves] : 0u);
+    // the largest's own low part; of several that are as large a lane's last, and of lanes the largest (as integers in the same
+    // order), so that it is the same in every call
+    if (__float_as_uint(top) == bits) {
+        float rest = 0.0f;
+#pragma unroll
+        for (int c = 0; c < CPL; ++c)
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (__builtin_fabsf(n[c][e]) == top) rest = __builtin_copysignf(1.0f, n[c][e]) * low[c][e];
+        const int32_t word = (int32_t)__float_as_uint(rest);
+        __hip_atomic_fetch_max(&slow, word < 0 ? word ^ 0x7fffffff : word, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+    }
+    __syncthreads();
     const float most = __uint_as_float(bits), scale = row_scale(most);
     if (threadIdx.x == 0) p.y_scale[row] = scale;
-    // 1 / scale in two parts: 448 / most, or 1 / scale at the floor
+    // 1 / scale in two parts: 448 / (most and its low part), or 1 / scale at the floor
     const bool floor = most / 448.0f < 1e-12f;
     const float over = floor ? 1.0f : 448.0f, under = floor ? scale : most;
-    const float R = over / under, R_low = __builtin_fmaf(-R, under, over) / under;
+    const float rest = floor ? 0.0f : __uint_as_float((uint32_t)(slow < 0 ? slow ^ 0x7fffffff : slow));
+    const float R = over / under, R_low = (__builtin_fmaf(-R, under, over) - R * rest) / under;
     const bool finite = __builtin_isfinite(scale);
     const __amdgpu_buffer_rsrc_t yr = row_buffer(p.y + row * p.ldy, p.K);
     const __amdgpu_buffer_rsrc_t nr = row_buffer(p.normed ? (uint8_t*)p.normed + row * p.ldn * element_bytes(B) : p.y, p.normed ? bbytes : 0);
