@@ -316,3 +316,26 @@ def test_rows_of_float32_are_refused(device):
     with pytest.raises(ValueError, match="bfloat16 or float16"):
         f(torch.randn(4, 512, device=device), adapters=bank(device, 2, 16, 512, 384, BF16, 2),
           index=torch.zeros(4, device=device, dtype=torch.int32))
+
+
+@pytest.mark.parametrize("T", [300, 1300])
+def test_graphs_of_the_other_forms(device, T):
+    """A step and a prompt, captured, replayed with other requests and rows between eager calls (which take workspaces of their own)."""
+    x, base = rows(device, T, 1024, 520, BF16, 1)
+    ad = bank(device, 4, 96, 1024, 520, BF16, 2)
+    index = torch.zeros(T, device=device, dtype=torch.int32)
+    adapter_add(x, base, ad, index)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = adapter_add(x, base, ad, index)
+        twice = adapter_add(x, out, ad, index)
+    for step in range(5):
+        index.copy_(choose(device, T, 4, ("random", "runs", "one")[step % 3], step))
+        x.copy_(rows(device, T, 1024, 8, BF16, 50 + step)[0])
+        graph.replay()
+        want = adapter_add(x, base, ad, index)
+        want_twice = adapter_add(x, want, ad, index)
+        torch.cuda.synchronize()
+        assert torch.equal(out, want) and torch.equal(twice, want_twice)
+        check(out, x, base, ad, index)

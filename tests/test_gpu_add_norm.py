@@ -238,3 +238,10 @@ def test_equal_maxima(device):
         for _ in range(20):
             again = vdn_fp8.add_norm_quantize(r, b, w, 1e-6, return_normed=True, **tables)
             assert all(torch.equal(p.view(torch.uint8), q.view(torch.uint8)) for p, q in zip(first, again))
+
+
+def test_more_rows_than_a_launch_takes(device):
+    M, K = (1 << 21) + 37, 8
+    r, b, w, gate, sc, sh, index = inputs(device, M, K, BF16, BF16, 5, 1)
+    got = vdn_fp8.add_norm_quantize(r, b, w, 1e-6, gate=gate, scale=sc, shift=sh, indices=index, return_normed=True)
+    check(got, formula(r, b, w, 1e-6, gate, sc, sh, index), BF16)

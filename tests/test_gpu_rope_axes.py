@@ -174,3 +174,15 @@ def test_offsets_beyond_32_bits(device):
     got = vdn_fp8.qk_prep_axes(query, key, nq, nk, rope, positions)
     for out, x, norm in zip(got, (q, k), (nq, nk)):
         check(out[-40:], x, norm, rope, positions[-40:])
+
+
+def test_more_tokens_than_a_launch_takes(device):
+    T, rope = (1 << 25) + 70, RopeAxes.make((8, 12, 12), device=device)
+    q, _, nq, _ = heads(device, 100, 1, 1, 64, BF16, 1)
+    query = torch.empty(T, 1, 64, device=device, dtype=BF16)
+    query.fill_(1.0)
+    query[-100:] = q
+    positions = torch.arange(T, device=device, dtype=torch.int32)[:, None].expand(T, 3)
+    out, none = vdn_fp8.qk_prep_axes(query, query[:, :0], nq, None, rope, positions)
+    assert none.shape == (T, 0, 64)
+    check(out[-100:], q, nq, rope, positions[-100:])
