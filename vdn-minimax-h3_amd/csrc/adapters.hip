@@ -970,11 +970,14 @@ Plan plan_of(int64_t T, int64_t K, int64_t N, int64_t L, int64_t R)
     } else {
         const int64_t steps = ceil_div(K, kBk), columns = ceil_div(N, kBn);
         p.rank_frags = (int)(R / 16);
-        // workgroups to fill the card, and two (k) or four (n) of each tile even so: a workgroup's first steps wait for memory
-        int64_t parts = ceil_div(kFill, p.tiles), blocks = kFill / p.tiles;
+        // Workgroups to fill the card (k), two rounds of them where the tiles alone are more than the compute units and would be an
+        // uneven one (20000 x 5376 -> 1024, rank 128, 16: 127 and 79 us with two parts, 117 and 74 with four); but seven steps of k in each, as
+        // its first ones wait for memory and the second product fetches every part (1600 tokens, rank 128: 33 us with 21 parts, 26 with
+        // six; 4800: 45 and 42).
+        int64_t parts = ceil_div(p.tiles > 256 ? 2 * kFill : kFill, p.tiles), blocks = kFill / p.tiles;
         const int64_t eighths = ceil_div(columns, 8);
         if (parts < 2) parts = 2;
-        if (parts > ceil_div(steps, 4)) parts = ceil_div(steps, 4);
+        if (parts > ceil_div(steps, 7)) parts = ceil_div(steps, 7);
         p.span_k = (int)(kBk * ceil_div(steps, parts));
         p.parts = (int)ceil_div(K, p.span_k);
         // Above 64 ranks two workgroups of k_expand_tile are all that a compute unit has registers for, and where four or more of a tile are
