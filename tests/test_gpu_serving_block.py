@@ -156,3 +156,43 @@ def test_a_step_in_a_graph(device):
         want = step(*other)
         torch.cuda.synchronize()
         assert all(torch.equal(a, b_) for a, b_ in zip(out, want)), n
+
+
+@pytest.mark.parametrize("choice", [{}, {"top": 2, "query_block": 32}], ids=["dense", "top"])
+def test_rows_that_attention_refuses_are_refused_before_the_store(device, choice):
+    """float32 rows, which the rotation and the store take and attention does not: with `rope` nothing is stored either."""
+    m = model(device)
+    cache, table = cache_of(device, 1, 2)
+    lengths = torch.full((1,), 4, dtype=torch.int32, device=device)
+    for t in cache:
+        t.view(torch.uint8).fill_(7)
+    x = torch.randn(4, HIDDEN, device=device)
+    projections = [torch.nn.Linear(HIDDEN, n * D, bias=False, device=device).requires_grad_(False) for n in (HQ, H, H)]
+    norms = [types.SimpleNamespace(weight=torch.ones(D, device=device), eps=1e-6) for _ in "qk"]
+    positions = torch.zeros(4, 3, dtype=torch.int32, device=device)
+    with pytest.raises(ValueError, match="bfloat16, float16"):
+        cached_attention(x, *projections, *norms, cache, table, lengths, rope=m.rope, positions=positions, **choice)
+    torch.cuda.synchronize()
+    assert all(bool((t.view(torch.uint8) == 7).all()) for t in cache)
+
+
+def test_float16_rows(device):
+    """A float16 block by `rope`: each call's result has the bits of its parts."""
+    m = model(device)
+    g = torch.Generator(device).manual_seed(2)
+    cache, table = cache_of(device, 2, 2)
+    other, _ = cache_of(device, 2, 2)
+    weights = [(torch.randn(n * D, HIDDEN, device=device, generator=g) / 32).half() for n in (HQ, H, H)]
+    projections = [lambda t, w=w: t @ w.T for w in weights]
+    norms = [types.SimpleNamespace(weight=torch.ones(D, device=device, dtype=torch.float16), eps=1e-6) for _ in "qk"]
+    for length in (30, 31):
+        T = 60 if length == 30 else 2
+        x = torch.randn(T, HIDDEN, device=device, generator=g).half()
+        lengths = torch.full((2,), length, dtype=torch.int32, device=device)
+        positions = torch.arange(T, device=device, dtype=torch.int32)[:, None].expand(T, 3)
+        got = cached_attention(x, *projections, *norms, cache, table, lengths, rope=m.rope, positions=positions, causal=True)
+        q, k, v = (p(x).unflatten(1, (-1, D)) for p in projections)
+        q, k = vdn_fp8.qk_prep_axes(q, k, *((n.weight, n.eps) for n in norms), m.rope, positions)
+        vdn_fp8.kv_append(k, v, other, table, lengths)
+        want = vdn_fp8.kv_attention(q, other, table, lengths, causal=True)
+        assert got.dtype == torch.float16 and torch.equal(got, want.flatten(1))

@@ -124,15 +124,19 @@ def _batch(page_table, lengths, q_start, tokens, pages, device):
     return _lib.KvBatchStruct(page_table.data_ptr(), ld if B > 1 else W, W, lengths.data_ptr(), start, B, tokens)
 
 
+def _not_rows(t, heads, d, name, dtypes):
+    names = ", ".join(str(x).replace("torch.", "") for x in dtypes)
+    return ValueError(f"{name} must be a {names} [T, {'heads' if heads is None else heads}, {d}] tensor "
+                      f"(got {t.dtype} {tuple(t.shape)})")
+
+
 def _rows(t, heads, d, name, dtypes):
     """[T, heads, d] with contiguous heads on the GPU, 16-byte aligned rows; a copy where it is not."""
     if not t.is_cuda:
         raise ValueError(f"the cache's kernels run on the GPU; {name} is a CPU tensor")
     shape = t.shape
     if len(shape) != 3 or t.dtype not in dtypes or shape[2] != d or (heads is not None and shape[1] != heads):
-        names = ", ".join(str(x).replace("torch.", "") for x in dtypes)
-        raise ValueError(f"{name} must be a {names} [T, {'heads' if heads is None else heads}, {d}] tensor "
-                         f"(got {t.dtype} {tuple(t.shape)})")
+        raise _not_rows(t, heads, d, name, dtypes)
     token, head, unit = t.stride()
     if unit != 1 or head != d or token % 8 or token < shape[1] * d or t.data_ptr() % 16:
         t = t.clone(memory_format=torch.contiguous_format)
@@ -283,6 +287,8 @@ def check_attention(query, cache, page_table, lengths, *, scale=None, q_start=No
         raise ValueError(f"max_query must not be negative (got {max_query})")
     if not query.is_cuda:
         raise ValueError("the cache's kernels run on the GPU; query is a CPU tensor")
+    if query.dtype not in _QUERY_DTYPES or query.shape[2] != d:
+        raise _not_rows(query, None, d, "query", _QUERY_DTYPES)
     # what the library refuses by sizes
     b = _batch(page_table, lengths, q_start, T, c.pages, dev)
     with _on(dev):
