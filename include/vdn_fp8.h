@@ -498,7 +498,8 @@ int vdn_fp8_add_norm_quantize(const void *residual, int stream_type, int64_t ldr
  *   out[t][n] = base[t][n] where index[t] is outside [0, L)
  * x [T, K], base and out [T, N], a [L, R, K], b [L, N, R] of dtype (bf16 or binary16), scale
  * binary32 [L], index [T]. The first product is accumulated and kept in binary32, and enters the
- * second so (one launch) or as two 16-bit parts (2^-17 of it or less is left out). out may be base itself
+ * second so (one launch) or as two 16-bit parts, which leave out 2^-17 of it or less (bf16; of what is above 2^-100) or
+ * 2^-23 of the token's largest or less (binary16). out may be base itself
  * (with its stride); nothing else may overlap (out over x, or over part of base, is VDN_FP8_EINVAL). The same
  * inputs give the same bits, and a token's do not depend on the others' values. workspace: device memory,
  * 16-byte aligned, of the size asked for with the same T, K, N, L, R (0: none is needed, NULL will do); it need

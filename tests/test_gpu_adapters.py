@@ -339,3 +339,49 @@ def test_graphs_of_the_other_forms(device, T):
         torch.cuda.synchronize()
         assert torch.equal(out, want) and torch.equal(twice, want_twice)
         check(out, x, base, ad, index)
+
+
+# Values in [1, 2) of 18 bits. Both 16-bit parts of one are multiples of 2^-17, as it is itself, so every sum below is one of a
+# few such multiples of at most 4 and is exact in binary32 in any order: what is off is the split alone, 2^-17 at most.
+@pytest.mark.parametrize("T", [40, 500, 1500])
+@pytest.mark.parametrize("R", [16, 48, 128])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_what_the_second_product_gets_of_the_first(device, T, R, dtype):
+    """h in three ranks: a value, less its two largest 16-bit parts. What is left of the sum is below 2^-17, and so is what the
+    kernel may lose of the value."""
+    g = torch.Generator().manual_seed(R)
+    h = 1 + torch.randint(0, 1 << 17, (T,), generator=g).double() / (1 << 17)
+    h[:4] = torch.tensor([1 + 2.0 ** -8 + 2.0 ** -16, 1 + 2.0 ** -7 - 2.0 ** -17, 1 + 2.0 ** -8 + 3 * 2.0 ** -17, 2 - 2.0 ** -17])
+    top = h.to(BF16).double()
+    middle = (h - top).to(BF16).double()
+    rest = h - top - middle
+    assert float(rest.abs().max()) <= 2.0 ** -17
+    K, N = 8, 136
+    x = torch.zeros(T, K, dtype=torch.float64)
+    x[:, 0], x[:, 1], x[:, 2] = top, middle, rest
+    a, b = torch.zeros(1, R, K), torch.zeros(1, N, R)
+    a[0, 0, :3] = 1
+    a[0, 1, 0] = a[0, 2, 1] = -1
+    b[0, :, :3] = 1
+    assert torch.equal(x.to(dtype).double(), x)
+    ad = Adapters(a.to(dtype).to(device), b.to(dtype).to(device), torch.ones(1, device=device))
+    index, base = torch.zeros(T, dtype=torch.int32, device=device), torch.zeros(T, N, dtype=dtype, device=device)
+    got = adapter_add(x.to(dtype).to(device), base, ad, index).double().cpu()
+    # (the result is rounded to its type: half a step of what is at most 2^-16)
+    assert torch.all((got - rest[:, None]).abs() <= 2.0 ** -17 + 2.0 ** -16 * torch.finfo(dtype).eps / 2), float((got - rest[:, None]).abs().max() * 2 ** 17)
+
+
+@pytest.mark.parametrize("T", [40, 500, 1500])
+def test_products_beyond_bfloat16(device, T):
+    """h between bfloat16's largest and binary32's, with a small B: the result is in range, with h's own accuracy."""
+    top = float(torch.finfo(BF16).max)
+    x, base = torch.zeros(T, 8, device=device, dtype=BF16), torch.zeros(T, 72, device=device, dtype=BF16)
+    x[:, 0] = top
+    x[:, 1] = 2.0 ** 119 * (1 + torch.arange(T, device=device) % 64 / 64)          # (below 2^120: h below 2^128)
+    x[1::2] *= -1
+    a, b = torch.zeros(1, 16, 8, device=device, dtype=BF16), torch.full((1, 72, 16), 2.0 ** -20, device=device, dtype=BF16)
+    a[0, 0, :2] = 1
+    ad = Adapters(a, b, torch.ones(1, device=device))
+    assert float((x.double() @ a[0].double().T).abs().max()) > top
+    index = torch.zeros(T, device=device, dtype=torch.int32)
+    check(adapter_add(x, base, ad, index), x, base, ad, index)

@@ -6,7 +6,7 @@
 // in two launches: k_shrink_* write h, binary32, in S parts summed over disjoint ranges of k; k_expand_* add the parts and
 // the second product to the base. A step of few tokens is one launch (k_few). All are bound by memory (2 R operations for
 // each element of x and of base, R <= 128), so the matrix cores have time to spare: h is not rounded to 16 bits between the
-// products but goes in as two of them, a high and a low part, which keeps 2^-17 of it and costs the second product twice over
+// products but goes in as two of them, a high and a low part, which lose 2^-17 of it at most and cost the second product twice over
 // (1.5 us of 61 at 6470 tokens of rank 128).
 //
 // On the card: 32760 tokens, 5120 -> 15360, rank 64: 70 + 374 us, 5.2 TB/s of the bytes that it cannot do without (a large copy
@@ -327,9 +327,12 @@ __global__ __launch_bounds__(kWaves * kLanes) void k_shrink_tile(AdapterArgs p)
 // out = base + scale h B^T
 // ---------------------------------------------------------------------------
 
-// Eight ranks of h as two operands of eight 16-bit values, high and low part. bf16: the upper half of the word and what it leaves
-// (16 bits in all, whatever the size). float16: relative to the power of two 2^e above the token's largest, e back in the result,
-// so that no h is too large for it.
+constexpr float kMostBf16 = 0x1.fep127f;
+
+// Eight ranks of h as two operands of eight 16-bit values, high and low part. bf16: h rounded to nearest and what that leaves, 2^-8 of
+// it at most, rounded likewise: 2^-17 of h is lost at most (a high part of truncated words would leave 2^-7, and lose 2^-16).
+// float16: relative to the power of two 2^e above the token's largest, e back in the result, so that no h is too large
+// for it; 2^-24 of that power of two is lost at most, whatever the size of h.
 template <int TYPE>
 __device__ __forceinline__ void split8(const float (&h)[8], float down, uint4& high, uint4& low)
 {
@@ -337,12 +340,11 @@ __device__ __forceinline__ void split8(const float (&h)[8], float down, uint4& h
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
         if (TYPE == kBf16) {
-            const uint32_t u0 = __float_as_uint(h[2 * e]), u1 = __float_as_uint(h[2 * e + 1]);
-            a[e] = (u0 >> 16) | (u1 & 0xffff0000u);
-            // (an infinity leaves nothing: the difference would be NaN)
-            const float l0 = __builtin_isfinite(h[2 * e]) ? h[2 * e] - __uint_as_float(u0 & 0xffff0000u) : 0.0f;
-            const float l1 = __builtin_isfinite(h[2 * e + 1]) ? h[2 * e + 1] - __uint_as_float(u1 & 0xffff0000u) : 0.0f;
-            b[e] = pack_bf16x2(l0, l1);
+            const float v0 = h[2 * e], v1 = h[2 * e + 1];
+            const bool in0 = __builtin_isfinite(v0), in1 = __builtin_isfinite(v1);
+            // (what would round to infinity takes bf16's largest; an infinity leaves nothing: the difference would be NaN)
+            a[e] = pack_bf16x2(in0 ? fminf(fmaxf(v0, -kMostBf16), kMostBf16) : v0, in1 ? fminf(fmaxf(v1, -kMostBf16), kMostBf16) : v1);
+            b[e] = pack_bf16x2(in0 ? v0 - bf16_lo(a[e]) : 0.0f, in1 ? v1 - bf16_hi(a[e]) : 0.0f);
         } else {
             f16x2_t hi, lo;
 #pragma unroll
