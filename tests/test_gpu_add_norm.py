@@ -245,3 +245,16 @@ def test_more_rows_than_a_launch_takes(device):
     r, b, w, gate, sc, sh, index = inputs(device, M, K, BF16, BF16, 5, 1)
     got = vdn_fp8.add_norm_quantize(r, b, w, 1e-6, gate=gate, scale=sc, shift=sh, indices=index, return_normed=True)
     check(got, formula(r, b, w, 1e-6, gate, sc, sh, index), BF16)
+
+
+@pytest.mark.parametrize("kind,rows", [(torch.uint8, 300), (torch.uint8, 20), (torch.int8, 200), (torch.int8, 128), (torch.int8, 129),
+                                       (torch.int16, 33000), (torch.bool, 2), (torch.bool, 1), (torch.int64, 300)])
+def test_indices_narrower_than_the_table(device, kind, rows):
+    """Indices of any integer type (or truth values), also of one that does not hold the table's last row: clamped as others are."""
+    g = torch.Generator().manual_seed(rows)
+    M, K = 40, 64
+    r, b, gate = (torch.randn(n, K, generator=g).to(BF16).to(device) for n in (M, M, rows))
+    index = torch.randint(-128, 128, (M,), generator=g).to(kind).to(device)
+    got = vdn_fp8.add_norm_quantize(r, b, None, 1e-6, gate=gate, indices=index)
+    want = vdn_fp8.add_norm_quantize(r, b, None, 1e-6, gate=gate, indices=index.long().clamp(0, rows - 1).int())
+    assert all(torch.equal(p.view(torch.uint8), q.view(torch.uint8)) for p, q in zip(got, want))

@@ -236,8 +236,8 @@ def add_norm_quantize(residual, branch, weight, eps, *, gate=None, scale=None, s
             raise ValueError("indices must hold one table row per token")
         check_index_range(indices, rows, "add_norm_quantize: indices")
         if indices.dtype is not torch.int32 or indices.get_device() != at or not indices.is_contiguous():
-            # (a wider index is clamped before it is narrowed)
-            indices = indices.to(r.device).clamp(0, rows - 1).to(torch.int32).contiguous()
+            # (clamped in 64 bits: a wider index before it is narrowed, and a narrower one's type need not hold the last row)
+            indices = indices.to(r.device, torch.int64).clamp(0, rows - 1).to(torch.int32).contiguous()
         of_indices = indices.data_ptr()
     # (empty_like is the shortest way to a new tensor: 1.1 us)
     like = r if ldr == K and r.is_contiguous() else torch.empty(M, K, device=r.device, dtype=stream)
