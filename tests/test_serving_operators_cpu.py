@@ -126,3 +126,17 @@ def test_rope_axes():
     for bad in ((), (0,), (-1, 9)):
         with pytest.raises(ValueError):
             RopeAxes.make(bad, device="cpu")
+
+
+def test_one_bank_for_three_projections_is_refused():
+    """A bank is a tuple of three itself: refused before a projection runs, not taken apart."""
+    bank = Adapters(torch.zeros(1, 16, 64).bfloat16(), torch.zeros(1, 64, 16).bfloat16(), torch.ones(1))
+    cache = vdn_fp8.KvCache.empty(1, 1, 64, "cpu")
+
+    def unreached(x):
+        raise AssertionError("a projection ran")
+
+    with pytest.raises(ValueError, match="three banks"):
+        vdn_fp8.softmax_attention.cached_attention(torch.zeros(4, 64).bfloat16(), unreached, unreached, unreached, None, None, cache,
+                                                   torch.zeros(1, 1, dtype=torch.int32), torch.full((1,), 4, dtype=torch.int32),
+                                                   adapters=bank, index=torch.zeros(4, dtype=torch.int32))

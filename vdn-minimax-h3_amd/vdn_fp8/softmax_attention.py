@@ -215,6 +215,8 @@ def cached_attention(x, to_q, to_k, to_v, norm_q, norm_k, cache, page_table, len
         raise ValueError("rope and positions go together, in place of rotary_emb")
     if (adapters is None) != (index is None) or (adapters is not None and len(adapters) != 3):
         raise ValueError("adapters (of to_q, to_k and to_v) and index go together")
+    if adapters is not None and any(isinstance(bank, torch.Tensor) for bank in adapters):   # (one bank has three parts as well)
+        raise ValueError("adapters must be three banks, of to_q, to_k and to_v (or None for one without); got the tensors of one")
     out = _project(x, (to_q, to_k, to_v))
     if adapters is not None:
         from .fp8_linear import Fp8Linear
