@@ -478,7 +478,8 @@ int vdn_fp8_kv_select(const vdn_fp8_kv_cache *cache, const vdn_fp8_kv_batch *bat
  * with i = index[m] (row 0 if NULL), clamped into [0, rows). n is not rounded before the codes.
  * stream_type: VDN_FP8_DTYPE_* of residual and hidden; dtype: of branch, gate, weight, mod_scale,
  * mod_shift and normed. gate, weight, mod_scale with mod_shift, index and normed may be NULL. hidden
- * may be residual or branch itself (with its stride); nothing else may overlap.
+ * may be residual or branch itself (with its stride and type); nothing else may overlap (hidden, y or
+ * normed over other rows is VDN_FP8_EINVAL).
  * Replaces: nothing in one call; `post`, then `pre`, then quantize_rows
  *           (src/models/ops/fused_block.py:41-49, fp8_linear.py:110-117), which round n to bf16 between.
  * Requires: stream_type = dtype, or VDN_FP8_DTYPE_F32; K % 8 == 0, 8 <= K <= 16384; strides

@@ -12,6 +12,7 @@ import pytest
 import torch
 
 import vdn_fp8
+import vdn_fp8._lib as L
 
 pytestmark = pytest.mark.gpu
 
@@ -258,3 +259,40 @@ def test_indices_narrower_than_the_table(device, kind, rows):
     got = vdn_fp8.add_norm_quantize(r, b, None, 1e-6, gate=gate, indices=index)
     want = vdn_fp8.add_norm_quantize(r, b, None, 1e-6, gate=gate, indices=index.long().clamp(0, rows - 1).int())
     assert all(torch.equal(p.view(torch.uint8), q.view(torch.uint8)) for p, q in zip(got, want))
+
+
+def call(r, b, w, hidden, y, s, normed):
+    """The C entry point, without tables."""
+    M, K = r.shape
+    types = {BF16: L.DTYPE_BF16, F16: L.DTYPE_F16, F32: L.DTYPE_F32}
+    L.check(L.load().vdn_fp8_add_norm_quantize(
+        r.data_ptr(), types[r.dtype], r.stride(0), b.data_ptr(), types[b.dtype], b.stride(0), M, K, None, 0, w.data_ptr(), 1e-6, None, None, 0, None,
+        0, hidden.data_ptr(), hidden.stride(0), y.data_ptr(), y.stride(0), s.data_ptr(), normed.data_ptr(), normed.stride(0),
+        torch.cuda.current_stream().cuda_stream), "add_norm_quantize")
+
+
+@pytest.mark.parametrize("M,K", [(1, 264), (16, 5120), (700, 4104)])
+@pytest.mark.parametrize("stream,dtype,over", [(*t, over) for t in TYPES for over in ("residual", "branch", "both") if over != "both" or t[0] is t[1]])
+def test_hidden_in_place(device, M, K, stream, dtype, over):
+    """hidden over residual, over a branch of its type, over both where they are one: the bits of a new tensor. Rows lie apart, and
+    what lies between them stays."""
+    r, b, w, *_ = inputs(device, M, K, stream, dtype, 1, M + K)
+    wide = [torch.full((M, K + 24), 7.0, device=device, dtype=t.dtype) for t in (r, b)]
+    if over == "both":
+        b = r.clone()
+        wide[1] = wide[0]
+    rows = [t[:, 8:8 + K] for t in wide]
+    rows[0].copy_(r), rows[1].copy_(b)
+    want = vdn_fp8.add_norm_quantize(r, b, w, 1e-6, return_normed=True)
+    y, s, normed = torch.empty(M, K, device=device, dtype=E4M3), torch.empty(M, 1, device=device), torch.empty(M, K, device=device, dtype=dtype)
+    hidden = rows[over == "branch"]
+    if over == "branch" and stream is not dtype:
+        kept = [t.clone() for t in wide]
+        with pytest.raises(ValueError, match="with its stride and type"):
+            call(*rows, w, hidden, y, s, normed)
+        assert all(torch.equal(t, k) for t, k in zip(wide, kept))
+        return
+    call(*rows, w, hidden, y, s, normed)
+    for got, t in zip((hidden, y, s, normed), want):
+        assert torch.equal(got.contiguous().view(torch.uint8), t.view(torch.uint8))
+    assert all(bool((t[:, :8] == 7).all() and (t[:, 8 + K:] == 7).all()) for t in wide)

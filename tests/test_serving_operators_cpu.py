@@ -140,3 +140,27 @@ def test_one_bank_for_three_projections_is_refused():
         vdn_fp8.softmax_attention.cached_attention(torch.zeros(4, 64).bfloat16(), unreached, unreached, unreached, None, None, cache,
                                                    torch.zeros(1, 1, dtype=torch.int32), torch.full((1,), 4, dtype=torch.int32),
                                                    adapters=bank, index=torch.zeros(4, dtype=torch.int32))
+
+
+def apart(**over):
+    """`norm` of four rows of 64 in places of their own (bf16), less what `over` puts elsewhere."""
+    return norm(**{**dict(r=FAKE, b=FAKE + (1 << 16), h=OTHER, y=OTHER + (1 << 16), s=OTHER + (1 << 18)), **over})
+
+
+@pytest.mark.parametrize("over,needle", [
+    # hidden over residual or branch with another stride, or in part: rows, columns that meet, columns that wrap into a row
+    (dict(h=FAKE, ldh=72), "residual or branch itself"), (dict(h=FAKE + (1 << 16), ldh=72), "residual or branch itself"),
+    (dict(h=FAKE + 128), "residual or branch itself"), (dict(h=FAKE + (1 << 16) + 3 * 128), "residual or branch itself"),
+    (dict(h=FAKE + 64, ldr=96, ldh=96), "residual or branch itself"), (dict(r=OTHER, h=OTHER + 112, ldr=96, ldh=96), "residual or branch itself"),
+    # a binary32 stream over a branch of 16 bits: a row of it is two of the branch's
+    (dict(h=FAKE + (1 << 16), stream=2), "residual or branch itself"), (dict(h=FAKE + (1 << 16), stream=2, M=1), "residual or branch itself"),
+    (dict(h=FAKE + (1 << 16), stream=2, dtype=1), "residual or branch itself"),
+    (dict(r=FAKE, h=FAKE, b=FAKE, stream=2), "residual or branch itself"),
+    # in place, and the other rows over them
+    (dict(h=FAKE, y=FAKE), "y and normed"), (dict(y=FAKE + 128), "y and normed"), (dict(y=FAKE + (1 << 16) + 3 * 128 + 120), "y and normed"),
+    (dict(y=OTHER), "y and normed"), (dict(n=FAKE), "y and normed"), (dict(n=FAKE + (1 << 16)), "y and normed"), (dict(n=OTHER), "y and normed"),
+    (dict(n=OTHER + (1 << 16) + 240), "y and normed"),
+])
+def test_rows_that_share_memory_are_einval(over, needle):
+    assert apart(**over) == L.EINVAL
+    assert needle in L.load().vdn_fp8_last_error().decode()

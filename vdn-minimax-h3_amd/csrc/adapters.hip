@@ -1081,16 +1081,6 @@ int check_sizes(int64_t T, int64_t K, int64_t N, int64_t L, int64_t R)
     return VDN_FP8_OK;
 }
 
-// Whether rows [T, columns] of 16-bit elements share memory with others. Two column ranges of one matrix do not.
-bool rows_overlap(const void* a, int64_t lda, int64_t of_a, const void* b, int64_t ldb, int64_t of_b, int64_t T)
-{
-    const int64_t from_a = (int64_t)(uintptr_t)a, from_b = (int64_t)(uintptr_t)b;
-    if (from_a + ((T - 1) * lda + of_a) * 2 <= from_b || from_b + ((T - 1) * ldb + of_b) * 2 <= from_a) return false;
-    if (lda != ldb) return true;
-    const int64_t ld = lda * 2, apart = ((from_b - from_a) % ld + ld) % ld;   // b's columns behind a's
-    return apart < of_a * 2 || apart + of_b * 2 > ld;
-}
-
 }  // namespace
 }  // namespace vdn
 
@@ -1120,8 +1110,8 @@ extern "C" int vdn_fp8_adapter_add(const void* x, int dtype, int64_t ldx, const 
     if (!aligned(x, 16) || !aligned(base, 16) || !aligned(out, 16) || !aligned(a, 16) || !aligned(b, 16) || !aligned(scale, 4) || !aligned(index, 4))
         return set_error(VDN_FP8_EINVAL, "%s: misaligned pointer (x, base, out, A, B 16 B)", what);
     // (workgroups read all of x, and write their columns of out when they are done with them)
-    if (rows_overlap(x, ldx, K, out, ldo, N, T)) return set_error(VDN_FP8_EINVAL, "%s: out must not overlap x", what);
-    if (out == base ? ldo != ldbase : rows_overlap(base, ldbase, N, out, ldo, N, T))
+    if (rows_overlap(x, ldx * 2, K * 2, out, ldo * 2, N * 2, T)) return set_error(VDN_FP8_EINVAL, "%s: out must not overlap x", what);
+    if (out == base ? ldo != ldbase : rows_overlap(base, ldbase * 2, N * 2, out, ldo * 2, N * 2, T))
         return set_error(VDN_FP8_EINVAL, "%s: out must be base itself, with its stride, or not overlap it", what);
     const Plan plan = plan_of(T, K, N, L ? L : 1, R);
     const int64_t need = L ? workspace_bytes_of(plan, R) : 0;

@@ -270,6 +270,17 @@ extern "C" int vdn_fp8_add_norm_quantize(const void* residual, int stream_type, 
         !aligned(normed, 16) || !aligned(gate, 16) || !aligned(weight, 16) || !aligned(mod_scale, 16) || !aligned(mod_shift, 16) ||
         !aligned(index, 4))
         return set_error(VDN_FP8_EINVAL, "%s: misaligned pointer (rows, weight and tables 16 B; y 8 B)", what);
+    // (workgroups write their rows when they are done with them, in any order)
+    struct Rows { const void* at; int64_t ld, bytes; };
+    const int64_t S = element_bytes(stream_type), B = element_bytes(dtype);
+    auto overlap = [&](const Rows& a, const Rows& b) { return a.at && b.at && rows_overlap(a.at, a.ld, a.bytes, b.at, b.ld, b.bytes, M); };
+    const Rows r{residual, ldr * S, K * S}, b{branch, ldb * B, K * B}, h{hidden, ldh * S, K * S}, codes{y, ldy, K}, n{normed, ldn * B, K * B};
+    if ((hidden == residual ? M > 1 && ldh != ldr : overlap(r, h)) ||
+        (hidden == branch ? stream_type != dtype || (M > 1 && ldh != ldb) : overlap(b, h)))
+        return set_error(VDN_FP8_EINVAL, "%s: hidden must be residual or branch itself, with its stride and type, or not overlap them", what);
+    for (const Rows& in : {r, b, h})
+        if (overlap(in, codes) || overlap(in, n)) return set_error(VDN_FP8_EINVAL, "%s: y and normed must not overlap the other rows", what);
+    if (overlap(codes, n)) return set_error(VDN_FP8_EINVAL, "%s: y and normed must not overlap the other rows", what);
     const AddNormArgs p{residual, ldr, branch, ldb, gate, ldgate, weight, mod_scale, mod_shift, ldmod, index, rows, eps, M, K,
                         hidden, ldh, (uint8_t*)y, ldy, y_scale, normed, ldn};
     if (stream_type == kF32)

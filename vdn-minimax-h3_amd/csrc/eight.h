@@ -94,4 +94,15 @@ __device__ __forceinline__ Eight<TYPE> encode8(const float (&x)[8])
     return v;
 }
 
+// host: whether two sets of `rows` rows share memory, of of_a and of_b bytes, lda and ldb bytes apart. Two column
+// ranges of one matrix do not.
+inline bool rows_overlap(const void* a, int64_t lda, int64_t of_a, const void* b, int64_t ldb, int64_t of_b, int64_t rows)
+{
+    const int64_t from_a = (int64_t)(uintptr_t)a, from_b = (int64_t)(uintptr_t)b;
+    if (from_a + (rows - 1) * lda + of_a <= from_b || from_b + (rows - 1) * ldb + of_b <= from_a) return false;
+    if (lda != ldb) return true;
+    const int64_t apart = ((from_b - from_a) % lda + lda) % lda;   // b's columns behind a's
+    return apart < of_a || apart + of_b > lda;
+}
+
 }  // namespace vdn
