@@ -527,7 +527,8 @@ int vdn_fp8_adapter_add(const void *x, int dtype, int64_t ldx, const void *base,
  *   out[i]  = n[i] for i >= rotary_dim
  * query [T, q_heads, d], key [T, k_heads, d], their outputs and weights [d] of dtype; positions
  * [T, axes] of position_type, row stride ldpos; inv_freq binary64 and axis (clamped into [0, axes))
- * [rotary_dim / 2]. Either side may have no heads. An output may be its input itself (with its stride).
+ * [rotary_dim / 2]. Either side may have no heads. An output may be its own input (with its stride); over
+ * other rows it is VDN_FP8_EINVAL.
  * Replaces: `_qk_prep` of q and of k (src/models/softmax_attention/kernels.py:8-45) and the tables of
  *           the caller's rotary embedding, whose bf16 rounding (`cos.to(x.dtype)`) is not taken over.
  * Requires: d in {64, 128, 256}; heads * d <= 65536; rotary_dim in [0, d], a multiple of 16 (pairs: 8); 1 to 8 axes;

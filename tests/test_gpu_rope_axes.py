@@ -9,6 +9,7 @@ import pytest
 import torch
 
 import vdn_fp8
+import vdn_fp8._lib as L
 from vdn_fp8 import RopeAxes
 
 pytestmark = pytest.mark.gpu
@@ -186,3 +187,24 @@ def test_more_tokens_than_a_launch_takes(device):
     out, none = vdn_fp8.qk_prep_axes(query, query[:, :0], nq, None, rope, positions)
     assert none.shape == (T, 0, 64)
     check(out[-100:], q, nq, rope, positions[-100:])
+
+
+@pytest.mark.parametrize("T", [1, 16, 1500])
+@pytest.mark.parametrize("d,dtype,pairs", [(64, F16, True), (128, BF16, False), (256, F32, False)])
+def test_outputs_in_place(device, T, d, dtype, pairs):
+    """The C entry with each output in its input's place, column slices of one fused matrix: the bits of new tensors, and the
+    columns of the values stay."""
+    Hq, H = 5, 3
+    rope = RopeAxes.make((d // 4, d // 4), pairs=pairs, device=device)
+    qkv = torch.randn(T, (Hq + 2 * H) * d, device=device).to(dtype)
+    before = qkv.clone()
+    q, k, v = (t.unflatten(1, (-1, d)) for t in qkv.split((Hq * d, H * d, H * d), 1))
+    w = (1 + 0.2 * torch.randn(d, device=device)).to(dtype)
+    pos = torch.randint(0, 3000, (T, 2), device=device).int()
+    want = vdn_fp8.qk_prep_axes(q, k, (w, 1e-6), None, rope, pos)
+    ld, kind = qkv.stride(0), {BF16: L.DTYPE_BF16, F16: L.DTYPE_F16, F32: L.DTYPE_F32}[dtype]
+    L.check(L.load().vdn_fp8_qk_prep_axes(
+        q.data_ptr(), Hq, ld, k.data_ptr(), H, ld, T, d, kind, 1, w.data_ptr(), 1e-6, 0, None, 0.0, rope.inv_freq.data_ptr(), rope.axis.data_ptr(), d,
+        int(pairs), pos.data_ptr(), L.POSITION_I32, 2, 2, q.data_ptr(), ld, k.data_ptr(), ld, torch.cuda.current_stream().cuda_stream), "qk_prep_axes")
+    assert torch.equal(q, want[0]) and torch.equal(k, want[1])
+    assert torch.equal(v, before.split((Hq * d, H * d, H * d), 1)[2].unflatten(1, (-1, d)))

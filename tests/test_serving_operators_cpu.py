@@ -164,3 +164,17 @@ def apart(**over):
 def test_rows_that_share_memory_are_einval(over, needle):
     assert apart(**over) == L.EINVAL
     assert needle in L.load().vdn_fp8_last_error().decode()
+
+
+@pytest.mark.parametrize("over", [
+    # an output over its own input with another stride, or in part
+    dict(oq=FAKE, ldoq=520), dict(ok=FAKE + (1 << 16), ldok=264), dict(oq=FAKE + 1024), dict(oq=FAKE + 3 * 1024 + 1008),
+    dict(ok=FAKE + (1 << 16) - 496), dict(ldk=272, ldok=272, ok=FAKE + (1 << 16) + 32),
+    # over the other side's input or output, also in place
+    dict(oq=FAKE + (1 << 16)), dict(ok=FAKE), dict(ok=OTHER), dict(ok=OTHER + 3 * 1024), dict(k=FAKE, oq=FAKE), dict(oq=FAKE, ok=FAKE + 512),
+    dict(k=FAKE + 768, ldq=640, ldk=640, oq=FAKE, ldoq=640),
+])
+def test_rotated_rows_that_share_memory_are_einval(over):
+    """Four tokens of 4 + 2 heads of 128 bf16 in places of their own, less what `over` puts elsewhere."""
+    assert rope(**{**dict(q=FAKE, k=FAKE + (1 << 16), oq=OTHER, ok=OTHER + (1 << 16)), **over}) == L.EINVAL
+    assert "own input" in L.load().vdn_fp8_last_error().decode()

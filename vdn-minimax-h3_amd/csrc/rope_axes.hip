@@ -263,6 +263,14 @@ extern "C" int vdn_fp8_qk_prep_axes(const void* query, int64_t q_heads, int64_t 
     if (bad(query, q_heads, ldq, out_q, ldoq) || bad(key, k_heads, ldk, out_k, ldok))
         return set_error(VDN_FP8_EINVAL, "%s: rows must be given, 16-byte aligned, with strides multiples of 8 and >= heads * d", what);
     if (!aligned(weight_q, 16) || !aligned(weight_k, 16)) return set_error(VDN_FP8_EINVAL, "%s: misaligned pointer (weights 16 B)", what);
+    // (waves write their slots of a token when they are done with them, in any order)
+    struct Rows { const void* at; int64_t ld, bytes; };
+    const int64_t E = element_bytes(dtype);
+    auto overlap = [&](const Rows& a, const Rows& b) { return a.bytes && b.bytes && rows_overlap(a.at, a.ld, a.bytes, b.at, b.ld, b.bytes, T); };
+    const Rows q{query, ldq * E, q_heads * d * E}, k{key, ldk * E, k_heads * d * E}, oq{out_q, ldoq * E, q.bytes}, ok{out_k, ldok * E, k.bytes};
+    if ((out_q == query ? q_heads && T > 1 && ldoq != ldq : overlap(q, oq)) || (out_k == key ? k_heads && T > 1 && ldok != ldk : overlap(k, ok)) ||
+        overlap(q, ok) || overlap(k, oq) || overlap(oq, ok))
+        return set_error(VDN_FP8_EINVAL, "%s: an output must be its own input, with its stride, or not overlap other rows", what);
     const RopeArgs p{{{query, ldq, (int)q_heads, 0, norm_q != 0, weight_q, eps_q, out_q, ldoq},
                       {key, ldk, (int)k_heads, 0, norm_k != 0, weight_k, eps_k, out_k, ldok}},
                      T, (int)d, (int)rotary_dim, inv_freq, axis, positions, ldpos, rotary_dim > 0 ? (int)axes : 0, position_type, 0, 0, 0};
