@@ -385,3 +385,22 @@ def test_products_beyond_bfloat16(device, T):
     assert float((x.double() @ a[0].double().T).abs().max()) > top
     index = torch.zeros(T, device=device, dtype=torch.int32)
     check(adapter_add(x, base, ad, index), x, base, ad, index)
+
+
+@pytest.mark.parametrize("K,T", [(7176, 7), (7176, 300), (13824, 1), (13824, 40), (13824, 64), (13824, 65), (13824, 700), (13824, 1100), (41000, 30),
+                                 (41000, 520), (41000, 1100), (1 << 17, 3), (1 << 17, 130), (1 << 17, 1030)])
+@pytest.mark.parametrize("R", [16, 48, 64, 128])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_long_rows(device, K, T, R, dtype):
+    """Rows that the form of one launch does not take, those of a feed-forward's down projection and the longest; more than 32 parts of
+    the first product."""
+    print(f"adapters K={K} T={T} R={R} {dtype}", flush=True)
+    N = 136
+    x, base = rows(device, T, K, N, dtype, K + T)
+    ad = bank(device, 3, R, K, N, dtype, R)
+    index = choose(device, T, 3, "random" if T < 100 else "runs", R)
+    got = adapter_add(x, base, ad, index)
+    check(got, x, base, ad, index)
+    mine = base.clone()
+    adapter_add(x, mine, ad, index, out=mine)
+    assert torch.equal(mine, got)
