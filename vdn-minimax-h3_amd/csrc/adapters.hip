@@ -7,10 +7,10 @@
 // the second product to the base. A step of few tokens is one launch (k_few). All are bound by memory (2 R operations for
 // each element of x and of base, R <= 128), so the matrix cores have time to spare: h is not rounded to 16 bits between the
 // products but goes in as two of them, a high and a low part, which lose 2^-17 of it at most and cost the second product twice over
-// (1.5 us of 61 at 6470 tokens of rank 128).
+// (1 us of 79 at 6470 tokens, 5376 -> 7168, rank 128).
 //
-// On the card: 32760 tokens, 5120 -> 15360, rank 64: 70 + 374 us, 5.2 TB/s of the bytes that it cannot do without (a large copy
-// reaches 5.1); 6470 tokens of six requests, 5376 -> 7168, rank 128: 31 + 53 us, 3.3 TB/s; 32 tokens of 12 adapters, 5120 -> 7168, rank 32:
+// On the card: 32760 tokens, 5120 -> 15360, rank 64: 72 + 377 us, 5.2 TB/s of the bytes that it cannot do without (a large copy
+// reaches 5.1); 6470 tokens of six requests, 5376 -> 7168, rank 128: 32 + 53 us, 3.3 TB/s; 32 tokens of 12 adapters, 5120 -> 7168, rank 32:
 // 14 us; one token of rank 16, 5120 -> 5120: 4.6 us.
 //
 // Which tokens share an adapter. A tile is 64 consecutive tokens; a wave holds their adapters one a lane and finds the distinct
@@ -245,8 +245,8 @@ __global__ __launch_bounds__(WK * kLanes) void k_shrink_step(AdapterArgs p)
 }
 
 // Many tokens: a workgroup of four waves takes a tile, 16 tokens a wave and all ranks (R = 16 RF). A matrix operand has 16 rows in 16 neighbouring
-// lanes, and read from memory like that every lane of a quarter wave touches a line of its own (x and A straight into operands:
-// 165 us at 32760 x 5120, rank 64). So both go through LDS: kBk consecutive k of 64 tokens and of R ranks are loaded
+// lanes, and read from memory like that every lane of a quarter wave touches a line of its own (the step's kernels, which read so, take two to five times as
+// long: figures at kStepTokens). So both go through LDS: kBk consecutive k of 64 tokens and of R ranks are loaded
 // as whole lines into registers, one step ahead. Chunk c of 16
 // bytes of a row lies at c ^ (row % 16): rows' writes and columns' reads both spread over all banks.
 constexpr int kWaves = 4;
@@ -566,9 +566,10 @@ __global__ __launch_bounds__(kWaves * kLanes) void k_expand_step(AdapterArgs p)
 // and B the second, column j of product f being column 8 j + f: a lane has eight consecutive columns of a token and 16 neighbouring
 // lanes 256 consecutive bytes of its row, so that base and out are read and written as whole lines. B's 128 rows go through LDS, loaded as whole
 // lines one step ahead: chunk c of row n lies at 17 (n % 8) + n / 8 of the plane of chunk c, the order in which product n % 8 reads it,
-// planes being spaced so that the writes, rows of neighbouring lanes, spread over the banks as well.
+// planes being spaced so that the writes, rows of neighbouring lanes, spread over the banks as well. (Conflicts are 0.38 to 0.48 of the LDS's
+// cycles all the same, and those 0.2 of the time.)
 constexpr int kBn = 128;
-// An out of at least this many bytes, the last-level cache's, is stored non-temporally (32760 x 15360: 367 us of k_expand_tile against 394).
+// An out of at least this many bytes, the last-level cache's, is stored non-temporally (32760 x 15360, rank 64: 442 us a call against 463).
 constexpr int64_t kOnceBytes = 256ll << 20;
 
 // h of 16 tokens of a wave, its parts added, rows of neighbouring lanes: binary32, a row padded by a chunk.
@@ -585,7 +586,7 @@ __device__ __forceinline__ void gather_h(const AdapterArgs& p, int64_t tile, con
         sum[i] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
         from[i] = row0 + row < count ? ((uint32_t)list[row0 + row] * (uint32_t)p.R + 4u * c) * 4u : kOutside;
     }
-    // (two parts at a time, all their loads ahead of the first sum: left to itself the compiler waits for each, 2 us a part)
+    // (two parts at a time, all their loads ahead of the first sum: left to itself the compiler may wait for each)
     for (int s = 0; s < p.S; s += 2) {
         const __amdgpu_buffer_rsrc_t part = part_buffer(p, tile, s), other = part_buffer(p, tile, s + 1 < p.S ? s + 1 : s);
         uint4 v[2][RF];
@@ -701,8 +702,8 @@ __global__ __launch_bounds__(kWaves * kLanes) void k_expand_tile(AdapterArgs p)
                 f32x4_t acc[8];
 #pragma unroll
                 for (int f = 0; f < 8; ++f) acc[f] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
-                // (columns of the next product under this one's: left to itself the compiler reads all eight ahead, 69 us against 66
-                // at 6470 tokens of rank 128)
+                // (columns of the next product under this one's: left to itself the compiler reads all eight ahead, 1% of a call's
+                // time)
                 uint4 v[2][RK];
                 auto read = [&](uint4 (&to)[RK], int f) {
 #pragma unroll
@@ -771,7 +772,8 @@ constexpr int kFewWaves = 16, kFewColumns = 512;
 constexpr int kFewRank = 64, kFewK = 7168;              // (LDS: 8 tokens' x and 512 rows of B of 32 ranks, or 4 tokens' and 64)
 constexpr int few_tokens(int rank_frags) { return rank_frags <= 2 ? 8 : 4; }
 
-// acc + the products of eight elements.
+// acc + the products of eight elements. (binary16 by conversions and single fma: one token of rank 32 6.5 us against bf16's 6.3, eight of
+// one adapter 18.4 against 12.9.)
 template <int TYPE>
 __device__ __forceinline__ float dot8(uint4 a, uint4 b, float acc)
 {
@@ -943,7 +945,19 @@ struct Plan {
     int slots;
 };
 
-constexpr int kStepTokens = 1024;   // at most these many take the step's form
+// At most these many tokens take the step's form, which costs less for each adapter of a few tokens. Both forms, us a call, step's and tiles':
+//                                        65 tokens      256            512            1024           1600
+//   16 adapters, one at random for each token, 5120 -> 5120
+//     rank 16                            11.8   40      16.5   41      25     42      39     52      53     80
+//     rank 64                            17     56      30     59      47     61      83     78      126    124
+//     rank 128                           27     92      60     98      106    103     202    134     286    201
+//   one adapter, 5120 -> 5120
+//     rank 16                            18     12      21     14      22     15      24     18      40     21
+//     rank 64                            27     18      38     19      39     19      60     22      91     27
+//     rank 128                           37     25      40     26      54     27      99     30      169    33
+// So the limit is where the forms cross for such tokens of rank 64; a batch of up to 1024 tokens in which a request has many would be two to
+// three times as fast in tiles, but the host does not read the index.
+constexpr int kStepTokens = 1024;
 constexpr int kFill = 512;          // workgroups that fill the card at two a compute unit
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
@@ -951,9 +965,11 @@ int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 Plan plan_of(int64_t T, int64_t K, int64_t N, int64_t L, int64_t R)
 {
     Plan p{};
-    // One launch where few tokens of an adapter are the rule, all in one tile, and h costs little to compute again for each 512 columns.
-    // One launch against two, rank 32, 5120 -> 7168, us on the card: one token 6.1 and 8.7, 12 tokens of as many adapters 9.7 and 11.7,
-    // 48 of 12 12.3 and 12.2 (and a call's host time is 10 us against 14).
+    // One launch where few tokens of an adapter are to be expected, all in one tile, and h costs little to compute again for each 512
+    // columns. One launch against two, rank 32, 5120 -> 7168, us on the card: one token 6.3 and 9.1, 12 tokens of as many adapters 10.5 and 12.0,
+    // 32 of 12 12.2 and 12.1, 48 of 12 12.8 and 12.4, 64 of 16 13.5 and 13.2 (and a call's host time is 10 us against 14). L is all that the
+    // host knows of how many adapters are used: where those of a large bank are few, one launch is slower from eight tokens of an adapter on
+    // (eight 12.9 and 9.6, 16 18 and 10, 64 55 and 21; rank 64: 22 and 11, 33 and 11, 98 and 29), and so are 64 tokens of 64 adapters (65 and 34).
     p.few = T <= kTile && T <= 4 * L && R <= kFewRank && K <= kFewK;
     p.step = T <= kStepTokens;
     p.tiles = ceil_div(T, kTile);
@@ -972,10 +988,11 @@ Plan plan_of(int64_t T, int64_t K, int64_t N, int64_t L, int64_t R)
     } else {
         const int64_t steps = ceil_div(K, kBk), columns = ceil_div(N, kBn);
         p.rank_frags = (int)(R / 16);
-        // Workgroups to fill the card (k), two rounds of them where the tiles alone are more than the compute units and would be an
-        // uneven one (20000 x 5376 -> 1024, rank 128, 16: 127 and 79 us with two parts, 117 and 74 with four); but seven steps of k in each, as
-        // its first ones wait for memory and the second product fetches every part (1600 tokens, rank 128: 33 us with 21 parts, 26 with
-        // six; 4800: 45 and 42).
+        // Workgroups to fill the card (k), two rounds of them where the tiles alone are more than the compute units, as those that hold the border
+        // between two requests take twice as long and would be the last of one round (5376 -> 1024, us a call with one round and with two: 23000
+        // tokens of three requests, rank 64 102 and 97, rank 128 128 and 122; 20000 of four, rank 16 78 and 70, rank 128 110 and 106; of one
+        // request 58 and 59, 75 and 80, 96 and 97 of ranks 16, 64, 128); but seven steps of k in each, as its first ones wait for memory and the
+        // second product fetches every part (rank 128, 1600 tokens: 31 us with 21 parts, 24 with six; 4800: 42 with seven, 38 with six).
         int64_t parts = ceil_div(p.tiles > 256 ? 2 * kFill : kFill, p.tiles), blocks = kFill / p.tiles;
         const int64_t eighths = ceil_div(columns, 8);
         if (parts < 2) parts = 2;
@@ -983,8 +1000,9 @@ Plan plan_of(int64_t T, int64_t K, int64_t N, int64_t L, int64_t R)
         p.span_k = (int)(kBk * ceil_div(steps, parts));
         p.parts = (int)ceil_div(K, p.span_k);
         // Above 64 ranks two workgroups of k_expand_tile are all that a compute unit has registers for, and where four or more of a tile are
-        // one round of them, an eighth left to tiles of two adapters, more would be two (6470 x 7168, rank 128: 61 us with four, 66 with
-        // seven; 3200 tokens 41 and 49. At rank 64 three go on a compute unit: 58 with four, 53 with seven).
+        // one round of them, an eighth left to tiles of two adapters, more would be two (5376 -> 7168, rank 128, us a call: 6470 tokens of six
+        // requests 82 with four and 90 with seven, 3200 of one 51 and 58. At rank 64 three go on a compute unit: 6470 tokens 63 with four, 60 with
+        // seven).
         const int64_t round = kFill * 7 / 8 / p.tiles;
         if (R > 64 && round >= 4) blocks = round;
         else if (blocks < eighths) blocks = eighths;

@@ -18,7 +18,9 @@ namespace {
 
 constexpr int kLanes = 64;
 constexpr int kMostWaves = 16;   // of a workgroup
-constexpr int64_t kFewRows = 512; // one chunk a thread up to here
+// One chunk a thread up to here, two beyond: us with one and with two, rows of 5120: 64 rows 4.2 and 4.4, 300 6.4 and 6.3, 512 7.7 and 7.9, 821
+// 11.6 and 10.4, 3485 31 and 29; rows of 4104: 512 7.1 and 7.2, 821 10.3 and 10.1, 1500 14.5 and 15.4, 3485 26.5 and 26.0.
+constexpr int64_t kFewRows = 512;
 
 struct AddNormArgs {
     const void* residual;
@@ -72,7 +74,7 @@ constexpr int64_t kOnceBytes = 256ll << 20;
 
 // A workgroup per row, of as many waves as its chunks fill: thread t holds chunk t, or t and t + threads, as
 // binary32 in registers from the addition to the codes, and the partial sums of squares and the maxima meet in
-// LDS. One chunk a thread makes a row short for the few of a step (16 of 5120: 4.1 us on the card); two halve what
+// LDS. One chunk a thread makes a row short for the few of a step (16 of 5120: 4.3 us on the card); two halve what
 // every wave does once, which costs time where there are many (32760 of 5376, gated and modulated: 243 us and
 // 5.1 TB/s, as fast as a copy of those bytes; with one chunk a thread 3% slower). All loads go out before the first of
 // them is used, the tables' as soon as the row's index is there; a table that is absent is a descriptor of no
@@ -164,8 +166,9 @@ __global__ __launch_bounds__(kMostWaves * kLanes) void k_add_norm(AddNormArgs p,
         for (int e = 0; e < 8; ++e) {
             // n + low: low is what the rounding of h rstd leaves out of n, and with a shift that of rstd (without one it cancels
             // against the scale's), without a shift that of the product with w. A code moves where such errors carry a value across a
-            // border between two, the largest's (below) for a whole row: 150 of the 176 million codes of 32760 x 5376 do and none
-            // of 16 x 5120 without a shift; 292 and 8 where n, the scale and the quotient are each rounded to binary32.
+            // border between two, the largest's (below) for a whole row: 110 to 140 of the 176 million codes of 32760 x 5376 (means of
+            // inputs of six seeds: 129) and none of 16 x 5120 without a shift (of twelve); 301 and 6.3 where n, the scale and the quotient
+            // are each rounded to binary32.
             const float t = n[c][e] * rstd, left = __builtin_fmaf(n[c][e], rstd, -t);
             const float t_low = AFFINE ? __builtin_fmaf(n[c][e], rstd_low, left) : left;
             if (AFFINE) {

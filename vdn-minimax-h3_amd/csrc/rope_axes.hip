@@ -20,8 +20,8 @@
 // its wave about 60 operations once, and not once for each of the lanes that need it. The little that the angles need is fetched ahead of
 // the slots (loads come back in order), so that they are ready when those are.
 //
-// On the card: 32760 tokens of 40 + 40 heads of 128 224 us, 6.0 TB/s read and written, with the VALU busy 0.9 of the time (235 with what
-// the angles need fetched behind the rows); 5329 tokens of 16 + 16 heads of 64 10.9; 6405 float32 tokens of 32 + 8 heads of 128 52,
+// On the card: 32760 tokens of 40 + 40 heads of 128 224 us, 6.0 TB/s read and written, with the VALU busy 0.86 of the time (235 with what
+// the angles need fetched behind the rows); 5329 tokens of 16 + 16 heads of 64 11.3; 6405 float32 tokens of 32 + 8 heads of 128 52,
 // 5.1 TB/s; 16 tokens of 40 + 8 heads 3.8, a chain of the positions' load, the angles and the store.
 #include <stdint.h>
 
@@ -192,7 +192,9 @@ __global__ __launch_bounds__(kWaves * kLanes) void k_rope_axes(RopeArgs p, int64
 // Outputs of at least this many bytes are stored non-temporally: beyond what the last-level cache holds,
 // cached stores only evict each other.
 constexpr int64_t kOnceBytes = 256ll << 20;
-constexpr int64_t kFewTokens = 1024;   // a slot a wave below this
+// A slot a wave below this, up to six from there on: us with one and with six, 40 + 40 heads of 128: 256 tokens 5.4 and 6.4, 512 8.6 and 8.3, 1024
+// 14.4 and 12.2; 40 + 8: 512 5.9 and 7.1, 800 8.4 and 8.8, 1024 9.9 and 9.6, 3000 22 and 17; 16 + 16 of 64: 1024 4.9 and 6.1, 3000 10.0 and 9.4.
+constexpr int64_t kFewTokens = 1024;
 
 template <int TYPE, int G, bool PAIRS>
 int launch(RopeArgs p, hipStream_t stream)
